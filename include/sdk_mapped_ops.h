@@ -50,7 +50,8 @@ typedef enum sdk_status {
   SDK_ERR_DEVICE = -4            /* HIP runtime reported an error */
 } sdk_status;
 
-typedef enum sdk_dtype { SDK_F32 = 0, SDK_F64 = 1 } sdk_dtype;
+/* SDK_BF16 and SDK_F16: the operators on token sequences only. */
+typedef enum sdk_dtype { SDK_F32 = 0, SDK_F64 = 1, SDK_BF16 = 2, SDK_F16 = 3 } sdk_dtype;
 
 /* ext_modules/include/enums.h:12-16 (exported by include/layers/enum_export.h:10-18) */
 typedef enum sdk_interp { SDK_NEAREST = 0, SDK_BILINEAR = 1, SDK_BISPHERICAL = 2 } sdk_interp;
@@ -793,6 +794,96 @@ int sdk_mapped_max_unpool_planned_bands(const void* grad_output, const int64_t* 
                                         int64_t height, int64_t width, int64_t out_height,
                                         int64_t out_width, int64_t kernel_size, int32_t interp,
                                         int32_t dtype, sdk_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * Operators on token sequences (spherical samples as tokens; not in the reference):
+ * attention with a learned bias for each bucket of relative positions, residual
+ * addition with root-mean-square norm, AdamW.  dtype: SDK_F32, SDK_BF16 or SDK_F16.
+ * Sums, softmax statistics and norms are float32.
+ * ------------------------------------------------------------------------- */
+
+/* Attention of `queries` tokens to `keys` tokens:
+ *   s[i][j] = scale * <query[i], key[j]> + bias_table[head][bucket_map[i][j]]
+ *   output[i] = sum over j of softmax_j(s[i])[j] * value[j]
+ * A pair (i, j) does not count if bucket_map[i][j] >= buckets, if j >= key_lengths[b], or, with
+ * `causal`, if j > i + key_lengths[b] - queries (the last query sees every key).  A query without
+ * pairs gets zeros, and -inf as its lse.  Keys and values at or beyond key_lengths[b] are not read;
+ * those of pairs that the map leaves out are, and have to be finite.
+ * A bias of -inf leaves its bucket out; finite ones beyond 2^100 / max(scale, 1 / scale) count as that.
+ *
+ * query, output [batch, heads, queries, dim]; key, value [batch, key_heads, keys, dim], heads a
+ * multiple of key_heads (head h reads key head h / (heads / key_heads)); bias_table [heads, buckets]
+ * dense, of `dtype` or float32 (table_dtype); bucket_map [queries, keys] bytes, or one such map for
+ * each batch element; key_lengths [batch] or NULL (every key counts).  Strides in elements, of the
+ * batch, head and token axes; the last axis is dense.  dim: a multiple of 8 up to 128, rows of every
+ * tensor 16-byte aligned; buckets: 1 .. 256; scale > 0.
+ * Backward: gradients that are NULL are not formed; grad_table [heads, buckets] of table_dtype.
+ * Every sum is formed in an order that depends on the sizes alone. */
+typedef struct sdk_bucket_attention {
+  const void* query;
+  const void* key;
+  const void* value;
+  const void* bias_table;
+  const uint8_t* bucket_map;
+  const int32_t* key_lengths;
+  void* output;             /* written by the forward, read by the backward */
+  float* lse;               /* [batch, heads, queries]: log2 of the sum of exp(s); forward: may be NULL */
+  const void* grad_output;
+  void* grad_query;
+  void* grad_key;
+  void* grad_value;
+  void* grad_table;
+  int64_t batch, heads, key_heads, queries, keys, dim, buckets;
+  int64_t query_strides[3], key_strides[3], value_strides[3], output_strides[3];
+  int64_t grad_output_strides[3], grad_query_strides[3], grad_key_strides[3], grad_value_strides[3];
+  int64_t map_strides[2];   /* batch (0: one map for all) and query axis */
+  double scale;
+  int32_t causal, dtype, table_dtype;
+} sdk_bucket_attention;
+
+size_t sdk_bucket_attention_workspace_bytes(const sdk_bucket_attention* a, int32_t backward);
+int sdk_bucket_attention_forward(const sdk_bucket_attention* a, void* workspace, size_t workspace_bytes,
+                                 sdk_stream_t stream);
+int sdk_bucket_attention_backward(const sdk_bucket_attention* a, void* workspace, size_t workspace_bytes,
+                                  sdk_stream_t stream);
+
+/* Rows of x + residual and their root-mean-square norm: out = weight * h / sqrt(mean(h^2) + eps),
+ * h = x + residual (residual NULL: h = x).  summed (may be NULL): h, rounded to dtype; inverse (may be
+ * NULL) [rows]: 1 / sqrt(mean(h^2) + eps), for the backward.  codes 0: out has dtype.  codes 1 or 2:
+ * out holds 8-bit codes, int8 or float8 e4m3, of out / scales[row], scales[row] = largest magnitude /
+ * 127 or / 448 (0, with codes 0, for rows below 2^-100).  width: up to 16384.  weight_dtype: dtype or
+ * SDK_F32.  Dense rows. */
+int sdk_add_rms_norm(const void* x, const void* residual, const void* weight, void* out, float* scales,
+                     void* summed, float* inverse, int64_t rows, int64_t width, double eps, int32_t codes,
+                     int32_t dtype, int32_t weight_dtype, sdk_stream_t stream);
+/* grad_x (the gradient of x and of residual): that of `grad` through the norm plus grad_sum (may be
+ * NULL).  grad_x or grad_weight may be NULL; the workspace is needed for grad_weight. */
+size_t sdk_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int sdk_add_rms_norm_backward(const void* grad, const void* grad_sum, const void* summed, const void* weight,
+                              const float* inverse, void* grad_x, void* grad_weight, void* workspace,
+                              size_t workspace_bytes, int64_t rows, int64_t width, int32_t dtype,
+                              int32_t weight_dtype, sdk_stream_t stream);
+/* out[row] = codes[row] * scales[row]; codes 1 (int8) or 2 (float8 e4m3). */
+int sdk_dequantize_rows(const void* codes_in, const float* scales, void* out, int64_t rows, int64_t width,
+                        int32_t codes, int32_t dtype, sdk_stream_t stream);
+
+/* One AdamW step (decoupled weight decay, both moments corrected for their start) over `count`
+ * tensors, in place.  The lists are host arrays of device pointers, read before the call returns;
+ * params and grads have `dtype`.  step: 1 for the first. */
+int sdk_adamw_step(void* const* params, const void* const* grads, float* const* avgs, float* const* sqs,
+                   const int64_t* sizes, int64_t count, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, int64_t step, int32_t dtype, sdk_stream_t stream);
+/* The same with moments in 8 bits: each 256 consecutive values of a tensor share a scale s, the largest
+ * magnitude among them.  First moment: int8 code c stands for c |c| / 127^2 s; second: uint8 code c for
+ * (c / 255)^4 s, at least code 1 where it is not zero.  Blocks whose largest value is below 2^-126
+ * hold zeros.  Scales: ceil(size / 256) floats. */
+int sdk_adamw_step_8bit(void* const* params, const void* const* grads, int8_t* const* avg_codes,
+                        float* const* avg_scales, uint8_t* const* sq_codes, float* const* sq_scales,
+                        const int64_t* sizes, int64_t count, double lr, double beta1, double beta2, double eps,
+                        double weight_decay, int64_t step, int32_t dtype, sdk_stream_t stream);
+/* The values that the codes of a moment stand for (second: 0 first moment, 1 second). */
+int sdk_adamw_moment_values(const void* codes, const float* scales, void* out, int64_t size, int32_t second,
+                            int32_t dtype, sdk_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,9 @@ kernels in libsdk_mapped_ops.so:
     _weighted_mapped_max_pooling, _mapped_avg_pooling, _weighted_mapped_avg_pooling,
     _uv_resample, _voting_resample
 
+and, beyond the reference, `_token_ops`: operators on token sequences (attention with a bucketed
+bias, residual RMS norm, AdamW).
+
 Importing the package loads the library and registers the operators; it raises
 ImportError when the library has not been built.
 """
@@ -20,4 +23,5 @@ from . import _capi
 _capi.load()
 
 from . import _ops  # noqa: E402  (registers torch.ops.sdk_mapped_ops.*)
+from . import _token_ops  # noqa: E402,F401  (the operators on token sequences)
 from . import _enums  # noqa: E402,F401

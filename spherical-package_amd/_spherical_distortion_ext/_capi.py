@@ -9,11 +9,26 @@ import os
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_ROOT, "libsdk_mapped_ops.so")
 
-SDK_F32, SDK_F64 = 0, 1
+SDK_F32, SDK_F64, SDK_BF16, SDK_F16 = 0, 1, 2, 3
 SDK_COMPUTE_NATIVE, SDK_COMPUTE_BF16, SDK_COMPUTE_UNFUSED, SDK_COMPUTE_SPLIT = 0, 1, 2, 3
 
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
 
+
+
+class BucketAttention(ctypes.Structure):
+    """sdk_bucket_attention."""
+    _fields_ = ([(n, _vp) for n in ("query", "key", "value", "bias_table", "bucket_map", "key_lengths", "output",
+                                    "lse", "grad_output", "grad_query", "grad_key", "grad_value", "grad_table")]
+                + [(n, _i64) for n in ("batch", "heads", "key_heads", "queries", "keys", "dim", "buckets")]
+                + [(n + "_strides", _i64 * 3) for n in ("query", "key", "value", "output", "grad_output",
+                                                        "grad_query", "grad_key", "grad_value")]
+                + [("map_strides", _i64 * 2), ("scale", ctypes.c_double), ("causal", _i32), ("dtype", _i32),
+                   ("table_dtype", _i32)])
+
+
+_attention = ctypes.POINTER(BucketAttention)
+_step_settings = [_i64] + [ctypes.c_double] * 5 + [_i64, _i32, _vp]
 # name -> argument types, in header order
 _CONV_DIMS = [_i64] * 8 + [_i32] * 4 + [_vp]
 SIGNATURES = {
@@ -78,13 +93,23 @@ SIGNATURES = {
     "sdk_mapped_max_unpool_planned": [_vp] * 6 + [_sz] + [_i64] * 7 + [_i32] * 3 + [_vp],
     "sdk_mapped_max_unpool_plan_bands": [_vp, _sz, _i64, _i64, _i32, _vp, _vp],
     "sdk_mapped_max_unpool_planned_bands": [_vp] * 5 + [_sz] + [_i64] * 7 + [_i32] * 2 + [_vp],
+    # operators on token sequences
+    "sdk_bucket_attention_forward": [_attention, _vp, _sz, _vp],
+    "sdk_bucket_attention_backward": [_attention, _vp, _sz, _vp],
+    "sdk_add_rms_norm": [_vp] * 7 + [_i64] * 2 + [ctypes.c_double] + [_i32] * 3 + [_vp],
+    "sdk_add_rms_norm_backward": [_vp] * 8 + [_sz] + [_i64] * 2 + [_i32] * 2 + [_vp],
+    "sdk_dequantize_rows": [_vp] * 3 + [_i64] * 2 + [_i32] * 2 + [_vp],
+    "sdk_adamw_step": [_vp] * 5 + _step_settings,
+    "sdk_adamw_step_8bit": [_vp] * 7 + _step_settings,
+    "sdk_adamw_moment_values": [_vp] * 3 + [_i64] + [_i32] * 2 + [_vp],
 }
 OTHER_SYMBOLS = ("sdk_last_error", "sdk_version", "sdk_mapped_conv_workspace_bytes",
                  "sdk_resample_to_map_workspace_bytes", "sdk_mapped_max_unpool_workspace_bytes",
                  "sdk_resample_to_uv_maps_workspace_bytes", "sdk_voting_resample_workspace_bytes",
                  "sdk_mapped_conv_plan_bytes", "sdk_mapped_conv_plan_bytes_columns",
                  "sdk_mapped_conv_columns_bytes",
-                 "sdk_mapped_avg_unpool_lists_bytes")
+                 "sdk_mapped_avg_unpool_lists_bytes", "sdk_bucket_attention_workspace_bytes",
+                 "sdk_add_rms_norm_backward_workspace_bytes")
 
 _lib = None
 
@@ -125,6 +150,10 @@ def load():
     lib.sdk_mapped_avg_unpool_lists_bytes.restype = _sz
     lib.sdk_mapped_avg_unpool_lists_bytes.argtypes = [_i64] * 5 + [_i32] * 3
     lib.sdk_mapped_conv_plan_bytes.restype = _sz
+    lib.sdk_bucket_attention_workspace_bytes.argtypes = [_attention, _i32]
+    lib.sdk_bucket_attention_workspace_bytes.restype = _sz
+    lib.sdk_add_rms_norm_backward_workspace_bytes.argtypes = [_i64] * 2
+    lib.sdk_add_rms_norm_backward_workspace_bytes.restype = _sz
     _lib = lib
     return lib
 

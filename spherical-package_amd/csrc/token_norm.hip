@@ -1,0 +1,359 @@
+// Addition of the residual and root-mean-square norm of rows, with gradients, and the same with rows in
+// 8 bits and a scale each.
+//
+//   h = x + r            y_j = w_j h_j inv,  inv = 1 / sqrt(mean_j h_j^2 + eps)
+//   dh_j = inv (w_j g_j - h_j inv^2 mean_i(w_i g_i h_i)) + s_j      (g, s: the gradients of y and h)
+//   dw_j = sum over rows of g_j h_j inv
+//
+// All of it is bound by memory: a row is read once, held in registers, and every sum over it (squares,
+// largest magnitude, w g h) is formed there.  Sums are float32.  The forward normalises the sum before it is
+// rounded to the tensors' type; the backward reads the rounded h, which the forward wrote.
+#include <algorithm>
+
+#include "token_types.hpp"
+
+namespace sdk {
+namespace token {
+namespace {
+
+// A row is dealt to THREADS threads, N chunks of V elements each: chunk k of thread t begins at
+// (k * THREADS + t) * V, so that a wave reads consecutive memory.  Workgroups of at least 256 threads:
+// narrow rows share one.
+template <int THREADS>
+constexpr int kGroup = THREADS < 256 ? 256 : THREADS;
+
+constexpr int kPlain = 0, kInt8 = 1, kFp8 = 2;
+constexpr float kSmallestRow = 0x1p-100f;   // rows below it are zeros in 8 bits: 1 / scale stays finite
+
+template <typename T, int V>
+__device__ __forceinline__ void load_weight(const void* w, int is_float, int64_t at, float (&f)[V]) {
+  if (is_float)
+    load_pack<float, V>((const float*)w + at, f);
+  else
+    load_pack<T, V>((const T*)w + at, f);
+}
+
+template <typename T, int V, int N, int THREADS>
+__global__ __launch_bounds__(kGroup<THREADS>) void norm_forward(
+    const T* x, const T* residual, const void* weight, int weight_float, void* out, float* scales,
+    T* summed, float* inverse, int64_t rows, int width, float eps, int codes) {
+  __shared__ float slots[kGroup<THREADS> / 64];
+  const int t = threadIdx.x % THREADS;
+  const int64_t row = (int64_t)blockIdx.x * (kGroup<THREADS> / THREADS) + threadIdx.x / THREADS;
+  const bool live = row < rows;
+  const int64_t base = row * width;
+  float h[N][V];
+  float sq = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+    if (live && j < width) {
+      load_pack<T, V>(x + base + j, h[k]);
+      if (residual) {
+        float r[V];
+        load_pack<T, V>(residual + base + j, r);
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[k][e] += r[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[k][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sq += h[k][e] * h[k][e];
+  }
+  if (summed) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = (k * THREADS + t) * V;
+      if (live && j < width) store_pack<T, V>(summed + base + j, h[k]);
+    }
+  }
+  sq = over_group<Add, THREADS>(sq, slots);
+  const float inv = 1.f / sqrtf(sq / (float)width + eps);
+  if (inverse && live && t == 0) inverse[row] = inv;
+  float largest = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+    if (j < width) {
+      float w[V];
+      load_weight<T, V>(weight, weight_float, j, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        h[k][e] = h[k][e] * inv * w[e];
+        if (codes != kPlain) largest = Largest::of(largest, fabsf(h[k][e]));
+      }
+      if (codes == kPlain && live) store_pack<T, V>((T*)out + base + j, h[k]);
+    }
+  }
+  if (codes == kPlain) return;
+  largest = over_group<Largest, THREADS>(largest, slots);
+  const float most = codes == kInt8 ? 127.f : 448.f;
+  const bool some = !(largest < kSmallestRow);   // a row with a NaN keeps it in its scale
+  const float up = some ? most / largest : 0.f;
+  if (live && t == 0) scales[row] = some ? largest * (1.f / most) : 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+    if (live && j < width) {
+      Pack<unsigned char, V> c;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        // v * up can pass the largest code by an ulp (127.00001, 448.00003): both roundings take it back
+        const float v = h[k][e] * up;
+        if (codes == kInt8)
+          c.v[e] = (unsigned char)(signed char)(int)rintf(v);
+        else
+          c.v[e] = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(
+                       fminf(fmaxf(v, -448.f), 448.f), 0.f, 0, false) & 0xff);
+      }
+      *reinterpret_cast<Pack<unsigned char, V>*>((unsigned char*)out + base + j) = c;
+    }
+  }
+}
+
+// Workgroup b takes rows b, b + gridDim.x, ... (times the rows that share a workgroup) and keeps its part of
+// dw in registers; the parts are joined in their order by norm_weight_grad.
+template <typename T, int V, int N, int THREADS>
+__global__ __launch_bounds__(kGroup<THREADS>) void norm_backward(
+    const T* grad, const T* grad_sum, const T* h_in, const void* weight, int weight_float,
+    const float* inverse, T* grad_x, float* parts, int64_t rows, int width) {
+  constexpr int SHARE = kGroup<THREADS> / THREADS;
+  __shared__ float slots[kGroup<THREADS> / 64];
+  const int t = threadIdx.x % THREADS, sub = threadIdx.x / THREADS;
+  float w[N][V], dw[N][V];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[k][e] = dw[k][e] = 0.f;
+    if (j < width) load_weight<T, V>(weight, weight_float, j, w[k]);
+  }
+  for (int64_t first = (int64_t)blockIdx.x * SHARE; first < rows; first += (int64_t)gridDim.x * SHARE) {
+    const int64_t row = first + sub, base = row * width;
+    const bool live = row < rows;
+    const float inv = live ? inverse[row] : 0.f;
+    float h[N][V], g[N][V], dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = (k * THREADS + t) * V;
+      if (live && j < width) {
+        load_pack<T, V>(h_in + base + j, h[k]);
+        load_pack<T, V>(grad + base + j, g[k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[k][e] = g[k][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        dw[k][e] += g[k][e] * (h[k][e] * inv);
+        g[k][e] *= w[k][e];
+        dot += g[k][e] * h[k][e];
+      }
+    dot = over_group<Add, THREADS>(dot, slots);
+    if (grad_x) {
+      const float along = inv * inv * (dot / (float)width);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int j = (k * THREADS + t) * V;
+        if (live && j < width) {
+          float s[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[e] = 0.f;
+          if (grad_sum) load_pack<T, V>(grad_sum + base + j, s);
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[e] += inv * (g[k][e] - h[k][e] * along);
+          store_pack<T, V>(grad_x + base + j, s);
+        }
+      }
+    }
+  }
+  if (!parts) return;
+  float* mine = parts + ((int64_t)blockIdx.x * SHARE + sub) * width;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (j + e < width) mine[j + e] = dw[k][e];
+  }
+}
+
+// dw[j] = sum over the parts, 64 columns a workgroup, a quarter of the parts a wave.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_weight_grad(const float* parts, int64_t count, int width,
+                                                        void* grad_weight, int is_float) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int j = blockIdx.x * 64 + lane;
+  const int64_t each = (count + 3) / 4, from = wave * each, to = from + each < count ? from + each : count;
+  float s = 0.f;
+  if (j < width)
+    for (int64_t i = from; i < to; ++i) s += parts[i * width + j];
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && j < width) {
+    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    if (is_float)
+      ((float*)grad_weight)[j] = s;
+    else
+      ((T*)grad_weight)[j] = (T)s;
+  }
+}
+
+// out = codes * scale of the row, a chunk of V codes a thread.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void dequantize(const unsigned char* codes, const float* scales, T* out,
+                                                  int64_t chunks, int per_row, int fp8) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= chunks) return;
+  const float s = scales[c / per_row];
+  const Pack<unsigned char, V> q = reinterpret_cast<const Pack<unsigned char, V>*>(codes)[c];
+  float f[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    f[e] = (fp8 ? __builtin_amdgcn_cvt_f32_fp8((int)q.v[e], 0) : (float)(signed char)q.v[e]) * s;
+  store_pack<T, V>(out + c * V, f);
+}
+
+// Threads of a row: at most 16 elements a thread.
+int threads_of(int64_t width) { return width <= 1024 ? 64 : width <= 4096 ? 256 : 1024; }
+constexpr int64_t kMostWidth = 16384;
+
+// Runs `CALL` with V, N and THREADS for rows of `width`; `wide`: 16-byte vectors fit rows and pointers.
+#define NORM_SHAPE_N(NN, CALL)                                            \
+  do {                                                                    \
+    constexpr int N = NN;                                                 \
+    if (threads == 64) { constexpr int THREADS = 64; CALL; }              \
+    else if (threads == 256) { constexpr int THREADS = 256; CALL; }       \
+    else { constexpr int THREADS = 1024; CALL; }                          \
+  } while (0)
+#define NORM_SHAPE(CALL)                                                  \
+  do {                                                                    \
+    const int threads = threads_of(width);                                \
+    if (wide) {                                                           \
+      constexpr int V = kWide<T>;                                         \
+      const int64_t n = ceil_div(width, (int64_t)threads * V);            \
+      if (n <= 1) NORM_SHAPE_N(1, CALL);                                  \
+      else if (n <= 2) NORM_SHAPE_N(2, CALL);                             \
+      else if constexpr (V <= 4) NORM_SHAPE_N(4, CALL);                   \
+    } else {                                                              \
+      constexpr int V = 1;                                                \
+      if (width <= 4 * threads) NORM_SHAPE_N(4, CALL);                    \
+      else NORM_SHAPE_N(16, CALL);                                        \
+    }                                                                     \
+  } while (0)
+
+int64_t backward_groups(int64_t rows, int64_t width) {
+  const int threads = threads_of(width), share = threads < 256 ? 256 / threads : 1;
+  const int64_t groups = threads == 1024 ? 512 : 1024;
+  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, share), groups));
+}
+
+int check(int64_t rows, int64_t width, int dtype, int weight_dtype) {
+  SDK_REQUIRE(rows >= 0, "rows = %lld must not be negative", (long long)rows);
+  SDK_REQUIRE(width >= 1 && width <= kMostWidth, "width = %lld must be between 1 and %lld",
+              (long long)width, (long long)kMostWidth);
+  SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
+  SDK_REQUIRE(weight_dtype == dtype || weight_dtype == SDK_F32,
+              "weight's dtype %d must be the rows' or float32", weight_dtype);
+  return SDK_OK;
+}
+
+}  // namespace
+}  // namespace token
+}  // namespace sdk
+
+using namespace sdk;
+using namespace sdk::token;
+
+extern "C" {
+
+int sdk_add_rms_norm(const void* x, const void* residual, const void* weight, void* out, float* scales,
+                     void* summed, float* inverse, int64_t rows, int64_t width, double eps, int32_t codes,
+                     int32_t dtype, int32_t weight_dtype, sdk_stream_t stream) {
+  if (int rc = check(rows, width, dtype, weight_dtype)) return rc;
+  SDK_REQUIRE(codes >= 0 && codes <= 2, "codes = %d must be 0 (none), 1 (int8) or 2 (float8 e4m3)", codes);
+  SDK_REQUIRE(eps >= 0, "eps must not be negative");
+  if (rows == 0) return SDK_OK;
+  SDK_REQUIRE(x && weight && out, "x, weight and out must not be NULL");
+  SDK_REQUIRE(codes == 0 || scales, "scales must not be NULL where the output is in 8 bits");
+  hipStream_t s = (hipStream_t)stream;
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, {
+    const bool wide = width % kWide<T> == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) &&
+                      aligned16(out) && aligned16(summed);
+    NORM_SHAPE(launch(norm_forward<T, V, N, THREADS>,
+                      dim3((unsigned)ceil_div(rows, kGroup<THREADS> / THREADS)), dim3(kGroup<THREADS>), s,
+                      (const T*)x, (const T*)residual, weight, (int)(weight_dtype == SDK_F32), out, scales,
+                      (T*)summed, inverse, rows, (int)width, (float)eps, (int)codes));
+  });
+  SDK_LAUNCH_CHECK("add_rms_norm");
+  return SDK_OK;
+}
+
+size_t sdk_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
+  if (rows < 1 || width < 1 || width > kMostWidth) return 0;
+  const int threads = threads_of(width), share = threads < 256 ? 256 / threads : 1;
+  return (size_t)backward_groups(rows, width) * share * width * sizeof(float);
+}
+
+int sdk_add_rms_norm_backward(const void* grad, const void* grad_sum, const void* summed, const void* weight,
+                              const float* inverse, void* grad_x, void* grad_weight, void* workspace,
+                              size_t workspace_bytes, int64_t rows, int64_t width, int32_t dtype,
+                              int32_t weight_dtype, sdk_stream_t stream) {
+  if (int rc = check(rows, width, dtype, weight_dtype)) return rc;
+  SDK_REQUIRE(weight && (grad_x || grad_weight), "weight and one gradient at least must not be NULL");
+  SDK_REQUIRE(rows == 0 || (grad && summed && inverse), "grad, summed and inverse must not be NULL");
+  const size_t need = grad_weight ? sdk_add_rms_norm_backward_workspace_bytes(rows, width) : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SDK_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t groups = rows ? backward_groups(rows, width) : 0;
+  const int share = threads_of(width) < 256 ? 256 / threads_of(width) : 1;
+  float* parts = grad_weight ? (float*)workspace : nullptr;
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, {
+    const bool wide = width % kWide<T> == 0 && aligned16(grad) && aligned16(grad_sum) && aligned16(summed) &&
+                      aligned16(weight) && aligned16(grad_x);
+    if (rows)
+      NORM_SHAPE(launch(norm_backward<T, V, N, THREADS>, dim3((unsigned)groups), dim3(kGroup<THREADS>), s,
+                        (const T*)grad, (const T*)grad_sum, (const T*)summed, weight,
+                        (int)(weight_dtype == SDK_F32), inverse, (T*)grad_x, parts, rows, (int)width));
+    if (grad_weight)
+      launch(norm_weight_grad<T>, dim3((unsigned)ceil_div(width, 64)), dim3(256), s, (const float*)parts,
+             groups * share, (int)width, grad_weight, (int)(weight_dtype == SDK_F32));
+  });
+  SDK_LAUNCH_CHECK("add_rms_norm_backward");
+  return SDK_OK;
+}
+
+int sdk_dequantize_rows(const void* codes, const float* scales, void* out, int64_t rows, int64_t width,
+                        int32_t codes_kind, int32_t dtype, sdk_stream_t stream) {
+  SDK_REQUIRE(rows >= 0 && width >= 1 && width < (int64_t)1 << 31, "rows %lld of width %lld", (long long)rows,
+              (long long)width);
+  SDK_REQUIRE(codes_kind == kInt8 || codes_kind == kFp8, "codes = %d must be 1 (int8) or 2 (float8 e4m3)",
+              codes_kind);
+  SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
+  if (rows == 0) return SDK_OK;
+  SDK_REQUIRE(codes && scales && out, "codes, scales and out must not be NULL");
+  hipStream_t s = (hipStream_t)stream;
+  const bool wide = width % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)out & 31) == 0;
+  const int64_t chunks = rows * width / (wide ? 8 : 1);
+  SDK_REQUIRE(ceil_div(chunks, 256) < (int64_t)1 << 31, "%lld rows of width %lld are too many",
+              (long long)rows, (long long)width);
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, {
+    if (wide)
+      launch(dequantize<T, 8>, dim3((unsigned)ceil_div(chunks, 256)), dim3(256), s,
+             (const unsigned char*)codes, scales, (T*)out, chunks, (int)(width / 8), (int)(codes_kind == kFp8));
+    else
+      launch(dequantize<T, 1>, dim3((unsigned)ceil_div(chunks, 256)), dim3(256), s,
+             (const unsigned char*)codes, scales, (T*)out, chunks, (int)width, (int)(codes_kind == kFp8));
+  });
+  SDK_LAUNCH_CHECK("dequantize_rows");
+  return SDK_OK;
+}
+
+}  // extern "C"

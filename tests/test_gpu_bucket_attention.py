@@ -1,0 +1,289 @@
+"""Attention with a bias for each bucket of relative positions, against its definition in float64 on the
+CPU: forward, the gradients of queries, keys, values and bias table, and the forms of serving.
+
+Tolerances, of the largest value of an output (norm-relative): a sum of products of values rounded to a type
+with unit roundoff u is off by a few u where the weights p and ds are rounded once before the second product and
+the result once more; 4 u covers both and the order of float32 sums: 2^-7 / 2 = 1.6e-2 for bfloat16, 2e-3 for
+float16.  float32: the exponent of exp2 is off by 2^-24 of its magnitude (up to 2^5 here), so p by 2^-24 * 32 * ln 2
+= 1.3e-6; sums over at most 700 terms of either sign add less than as much again: 4e-6.
+ds is the difference of two float32 sums over the head's values, which cancel where a row has one key: an absolute
+term of 2^-22 of the sum's terms comes on top of the relative one.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TOL = {torch.float32: 4e-6, torch.bfloat16: 1.6e-2, torch.float16: 2e-3}
+
+
+def _exact(q, k, v, table, bmap, lengths=None, causal=False, scale=None, grad=None):
+    """Definition in float64 on the CPU; with grad also the gradients of q, k, v and table."""
+    q, k, v, table = (t.detach().double().cpu() for t in (q, k, v, table))
+    bmap = bmap.cpu().long()
+    B, H, Lq, D = q.shape
+    Hk, Lk = k.shape[1:3]
+    G, NB = H // Hk, table.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    maps = bmap if bmap.dim() == 3 else bmap.expand(B, Lq, Lk)
+    out, dq, dk, dv, dt = (torch.zeros_like(t) for t in (q, q, k, v, table))
+    for b in range(B):
+        n = Lk if lengths is None else int(lengths[b])
+        m = maps[b, :, :n]
+        seen = m < NB
+        if causal:
+            seen = seen & (torch.arange(n)[None] <= torch.arange(Lq)[:, None] + (n - Lq))
+        for h in range(H):
+            kk, vv = k[b, h // G, :n], v[b, h // G, :n]
+            s = scale * (q[b, h] @ kk.T) + table[h][m.clamp(max=NB - 1)]
+            s = s.masked_fill(~seen, -math.inf)
+            top = s.amax(1, keepdim=True) if n else torch.zeros(Lq, 1, dtype=torch.float64)
+            p = torch.exp(s - torch.where(top.isinf(), 0.0, top))
+            total = p.sum(1, keepdim=True)
+            p = torch.where(total > 0, p / total, 0.0)
+            out[b, h] = p @ vv
+            if grad is not None:
+                g = grad[b, h].double().cpu()
+                ds = p * (g @ vv.T - (g * out[b, h]).sum(1, keepdim=True))
+                dq[b, h] = scale * ds @ kk
+                dk[b, h // G, :n] += scale * ds.T @ q[b, h]
+                dv[b, h // G, :n] += p.T @ g
+                dt[h].index_add_(0, m[seen], ds[seen])
+    return out if grad is None else (out, dq, dk, dv, dt)
+
+
+def _close(got, want, tol, terms=0.0):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape
+    assert bool(torch.isfinite(got).all())
+    if got.numel():
+        assert float((got - want).abs().max()) <= tol * float(want.abs().max()) + 2.0 ** -22 * terms
+
+
+def _terms(q, k, v, do):
+    """Size of the terms that cancel in the gradients: |do| |v| of a pair times the other operand."""
+    each = float(do.detach().double().norm(dim=-1).max() * v.detach().double().norm(dim=-1).max())
+    return (0.0, each * float(k.detach().abs().max()), each * float(q.detach().abs().max()), 0.0, each)
+
+
+def _inputs(B, H, Hk, Lq, Lk, D, NB, dtype, seed, out_share=0.0, per_batch=False):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, do = (torch.randn(*s, generator=g).to(dtype).to(DEV)
+                   for s in ((B, H, Lq, D), (B, Hk, Lk, D), (B, Hk, Lk, D), (B, H, Lq, D)))
+    table = torch.randn(H, NB, generator=g).to(DEV)
+    bmap = torch.randint(0, NB, ((B, Lq, Lk) if per_batch else (Lq, Lk)), generator=g)
+    if out_share:
+        bmap[torch.rand(bmap.shape, generator=g) < out_share] = 255
+    return q, k, v, table, bmap.to(torch.uint8).to(DEV), do
+
+
+SHAPES = [  # B, H, Hk, Lq, Lk, D, buckets
+    (1, 1, 1, 1, 1, 8, 1),
+    (2, 3, 1, 7, 5, 16, 2),
+    (1, 4, 2, 31, 33, 24, 9),
+    (2, 2, 2, 64, 64, 32, 32),
+    (1, 6, 2, 65, 127, 40, 33),
+    (1, 2, 1, 129, 191, 64, 64),
+    (2, 4, 1, 128, 257, 72, 65),
+    (1, 3, 3, 200, 130, 128, 129),
+    (1, 2, 2, 33, 700, 96, 250),
+    (1, 8, 1, 5, 600, 128, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_gradients(shape, dtype):
+    from spherical_distortion import functional as F
+    B, H, Hk, Lq, Lk, D, NB = shape
+    q, k, v, table, bmap, do = _inputs(*shape, dtype, seed=sum(shape), out_share=0.1 if NB < 255 else 0.0)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = F.bucket_attention(*leaves, bmap)
+    grads = torch.autograd.grad(out, leaves, do)
+    want = _exact(q, k, v, table, bmap, grad=do)
+    for got, ref, terms in zip((out, *grads), want, _terms(q, k, v, do)):
+        _close(got, ref, TOL[dtype], terms)
+    assert [g.dtype for g in grads] == [dtype] * 3 + [torch.float32]
+    with torch.no_grad():
+        assert torch.equal(F.bucket_attention(*leaves, bmap), out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lq,lk", [(100, 100), (37, 260), (260, 37), (1, 300), (3, 70)])
+def test_lengths_causal_and_maps_of_each_sequence(dtype, causal, lq, lk):
+    """Lengths of zero, one and all; keys and values beyond a length hold NaN and infinity."""
+    from spherical_distortion import functional as F
+    lengths = torch.tensor([lk, 0, 1, lk // 2], dtype=torch.int32)
+    q, k, v, table, bmap, do = _inputs(4, 4, 2, lq, lk, 48, 20, dtype, seed=lq + lk, out_share=0.2, per_batch=True)
+    for b in range(4):
+        k[b, :, int(lengths[b]):] = math.nan
+        v[b, :, int(lengths[b]):] = math.inf
+    clean_k, clean_v = k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = F.bucket_attention(*leaves, bmap, key_lengths=lengths.to(DEV), causal=causal)
+    grads = torch.autograd.grad(out, leaves, do)
+    want = _exact(q, clean_k, clean_v, table, bmap, lengths, causal, grad=do)
+    for got, ref, terms in zip((out, *grads), want, _terms(q, clean_k, clean_v, do)):
+        _close(got, ref, TOL[dtype], terms)
+    assert not bool(out[1].any())   # a sequence without keys
+
+
+def test_rows_and_columns_without_pairs():
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(2, 2, 1, 150, 170, 32, 12, torch.float32, seed=3)
+    bmap[17] = 200
+    bmap[128:] = 12          # the first value that is no bucket
+    bmap[:, 40:60] = 255
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = F.bucket_attention(*leaves, bmap)
+    grads = torch.autograd.grad(out, leaves, do)
+    for got, ref in zip((out, *grads), _exact(q, k, v, table, bmap, grad=do)):
+        _close(got, ref, TOL[torch.float32])
+    for t in (out[:, :, 17], out[:, :, 128:], grads[0][:, :, 17], grads[1][:, :, 40:60], grads[2][:, :, 40:60]):
+        assert not bool(t.any())
+    everything = torch.full_like(bmap, 255)
+    out = F.bucket_attention(*leaves, everything)
+    assert not bool(out.any())
+    for t in torch.autograd.grad(out, leaves, do):
+        assert not bool(t.any())
+
+
+@pytest.mark.parametrize("lowest", [torch.finfo(torch.float32).min, -math.inf, -1e30])
+def test_biases_that_mask(lowest):
+    """A bias of the type's lowest value: the pair's weight is zero beside others, and equal among
+    themselves; -inf leaves the pair out."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 2, 2, 70, 90, 64, 6, torch.float32, seed=5)
+    table[0, 2] = lowest
+    table[1, :] = lowest
+    bmap[9] = 2
+    out = F.bucket_attention(q, k, v, table, bmap)
+    want = _exact(q, k, v, table, bmap)
+    _close(out, want, TOL[torch.float32])
+
+
+def test_bias_table_of_the_queries_type_and_scale():
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(2, 4, 2, 90, 110, 64, 30, torch.bfloat16, seed=6)
+    table = table.to(torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    for scale in (0.01, 1.5):
+        out = F.bucket_attention(*leaves, bmap, scale=scale)
+        grads = torch.autograd.grad(out, leaves, do)
+        assert grads[3].dtype == torch.bfloat16
+        for got, ref in zip((out, *grads), _exact(q, k, v, table, bmap, scale=scale, grad=do)):
+            _close(got, ref, TOL[torch.bfloat16])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_unaligned_views(dtype):
+    """Heads packed beside each other, a map that is a view of a larger one at an odd address, rows that
+    are not 16-byte aligned."""
+    from spherical_distortion import functional as F
+    g = torch.Generator().manual_seed(8)
+    B, H, L, D, NB = 2, 3, 77, 32, 11
+    packed = torch.randn(B, L, 3, H, D, generator=g).to(dtype).to(DEV)
+    q, k, v = (packed[:, :, i].transpose(1, 2) for i in range(3))
+    table = torch.randn(H, NB, generator=g).to(DEV)
+    big = torch.randint(0, NB, (L + 2, L + 6), generator=g).to(torch.uint8).to(DEV)
+    bmap = big[1:-1, 5:-1]
+    _close(F.bucket_attention(q, k, v, table, bmap), _exact(q, k, v, table, bmap), TOL[dtype])
+    wide = torch.randn(B, H, L, D + 3, generator=g).to(dtype).to(DEV)
+    odd = wide[..., 1:-2]
+    do = torch.randn(B, H, D, L, generator=g).to(dtype).to(DEV).transpose(2, 3)
+    leaves = [t.detach().requires_grad_() for t in (odd, k, v, table)]
+    out = F.bucket_attention(*leaves, bmap.t().contiguous().t())
+    grads = torch.autograd.grad(out, leaves, do)
+    for got, ref in zip((out, *grads), _exact(odd, k, v, table, bmap, grad=do)):
+        _close(got, ref, TOL[dtype])
+
+
+def test_gradients_against_differences():
+    """Central differences of a weighted sum of the outputs in float32: its value is about 10, so a step of
+    2^-6 gives quotients off by about 10 * 2^-22 / 2^-6 = 2e-4 from rounding and 1e-4 from the third
+    derivative: 2e-3 of a gradient of order one."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 2, 1, 9, 11, 16, 5, torch.float32, seed=11)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    grads = torch.autograd.grad(F.bucket_attention(*leaves, bmap), leaves, do)
+    step = 2.0 ** -6
+    g = torch.Generator().manual_seed(1)
+    for i, grad in enumerate(grads):
+        for _ in range(4):
+            at = [int(torch.randint(0, n, (1,), generator=g)) for n in grad.shape]
+            sides = []
+            for sign in (1, -1):
+                moved = [t.detach().clone() for t in leaves]
+                moved[i][tuple(at)] += sign * step
+                sides.append((F.bucket_attention(*moved, bmap).double() * do.double()).sum())
+            want = float(sides[0] - sides[1]) / (2 * step)
+            assert abs(float(grad[tuple(at)]) - want) <= 2e-3 * max(1.0, abs(want))
+
+
+def test_gradients_that_are_not_wanted_and_repeated_runs():
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(2, 4, 2, 140, 150, 64, 40, torch.bfloat16, seed=12)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    full = torch.autograd.grad(F.bucket_attention(*leaves, bmap), leaves, do)
+    again = torch.autograd.grad(F.bucket_attention(*leaves, bmap), leaves, do)
+    for a, b in zip(full, again):
+        assert torch.equal(a, b)   # every sum has one order
+    for i in range(4):
+        one = [t.detach().requires_grad_(j == i) for j, t in enumerate(leaves)]
+        got, = torch.autograd.grad(F.bucket_attention(*one, bmap), [one[i]], do)
+        assert torch.equal(got, full[i])
+
+
+def test_empty_sizes():
+    from spherical_distortion import functional as F
+    for B, Lq, Lk in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
+        q, k, v, table, bmap, do = _inputs(B, 2, 1, Lq, Lk, 16, 3, torch.float32, seed=1)
+        leaves = [t.requires_grad_() for t in (q, k, v, table)]
+        out = F.bucket_attention(*leaves, bmap)
+        assert out.shape == (B, 2, Lq, 16) and not bool(out.any())
+        for t, g in zip(leaves, torch.autograd.grad(out, leaves, do)):
+            assert g.shape == t.shape and not bool(g.any())
+
+
+def test_another_stream_and_a_graph():
+    """The pass on a side stream, and a captured one replayed with new inputs."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 4, 1, 2, 900, 64, 30, torch.bfloat16, seed=13)
+    want = F.bucket_attention(q, k, v, table, bmap)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = F.bucket_attention(q, k, v, table, bmap)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = F.bucket_attention(q, k, v, table, bmap)
+    for seed in (20, 21, 22):
+        fresh = _inputs(1, 4, 1, 2, 900, 64, 30, torch.bfloat16, seed=seed)
+        for old, new in zip((q, k, v, table), fresh):
+            old.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, F.bucket_attention(q, k, v, table, bmap))
+
+
+def test_refusals():
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(2, 4, 2, 8, 9, 16, 3, torch.float32, seed=1)
+    call = F.bucket_attention
+    call(q, k, v, table, bmap)
+    for bad in (dict(query=q.double()), dict(key=k.half()), dict(query=q[0]), dict(value=v[:, :, :-1]),
+                dict(key=k[:, :1].expand(2, 3, 9, 16)[:, :3], value=v[:, :1].expand(2, 3, 9, 16)),
+                dict(query=q[..., :12], key=k[..., :12], value=v[..., :12]), dict(bias_table=table[:2]),
+                dict(bias_table=table.half()), dict(bias_table=table.repeat(1, 100)), dict(bucket_map=bmap.int()),
+                dict(bucket_map=bmap[:, :-1]), dict(bucket_map=bmap.expand(3, 8, 9)), dict(scale=0.0),
+                dict(scale=math.inf), dict(scale=-1.0), dict(key_lengths=torch.tensor([1, 2], device=DEV)),
+                dict(key_lengths=torch.ones(3, dtype=torch.int32, device=DEV)),
+                dict(key_lengths=torch.ones(2, dtype=torch.int32)), dict(bucket_map=bmap.cpu())):
+        args = dict(query=q, key=k, value=v, bias_table=table, bucket_map=bmap) | bad
+        with pytest.raises(RuntimeError):
+            call(**args)
