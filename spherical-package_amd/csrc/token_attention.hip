@@ -23,6 +23,10 @@ constexpr int kTable = 256;
 template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 1 : 2;   // 32-token parts of a tile
 
+// Waves of a SIMD in the backward: with two, accumulators lie among the 256 registers of a wave.
+template <int DP>
+constexpr int kBackwardWaves = DP <= 64 ? 2 : 1;
+
 // A wave's 32 columns of B: rows first + lane % 32 of a tensor, values 16 c + 8 h .. + 7 in operand c; rows at or
 // beyond `end` are zeros.
 template <typename T, int DP>
@@ -52,6 +56,13 @@ __device__ __forceinline__ void store_columns(T* base, int64_t stride, int64_t r
     }
 }
 
+// Between a wave's writes to LDS and its other lanes' reads: LDS keeps a wave's order, so it is the compiler alone
+// that must not exchange them.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Where split `split` of `splits` begins among `tiles`.
 __device__ __forceinline__ int64_t split_at(int64_t tiles, int split, int splits) { return tiles * split / splits; }
 
@@ -60,7 +71,7 @@ __device__ __forceinline__ int64_t split_at(int64_t tiles, int split, int splits
 // columns, so a query's maximum and sum are one lane's (and the lane's 32 further on).
 // splits > 1: each takes a part of the keys and leaves its normalised output and log2 of its sum for `join`.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void attend(const Attention a, int splits, unsigned tiles, float* part_out,
+__global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int splits, unsigned tiles, float* part_out,
                                                    float* part_lse) {
   constexpr int NT = kParts<T>, KEYS = 32 * NT;
   __shared__ __attribute__((aligned(16))) Tile<T, DP, NT> keys, values;
@@ -175,6 +186,166 @@ __global__ __launch_bounds__(kThreads) void attend(const Attention a, int splits
   if (a.lse && h == 0) a.lse[row] = lse2;
 }
 
+// ------------------------------------------------------------------------------------------ few queries
+// At most 32 rows (a key head's query heads times the queries) against many keys: bound by reading the keys and
+// values once.  A workgroup takes a part of one key head's keys for all of its rows; its waves walk 32 keys each
+// by themselves, without barriers: keys go from memory into the product's registers, values through the wave's
+// own tile in LDS, both requested a step ahead.  The waves' states are joined in LDS at the end.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_few(
+    const Attention a, int splits, float* part_out, float* part_lse) {
+  constexpr int kVectors = DP / kWide<T>, kCount = 32 * kVectors / 64;
+  constexpr int kState = 2 * 32 * (DP + 1);   // floats of two waves' states
+  __shared__ __attribute__((aligned(16))) union {
+    Tile<T, DP, 1> values[kWaves];
+    float state[kState];
+  } lds;
+  __shared__ float level[kWaves / 2][2][32];
+  extern __shared__ float table[];   // [query head of the key head][257]: equal buckets of two heads in two banks
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, h = lane / 32;
+  const unsigned id = by_die(blockIdx.x, gridDim.x);
+  const int split = (int)(id % (unsigned)splits);
+  const unsigned bh = id / (unsigned)splits;
+  const int shared_head = (int)(bh % (unsigned)a.key_heads), b = (int)(bh / (unsigned)a.key_heads);
+  const int group = a.heads / a.key_heads, rows = group * (int)a.queries;
+  const int r = std::min(lane % 32, rows - 1), head = shared_head * group + r / (int)a.queries;
+  const int64_t query = r % (int)a.queries;
+  for (int i = threadIdx.x; i < group * kTable; i += kThreads)
+    table[i / kTable * (kTable + 1) + i % kTable] =
+        a.bias(shared_head * group + i / kTable, i % kTable, __is_same(T, bf16));
+  const float* bias = table + r / (int)a.queries * (kTable + 1);
+  const T* kp = (const T*)a.k + b * a.ks[0] + shared_head * a.ks[1];
+  const T* vp = (const T*)a.v + b * a.vs[0] + shared_head * a.vs[1];
+  const int64_t len = a.length(b);
+  const int64_t last = a.causal ? len - a.queries + query : len - 1;
+  const int64_t blocks = (len + 31) / 32;
+  const int64_t from = split_at(blocks, split, splits) * 32, to = std::min(len, split_at(blocks, split + 1, splits) * 32);
+  const uint8_t* map = a.map + b * a.ms[0] + query * a.ms[1];
+  // the token whose key this lane supplies: row lane % 32 of the product
+  const int token = 16 * (lane / 4 % 2) + 4 * (lane % 32 / 8) + lane % 4;
+
+  Operand<T> q[DP / 16];
+  load_columns<T, DP>(q, (const T*)a.q + b * a.qs[0] + head * a.qs[1], a.qs[2], query, a.queries, a.dim, lane);
+  floatx16 o[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+  float most = -INFINITY, sum = 0.f;
+  __syncthreads();
+
+  Operand<T> k[DP / 16];
+  Pack<T, kWide<T>> x[kCount];
+  Buckets bucket;
+  auto request = [&](int64_t k0) {
+    load_columns<T, DP>(k, kp, a.ks[2], k0 + token, to, a.dim, lane);
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      const int at = n * 64 + lane, d = at % kVectors * kWide<T>;
+      const int64_t row = k0 + at / kVectors;
+      if (row < to && d < a.dim) {
+        x[n] = *reinterpret_cast<const Pack<T, kWide<T>>*>(vp + row * a.vs[2] + d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kWide<T>; ++e) x[n].v[e] = (T)0.f;
+      }
+    }
+    bucket.load(map, k0 + 16 * h, a.keys);
+  };
+  Tile<T, DP, 1>& values = lds.values[wave];
+  int64_t k0 = from + 32 * wave;
+  if (k0 < to) request(k0);
+  for (; k0 < to; k0 += 32 * kWaves) {
+    floatx16 s;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[v] = bias[bucket[v]];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) s = product(k[c], q[c], s);
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      const int at = n * 64 + lane;
+      *reinterpret_cast<Pack<T, kWide<T>>*>(
+          &values.v[row_of<1>(at / kVectors) * Tile<T, DP, 1>::kStride + at % kVectors * kWide<T>]) = x[n];
+    }
+    if (k0 + 32 * kWaves < to) request(k0 + 32 * kWaves);
+    if (k0 + 32 > last + 1) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        if (k0 + 16 * h + v > last) s[v] = -INFINITY;
+    }
+    float now = s[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) now = fmaxf(now, s[v]);
+    now = fmaxf(now, other_half(now));
+    if (__any(now > most)) {
+      const float grown = fmaxf(now, most);
+      const float by = grown == -INFINITY ? 1.f : exp2f((most - grown) * a.scale2);
+      most = grown;
+      sum *= by;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= by;
+    }
+    const float off = most == -INFINITY ? 0.f : most * a.scale2;
+    float p[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      p[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -off));
+      sum += p[v];
+    }
+    wave_order();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const Operand<T> w = rounded<T>(p + 8 * half);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] = product(values.columns(0, half, d, lane), w, o[d]);
+    }
+    wave_order();
+  }
+  sum += other_half(sum);
+  // waves 2 and 3 hand their states to 0 and 1, then 1 to 0
+#pragma unroll
+  for (int step = kWaves / 2; step > 0; step /= 2) {
+    __syncthreads();
+    const int slot = wave % step;
+    float* state = lds.state + slot * 32 * (DP + 1) + lane % 32 * (DP + 1);   // DP + 1: columns in other banks
+    if (wave >= step && wave < 2 * step) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) state[32 * d + 8 * (v / 4) + 4 * h + v % 4] = o[d][v];
+      level[slot][0][lane % 32] = most;
+      level[slot][1][lane % 32] = sum;
+    }
+    __syncthreads();
+    if (wave < step) {
+      const float other = level[slot][0][lane % 32], grown = fmaxf(most, other);
+      const float mine = grown == -INFINITY ? 1.f : exp2f((most - grown) * a.scale2);
+      const float theirs = grown == -INFINITY ? 1.f : exp2f((other - grown) * a.scale2);
+      most = grown;
+      sum = sum * mine + level[slot][1][lane % 32] * theirs;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          o[d][v] = o[d][v] * mine + state[32 * d + 8 * (v / 4) + 4 * h + v % 4] * theirs;
+    }
+  }
+  if (wave != 0 || lane % 32 >= rows) return;
+  const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  const float lse2 = sum > 0.f || sum != sum ? fmaf(most, a.scale2, log2f(sum)) : -INFINITY;
+  const int64_t row = ((int64_t)b * a.heads + head) * a.queries + query;
+  if (splits > 1) {
+    const int64_t all = (int64_t)a.batch * a.heads * a.queries;
+    store_columns<float, DP>(part_out + split * all * a.dim, a.dim, row, a.dim, lane, o, by);
+    if (h == 0) part_lse[split * all + row] = lse2;
+    return;
+  }
+  store_columns<T, DP>((T*)a.out + b * a.os[0] + head * a.os[1], a.os[2], query, a.dim, lane, o, by);
+  if (a.lse && h == 0) a.lse[row] = lse2;
+}
+
 // The splits of a row: weights 2^(lse2 - largest), a wave a row.
 template <typename T>
 __global__ __launch_bounds__(256) void join(const Attention a, int splits, const float* part_out,
@@ -246,11 +417,34 @@ __global__ __launch_bounds__(256) void turn_map(const Attention a, uint8_t* turn
 }
 
 // dq and the bias table's gradient: as the forward, a workgroup walks the keys with 128 queries.  Each lane adds
-// its ds to the bucket's sum in a column of its own (`columns` of them a wave: 64 up to 64 buckets, fewer beyond,
-// then the lanes that share one take turns), so that every sum has one order.
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void grad_queries(const Attention a, unsigned tiles, const float* delta,
-                                                         const float* lse2, float* table_parts, int columns) {
+// its ds to the bucket's sum in a column of its own (COLUMNS of them a wave: 64 up to 64 buckets, fewer beyond,
+// then the lanes that share one take turns; 0: no table gradient), so that every sum has one order.
+// Four at a time: read, add, write, and where two of the four meet the second takes the first's sum.  (An LDS
+// float add of 64 lanes takes 193 cycles of a CU whatever its addresses, this 13.)
+template <int COLUMNS>
+__device__ __forceinline__ void add_by_bucket(float* column, const Buckets& bucket, int buckets, const float* x) {
+#pragma unroll
+  for (int v = 0; v < 16; v += 4) {
+    int at[4];
+    float sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] = std::min((int)bucket[v + i], buckets) * COLUMNS;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = column[at[i]];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum[i] += x[v + i];
+#pragma unroll
+      for (int j = i + 1; j < 4; ++j) sum[j] = at[j] == at[i] ? sum[i] : sum[j];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) column[at[i]] = sum[i];
+  }
+}
+
+template <typename T, int DP, int COLUMNS>
+__global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(const Attention a, unsigned tiles, const float* delta,
+                                                         const float* lse2, float* table_parts) {
   constexpr int NT = kParts<T>, KEYS = 32 * NT;
   __shared__ __attribute__((aligned(16))) Tile<T, DP, NT> keys, values;
   __shared__ float table[kTable];
@@ -262,9 +456,8 @@ __global__ __launch_bounds__(kThreads) void grad_queries(const Attention a, unsi
   const T* kp = (const T*)a.k + b * a.ks[0] + shared_head * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + shared_head * a.vs[1];
   table[threadIdx.x] = a.bias(head, threadIdx.x, __is_same(T, bf16));
-  float* mine = sums + wave * (a.buckets + 1) * columns;
-  if (table_parts)
-    for (int i = lane; i < (a.buckets + 1) * columns; i += 64) mine[i] = 0.f;
+  float* mine = sums + wave * (a.buckets + 1) * COLUMNS;
+  for (int i = lane; i < (a.buckets + 1) * COLUMNS; i += 64) mine[i] = 0.f;
 
   const int64_t first = (int64_t)tile * (32 * kWaves), query = first + wave * 32 + lane % 32;
   const int64_t len = a.length(b), shift = len - a.queries;
@@ -327,16 +520,15 @@ __global__ __launch_bounds__(kThreads) void grad_queries(const Attention a, unsi
 #pragma unroll
       for (int v = 0; v < 16; ++v)
         ds[t][v] = __builtin_amdgcn_exp2f(fmaf(s[t][v], a.scale2, -my_lse)) * e[t][v];
-    if (table_parts) {
-      for (int turn = 0; turn < 64 / columns; ++turn)
-        if (lane / columns == turn)
+    if constexpr (COLUMNS > 0) {
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+      for (int turn = 0; turn < 64 / COLUMNS; ++turn) {
+        if (lane / COLUMNS == turn) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              const int at = std::min((int)bucket[t][v], a.buckets) * columns + lane % columns;
-              __hip_atomic_fetch_add(mine + at, ds[t][v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            }
+          for (int t = 0; t < NT; ++t) add_by_bucket<COLUMNS>(mine + lane % COLUMNS, bucket[t], a.buckets, ds[t]);
+        }
+        if (COLUMNS < 64) wave_order();   // the next turn's lanes read what these wrote
+      }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -349,13 +541,13 @@ __global__ __launch_bounds__(kThreads) void grad_queries(const Attention a, unsi
   }
   if (a.dq && query < a.queries)
     store_columns<T, DP>((T*)a.dq + b * a.dqs[0] + head * a.dqs[1], a.dqs[2], query, a.dim, lane, dq, a.scale);
-  if (table_parts) {
+  if constexpr (COLUMNS > 0) {
     __syncthreads();
     for (int i = threadIdx.x; i < a.buckets; i += kThreads) {
       float x = 0.f;
       for (int w = 0; w < kWaves; ++w)
-        for (int c = 0; c < columns; ++c)   // begun at the bucket's own column: other banks for other lanes
-          x += sums[(w * (a.buckets + 1) + i) * columns + (c + i) % columns];
+        for (int c = 0; c < COLUMNS; ++c)   // begun at the bucket's own column: other banks for other lanes
+          x += sums[(w * (a.buckets + 1) + i) * COLUMNS + (c + i) % COLUMNS];
       table_parts[((int64_t)bh * tiles + tile) * a.buckets + i] = x;
     }
   }
@@ -390,7 +582,7 @@ __global__ __launch_bounds__(256) void join_table(const Attention a, unsigned ti
 // dk and dv: a workgroup keeps 128 keys, 32 a wave, and walks the queries of every head that reads them:
 // S = Q K^T has the keys in columns.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void grad_keys(const Attention a, unsigned tiles, const float* delta,
+__global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(const Attention a, unsigned tiles, const float* delta,
                                                       const float* lse2, const uint8_t* turned, int64_t pitch) {
   constexpr int NT = kParts<T>, ROWS = 32 * NT;
   __shared__ __attribute__((aligned(16))) Tile<T, DP, NT> queries, grads;
@@ -444,35 +636,29 @@ __global__ __launch_bounds__(kThreads) void grad_keys(const Attention a, unsigne
         next_q.load(qp, a.qs[2], q0 + ROWS, a.queries, a.dim);
         next_g.load(gp, a.gs[2], q0 + ROWS, a.queries, a.dim);
       }
-      floatx16 s[NT], e[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[t][i] = table[bucket[t][i]];
-          e[t][i] = row_delta[16 * NT * h + 16 * t + i];
-        }
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          s[t] = product(queries.rows(t, c, lane), k[c], s[t]);
-          e[t] = product(grads.rows(t, c, lane), v[c], e[t]);
-        }
-      if (q0 < seen) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (q0 + 16 * NT * h + 16 * t + i < seen) s[t][i] = -INFINITY;
-      }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        floatx16 s, e;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[i] = table[bucket[t][i]];
+          e[i] = row_delta[16 * NT * h + 16 * t + i];
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+          s = product(queries.rows(t, c, lane), k[c], s);
+          e = product(grads.rows(t, c, lane), v[c], e);
+        }
+        if (q0 < seen) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (q0 + 16 * NT * h + 16 * t + i < seen) s[i] = -INFINITY;
+        }
         float p[16], ds[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], a.scale2, row_lse[16 * NT * h + 16 * t + i]));
-          ds[i] = p[i] * e[t][i];
+          p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, row_lse[16 * NT * h + 16 * t + i]));
+          ds[i] = p[i] * e[i];
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -553,10 +739,14 @@ Attention on_device(const sdk_bucket_attention* a) {
   return d;
 }
 
+// Whether a key head's rows go to attend_few.
+bool few_rows(const sdk_bucket_attention* a) { return a->heads / a->key_heads * a->queries <= 32; }
+
 // Parts that the keys are dealt to: enough workgroups for the 256 CUs, at least 256 keys each.
 int splits_of(const sdk_bucket_attention* a) {
-  const int64_t groups = a->batch * a->heads * ceil_div(a->queries, 32 * kWaves);
-  if (groups >= 256 || groups == 0) return 1;
+  const bool few = few_rows(a);
+  const int64_t groups = few ? a->batch * a->key_heads : a->batch * a->heads * ceil_div(a->queries, 32 * kWaves);
+  if (groups >= (few ? 512 : 256) || groups == 0) return 1;
   return (int)std::max<int64_t>(1, std::min(ceil_div(512, groups), a->keys / 256));
 }
 
@@ -574,6 +764,20 @@ BackwardSpace backward_space(const sdk_bucket_attention* a) {
   w.turned = w.parts + up(a->batch * a->heads * ceil_div(a->queries, 32 * kWaves) * a->buckets * 4);
   w.total = w.turned + up((a->map_strides[0] ? a->batch : 1) * a->keys * w.pitch);
   return w;
+}
+
+template <typename T, int DP, int COLUMNS>
+int launch_grad_queries(const Attention& d, unsigned tiles, const float* delta, const float* lse2, float* parts,
+                        hipStream_t s) {
+  const size_t smem = (size_t)kWaves * (d.buckets + 1) * COLUMNS * sizeof(float);
+  auto* kernel = grad_queries<T, DP, COLUMNS>;
+  if (smem > (32 << 10)) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != hipSuccess) return fail(SDK_ERR_DEVICE, "LDS of %zu bytes: %s", smem, hipGetErrorString(e));
+  }
+  kernel<<<dim3(tiles * (unsigned)(d.batch * d.heads)), dim3(kThreads), smem, s>>>(d, tiles, delta, lse2, parts);
+  return SDK_OK;
 }
 
 int check_inputs(const sdk_bucket_attention* a) {
@@ -619,7 +823,14 @@ int sdk_bucket_attention_forward(const sdk_bucket_attention* a, void* workspace,
   float* part_lse = part_out ? part_out + splits * rows * a->dim : nullptr;
   hipStream_t s = (hipStream_t)stream;
   SDK_DISPATCH_TOKEN_DTYPE(a->dtype, {
-    ATTENTION_DIM(a->dim, launch(attend<T, DP>, dim3(tiles * (unsigned)(a->batch * a->heads) * splits),
+    if (few_rows(a)) {
+      const int group = d.heads / d.key_heads;
+      ATTENTION_DIM(a->dim, {
+        attend_few<T, DP><<<dim3((unsigned)(a->batch * a->key_heads) * splits), dim3(kThreads),
+                            group*(kTable + 1) * sizeof(float), s>>>(d, splits, part_out, part_lse);
+      });
+    } else
+      ATTENTION_DIM(a->dim, launch(attend<T, DP>, dim3(tiles * (unsigned)(a->batch * a->heads) * splits),
                                  dim3(kThreads), s, d, splits, tiles, part_out, part_lse));
     if (splits > 1)
       launch(join<T>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), s, d, splits, (const float*)part_out,
@@ -655,20 +866,17 @@ int sdk_bucket_attention_backward(const sdk_bucket_attention* a, void* workspace
   uint8_t* turned = (uint8_t*)(ws + w.turned);
   const unsigned q_tiles = (unsigned)ceil_div(a->queries, 32 * kWaves), k_tiles = (unsigned)ceil_div(a->keys, 32 * kWaves);
   const int64_t rows = a->batch * a->heads * a->queries;
-  const int columns = a->buckets <= 64 ? 64 : a->buckets <= 128 ? 32 : 16;
+  const int columns = !a->grad_table ? 0 : a->buckets <= 64 ? 64 : a->buckets <= 128 ? 32 : 16;
   SDK_DISPATCH_TOKEN_DTYPE(a->dtype, {
     if (any) {
       launch(row_terms<T>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), s, d, delta, lse2);
       if (a->grad_query || a->grad_table) {
-        const size_t smem = a->grad_table ? (size_t)kWaves * (a->buckets + 1) * columns * sizeof(float) : 0;
         ATTENTION_DIM(a->dim, {
-          if (smem > (32 << 10)) {
-            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(grad_queries<T, DP>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != hipSuccess) return fail(SDK_ERR_DEVICE, "LDS of %zu bytes: %s", smem, hipGetErrorString(e));
-          }
-          grad_queries<T, DP><<<dim3(q_tiles * (unsigned)(a->batch * a->heads)), dim3(kThreads), smem, s>>>(
-              d, q_tiles, (const float*)delta, (const float*)lse2, a->grad_table ? parts : nullptr, columns);
+          int rc = columns == 0    ? launch_grad_queries<T, DP, 0>(d, q_tiles, delta, lse2, parts, s)
+                   : columns == 64 ? launch_grad_queries<T, DP, 64>(d, q_tiles, delta, lse2, parts, s)
+                   : columns == 32 ? launch_grad_queries<T, DP, 32>(d, q_tiles, delta, lse2, parts, s)
+                                   : launch_grad_queries<T, DP, 16>(d, q_tiles, delta, lse2, parts, s);
+          if (rc != SDK_OK) return rc;
         });
       }
     }

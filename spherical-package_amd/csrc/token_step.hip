@@ -12,6 +12,7 @@
 // Bound by memory: 28 bytes a value with float32 parameters and moments, 16 with moments in 8 bits.  All
 // arithmetic is float32, each operation rounded by itself in the order above (nothing is contracted), with
 // exact division and square root.
+#include <algorithm>
 #include <cmath>
 
 #include "token_types.hpp"
@@ -126,7 +127,38 @@ __device__ __forceinline__ float scale_of(float largest, float& inverse) {
 constexpr int kRounds8 = 4;                         // blocks of 256 values a wave
 constexpr int kPerGroup8 = 4 * kRounds8 * kBlock;
 
-// A wave takes a block of 256 values, four consecutive ones a lane.
+// One block of 256 values, four consecutive ones a lane, on its way through a step.
+template <typename T>
+struct Block8 {
+  float p[4], g[4], m_scale, v_scale;
+  Pack<signed char, 4> cm;
+  Pack<unsigned char, 4> cv;
+
+  __device__ __forceinline__ void step(const Settings& s, int left) {   // left: values from this lane's first to the end
+    float m[4], v[4], m_most = 0.f, v_most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // beyond the tensor's end the values are zeros whatever the scale holds
+      m[e] = e < left ? avg_value(cm.v[e], m_scale) : 0.f;
+      v[e] = e < left ? sq_value(cv.v[e], v_scale) : 0.f;
+      update(p[e], g[e], m[e], v[e], s);
+      m_most = Largest::of(m_most, fabsf(m[e]));
+      v_most = Largest::of(v_most, v[e]);
+    }
+    float m_inv, v_inv;
+    m_scale = scale_of(over_wave<Largest>(m_most), m_inv);
+    v_scale = scale_of(over_wave<Largest>(v_most), v_inv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float c = rintf(sqrtf(fabsf(m[e]) * m_inv) * 127.f);
+      cm.v[e] = (signed char)(int)(m[e] < 0.f ? -c : c);
+      const float d = rintf(sqrtf(sqrtf(v[e] * v_inv)) * 255.f);
+      cv.v[e] = (unsigned char)(int)(v[e] > 0.f && v_inv > 0.f && d < 1.f ? 1.f : d);
+    }
+  }
+};
+
+// A wave takes four blocks, all of them requested before the first is worked on.
 template <typename T>
 __global__ __launch_bounds__(256) void adamw8(const Tensors8 t, const Settings s) {
   const int i = tensor_of(t.start);
@@ -138,87 +170,80 @@ __global__ __launch_bounds__(256) void adamw8(const Tensors8 t, const Settings s
   const int64_t n = t.n[i], from = (int64_t)(blockIdx.x - t.start[i]) * kPerGroup8;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool wide = (((uintptr_t)p | (uintptr_t)g) % (4 * sizeof(T)) | ((uintptr_t)mc | (uintptr_t)vc) % 4) == 0;
+  if (wide && from + kPerGroup8 <= n) {
+    Block8<T> x[kRounds8];
 #pragma unroll
-  for (int r = 0; r < kRounds8; ++r) {
-    const int64_t first = from + (int64_t)(r * 4 + wave) * kBlock;
-    if (first >= n) break;
-    const int64_t at = first + lane * 4, block = first / kBlock;
-    const bool whole = wide && first + kBlock <= n;
-    float fp[4], fg[4];
-    Pack<signed char, 4> cm;
-    Pack<unsigned char, 4> cv;
-    if (whole) {
-      load_pack<T, 4>(p + at, fp);
-      load_pack<T, 4>(g + at, fg);
-      cm = *reinterpret_cast<const Pack<signed char, 4>*>(mc + at);
-      cv = *reinterpret_cast<const Pack<unsigned char, 4>*>(vc + at);
-    } else {
+    for (int r = 0; r < kRounds8; ++r) {
+      const int64_t first = from + (int64_t)(r * 4 + wave) * kBlock, at = first + lane * 4;
+      load_pack<T, 4>(p + at, x[r].p);
+      load_pack<T, 4>(g + at, x[r].g);
+      x[r].cm = *reinterpret_cast<const Pack<signed char, 4>*>(mc + at);
+      x[r].cv = *reinterpret_cast<const Pack<unsigned char, 4>*>(vc + at);
+      x[r].m_scale = ms[first / kBlock];
+      x[r].v_scale = vs[first / kBlock];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = at + e < n;
-        fp[e] = in ? (float)p[at + e] : 0.f;
-        fg[e] = in ? (float)g[at + e] : 0.f;
-        cm.v[e] = in ? mc[at + e] : (signed char)0;
-        cv.v[e] = in ? vc[at + e] : (unsigned char)0;
+    for (int r = 0; r < kRounds8; ++r) {
+      const int64_t first = from + (int64_t)(r * 4 + wave) * kBlock, at = first + lane * 4;
+      x[r].step(s, 4);
+      store_pack<T, 4>(p + at, x[r].p);
+      *reinterpret_cast<Pack<signed char, 4>*>(mc + at) = x[r].cm;
+      *reinterpret_cast<Pack<unsigned char, 4>*>(vc + at) = x[r].cv;
+      if (lane == 0) {
+        ms[first / kBlock] = x[r].m_scale;
+        vs[first / kBlock] = x[r].v_scale;
       }
     }
-    const float m_scale = ms[block], v_scale = vs[block];
-    float fm[4], fv[4], m_most = 0.f, v_most = 0.f;
+    return;
+  }
+  for (int r = 0; r < kRounds8; ++r) {
+    const int64_t first = from + (int64_t)(r * 4 + wave) * kBlock, at = first + lane * 4;
+    if (first >= n) break;
+    const int left = (int)std::min<int64_t>(4, n - at);
+    Block8<T> x;
+    x.m_scale = ms[first / kBlock];
+    x.v_scale = vs[first / kBlock];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      // beyond the tensor's end the values are zeros whatever the scale holds
-      const bool in = whole || at + e < n;
-      fm[e] = in ? avg_value(cm.v[e], m_scale) : 0.f;
-      fv[e] = in ? sq_value(cv.v[e], v_scale) : 0.f;
-      update(fp[e], fg[e], fm[e], fv[e], s);
-      m_most = Largest::of(m_most, fabsf(fm[e]));
-      v_most = Largest::of(v_most, fv[e]);
+      x.p[e] = e < left ? (float)p[at + e] : 0.f;
+      x.g[e] = e < left ? (float)g[at + e] : 0.f;
+      x.cm.v[e] = e < left ? mc[at + e] : (signed char)0;
+      x.cv.v[e] = e < left ? vc[at + e] : (unsigned char)0;
     }
-    float m_inv, v_inv;
-    m_most = scale_of(over_wave<Largest>(m_most), m_inv);
-    v_most = scale_of(over_wave<Largest>(v_most), v_inv);
+    x.step(s, left);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float c = rintf(sqrtf(fabsf(fm[e]) * m_inv) * 127.f);
-      cm.v[e] = (signed char)(int)(fm[e] < 0.f ? -c : c);
-      const float d = rintf(sqrtf(sqrtf(fv[e] * v_inv)) * 255.f);
-      cv.v[e] = (unsigned char)(int)(fv[e] > 0.f && v_inv > 0.f && d < 1.f ? 1.f : d);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (e < left) {
+        p[at + e] = (T)x.p[e];
+        mc[at + e] = x.cm.v[e];
+        vc[at + e] = x.cv.v[e];
+      }
     if (lane == 0) {
-      ms[block] = m_most;
-      vs[block] = v_most;
-    }
-    if (whole) {
-      store_pack<T, 4>(p + at, fp);
-      *reinterpret_cast<Pack<signed char, 4>*>(mc + at) = cm;
-      *reinterpret_cast<Pack<unsigned char, 4>*>(vc + at) = cv;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (at + e < n) {
-          p[at + e] = (T)fp[e];
-          mc[at + e] = cm.v[e];
-          vc[at + e] = cv.v[e];
-        }
+      ms[first / kBlock] = x.m_scale;
+      vs[first / kBlock] = x.v_scale;
     }
   }
 }
 
-// The values that codes stand for, four a thread.
+// The values that codes stand for, 16 a thread (one scale: kBlock is a multiple of 16).
 template <typename T>
 __global__ __launch_bounds__(256) void moment_values(const unsigned char* codes, const float* scales, T* out,
                                                      int64_t n, int second, int wide) {
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
   if (at >= n) return;
-  const float scale = scales[at / kBlock];   // kBlock is a multiple of four: one scale for the four
-  float f[4];
-  if (wide && at + 4 <= n) {
-    const Pack<unsigned char, 4> c = *reinterpret_cast<const Pack<unsigned char, 4>*>(codes + at);
+  const float scale = scales[at / kBlock];
+  if (wide && at + 16 <= n) {
+    const Pack<unsigned char, 16> c = *reinterpret_cast<const Pack<unsigned char, 16>*>(codes + at);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = second ? sq_value(c.v[e], scale) : avg_value((signed char)c.v[e], scale);
-    store_pack<T, 4>(out + at, f);
+    for (int k = 0; k < 16; k += kWide<T>) {
+      float f[kWide<T>];
+#pragma unroll
+      for (int e = 0; e < kWide<T>; ++e)
+        f[e] = second ? sq_value(c.v[k + e], scale) : avg_value((signed char)c.v[k + e], scale);
+      store_pack<T, kWide<T>>(out + at + k, f);
+    }
   } else {
-    for (int e = 0; e < 4 && at + e < n; ++e) {
+    for (int e = 0; e < 16 && at + e < n; ++e) {
       const unsigned char c = codes[at + e];
       out[at + e] = (T)(second ? sq_value(c, scale) : avg_value((signed char)c, scale));
     }
@@ -344,8 +369,8 @@ int sdk_adamw_moment_values(const void* codes, const float* scales, void* out, i
   SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
   if (size == 0) return SDK_OK;
   SDK_REQUIRE(codes && scales && out, "codes, scales and out must not be NULL");
-  const int wide = ((uintptr_t)codes & 3) == 0 && ((uintptr_t)out & 15) == 0;
-  SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(moment_values<T>, dim3((unsigned)ceil_div(size, 1024)), dim3(256),
+  const int wide = ((uintptr_t)codes & 15) == 0 && ((uintptr_t)out & 15) == 0;
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(moment_values<T>, dim3((unsigned)ceil_div(size, 4096)), dim3(256),
                                          (hipStream_t)stream, (const unsigned char*)codes, scales, (T*)out, size,
                                          (int)(second != 0), wide));
   SDK_LAUNCH_CHECK("adamw_moment_values");
