@@ -342,9 +342,20 @@ _SCHEMAS = (
     ("adamw_moment_values", "(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor", adamw_moment_values),
 )
 
+
+
+def _native_names():
+    if _ops._native is None:
+        return frozenset()
+    _ops._native.sdk_torch_token_ops.restype = ctypes.c_char_p
+    return frozenset(_ops._native.sdk_torch_token_ops().decode().split(","))
+
+
+NATIVE_OPS = _native_names()
 _library = torch.library.Library(_ops._NS, "FRAGMENT")
 for _name, _schema, _fn in _SCHEMAS:
     _library.define(_name + _schema)
-    _library.impl(_name, _fn, "CUDA")
+    if _name not in NATIVE_OPS:
+        _library.impl(_name, _fn, "CUDA")
 ops = _ops.ops
 PYTHON_IMPL = {_name: _fn for _name, _schema, _fn in _SCHEMAS}

@@ -1,0 +1,360 @@
+// Compiled PyTorch-ROCm layer of the operators on token sequences: the checks, allocation, stream fetch and
+// C-ABI call of _spherical_distortion_ext/_token_ops.py (which defines the schemas and keeps a Python
+// implementation of each) in C++, where a call of a few microseconds on the GPU is not bound by its host side.
+// Part of libsdk_torch_ops.so; no device code here.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/library.h>
+
+#include <cmath>
+#include <cstdint>
+#include <optional>
+#include <vector>
+
+#include "sdk_mapped_ops.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+constexpr int64_t kBlock = 256;   // values of a moment in 8 bits that share a scale
+
+bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+void* ptr(const Tensor& t) { return t.data_ptr(); }
+void* ptr(const OptTensor& t) { return has(t) ? t->data_ptr() : nullptr; }
+
+int dtype_of(at::ScalarType t, const char* name) {
+  if (t == at::kFloat) return SDK_F32;
+  if (t == at::kBFloat16) return SDK_BF16;
+  TORCH_CHECK(t == at::kHalf, "unsupported dtype ", t, " of ", name, " (float32, bfloat16 and float16 only)");
+  return SDK_F16;
+}
+
+void on_gpu(const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), "this backend runs on the GPU only: tensors must be CUDA/HIP tensors");
+}
+void beside(const Tensor& ref, const char* name, const Tensor& t) {
+  TORCH_CHECK(t.is_cuda() && t.device() == ref.device(), name, " must be a CUDA tensor on ", ref.device());
+}
+void beside(const Tensor& ref, const char* name, const OptTensor& t) {
+  if (has(t)) beside(ref, name, *t);
+}
+void dense(const char* name, const Tensor& t) { TORCH_CHECK(t.is_contiguous(), name, " must be contiguous"); }
+void dense(const char* name, const OptTensor& t) {
+  if (has(t)) dense(name, *t);
+}
+
+hipStream_t stream_of(const Tensor& ref) {
+  return c10::hip::getCurrentHIPStream(ref.device().index()).stream();
+}
+
+#define TOKEN_CALL(name, ...)                                                                             \
+  do {                                                                                                    \
+    const int rc__ = name(__VA_ARGS__);                                                                   \
+    TORCH_CHECK(rc__ == 0, #name, " failed (status ", rc__, "): ", sdk_last_error());                     \
+  } while (0)
+
+Tensor nothing(const Tensor& like) { return at::empty({0}, like.options()); }
+
+// ------------------------------------------------------------------------------------------ attention
+// `t`, or a dense copy where its rows are not 16-byte aligned or its last axis is not dense.
+Tensor rows_ready(const Tensor& t) {
+  const int64_t each = 16 / (int64_t)t.element_size();
+  bool ok = (uintptr_t)t.data_ptr() % 16 == 0 && (t.size(-1) == 1 || t.stride(-1) == 1);
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % each == 0);
+  return ok ? t : t.contiguous();
+}
+
+// Batch, head and token strides; those of axes of length one do not count.
+void strides(const Tensor& t, int64_t (&s)[3]) {
+  for (int i = 0; i < 3; ++i) s[i] = t.size(i) == 1 ? 0 : t.stride(i);
+}
+
+void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& map,
+                     const OptTensor& lengths, double scale) {
+  on_gpu(q);
+  beside(q, "key", k), beside(q, "value", v), beside(q, "bias_table", table), beside(q, "bucket_map", map);
+  beside(q, "key_lengths", lengths);
+  (void)dtype_of(q.scalar_type(), "query");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "query and key must be [batch, heads, tokens, dim], got ", q.sizes(),
+              " and ", k.sizes());
+  const int64_t B = q.size(0), H = q.size(1), Lq = q.size(2), D = q.size(3);
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == B && k.size(3) == D, "key ", k.sizes(), " and value ",
+              v.sizes(), " must be [", B, ", key heads, keys, ", D, "]");
+  const int64_t Hk = k.size(1), Lk = k.size(2);
+  TORCH_CHECK(Hk >= 1 && H >= 1 && H % Hk == 0, "heads = ", H, " must be a multiple of key heads = ", Hk);
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+              "key and value must have dtype ", q.scalar_type(), " (got ", k.scalar_type(), " and ", v.scalar_type(),
+              ")");
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "dim = ", D, " must be a multiple of 8 up to 128");
+  TORCH_CHECK(table.dim() == 2 && table.size(0) == H && table.size(1) >= 1 && table.size(1) <= 256, "bias_table ",
+              table.sizes(), " must be [", H, ", buckets], 1 to 256 buckets");
+  TORCH_CHECK(table.scalar_type() == q.scalar_type() || table.scalar_type() == at::kFloat,
+              "bias_table must have dtype ", q.scalar_type(), " or float32 (got ", table.scalar_type(), ")");
+  TORCH_CHECK(map.scalar_type() == at::kByte, "bucket_map must have dtype uint8 (got ", map.scalar_type(), ")");
+  TORCH_CHECK((map.dim() == 2 || (map.dim() == 3 && map.size(0) == B)) && map.size(-2) == Lq && map.size(-1) == Lk,
+              "bucket_map ", map.sizes(), " must be [", Lq, ", ", Lk, "] or [", B, ", ", Lq, ", ", Lk, "]");
+  if (has(lengths)) {
+    TORCH_CHECK(lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == B,
+                "key_lengths must be int32 of shape [", B, "], got ", lengths->scalar_type(), " ", lengths->sizes());
+    dense("key_lengths", lengths);
+  }
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite, got ", scale);
+}
+
+// The argument block; the tensors may be replaced by dense copies, which the caller keeps.
+sdk_bucket_attention attention_args(Tensor& q, Tensor& k, Tensor& v, Tensor& table, Tensor& map,
+                                    const OptTensor& lengths, bool causal, double scale) {
+  q = rows_ready(q), k = rows_ready(k), v = rows_ready(v), table = table.contiguous();
+  if (map.size(-1) != 1 && map.stride(-1) != 1) map = map.contiguous();
+  sdk_bucket_attention a = {};
+  a.query = ptr(q), a.key = ptr(k), a.value = ptr(v), a.bias_table = ptr(table);
+  a.bucket_map = (const uint8_t*)ptr(map), a.key_lengths = (const int32_t*)ptr(lengths);
+  a.batch = q.size(0), a.heads = q.size(1), a.queries = q.size(2), a.dim = q.size(3);
+  a.key_heads = k.size(1), a.keys = k.size(2), a.buckets = table.size(1);
+  strides(q, a.query_strides), strides(k, a.key_strides), strides(v, a.value_strides);
+  a.map_strides[0] = map.dim() == 3 ? map.stride(0) : 0, a.map_strides[1] = map.stride(-2);
+  a.scale = scale, a.causal = causal;
+  a.dtype = dtype_of(q.scalar_type(), "query"), a.table_dtype = dtype_of(table.scalar_type(), "bias_table");
+  return a;
+}
+
+Tensor workspace(const Tensor& ref, size_t bytes) {
+  return bytes ? at::empty({(int64_t)bytes}, ref.options().dtype(at::kByte)) : Tensor();
+}
+
+std::tuple<Tensor, Tensor> bucket_attention_forward(Tensor q, Tensor k, Tensor v, Tensor table, Tensor map,
+                                                    const OptTensor& lengths, bool causal, double scale) {
+  check_attention(q, k, v, table, map, lengths, scale);
+  c10::DeviceGuard guard(q.device());
+  sdk_bucket_attention a = attention_args(q, k, v, table, map, lengths, causal, scale);
+  Tensor out = at::empty_like(q), lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
+  a.output = ptr(out), a.lse = (float*)ptr(lse);
+  strides(out, a.output_strides);
+  const size_t need = sdk_bucket_attention_workspace_bytes(&a, 0);
+  Tensor ws = workspace(q, need);
+  TOKEN_CALL(sdk_bucket_attention_forward, &a, need ? ptr(ws) : nullptr, need, stream_of(q));
+  return {out, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> bucket_attention_backward(
+    Tensor grad, Tensor q, Tensor k, Tensor v, Tensor table, Tensor map, const OptTensor& lengths, Tensor out,
+    Tensor lse, bool causal, double scale, bool need_query, bool need_keys, bool need_table) {
+  check_attention(q, k, v, table, map, lengths, scale);
+  beside(q, "grad_output", grad), beside(q, "output", out), beside(q, "lse", lse);
+  TORCH_CHECK(grad.sizes() == q.sizes() && out.sizes() == q.sizes() && lse.sizes() == q.sizes().slice(0, 3),
+              "grad_output, output and lse must have the shapes of the forward's results");
+  TORCH_CHECK(grad.scalar_type() == q.scalar_type() && out.scalar_type() == q.scalar_type() &&
+                  lse.scalar_type() == at::kFloat,
+              "grad_output and output must have dtype ", q.scalar_type(), ", lse float32");
+  c10::DeviceGuard guard(q.device());
+  sdk_bucket_attention a = attention_args(q, k, v, table, map, lengths, causal, scale);
+  grad = rows_ready(grad), out = rows_ready(out), lse = lse.contiguous();
+  a.grad_output = ptr(grad), a.output = ptr(out), a.lse = (float*)ptr(lse);
+  strides(grad, a.grad_output_strides), strides(out, a.output_strides);
+  Tensor dq = need_query ? at::empty_like(q) : nothing(q);
+  Tensor dk = need_keys ? at::empty_like(k) : nothing(k), dv = need_keys ? at::empty_like(v) : nothing(v);
+  Tensor dt = need_table ? at::empty_like(table) : nothing(table);
+  if (need_query) a.grad_query = ptr(dq), strides(dq, a.grad_query_strides);
+  if (need_keys) {
+    a.grad_key = ptr(dk), a.grad_value = ptr(dv);
+    strides(dk, a.grad_key_strides), strides(dv, a.grad_value_strides);
+  }
+  if (need_table) a.grad_table = ptr(dt);
+  const size_t need = sdk_bucket_attention_workspace_bytes(&a, 1);
+  Tensor ws = workspace(q, need);
+  TOKEN_CALL(sdk_bucket_attention_backward, &a, need ? ptr(ws) : nullptr, need, stream_of(q));
+  return {dq, dk, dv, dt};
+}
+
+// ------------------------------------------------------------------------------------------ norm
+void check_norm(const Tensor& x, const OptTensor& residual, const Tensor& weight) {
+  on_gpu(x);
+  beside(x, "residual", residual), beside(x, "weight", weight);
+  dense("x", x), dense("residual", residual), dense("weight", weight);
+  (void)dtype_of(x.scalar_type(), "x");
+  TORCH_CHECK(x.dim() >= 1 && weight.dim() == 1 && weight.size(0) == x.size(-1), "weight ", weight.sizes(),
+              " must have one value for each of the last axis of x ", x.sizes());
+  TORCH_CHECK(x.size(-1) >= 1 && x.size(-1) <= 16384, "width = ", x.size(-1), " must be between 1 and 16384");
+  TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
+              "weight must have dtype ", x.scalar_type(), " or float32 (got ", weight.scalar_type(), ")");
+  if (has(residual))
+    TORCH_CHECK(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(),
+                "residual must be like x: ", x.sizes(), " ", x.scalar_type(), ", got ", residual->sizes(), " ",
+                residual->scalar_type());
+}
+
+void norm(const Tensor& x, const OptTensor& residual, const Tensor& weight, const Tensor& out, float* scales,
+          const Tensor& summed, float* inverse, double eps, int codes) {
+  const int64_t width = x.size(-1);
+  TOKEN_CALL(sdk_add_rms_norm, ptr(x), ptr(residual), ptr(weight), ptr(out), scales,
+             has(residual) ? ptr(summed) : nullptr, inverse, x.numel() / width, width, eps, codes,
+             dtype_of(x.scalar_type(), "x"), dtype_of(weight.scalar_type(), "weight"), stream_of(x));
+}
+
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const OptTensor& residual, const Tensor& weight,
+                                                double eps) {
+  check_norm(x, residual, weight);
+  c10::DeviceGuard guard(x.device());
+  Tensor out = at::empty_like(x), summed = has(residual) ? at::empty_like(x) : nothing(x);
+  Tensor inverse = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  norm(x, residual, weight, out, nullptr, summed, (float*)ptr(inverse), eps, 0);
+  return {out, summed, inverse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm_quantized(const Tensor& x, const OptTensor& residual,
+                                                          const Tensor& weight, double eps, bool fp8) {
+  check_norm(x, residual, weight);
+  c10::DeviceGuard guard(x.device());
+  Tensor codes = at::empty(x.sizes(), x.options().dtype(fp8 ? at::kFloat8_e4m3fn : at::kChar));
+  Tensor summed = has(residual) ? at::empty_like(x) : nothing(x);
+  Tensor scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  norm(x, residual, weight, codes, (float*)ptr(scales), summed, nullptr, eps, fp8 ? 2 : 1);
+  return {codes, scales, summed};
+}
+
+std::tuple<Tensor, Tensor> add_rms_norm_backward(const Tensor& grad, const OptTensor& grad_sum, const Tensor& summed,
+                                                 const Tensor& weight, const Tensor& inverse, bool need_x,
+                                                 bool need_weight) {
+  check_norm(summed, OptTensor(), weight);
+  beside(summed, "grad", grad), beside(summed, "grad_sum", grad_sum), beside(summed, "inverse", inverse);
+  for (const auto& t : {std::pair<const char*, OptTensor>{"grad", grad}, {"grad_sum", grad_sum}})
+    if (has(t.second))
+      TORCH_CHECK(t.second->sizes() == summed.sizes() && t.second->scalar_type() == summed.scalar_type(), t.first,
+                  " must be like the sums: ", summed.sizes(), " ", summed.scalar_type(), ", got ", t.second->sizes(),
+                  " ", t.second->scalar_type());
+  dense("grad", grad), dense("grad_sum", grad_sum), dense("inverse", inverse);
+  const int64_t width = summed.size(-1), rows = summed.numel() / width;
+  TORCH_CHECK(inverse.scalar_type() == at::kFloat && inverse.numel() == rows,
+              "inverse must be float32 with one value for each row");
+  c10::DeviceGuard guard(summed.device());
+  Tensor dx = need_x ? at::empty_like(summed) : nothing(summed);
+  Tensor dw = need_weight ? at::empty_like(weight) : nothing(weight);
+  if (!need_x && !need_weight) return {dx, dw};
+  const size_t need = need_weight ? sdk_add_rms_norm_backward_workspace_bytes(rows, width) : 0;
+  Tensor ws = workspace(summed, need);
+  TOKEN_CALL(sdk_add_rms_norm_backward, ptr(grad), ptr(grad_sum), ptr(summed), ptr(weight),
+             (const float*)ptr(inverse), need_x ? ptr(dx) : nullptr, need_weight ? ptr(dw) : nullptr,
+             need ? ptr(ws) : nullptr, need, rows, width, dtype_of(summed.scalar_type(), "summed"),
+             dtype_of(weight.scalar_type(), "weight"), stream_of(summed));
+  return {dx, dw};
+}
+
+Tensor dequantize_rows(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+  on_gpu(codes);
+  beside(codes, "scales", scales);
+  dense("codes", codes), dense("scales", scales);
+  const bool fp8 = codes.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(fp8 || codes.scalar_type() == at::kChar, "codes must be int8 or float8_e4m3fn (got ",
+              codes.scalar_type(), ")");
+  const int to = dtype_of(dtype, "the result");
+  TORCH_CHECK(codes.dim() >= 1 && codes.size(-1) >= 1 && scales.scalar_type() == at::kFloat &&
+                  scales.sizes() == codes.sizes().slice(0, codes.dim() - 1),
+              "scales must be float32 with one value for each row of codes ", codes.sizes(), ", got ",
+              scales.scalar_type(), " ", scales.sizes());
+  c10::DeviceGuard guard(codes.device());
+  Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype));
+  const int64_t width = codes.size(-1);
+  TOKEN_CALL(sdk_dequantize_rows, ptr(codes), (const float*)ptr(scales), ptr(out), codes.numel() / width, width,
+             fp8 ? 2 : 1, to, stream_of(codes));
+  return out;
+}
+
+// ------------------------------------------------------------------------------------------ AdamW
+// The pointers of `tensors`, one for each parameter: like it, or `each` values to a scale.
+std::vector<void*> pointers(const char* name, at::TensorList params, at::TensorList tensors, at::ScalarType dtype,
+                            bool scales) {
+  TORCH_CHECK(tensors.size() == params.size(), tensors.size(), " ", name, " for ", params.size(), " params");
+  std::vector<void*> out(tensors.size());
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    const Tensor &t = tensors[i], &p = params[i];
+    TORCH_CHECK(t.scalar_type() == dtype && t.device() == params[0].device(), name, "[", i, "] must have dtype ",
+                dtype, " on ", params[0].device(), " (got ", t.scalar_type(), " on ", t.device(), ")");
+    const bool fits = scales ? t.dim() == 1 && t.size(0) == (p.numel() + kBlock - 1) / kBlock : t.sizes() == p.sizes();
+    TORCH_CHECK(fits, name, "[", i, "] has shape ", t.sizes(), " for a parameter ", p.sizes());
+    TORCH_CHECK(t.is_contiguous(), name, "[", i, "] must be contiguous");
+    out[i] = t.data_ptr();
+  }
+  return out;
+}
+
+std::vector<int64_t> sizes_of(at::TensorList params) {
+  std::vector<int64_t> n(params.size());
+  for (size_t i = 0; i < params.size(); ++i) n[i] = params[i].numel();
+  return n;
+}
+
+void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList avgs, at::TensorList sqs, double lr,
+                double beta1, double beta2, double eps, double weight_decay, int64_t step) {
+  if (params.empty()) return;
+  on_gpu(params[0]);
+  const at::ScalarType type = params[0].scalar_type();
+  const int dtype = dtype_of(type, "params");
+  const auto p = pointers("params", params, params, type, false), g = pointers("grads", params, grads, type, false);
+  const auto m = pointers("exp_avgs", params, avgs, at::kFloat, false);
+  const auto v = pointers("exp_avg_sqs", params, sqs, at::kFloat, false);
+  const auto n = sizes_of(params);
+  c10::DeviceGuard guard(params[0].device());
+  TOKEN_CALL(sdk_adamw_step, p.data(), g.data(), (float* const*)m.data(), (float* const*)v.data(), n.data(),
+             (int64_t)n.size(), lr, beta1, beta2, eps, weight_decay, step, dtype, stream_of(params[0]));
+}
+
+void adamw_step_8bit(at::TensorList params, at::TensorList grads, at::TensorList avg_codes, at::TensorList avg_scales,
+                     at::TensorList sq_codes, at::TensorList sq_scales, double lr, double beta1, double beta2,
+                     double eps, double weight_decay, int64_t step) {
+  if (params.empty()) return;
+  on_gpu(params[0]);
+  const at::ScalarType type = params[0].scalar_type();
+  const int dtype = dtype_of(type, "params");
+  const auto p = pointers("params", params, params, type, false), g = pointers("grads", params, grads, type, false);
+  const auto mc = pointers("avg_codes", params, avg_codes, at::kChar, false);
+  const auto ms = pointers("avg_scales", params, avg_scales, at::kFloat, true);
+  const auto vc = pointers("sq_codes", params, sq_codes, at::kByte, false);
+  const auto vs = pointers("sq_scales", params, sq_scales, at::kFloat, true);
+  const auto n = sizes_of(params);
+  c10::DeviceGuard guard(params[0].device());
+  TOKEN_CALL(sdk_adamw_step_8bit, p.data(), g.data(), (int8_t* const*)mc.data(), (float* const*)ms.data(),
+             (uint8_t* const*)vc.data(), (float* const*)vs.data(), n.data(), (int64_t)n.size(), lr, beta1, beta2, eps,
+             weight_decay, step, dtype, stream_of(params[0]));
+}
+
+Tensor adamw_moment_values(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+  on_gpu(codes);
+  beside(codes, "scales", scales);
+  dense("codes", codes), dense("scales", scales);
+  const bool second = codes.scalar_type() == at::kByte;
+  TORCH_CHECK(second || codes.scalar_type() == at::kChar,
+              "codes must be int8 (first moment) or uint8 (second), got ", codes.scalar_type());
+  const int to = dtype_of(dtype, "the result");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.dim() == 1 &&
+                  scales.size(0) == (codes.numel() + kBlock - 1) / kBlock,
+              "scales must be float32 of shape [", (codes.numel() + kBlock - 1) / kBlock, "], got ",
+              scales.scalar_type(), " ", scales.sizes());
+  c10::DeviceGuard guard(codes.device());
+  Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype));
+  TOKEN_CALL(sdk_adamw_moment_values, ptr(codes), (const float*)ptr(scales), ptr(out), codes.numel(), (int)second, to,
+             stream_of(codes));
+  return out;
+}
+
+}  // namespace
+
+TORCH_LIBRARY_IMPL(sdk_mapped_ops, CUDA, m) {
+  m.impl("bucket_attention_forward", &bucket_attention_forward);
+  m.impl("bucket_attention_backward", &bucket_attention_backward);
+  m.impl("add_rms_norm", &add_rms_norm);
+  m.impl("add_rms_norm_quantized", &add_rms_norm_quantized);
+  m.impl("add_rms_norm_backward", &add_rms_norm_backward);
+  m.impl("dequantize_rows", &dequantize_rows);
+  m.impl("adamw_step", &adamw_step);
+  m.impl("adamw_step_8bit", &adamw_step_8bit);
+  m.impl("adamw_moment_values", &adamw_moment_values);
+}
+
+// Names of the operators above, for the Python side (which implements those that are missing here).
+extern "C" const char* sdk_torch_token_ops(void) {
+  return "bucket_attention_forward,bucket_attention_backward,add_rms_norm,add_rms_norm_quantized,"
+         "add_rms_norm_backward,dequantize_rows,adamw_step,adamw_step_8bit,adamw_moment_values";
+}
