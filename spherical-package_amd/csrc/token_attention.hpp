@@ -10,6 +10,9 @@
 // row `row_of(k)`.  A lane reads the buckets of its 16 pairs as 16 consecutive bytes, and the values it holds are
 // the next product's B operand as they are: the sum's index may be permuted if A's rows are named alike.
 #pragma once
+#include <algorithm>
+#include <type_traits>
+
 #include "sdk_mfma.hpp"
 #include "token_types.hpp"
 
@@ -19,14 +22,16 @@ namespace token {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// Eight values of k of an operand.
+// Eight values of k of an operand.  float32 runs on the bf16 matrix unit: a float is the exact sum of three bf16
+// pieces (hi, mid, lo), and six of the nine products of pieces, all but those below 2^-26 of the product, are added
+// in float32.  (The unit's own float32 product takes 512 cycles for 16 values of k, these six 192.)
 template <typename T>
 struct Operand {
   unsigned u[4];
 };
 template <>
 struct Operand<float> {
-  float u[8];
+  Operand<bf16> piece[3];
 };
 
 __device__ __forceinline__ floatx16 product(const Operand<bf16>& a, const Operand<bf16>& b, floatx16 c) {
@@ -37,25 +42,34 @@ __device__ __forceinline__ floatx16 product(const Operand<f16>& a, const Operand
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                 0);
 }
-// float32: eight products of two values of k each, value s of both lane halves in product s.
 __device__ __forceinline__ floatx16 product(const Operand<float>& a, const Operand<float>& b, floatx16 c) {
-#pragma unroll
-  for (int s = 0; s < 8; ++s) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.u[s], b.u[s], c, 0, 0, 0);
-  return c;
+  c = product(a.piece[2], b.piece[0], c);
+  c = product(a.piece[0], b.piece[2], c);
+  c = product(a.piece[1], b.piece[1], c);
+  c = product(a.piece[1], b.piece[0], c);
+  c = product(a.piece[0], b.piece[1], c);
+  return product(a.piece[0], b.piece[0], c);
+}
+
+// Two floats' pieces, packed.  Each piece is rounded to nearest, so what is left out has either sign.
+__device__ __forceinline__ void split_pair(float x, float y, unsigned& hi, unsigned& mid, unsigned& lo) {
+  hi = pack_bf16x2(x, y);
+  x -= __uint_as_float(hi << 16), y -= __uint_as_float(hi & 0xffff0000u);
+  mid = pack_bf16x2(x, y);
+  x -= __uint_as_float(mid << 16), y -= __uint_as_float(mid & 0xffff0000u);
+  lo = pack_bf16x2(x, y);
 }
 
 template <typename T>
 __device__ __forceinline__ Operand<T> rounded(const float* f) {
   Operand<T> r;
-  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.u[i] = f[i];
-  } else if constexpr (__is_same(T, bf16)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.u[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      split_pair(f[2 * i], f[2 * i + 1], r.piece[0].u[i], r.piece[1].u[i], r.piece[2].u[i]);
+    } else if constexpr (__is_same(T, bf16)) {
+      r.u[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+    } else {
       const f32x2 v = {f[2 * i], f[2 * i + 1]};
       r.u[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
     }
@@ -63,18 +77,21 @@ __device__ __forceinline__ Operand<T> rounded(const float* f) {
   return r;
 }
 
+// Eight consecutive values in memory, 16-byte aligned; `in` false: zeros, not read.
 template <typename T>
-__device__ __forceinline__ Operand<T> zeros() {
-  Operand<T> r;
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(r.u) / 4); ++i) r.u[i] = 0;
+__device__ __forceinline__ Operand<T> load_operand(const T* p, bool in) {
+  Operand<T> r = {};
+  if (in) {
+    if constexpr (sizeof(T) == 4) {
+      float f[8];
+      load_pack<float, 4>(p, *reinterpret_cast<float(*)[4]>(f));
+      load_pack<float, 4>(p + 4, *reinterpret_cast<float(*)[4]>(f + 4));
+      r = rounded<T>(f);
+    } else {
+      r = *reinterpret_cast<const Operand<T>*>(__builtin_assume_aligned(p, 16));
+    }
+  }
   return r;
-}
-
-// Eight consecutive values, 16-byte aligned (in memory or LDS).
-template <typename T>
-__device__ __forceinline__ Operand<T> load_operand(const T* p) {
-  return *reinterpret_cast<const Operand<T>*>(__builtin_assume_aligned(p, 16));
 }
 
 template <int NT>
@@ -83,81 +100,222 @@ __device__ __forceinline__ int row_of(int token) {
   return 32 * t + 8 * (v / 4) + 4 * h + v % 4;
 }
 
-// A tile of 32 NT tokens, DP values each, in LDS.  16 bytes beside each row spread rows over the banks.
+// A tile of 32 NT tokens, DP values each, in LDS; float32 as three planes of pieces.  16 bytes beside each row
+// spread rows over the banks.
 template <typename T, int DP, int NT>
 struct Tile {
-  static constexpr int kRows = 32 * NT, kStride = DP + 16 / (int)sizeof(T);
-  T v[kRows * kStride];
+  using Half = std::conditional_t<sizeof(T) == 4, bf16, T>;
+  static constexpr int kRows = 32 * NT, kStride = DP + 8, kPlanes = sizeof(T) == 4 ? 3 : 1;
+  Half v[kPlanes][kRows * kStride];
 
-  // rows of A, values 16 c + 8 h .. + 7
-  __device__ __forceinline__ Operand<T> rows(int t, int c, int lane) const {
-    return load_operand<T>(v + (32 * t + lane % 32) * kStride + 16 * c + 8 * (lane / 32));
-  }
-  // columns of the tile as A: row i of A = column 32 d + i, k = the 16 tokens that registers 8 half .. 8 half + 7 of
-  // part t hold
-  __device__ __forceinline__ Operand<T> columns(int t, int half, int d, int lane) const {
-    const int first = 32 * t + 16 * half + 4 * (lane / 32);
-    Operand<T> r;
-    if constexpr (sizeof(T) == 4) {
+  // What a lane reads of a tile, by its own addresses: everything but the lane's part is a constant offset.
+  struct View {
+    const Half *row, *column;
+
+    // rows of A, values 16 c + 8 h .. + 7
+    __device__ __forceinline__ Operand<T> rows(int t, int c) const {
+      const int at = 32 * t * kStride + 16 * c;
+      Operand<T> r;
+      if constexpr (kPlanes == 3) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) r.u[s] = v[(first + s % 4 + 8 * (s / 4)) * kStride + 32 * d + lane % 32];
-    } else {
-      const T* p = v + (first + lane % 16 / 4) * kStride + 32 * d + 16 * (lane / 16 % 2) + 4 * (lane % 4);
-      const Bf16Frag f = tr_frag((const char*)p, (const char*)(p + 8 * kStride));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.u[i] = f.u[i];
+        for (int i = 0; i < 3; ++i) r.piece[i] = straight<bf16>(row + i * kRows * kStride + at);
+      } else {
+        r = straight<T>(row + at);
+      }
+      return r;
     }
+    // the first piece of float32 rows alone
+    __device__ __forceinline__ Operand<bf16> first_piece(int t, int c) const {
+      return straight<bf16>(row + 32 * t * kStride + 16 * c);
+    }
+    // columns of the tile as A: row i of A = column 32 d + i, k = the 16 tokens that registers 8 half .. 8 half + 7
+    // of part t hold
+    __device__ __forceinline__ Operand<T> columns(int t, int half, int d) const {
+      const int at = (32 * t + 16 * half) * kStride + 32 * d;
+      Operand<T> r;
+      if constexpr (kPlanes == 3) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) r.piece[i] = turned<bf16>(column + i * kRows * kStride + at);
+      } else {
+        r = turned<T>(column + at);
+      }
+      return r;
+    }
+  };
+  __device__ __forceinline__ View view(int lane) const {
+    return {v[0] + (lane % 32) * kStride + 8 * (lane / 32),
+            v[0] + (4 * (lane / 32) + lane % 16 / 4) * kStride + 16 * (lane / 16 % 2) + 4 * (lane % 4)};
+  }
+  // kWide values of a token from d on
+  __device__ __forceinline__ void store(int token, int d, const Pack<T, kWide<T>>& x) {
+    const int at = row_of<NT>(token) * kStride + d;
+    if constexpr (kPlanes == 3) {
+      unsigned p[3][2];
+      split_pair(x.v[0], x.v[1], p[0][0], p[1][0], p[2][0]);
+      split_pair(x.v[2], x.v[3], p[0][1], p[1][1], p[2][1]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(v[i] + at) = make_uint2(p[i][0], p[i][1]);
+    } else {
+      *reinterpret_cast<Pack<T, kWide<T>>*>(v[0] + at) = x;
+    }
+  }
+
+ private:
+  template <typename H>
+  __device__ static __forceinline__ Operand<H> straight(const Half* p) {
+    return *reinterpret_cast<const Operand<H>*>(__builtin_assume_aligned(p, 16));
+  }
+  template <typename H>
+  __device__ static __forceinline__ Operand<H> turned(const Half* p) {
+    const Bf16Frag f = tr_frag((const char*)p, (const char*)(p + 8 * kStride));
+    Operand<H> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.u[i] = f.u[i];
     return r;
   }
 };
 
-// A tile on its way from memory to LDS, in the registers of the workgroup's THREADS threads.  Tokens at or
-// beyond `end` and values at or beyond `dim` are zeros and are not read.
+// begin(v) plus the products of the tile's rows with x.  float32: the five small products of each pair first, from
+// zero, and `begin` last: the unit drops what falls below the sum's last bit, which adds up over the steps.  The
+// rows' first pieces are read twice for it (the fence keeps them from staying in registers).
+template <typename T, int DP, typename View, typename Begin>
+__device__ __forceinline__ floatx16 dot_tile(const View& view, int t, const Operand<T> (&x)[DP / 16], Begin begin) {
+  floatx16 c;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const Operand<T> a = view.rows(t, i);
+      c = product(a.piece[2], x[i].piece[0], c);
+      c = product(a.piece[0], x[i].piece[2], c);
+      c = product(a.piece[1], x[i].piece[1], c);
+      c = product(a.piece[1], x[i].piece[0], c);
+      c = product(a.piece[0], x[i].piece[1], c);
+    }
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) c = product(view.first_piece(t, i), x[i].piece[0], c);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] += begin(v);
+  } else {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] = begin(v);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) c = product(view.rows(t, i), x[i], c);
+  }
+  return c;
+}
+
+// A tile on its way from memory to LDS, in the registers of the workgroup's THREADS threads.  The tile's `left`
+// tokens and `dim` values are read, zeros stand for the others: a buffer descriptor that ends with the last token
+// tells them apart, and a thread's vectors lie at the same 32-bit offsets of every tile (the host checks that 64
+// tokens span less than 2^31 bytes).  Tile and descriptor are the workgroup's own, in scalar registers.
 template <typename T, int DP, int NT, int THREADS>
 struct Carry {
   static constexpr int kVectors = DP / kWide<T>, kCount = 32 * NT * kVectors / THREADS;
   static_assert(32 * NT * kVectors % THREADS == 0, "every thread carries as many vectors");
-  Pack<T, kWide<T>> v[kCount];
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 v[kCount];
+  unsigned at[kCount];
 
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int64_t first, int64_t end, int dim) {
+  __device__ __forceinline__ Carry(int64_t stride, int dim) {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
-      const int at = n * THREADS + threadIdx.x, token = at / kVectors, d = at % kVectors * kWide<T>;
-      if (first + token < end && d < dim) {
-        v[n] = *reinterpret_cast<const Pack<T, kWide<T>>*>(base + (first + token) * stride + d);
-      } else {
+      const int i = n * THREADS + threadIdx.x, d = i % kVectors * kWide<T>;
+      at[n] = d < dim ? (unsigned)((i / kVectors) * (int)stride + d) * (unsigned)sizeof(T) : 0xfffffff0u;
+    }
+  }
+  __device__ __forceinline__ void load(const T* tile, int64_t stride, int left, int dim) {
+    const int rows = std::min(left, 32 * NT);
+    const unsigned bytes = rows > 0 ? (unsigned)((rows - 1) * (int)stride + dim) * (unsigned)sizeof(T) : 0u;
+    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(tile), 0, bytes, 0x00020000);
 #pragma unroll
-        for (int e = 0; e < kWide<T>; ++e) v[n].v[e] = (T)0.f;
-      }
+    for (int n = 0; n < kCount; ++n) v[n] = __builtin_amdgcn_raw_buffer_load_b128(all, at[n], 0, 0);
+  }
+  __device__ __forceinline__ void scale(float by) {
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      Pack<T, kWide<T>> x = __builtin_bit_cast(Pack<T, kWide<T>>, v[n]);
+#pragma unroll
+      for (int e = 0; e < kWide<T>; ++e) x.v[e] = (T)((float)x.v[e] * by);
+      v[n] = __builtin_bit_cast(u32x4, x);
     }
   }
   __device__ __forceinline__ void store(Tile<T, DP, NT>& tile) const {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
-      const int at = n * THREADS + threadIdx.x, token = at / kVectors, d = at % kVectors * kWide<T>;
-      *reinterpret_cast<Pack<T, kWide<T>>*>(&tile.v[row_of<NT>(token) * Tile<T, DP, NT>::kStride + d]) = v[n];
+      const int i = n * THREADS + threadIdx.x;
+      tile.store(i / kVectors, i % kVectors * kWide<T>, __builtin_bit_cast(Pack<T, kWide<T>>, v[n]));
     }
   }
 };
 
-// The buckets of a lane's 16 pairs: 16 bytes at any address; at the map's end byte by byte.
+// The buckets of a lane's 16 pairs: 16 bytes at any address; near the map's end byte by byte.
 struct Buckets {
   unsigned w[4];
-  __device__ __forceinline__ void load(const uint8_t* row, int64_t first, int64_t count) {
-    if (first + 16 <= count) {
-      __builtin_memcpy(w, row + first, 16);
-    } else {
+  __device__ __forceinline__ void load(const uint8_t* row) { __builtin_memcpy(w, row, 16); }
+  __device__ __forceinline__ void load(const uint8_t* row, int left) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = 0;
+    for (int i = 0; i < 4; ++i) w[i] = 0;
+    for (int i = 0; i < 16 && i < left; ++i) {
+      const unsigned x = (unsigned)row[i] << (8 * (i % 4));
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (first + i < count) w[i / 4] |= (unsigned)row[first + i] << (8 * (i % 4));
+      for (int k = 0; k < 4; ++k) w[k] |= i / 4 == k ? x : 0u;
     }
   }
   __device__ __forceinline__ unsigned operator[](int v) const { return w[v / 4] >> (8 * (v % 4)) & 255u; }
 };
+// The buckets of a tile's parts from key `first` on.
+template <int NT>
+__device__ __forceinline__ void load_buckets(Buckets (&b)[NT], const uint8_t* row, int first, int count, int h) {
+  if (first + 32 * NT <= count) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) b[t].load(row + first + 16 * NT * h + 16 * t);
+  } else {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      b[t].load(row + first + 16 * NT * h + 16 * t, count - (first + 16 * NT * h + 16 * t));
+  }
+}
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// The value of the lane 32 away.
+__device__ __forceinline__ float other_half(float x) {
+  const unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(threadIdx.x % 64 < 32 ? r[1] : r[0]);
+}
+// Largest of the lane's and the other half's value (NaN: the other one).
+__device__ __forceinline__ float max_halves(float x) {
+  const unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// sum + the eight weights f, as the product takes them (16-bit: rounded, two at a time).
+template <typename T>
+__device__ __forceinline__ float add_weights(const Operand<T>& w, const float* f, float sum) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += f[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (__is_same(T, bf16)) {
+        const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w.u[i]), one, sum, false);
+      } else {
+        const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+        sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w.u[i]), one, sum, false);
+      }
+    }
+  }
+  return sum;
+}
+
+// A query's running maximum may fall behind by this much (a factor of 2^8 of the weights) before its sums are
+// brought to a new one.
+constexpr float kBehind = 8.f;
 
 // Workgroups follow each other round the eight dies; consecutive tiles of one head share its keys and values, so
 // each die gets a consecutive range of tiles.
@@ -174,13 +332,12 @@ struct Attention {
   void *dq, *dk, *dv, *dtable;
   float* lse;
   int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3], ms[2];
-  int64_t queries, keys;
-  int batch, heads, key_heads, dim, buckets, causal, table_float;
+  int queries, keys, batch, heads, key_heads, dim, buckets, causal, table_float;
   float scale, scale2, limit;
 
-  __device__ __forceinline__ int64_t length(int b) const {
+  __device__ __forceinline__ int length(int b) const {
     if (!lengths) return keys;
-    const int64_t n = lengths[b];
+    const int n = __builtin_amdgcn_readfirstlane(lengths[b]);
     return n < 0 ? 0 : n > keys ? keys : n;
   }
   // bias / scale of a bucket: scores enter the softmax as scale2 * (q k + bias / scale)
@@ -193,6 +350,98 @@ struct Attention {
     return fabsf(x) < INFINITY ? fminf(fmaxf(y, -limit), limit) : x;
   }
 };
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTable = 256;
+
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 1 : 2;   // 32-token parts of a tile
+
+// A wave's 32 columns of B: row `row` of a tensor, values 16 c + 8 h .. + 7 in operand c; zeros unless `in`.
+template <typename T, int DP>
+__device__ __forceinline__ void load_columns(Operand<T> (&x)[DP / 16], const T* base, int64_t stride, int row, bool in,
+                                             int dim, int lane) {
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    const int d = 16 * c + 8 * (lane / 32);
+    x[c] = load_operand<T>(base + row * stride + d, in && d < dim);
+  }
+}
+
+// The wave's accumulators D[value 32 d + ..][column] to row `row` of a tensor, times `by`.
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(T* base, int64_t stride, int64_t row, int dim, int lane,
+                                              const floatx16 (&acc)[DP / 32], float by) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int at = 32 * d + 8 * a + 4 * (lane / 32);
+      if (at < dim) {
+        const float f[4] = {acc[d][4 * a] * by, acc[d][4 * a + 1] * by, acc[d][4 * a + 2] * by,
+                            acc[d][4 * a + 3] * by};
+        store_pack<T, 4>(base + row * stride + at, f);
+      }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void clear(floatx16 (&x)[N]) {
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[d][v] = 0.f;
+}
+
+// Between a wave's writes to LDS and its other lanes' reads: LDS keeps a wave's order, so it is the compiler alone
+// that must not exchange them.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Where split `split` of `splits` begins among `tiles`.
+__device__ __forceinline__ int split_at(int tiles, int split, int splits) {
+  return (int)((int64_t)tiles * split / splits);
+}
+
+// Which tile of which head (counted with the batch) and which split of it a workgroup takes.  In causal calls
+// the tiles differ in work: the longest ones first (`ascending`: those with small numbers), all heads' together.
+struct Work {
+  int tile, head, split;
+  __device__ __forceinline__ Work(int tiles, int heads, int splits, bool causal, bool ascending) {
+    if (causal) {
+      unsigned id = blockIdx.x;
+      head = (int)(id % (unsigned)heads);
+      id /= (unsigned)heads;
+      split = (int)(id % (unsigned)splits);
+      tile = (int)(id / (unsigned)splits);
+      if (!ascending) tile = tiles - 1 - tile;
+    } else {
+      unsigned id = by_die(blockIdx.x, gridDim.x);
+      split = (int)(id % (unsigned)splits);
+      id /= (unsigned)splits;
+      tile = (int)(id % (unsigned)tiles);
+      head = (int)(id / (unsigned)tiles);
+    }
+  }
+};
+
+// host
+Attention on_device(const sdk_bucket_attention* a);
+bool few_rows(const sdk_bucket_attention* a);       // whether a key head's rows go to the kernel of few queries
+int forward_splits(const sdk_bucket_attention* a);
+size_t backward_bytes(const sdk_bucket_attention* a);
+int run_forward(const sdk_bucket_attention* a, void* workspace, hipStream_t s);
+int run_backward(const sdk_bucket_attention* a, void* workspace, hipStream_t s);
+
+// Runs `CALL` with DP, the padded dim.
+#define ATTENTION_DIM(dim, ...)                                  \
+  do {                                                           \
+    if ((dim) <= 32) { constexpr int DP = 32; __VA_ARGS__; }     \
+    else if ((dim) <= 64) { constexpr int DP = 64; __VA_ARGS__; } \
+    else { constexpr int DP = 128; __VA_ARGS__; }                \
+  } while (0)
 
 }  // namespace token
 }  // namespace sdk

@@ -1,0 +1,529 @@
+// Backward of attention with a bias for each bucket of relative positions (token_attention.hpp: operands and tiles).
+//
+//   p_ij = exp(s_ij - lse_i)      D_i = <do_i, o_i>      ds_ij = p_ij (<do_i, v_j> - D_i)
+//   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i      dv_j = sum_i p_ij do_i
+//   dT[head][b] = sum of ds_ij over the pairs of bucket b
+//
+// The scores are formed again from the lse, once with the queries in registers (dq, dT) and once with the keys (dk,
+// dv): seven products instead of five, and no sum whose order depends on scheduling.
+//
+// float16 has few exponents: p (about 1 / keys) and ds would fall among its subnormal numbers.  There p is held times
+// 2^8, and do times a power of two that brings its largest magnitude to 2^-7 .. 2^-6 (ds then overflows beside values
+// beyond 128 alone); both are taken out of the sums,
+// exactly.
+#include "token_attention.hpp"
+
+namespace sdk {
+namespace token {
+namespace {
+
+// Waves of a SIMD: with two, accumulators lie among the 256 registers of a wave.
+template <int DP>
+constexpr int kBackwardWaves = DP <= 64 ? 2 : 1;
+
+template <typename T>
+constexpr float kLift = __is_same(T, f16) ? 8.f : 0.f;   // log2 of what p is held times
+
+// What do is held times: from the bits of its largest magnitude.
+template <typename T>
+__device__ __forceinline__ float gradient_scale(const unsigned* top) {
+  if constexpr (!__is_same(T, f16)) return 1.f;
+  const unsigned exponent = *top >> 23;
+  return exponent == 0 || exponent >= 255 ? 1.f : __uint_as_float((247 - exponent) << 23);
+}
+
+// ------------------------------------------------------------------------------------------ terms of a row
+__global__ void clear_word(unsigned* word) { *word = 0; }
+
+// D_i and log2 of the softmax's sum (+inf for a query without pairs: its p are zeros); float16: the largest |do|.
+// A row is read by LANES lanes, 16 bytes each.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta, float* lse2, unsigned* top) {
+  __shared__ float slots[4];
+  const int lane = threadIdx.x % LANES, d = kWide<T> * lane;
+  const int64_t rows = (int64_t)a.batch * a.heads * a.queries;
+  float most = 0.f;
+  for (int64_t first = (int64_t)blockIdx.x * (256 / LANES); first < rows; first += (int64_t)gridDim.x * (256 / LANES)) {
+    const int64_t row = first + threadIdx.x / LANES;
+    float dot = 0.f;
+    if (row < rows) {
+      const int64_t query = row % a.queries, bh = row / a.queries;
+      const int head = (int)(bh % a.heads), b = (int)(bh / a.heads);
+      if (d < a.dim) {
+        float x[kWide<T>], y[kWide<T>];
+        load_pack<T, kWide<T>>((const T*)a.out + b * a.os[0] + head * a.os[1] + query * a.os[2] + d, x);
+        load_pack<T, kWide<T>>((const T*)a.grad + b * a.gs[0] + head * a.gs[1] + query * a.gs[2] + d, y);
+#pragma unroll
+        for (int e = 0; e < kWide<T>; ++e) {
+          dot = fmaf(x[e], y[e], dot);
+          if constexpr (__is_same(T, f16)) most = Largest::of(most, fabsf(y[e]));
+        }
+      }
+    }
+#pragma unroll
+    for (int n = LANES / 2; n > 0; n /= 2) dot += __shfl_xor(dot, n);
+    if (row < rows && lane == 0) {
+      const float l = a.lse[row];
+      delta[row] = dot;
+      lse2[row] = l == -INFINITY ? INFINITY : l;
+    }
+  }
+  if constexpr (__is_same(T, f16)) {   // the order of a maximum does not matter
+    most = over_group<Largest, 256>(most, slots);
+    if (threadIdx.x == 0) atomicMax(top, __float_as_uint(most) & 0x7fffffffu);
+  }
+}
+
+// map[query][key] to turned[key][query], rows of `pitch` bytes, 64 x 64 bytes a workgroup.
+__global__ __launch_bounds__(256) void turn_map(const Attention a, uint8_t* turned, int pitch) {
+  __shared__ uint8_t block[64][65];
+  const int across = pitch / 64, q0 = (int)(blockIdx.x % across) * 64, k0 = (int)(blockIdx.x / across) * 64;
+  const uint8_t* map = a.map + (int64_t)blockIdx.y * a.ms[0];
+  const int x = threadIdx.x % 64;
+  for (int y = threadIdx.x / 64; y < 64; y += 4)
+    block[y][x] = q0 + y < a.queries && k0 + x < a.keys ? map[(q0 + y) * a.ms[1] + k0 + x] : 255;
+  __syncthreads();
+  uint8_t* to = turned + (int64_t)blockIdx.y * a.keys * pitch;
+  for (int y = threadIdx.x / 64; y < 64; y += 4)
+    if (k0 + y < a.keys) to[(int64_t)(k0 + y) * pitch + q0 + x] = block[x][y];
+}
+
+// ------------------------------------------------------------------------------------------ dq and the bias table
+// Adds x to the sums of its buckets in one lane's column, four at a time: read, add, write, and where two of the
+// four meet the second takes the first's sum.  (An LDS float add of 64 lanes takes 193 cycles of a CU whatever its
+// addresses, this 13.)
+template <int COLUMNS>
+__device__ __forceinline__ void add_by_bucket(float* column, const Buckets& bucket, int buckets, const float* x) {
+#pragma unroll
+  for (int v = 0; v < 16; v += 4) {
+    int at[4];
+    float sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] = std::min((int)bucket[v + i], buckets) * COLUMNS;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = column[at[i]];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum[i] += x[v + i];
+#pragma unroll
+      for (int j = i + 1; j < 4; ++j) sum[j] = at[j] == at[i] ? sum[i] : sum[j];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) column[at[i]] = sum[i];
+  }
+}
+
+// As the forward, a workgroup walks the keys (or a split of them) with 128 queries.  Each lane adds its ds to the
+// bucket's sum in a column of its own (COLUMNS of them a wave: 64 up to 64 buckets, fewer beyond, then the lanes
+// that share one take turns; 0: no table gradient), so that every sum has one order.
+// part: splits > 1: float32 sums of the splits, [split][row][dim].
+template <typename T, int DP, int COLUMNS>
+__global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
+    const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top, float* part,
+    float* table_parts) {
+  constexpr int NT = kParts<T>, KEYS = 32 * NT;
+  __shared__ __attribute__((aligned(16))) struct {
+    float table[kTable];   // at address zero: a lookup's address is four times the bucket
+    Tile<T, DP, NT> keys, values;
+  } lds;
+  auto& table = lds.table;
+  auto &keys = lds.keys, &values = lds.values;
+  extern __shared__ float sums[];   // [wave][bucket, the last for pairs that do not count][column]
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, h = lane / 32;
+  const Work work(tiles, a.batch * a.heads, splits, a.causal, false);
+  const int head = work.head % a.heads, b = work.head / a.heads;
+  const int shared_head = head / (a.heads / a.key_heads);
+  const T* kp = (const T*)a.k + b * a.ks[0] + shared_head * a.ks[1];
+  const T* vp = (const T*)a.v + b * a.vs[0] + shared_head * a.vs[1];
+  table[threadIdx.x] = a.bias(head, threadIdx.x, __is_same(T, bf16));
+  float* mine = sums + wave * (a.buckets + 1) * COLUMNS;
+  for (int i = lane; i < (a.buckets + 1) * COLUMNS; i += 64) mine[i] = 0.f;
+
+  const int first = work.tile * (32 * kWaves), query = first + wave * 32 + lane % 32;
+  const int len = a.length(b), shift = len - a.queries;
+  const int end = a.causal ? std::min(len, std::min(first + 32 * kWaves, a.queries) + shift) : len;
+  const int blocks = end > 0 ? (end + KEYS - 1) / KEYS : 0;
+  const int from = split_at(blocks, work.split, splits) * KEYS;
+  const int to = std::min(end, split_at(blocks, work.split + 1, splits) * KEYS);
+  const int clamped = std::min(query, a.queries - 1);
+  const int64_t row = (int64_t)work.head * a.queries + clamped;
+  const uint8_t* map = a.map + b * a.ms[0] + clamped * a.ms[1];
+  const int last = a.causal ? std::min(len - 1, clamped + shift) : len - 1;
+  const bool in = query < a.queries;
+  const float held = gradient_scale<T>(top);
+  const float my_lse = in ? lse2[row] - kLift<T> : INFINITY, my_delta = in ? delta[row] * held : 0.f;
+
+  Operand<T> q[DP / 16], g[DP / 16];
+  load_columns<T, DP>(q, (const T*)a.q + b * a.qs[0] + head * a.qs[1], a.qs[2], query, in, a.dim, lane);
+  load_columns<T, DP>(g, (const T*)a.grad + b * a.gs[0] + head * a.gs[1], a.gs[2], query, in, a.dim, lane);
+  if constexpr (__is_same(T, f16)) {
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      f16x8 x = __builtin_bit_cast(f16x8, g[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (f16)((float)x[e] * held);
+      g[c] = __builtin_bit_cast(Operand<T>, x);
+    }
+  }
+  floatx16 dq[DP / 32];
+  clear(dq);
+
+  Carry<T, DP, NT, kThreads> next_k(a.ks[2], a.dim), next_v(a.vs[2], a.dim);
+  Buckets bucket[NT];
+  auto request = [&](int k0) {
+    next_k.load(kp + k0 * a.ks[2], a.ks[2], to - k0, a.dim);
+    next_v.load(vp + k0 * a.vs[2], a.vs[2], to - k0, a.dim);
+  };
+  const auto key_view = keys.view(lane), value_view = values.view(lane);
+  if (from < to) {
+    request(from);
+    load_buckets<NT>(bucket, map, from, a.keys, h);
+  }
+  for (int k0 = from; k0 < to; k0 += KEYS) {
+    __syncthreads();
+    next_k.store(keys);
+    next_v.store(values);
+    __syncthreads();
+    if (k0 + KEYS < to) request(k0 + KEYS);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      floatx16 s = dot_tile<T, DP>(key_view, t, q, [&](int v) { return table[bucket[t][v]]; });
+      const floatx16 e = dot_tile<T, DP>(value_view, t, g, [&](int) { return -my_delta; });
+      if (k0 + KEYS > last + 1) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (k0 + 16 * NT * h + 16 * t + v > last) s[v] = -INFINITY;
+      }
+      float ds[16];
+#pragma unroll
+      for (int v = 0; v < 16; ++v) ds[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -my_lse)) * e[v];
+      if constexpr (COLUMNS > 0) {
+#pragma unroll
+        for (int turn = 0; turn < 64 / COLUMNS; ++turn) {
+          if (lane / COLUMNS == turn) add_by_bucket<COLUMNS>(mine + lane % COLUMNS, bucket[t], a.buckets, ds);
+          if (COLUMNS < 64) wave_order();   // the next turn's lanes read what these wrote
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const Operand<T> w = rounded<T>(ds + 8 * half);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) dq[d] = product(key_view.columns(t, half, d), w, dq[d]);
+      }
+    }
+    if (k0 + KEYS < to) load_buckets<NT>(bucket, map, k0 + KEYS, a.keys, h);
+  }
+  const float back = exp2f(-kLift<T>) / held;
+  if (in && splits > 1)
+    store_columns<float, DP>(part + ((int64_t)work.split * a.batch * a.heads * a.queries + row) * a.dim, a.dim, 0, a.dim,
+                             lane, dq, a.scale * back);
+  else if (in && a.dq)
+    store_columns<T, DP>((T*)a.dq + b * a.dqs[0] + head * a.dqs[1], a.dqs[2], query, a.dim, lane, dq, a.scale * back);
+  if constexpr (COLUMNS > 0) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.buckets; i += kThreads) {
+      float x = 0.f;
+      for (int w = 0; w < kWaves; ++w)
+        for (int c = 0; c < COLUMNS; ++c)   // begun at the bucket's own column: other banks for other lanes
+          x += sums[(w * (a.buckets + 1) + i) * COLUMNS + (c + i) % COLUMNS];
+      table_parts[(((int64_t)work.head * tiles + work.tile) * splits + work.split) * a.buckets + i] = x * back;
+    }
+  }
+}
+
+// dT[head][bucket]: a workgroup an entry; the `each` parts of every batch element are added in an order of their own,
+// in double.
+template <typename T>
+__global__ __launch_bounds__(256) void join_table(const Attention a, int each, const float* parts) {
+  __shared__ double sums[256];
+  const int head = blockIdx.x / a.buckets, bucket = blockIdx.x % a.buckets;
+  double x = 0;
+  const int64_t count = (int64_t)a.batch * each;
+  for (int64_t i = threadIdx.x; i < count; i += 256)
+    x += parts[((i / each * a.heads + head) * each + i % each) * a.buckets + bucket];
+  sums[threadIdx.x] = x;
+  __syncthreads();
+  for (int n = 128; n > 0; n /= 2) {
+    if ((int)threadIdx.x < n) sums[threadIdx.x] += sums[threadIdx.x + n];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const int64_t at = (int64_t)head * a.buckets + bucket;
+    if (a.table_float)
+      ((float*)a.dtable)[at] = (float)sums[0];
+    else
+      ((T*)a.dtable)[at] = (T)(float)sums[0];
+  }
+}
+
+// ------------------------------------------------------------------------------------------ dk and dv
+// A workgroup keeps 128 keys, 32 a wave, and walks the queries of every head that reads them (or a split of these
+// tiles): S = Q K^T has the keys in columns.  The next tile is requested while this one is worked on, into the
+// other buffer.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(
+    const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top,
+    const uint8_t* turned, int pitch, float* part) {
+  constexpr int NT = kParts<T>, ROWS = 32 * NT;
+  __shared__ __attribute__((aligned(16))) struct {
+    float table[kTable];
+    float row_lse[2][ROWS], row_delta[2][ROWS];
+    Tile<T, DP, NT> queries[2], grads[2];
+  } lds;
+  auto& table = lds.table;
+  auto &row_lse = lds.row_lse, &row_delta = lds.row_delta;
+  auto &queries = lds.queries, &grads = lds.grads;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, h = lane / 32;
+  const Work work(tiles, a.batch * a.key_heads, splits, a.causal, true);
+  const int shared_head = work.head % a.key_heads, b = work.head / a.key_heads;
+  const int group = a.heads / a.key_heads;
+  const int first = work.tile * (32 * kWaves), key = first + wave * 32 + lane % 32;
+  const int len = a.length(b), shift = len - a.queries;
+  const uint8_t* map = turned + ((a.ms[0] ? (int64_t)b * a.keys : 0) + std::min(key, a.keys - 1)) * pitch;
+  const float held = gradient_scale<T>(top);
+
+  Operand<T> k[DP / 16], v[DP / 16];
+  load_columns<T, DP>(k, (const T*)a.k + b * a.ks[0] + shared_head * a.ks[1], a.ks[2], key, key < len, a.dim, lane);
+  load_columns<T, DP>(v, (const T*)a.v + b * a.vs[0] + shared_head * a.vs[1], a.vs[2], key, key < len, a.dim, lane);
+  floatx16 dk[DP / 32], dv[DP / 32];
+  clear(dk);
+  clear(dv);
+
+  // tiles of queries that see some key of the workgroup, head after head
+  const int from = a.causal ? std::max(0, first - shift) / ROWS * ROWS : 0;
+  const int each = first < len && from < a.queries ? (a.queries - from + ROWS - 1) / ROWS : 0;
+  const int begin = split_at(group * each, work.split, splits), stop = split_at(group * each, work.split + 1, splits);
+  const int seen = a.causal ? key - shift : 0;   // this lane's first query
+
+  Carry<T, DP, NT, kThreads> next_q(a.qs[2], a.dim), next_g(a.gs[2], a.dim);
+  Buckets bucket[NT];
+  float next_lse = 0.f, next_delta = 0.f;
+  auto request = [&](int unit) {
+    const int head = shared_head * group + unit / each, q0 = from + unit % each * ROWS;
+    next_q.load((const T*)a.q + b * a.qs[0] + head * a.qs[1] + q0 * a.qs[2], a.qs[2], a.queries - q0, a.dim);
+    next_g.load((const T*)a.grad + b * a.gs[0] + head * a.gs[1] + q0 * a.gs[2], a.gs[2], a.queries - q0, a.dim);
+    if (threadIdx.x < ROWS) {
+      const int q = q0 + threadIdx.x;
+      const int64_t row = ((int64_t)b * a.heads + head) * a.queries + q;
+      next_lse = INFINITY, next_delta = 0.f;
+      if (q < a.queries) next_lse = lse2[row], next_delta = delta[row];   // worked on in put: nothing waits here
+    }
+  };
+  auto put = [&](int buffer) {
+    next_q.store(queries[buffer]);
+    if constexpr (__is_same(T, f16)) next_g.scale(held);
+    next_g.store(grads[buffer]);
+    if (threadIdx.x < ROWS) {
+      row_lse[buffer][threadIdx.x] = kLift<T> - next_lse;
+      row_delta[buffer][threadIdx.x] = -next_delta * held;
+    }
+  };
+  auto put_bias = [&](int unit) {
+    table[threadIdx.x] = a.bias(shared_head * group + unit / each, threadIdx.x, __is_same(T, bf16));
+  };
+  auto buckets_of = [&](int unit) {   // rows of the turned map are padded to whole tiles
+#pragma unroll
+    for (int t = 0; t < NT; ++t) bucket[t].load(map + from + unit % each * ROWS + 16 * NT * h + 16 * t);
+  };
+  if (begin < stop) {
+    request(begin);
+    buckets_of(begin);
+    put(0);
+    put_bias(begin);
+  }
+  __syncthreads();
+  for (int unit = begin; unit < stop; ++unit) {
+    const int now = (unit - begin) % 2, q0 = from + unit % each * ROWS;
+    const bool more = unit + 1 < stop;
+    if (more) request(unit + 1);
+    const auto query_view = queries[now].view(lane), grad_view = grads[now].view(lane);
+    const float *now_lse = row_lse[now] + 16 * NT * h, *now_delta = row_delta[now] + 16 * NT * h;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      floatx16 s = dot_tile<T, DP>(query_view, t, k, [&](int i) { return table[bucket[t][i]]; });
+      const floatx16 e = dot_tile<T, DP>(grad_view, t, v, [&](int i) { return now_delta[16 * t + i]; });
+      if (q0 < seen) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (q0 + 16 * NT * h + 16 * t + i < seen) s[i] = -INFINITY;
+      }
+      float p[16], ds[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, now_lse[16 * t + i]));
+        ds[i] = p[i] * e[i];
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const Operand<T> w = rounded<T>(p + 8 * half), x = rounded<T>(ds + 8 * half);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          dv[d] = product(grad_view.columns(t, half, d), w, dv[d]);
+          dk[d] = product(query_view.columns(t, half, d), x, dk[d]);
+        }
+      }
+    }
+    if (more) buckets_of(unit + 1);
+    if (more) put(1 - now);
+    __syncthreads();
+    if (more && (unit + 1) % each == 0) {   // the next tile is another head's
+      put_bias(unit + 1);
+      __syncthreads();
+    }
+  }
+  if (key >= a.keys) return;
+  if (key >= len) {   // columns of keys that do not count
+    clear(dk);
+    clear(dv);
+  }
+  const float back = exp2f(-kLift<T>) / held;
+  if (splits > 1) {
+    const int64_t rows = (int64_t)a.batch * a.key_heads * a.keys, row = (int64_t)work.head * a.keys + key;
+    float* to = part + ((int64_t)work.split * 2 * rows + row) * a.dim;
+    store_columns<float, DP>(to, a.dim, 0, a.dim, lane, dk, a.scale * back);
+    store_columns<float, DP>(to + rows * a.dim, a.dim, 0, a.dim, lane, dv, back);
+    return;
+  }
+  if (a.dk)
+    store_columns<T, DP>((T*)a.dk + b * a.dks[0] + shared_head * a.dks[1], a.dks[2], key, a.dim, lane, dk, a.scale * back);
+  if (a.dv) store_columns<T, DP>((T*)a.dv + b * a.dvs[0] + shared_head * a.dvs[1], a.dvs[2], key, a.dim, lane, dv, back);
+}
+
+// ------------------------------------------------------------------------------------------ splits
+// out[row] = sum of the splits' parts in their order, four values a thread; part [split][.. rows ..][dim], `pitch`
+// values from split to split.
+template <typename T>
+__global__ __launch_bounds__(256) void join_splits(const float* part, int64_t pitch, int splits, T* out, int64_t s0,
+                                                   int64_t s1, int64_t s2, int64_t rows, int tokens, int heads, int dim) {
+  const int per_row = dim / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per_row;
+  if (row >= rows) return;
+  const int d = (int)(i % per_row) * 4;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    float y[4];
+    load_pack<float, 4>(part + s * pitch + row * dim + d, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += y[e];
+  }
+  const int64_t bh = row / tokens, token = row % tokens;
+  store_pack<T, 4>(out + bh / heads * s0 + bh % heads * s1 + token * s2 + d, x);
+}
+
+// Parts that a walk of `steps` tiles is dealt to, for `groups` workgroups without: enough of them for the 256 CUs,
+// at least four tiles each.
+int splits_for(int64_t groups, int64_t steps) {
+  if (groups >= 256 || groups == 0) return 1;
+  return (int)std::max<int64_t>(1, std::min(ceil_div(512, groups), steps / 4));
+}
+
+struct Space {
+  int query_splits, key_splits, pitch;
+  int64_t top, delta, lse2, parts, turned, part, total;
+};
+Space space_of(const sdk_bucket_attention* a) {
+  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  Space w;
+  const int64_t tile = 32 * (a->dtype == SDK_F32 ? kParts<float> : kParts<bf16>), rows = 32 * kWaves;
+  const int64_t q_rows = a->batch * a->heads * a->queries, k_rows = a->batch * a->key_heads * a->keys;
+  const int64_t q_groups = a->batch * a->heads * ceil_div(a->queries, rows);
+  w.query_splits = splits_for(q_groups, ceil_div(a->keys, tile));
+  w.key_splits = splits_for(a->batch * a->key_heads * ceil_div(a->keys, rows),
+                            a->heads / a->key_heads * ceil_div(a->queries, tile));
+  w.pitch = (int)ceil_div(a->queries, 64) * 64;
+  w.top = 0;
+  w.delta = 256;
+  w.lse2 = w.delta + up(q_rows * 4);
+  w.parts = w.lse2 + up(q_rows * 4);
+  w.turned = w.parts + up(q_groups * w.query_splits * a->buckets * 4);
+  w.part = w.turned + up((a->map_strides[0] ? a->batch : 1) * a->keys * w.pitch);
+  // the parts of dq, then those of dk and dv, lie in the same place
+  const int64_t q_part = w.query_splits > 1 ? w.query_splits * q_rows : 0;
+  const int64_t k_part = w.key_splits > 1 ? w.key_splits * 2 * k_rows : 0;
+  w.total = w.part + up(std::max(q_part, k_part) * a->dim * 4);
+  return w;
+}
+
+template <typename T, int DP, int COLUMNS>
+int launch_grad_queries(const Attention& d, const Space& w, char* ws, hipStream_t s) {
+  const size_t smem = (size_t)kWaves * (d.buckets + 1) * COLUMNS * sizeof(float);
+  const int tiles = (int)ceil_div(d.queries, 32 * kWaves);
+  auto* kernel = grad_queries<T, DP, COLUMNS>;
+  if (smem > (32 << 10)) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != hipSuccess) return fail(SDK_ERR_DEVICE, "LDS of %zu bytes: %s", smem, hipGetErrorString(e));
+  }
+  kernel<<<dim3((unsigned)tiles * (unsigned)(d.batch * d.heads) * w.query_splits), dim3(kThreads), smem, s>>>(
+      d, w.query_splits, tiles, (const float*)(ws + w.delta), (const float*)(ws + w.lse2),
+      (const unsigned*)(ws + w.top), (float*)(ws + w.part), (float*)(ws + w.parts));
+  return SDK_OK;
+}
+
+template <typename T>
+void launch_join(const Attention& d, const float* part, int64_t pitch, int splits, void* out, const int64_t (&st)[3],
+                 int tokens, int heads, hipStream_t s) {
+  const int64_t rows = (int64_t)d.batch * heads * tokens;
+  launch(join_splits<T>, dim3((unsigned)ceil_div(rows * (d.dim / 4), 256)), dim3(256), s, part, pitch, splits, (T*)out,
+         st[0], st[1], st[2], rows, tokens, heads, d.dim);
+}
+
+template <typename T>
+int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t s) {
+  const Space w = space_of(a);
+  const bool any = a->batch > 0 && a->queries > 0;
+  const int64_t rows = a->batch * a->heads * a->queries;
+  float *delta = (float*)(ws + w.delta), *lse2 = (float*)(ws + w.lse2), *part = (float*)(ws + w.part);
+  unsigned* top = (unsigned*)(ws + w.top);
+  const int columns = !a->grad_table ? 0 : a->buckets <= 64 ? 64 : a->buckets <= 128 ? 32 : 16;
+  if (any) {
+    constexpr int LANES = 128 / kWide<T>;
+    if (__is_same(T, f16)) launch(clear_word, dim3(1), dim3(1), s, top);
+    // few workgroups where each ends with an atomic: 16384 of them took 190 us
+    const int64_t groups = std::min<int64_t>(ceil_div(rows, 256 / LANES), __is_same(T, f16) ? 1024 : 1 << 30);
+    launch(row_terms<T, LANES>, dim3((unsigned)groups), dim3(256), s, d, delta, lse2, top);
+    if (a->grad_query || a->grad_table) {
+      int rc = SDK_OK;
+      ATTENTION_DIM(a->dim, rc = columns == 0    ? launch_grad_queries<T, DP, 0>(d, w, ws, s)
+                                 : columns == 64 ? launch_grad_queries<T, DP, 64>(d, w, ws, s)
+                                 : columns == 32 ? launch_grad_queries<T, DP, 32>(d, w, ws, s)
+                                                 : launch_grad_queries<T, DP, 16>(d, w, ws, s));
+      if (rc != SDK_OK) return rc;
+      if (w.query_splits > 1 && a->grad_query)
+        launch_join<T>(d, part, rows * a->dim, w.query_splits, d.dq, d.dqs, d.queries, d.heads, s);
+    }
+  }
+  if (a->grad_table)
+    launch(join_table<T>, dim3((unsigned)(a->heads * a->buckets)), dim3(256), s, d,
+           any ? (int)ceil_div(a->queries, 32 * kWaves) * w.query_splits : 0, (const float*)(ws + w.parts));
+  if ((a->grad_key || a->grad_value) && a->batch > 0 && a->keys > 0) {
+    uint8_t* turned = (uint8_t*)(ws + w.turned);
+    const int tiles = (int)ceil_div(a->keys, 32 * kWaves);
+    if (any)
+      launch(turn_map, dim3((unsigned)(w.pitch / 64 * ceil_div(a->keys, 64)), (unsigned)(a->map_strides[0] ? a->batch : 1)),
+             dim3(256), s, d, turned, w.pitch);
+    ATTENTION_DIM(a->dim, launch(grad_keys<T, DP>, dim3((unsigned)(tiles * a->batch * a->key_heads) * w.key_splits),
+                                 dim3(kThreads), s, d, w.key_splits, tiles, (const float*)delta, (const float*)lse2,
+                                 (const unsigned*)top, (const uint8_t*)turned, w.pitch, part));
+    if (w.key_splits > 1) {
+      const int64_t values = a->batch * a->key_heads * a->keys * a->dim;
+      if (a->grad_key) launch_join<T>(d, part, 2 * values, w.key_splits, d.dk, d.dks, d.keys, d.key_heads, s);
+      if (a->grad_value)
+        launch_join<T>(d, part + values, 2 * values, w.key_splits, d.dv, d.dvs, d.keys, d.key_heads, s);
+    }
+  }
+  SDK_LAUNCH_CHECK("bucket_attention_backward");
+  return SDK_OK;
+}
+
+}  // namespace
+
+size_t backward_bytes(const sdk_bucket_attention* a) { return (size_t)space_of(a).total; }
+
+int run_backward(const sdk_bucket_attention* a, void* workspace, hipStream_t s) {
+  const Attention d = on_device(a);
+  SDK_DISPATCH_TOKEN_DTYPE(a->dtype, return run<T>(a, d, (char*)workspace, s));
+}
+
+}  // namespace token
+}  // namespace sdk

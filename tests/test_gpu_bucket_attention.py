@@ -165,6 +165,19 @@ def test_biases_that_mask(lowest):
     _close(out, want, TOL[torch.float32])
 
 
+@pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** 12])
+def test_small_and_large_gradients_of_float16(size):
+    """Gradients as a loss scale leaves them: weights of 1 / 600 times gradients of 2^-12 lie far below float16's
+    normal numbers, and times 2^12 near its largest.  Results that fall below 2^-14 are rounded to 2^-25."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 4, 2, 300, 600, 64, 20, torch.float16, seed=7)
+    do = do * size
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    grads = torch.autograd.grad(F.bucket_attention(*leaves, bmap), leaves, do)
+    for got, ref in zip(grads, _exact(q, k, v, table, bmap, grad=do)[1:]):
+        assert float((got.double().cpu() - ref).abs().max()) <= TOL[torch.float16] * float(ref.abs().max()) + 2.0 ** -25
+
+
 def test_bias_table_of_the_queries_type_and_scale():
     from spherical_distortion import functional as F
     q, k, v, table, bmap, do = _inputs(2, 4, 2, 90, 110, 64, 30, torch.bfloat16, seed=6)
