@@ -258,6 +258,7 @@ struct Buckets {
   __device__ __forceinline__ void load(const uint8_t* row, int left) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = 0;
+#pragma unroll 1
     for (int i = 0; i < 16 && i < left; ++i) {
       const unsigned x = (unsigned)row[i] << (8 * (i % 4));
 #pragma unroll
@@ -399,6 +400,10 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+
+// Waits for every load so far.  Before a loop: the compiler, which cannot tell a first step from a later one, would
+// otherwise wait in each step for what the loop uses of before it, and with it for the step's own requests.
+__device__ __forceinline__ void landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0) alone
 
 // Where split `split` of `splits` begins among `tiles`.
 __device__ __forceinline__ int split_at(int tiles, int split, int splits) {

@@ -169,21 +169,22 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
   clear(dq);
 
   Carry<T, DP, NT, kThreads> next_k(a.ks[2], a.dim), next_v(a.vs[2], a.dim);
-  Buckets bucket[NT];
+  Buckets bucket[NT], next_bucket[NT];
   auto request = [&](int k0) {
     next_k.load(kp + k0 * a.ks[2], a.ks[2], to - k0, a.dim);
     next_v.load(vp + k0 * a.vs[2], a.vs[2], to - k0, a.dim);
+    load_buckets<NT>(next_bucket, map, k0, a.keys, h);
   };
   const auto key_view = keys.view(lane), value_view = values.view(lane);
-  if (from < to) {
-    request(from);
-    load_buckets<NT>(bucket, map, from, a.keys, h);
-  }
+  if (from < to) request(from);
+  landed();
   for (int k0 = from; k0 < to; k0 += KEYS) {
     __syncthreads();
     next_k.store(keys);
     next_v.store(values);
     __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) bucket[t] = next_bucket[t];
     if (k0 + KEYS < to) request(k0 + KEYS);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -211,7 +212,6 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
         for (int d = 0; d < DP / 32; ++d) dq[d] = product(key_view.columns(t, half, d), w, dq[d]);
       }
     }
-    if (k0 + KEYS < to) load_buckets<NT>(bucket, map, k0 + KEYS, a.keys, h);
   }
   const float back = exp2f(-kLift<T>) / held;
   if (in && splits > 1)
@@ -296,12 +296,15 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(
   const int seen = a.causal ? key - shift : 0;   // this lane's first query
 
   Carry<T, DP, NT, kThreads> next_q(a.qs[2], a.dim), next_g(a.gs[2], a.dim);
-  Buckets bucket[NT];
+  Buckets bucket[NT], next_bucket[NT];
   float next_lse = 0.f, next_delta = 0.f;
   auto request = [&](int unit) {
     const int head = shared_head * group + unit / each, q0 = from + unit % each * ROWS;
     next_q.load((const T*)a.q + b * a.qs[0] + head * a.qs[1] + q0 * a.qs[2], a.qs[2], a.queries - q0, a.dim);
     next_g.load((const T*)a.grad + b * a.gs[0] + head * a.gs[1] + q0 * a.gs[2], a.gs[2], a.queries - q0, a.dim);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)   // rows of the turned map are padded to whole tiles
+      next_bucket[t].load(map + q0 + 16 * NT * h + 16 * t);
     if (threadIdx.x < ROWS) {
       const int q = q0 + threadIdx.x;
       const int64_t row = ((int64_t)b * a.heads + head) * a.queries + q;
@@ -321,21 +324,19 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(
   auto put_bias = [&](int unit) {
     table[threadIdx.x] = a.bias(shared_head * group + unit / each, threadIdx.x, __is_same(T, bf16));
   };
-  auto buckets_of = [&](int unit) {   // rows of the turned map are padded to whole tiles
-#pragma unroll
-    for (int t = 0; t < NT; ++t) bucket[t].load(map + from + unit % each * ROWS + 16 * NT * h + 16 * t);
-  };
   if (begin < stop) {
     request(begin);
-    buckets_of(begin);
     put(0);
     put_bias(begin);
   }
+  landed();
   __syncthreads();
   for (int unit = begin; unit < stop; ++unit) {
     const int now = (unit - begin) % 2, q0 = from + unit % each * ROWS;
     const bool more = unit + 1 < stop;
-    if (more) request(unit + 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) bucket[t] = next_bucket[t];
+    if (more) request(unit + 1);   // everything in it has landed by `put`: until then no load is waited for
     const auto query_view = queries[now].view(lane), grad_view = grads[now].view(lane);
     const float *now_lse = row_lse[now] + 16 * NT * h, *now_delta = row_delta[now] + 16 * NT * h;
 #pragma unroll
@@ -363,7 +364,6 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(
         }
       }
     }
-    if (more) buckets_of(unit + 1);
     if (more) put(1 - now);
     __syncthreads();
     if (more && (unit + 1) % each == 0) {   // the next tile is another head's

@@ -53,19 +53,20 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
   float level = -INFINITY, off = 0.f, sum = 0.f;
 
   Carry<T, DP, NT, kThreads> next_k(a.ks[2], a.dim), next_v(a.vs[2], a.dim);
-  Buckets bucket[NT];
+  Buckets bucket[NT], next_bucket[NT];
   auto request = [&](int k0) {
     next_k.load(kp + k0 * a.ks[2], a.ks[2], to - k0, a.dim);
     next_v.load(vp + k0 * a.vs[2], a.vs[2], to - k0, a.dim);
+    load_buckets<NT>(next_bucket, map, k0, a.keys, h);
   };
   if (from < to) {
     request(from);
-    load_buckets<NT>(bucket, map, from, a.keys, h);
     if (BUFFERS == 2) {
       next_k.store(keys[0]);
       next_v.store(values[0]);
     }
   }
+  landed();
   if (BUFFERS == 2) __syncthreads();
   int now_in = 0;
   for (int k0 = from; k0 < to; k0 += KEYS) {
@@ -77,12 +78,13 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
     }
     const auto key_view = keys[now_in].view(lane), value_view = values[now_in].view(lane);
     const bool more = k0 + KEYS < to;
-    if (more) request(k0 + KEYS);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) bucket[t] = next_bucket[t];
+    if (more) request(k0 + KEYS);   // with two buffers it has landed when it is stored: until then no load is waited for
     floatx16 s[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
       s[t] = dot_tile<T, DP>(key_view, t, q, [&](int v) { return table[bucket[t][v]]; });
-    if (more) load_buckets<NT>(bucket, map, k0 + KEYS, a.keys, h);
     if (k0 + KEYS > last + 1) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
