@@ -32,6 +32,17 @@ __device__ __forceinline__ float gradient_scale(const unsigned* top) {
   return exponent == 0 || exponent >= 255 ? 1.f : __uint_as_float((247 - exponent) << 23);
 }
 
+template <typename T>
+__device__ __forceinline__ void flip(Operand<T>& x, bool odd) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) flip(x.piece[i], odd);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.u[i] ^= odd ? 0x80008000u : 0u;
+  }
+}
+
 // ------------------------------------------------------------------------------------------ terms of a row
 __global__ void clear_word(unsigned* word) { *word = 0; }
 
@@ -151,7 +162,8 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
   const int last = a.causal ? std::min(len - 1, clamped + shift) : len - 1;
   const bool in = query < a.queries;
   const float held = gradient_scale<T>(top);
-  const float my_lse = in ? lse2[row] - kLift<T> : INFINITY, my_delta = in ? delta[row] * held : 0.f;
+  const float my_lse = in ? lse2[row] - kLift<T> : INFINITY;
+  float my_delta = in ? delta[row] * held : 0.f;
 
   Operand<T> q[DP / 16], g[DP / 16];
   load_columns<T, DP>(q, (const T*)a.q + b * a.qs[0] + head * a.qs[1], a.qs[2], query, in, a.dim, lane);
@@ -165,6 +177,12 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
       g[c] = __builtin_bit_cast(Operand<T>, x);
     }
   }
+  // Odd lanes work with -do and -D, so that ds has the other sign: what the matrix unit's rounding leaves to one side
+  // would add up in the table's sums, which cancel over many rows.  A lane's row and column are all of one sign.
+  const float sign = lane % 2 ? -1.f : 1.f;
+  my_delta *= sign;
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) flip(g[c], lane % 2);
   floatx16 dq[DP / 32];
   clear(dq);
 
@@ -205,27 +223,27 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
           if (COLUMNS < 64) wave_order();   // the next turn's lanes read what these wrote
         }
       }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const Operand<T> w = rounded<T>(ds + 8 * half);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) dq[d] = product(key_view.columns(t, half, d), w, dq[d]);
-      }
+      const Operand<T> w[2] = {rounded<T>(ds), rounded<T>(ds + 8)};
+      add_columns<T>(dq, key_view, t, w);
     }
   }
   const float back = exp2f(-kLift<T>) / held;
   if (in && splits > 1)
     store_columns<float, DP>(part + ((int64_t)work.split * a.batch * a.heads * a.queries + row) * a.dim, a.dim, 0, a.dim,
-                             lane, dq, a.scale * back);
+                             lane, dq, a.scale * back * sign);
   else if (in && a.dq)
-    store_columns<T, DP>((T*)a.dq + b * a.dqs[0] + head * a.dqs[1], a.dqs[2], query, a.dim, lane, dq, a.scale * back);
+    store_columns<T, DP>((T*)a.dq + b * a.dqs[0] + head * a.dqs[1], a.dqs[2], query, a.dim, lane, dq,
+                         a.scale * back * sign);
   if constexpr (COLUMNS > 0) {
     __syncthreads();
     for (int i = threadIdx.x; i < a.buckets; i += kThreads) {
       float x = 0.f;
       for (int w = 0; w < kWaves; ++w)
-        for (int c = 0; c < COLUMNS; ++c)   // begun at the bucket's own column: other banks for other lanes
-          x += sums[(w * (a.buckets + 1) + i) * COLUMNS + (c + i) % COLUMNS];
+        for (int c = 0; c < COLUMNS; ++c) {   // begun at the bucket's own column: other banks for other lanes
+          const int column = (c + i) % COLUMNS;
+          const float y = sums[(w * (a.buckets + 1) + i) * COLUMNS + column];
+          x += column % 2 ? -y : y;
+        }
       table_parts[(((int64_t)work.head * tiles + work.tile) * splits + work.split) * a.buckets + i] = x * back;
     }
   }
@@ -348,21 +366,17 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(
         for (int i = 0; i < 16; ++i)
           if (q0 + 16 * NT * h + 16 * t + i < seen) s[i] = -INFINITY;
       }
-      float p[16], ds[16];
+      float p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, now_lse[16 * t + i]));
-        ds[i] = p[i] * e[i];
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, now_lse[16 * t + i]));
+      {
+        const Operand<T> w[2] = {rounded<T>(p), rounded<T>(p + 8)};
+        add_columns<T>(dv, grad_view, t, w);
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const Operand<T> w = rounded<T>(p + 8 * half), x = rounded<T>(ds + 8 * half);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          dv[d] = product(grad_view.columns(t, half, d), w, dv[d]);
-          dk[d] = product(query_view.columns(t, half, d), x, dk[d]);
-        }
-      }
+      for (int i = 0; i < 16; ++i) p[i] *= e[i];   // ds
+      const Operand<T> w[2] = {rounded<T>(p), rounded<T>(p + 8)};
+      add_columns<T>(dk, query_view, t, w);
     }
     if (more) put(1 - now);
     __syncthreads();

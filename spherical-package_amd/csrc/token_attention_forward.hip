@@ -110,17 +110,18 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
         for (int v = 0; v < 16; ++v) o[d][v] *= by;
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+      Operand<T> w[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * half + i], a.scale2, -off));
-        const Operand<T> w = rounded<T>(p);
-        sum = add_weights<T>(w, p, sum);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) o[d] = product(value_view.columns(t, half, d), w, o[d]);
+        w[half] = rounded<T>(p);
+        sum = add_weights<T>(w[half], p, sum);
       }
+      add_columns<T>(o, value_view, t, w);
+    }
     if (BUFFERS == 2) {
       now_in ^= 1;
       if (more) {
@@ -258,12 +259,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
       sum += p[v];
     }
     wave_order();
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const Operand<T> w = rounded<T>(p + 8 * half);
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d) o[d] = product(value_view.columns(0, half, d), w, o[d]);
-    }
+    const Operand<T> w[2] = {rounded<T>(p), rounded<T>(p + 8)};
+    add_columns<T>(o, value_view, 0, w);
     wave_order();
   }
   sum += other_half(sum);
