@@ -100,27 +100,18 @@ __global__ __launch_bounds__(256) void turn_map(const Attention a, uint8_t* turn
 }
 
 // ------------------------------------------------------------------------------------------ dq and the bias table
-// Adds x to the sums of its buckets in one lane's column, four at a time: read, add, write, and where two of the
-// four meet the second takes the first's sum.  (An LDS float add of 64 lanes takes 193 cycles of a CU whatever its
-// addresses, this 13.)
+// Adds x to the sums of its buckets in one lane's column, two at a time: read, add, write, and where the two meet the
+// second takes the first's sum.  (An LDS float add of 64 lanes takes 193 cycles of a CU whatever its addresses, this
+// 13; by four or eight the comparisons cost more than the waits they save: 842 and 971 us of the kernel at 8192 x
+// 8192 pairs of 16 heads, 817 by two.)
 template <int COLUMNS>
 __device__ __forceinline__ void add_by_bucket(float* column, const Buckets& bucket, int buckets, const float* x) {
 #pragma unroll
-  for (int v = 0; v < 16; v += 4) {
-    int at[4];
-    float sum[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) at[i] = std::min((int)bucket[v + i], buckets) * COLUMNS;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = column[at[i]];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum[i] += x[v + i];
-#pragma unroll
-      for (int j = i + 1; j < 4; ++j) sum[j] = at[j] == at[i] ? sum[i] : sum[j];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) column[at[i]] = sum[i];
+  for (int v = 0; v < 16; v += 2) {
+    const int at = std::min((int)bucket[v], buckets) * COLUMNS, next = std::min((int)bucket[v + 1], buckets) * COLUMNS;
+    const float sum = column[at] + x[v], other = column[next];
+    column[at] = sum;
+    column[next] = (next == at ? sum : other) + x[v + 1];
   }
 }
 
@@ -203,7 +194,7 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < NT; ++t) bucket[t] = next_bucket[t];
-    if (k0 + KEYS < to) request(k0 + KEYS);
+    request(k0 + KEYS);   // beyond the last tile nothing is read
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       floatx16 s = dot_tile<T, DP>(key_view, t, q, [&](int v) { return table[bucket[t][v]]; });
@@ -424,11 +415,13 @@ __global__ __launch_bounds__(256) void join_splits(const float* part, int64_t pi
   store_pack<T, 4>(out + bh / heads * s0 + bh % heads * s1 + token * s2 + d, x);
 }
 
-// Parts that a walk of `steps` tiles is dealt to, for `groups` workgroups without: enough of them for the 256 CUs,
-// at least four tiles each.
-int splits_for(int64_t groups, int64_t steps) {
-  if (groups >= 256 || groups == 0) return 1;
-  return (int)std::max<int64_t>(1, std::min(ceil_div(512, groups), steps / 4));
+// Parts that a walk of `steps` tiles is dealt to, for `groups` workgroups without: two workgroups a CU, in causal
+// calls, whose tiles differ in work, four; at least four tiles each.  (256 workgroups of dk and dv, 8192 x 8192 pairs
+// of 16 heads: 967 us as they are, 640 as two parts each and a join.)
+int splits_for(int64_t groups, int64_t steps, bool causal) {
+  const int64_t wanted = causal ? 1024 : 512;
+  if (groups >= wanted || groups == 0) return 1;
+  return (int)std::max<int64_t>(1, std::min(ceil_div(wanted, groups), steps / 4));
 }
 
 struct Space {
@@ -441,9 +434,9 @@ Space space_of(const sdk_bucket_attention* a) {
   const int64_t tile = 32 * (a->dtype == SDK_F32 ? kParts<float> : kParts<bf16>), rows = 32 * kWaves;
   const int64_t q_rows = a->batch * a->heads * a->queries, k_rows = a->batch * a->key_heads * a->keys;
   const int64_t q_groups = a->batch * a->heads * ceil_div(a->queries, rows);
-  w.query_splits = splits_for(q_groups, ceil_div(a->keys, tile));
+  w.query_splits = splits_for(q_groups, ceil_div(a->keys, tile), a->causal);
   w.key_splits = splits_for(a->batch * a->key_heads * ceil_div(a->keys, rows),
-                            a->heads / a->key_heads * ceil_div(a->queries, tile));
+                            a->heads / a->key_heads * ceil_div(a->queries, tile), a->causal);
   w.pitch = (int)ceil_div(a->queries, 64) * 64;
   w.top = 0;
   w.delta = 256;

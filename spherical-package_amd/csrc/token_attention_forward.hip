@@ -69,6 +69,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
   landed();
   if (BUFFERS == 2) __syncthreads();
   int now_in = 0;
+  bool first_tile = true;
   for (int k0 = from; k0 < to; k0 += KEYS) {
     if (BUFFERS == 1) {
       __syncthreads();
@@ -77,10 +78,11 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
       __syncthreads();
     }
     const auto key_view = keys[now_in].view(lane), value_view = values[now_in].view(lane);
-    const bool more = k0 + KEYS < to;
 #pragma unroll
     for (int t = 0; t < NT; ++t) bucket[t] = next_bucket[t];
-    if (more) request(k0 + KEYS);   // with two buffers it has landed when it is stored: until then no load is waited for
+    // Beyond the last tile nothing is read.  With two buffers it has landed when it is stored: until then no load is
+    // waited for.
+    request(k0 + KEYS);
     floatx16 s[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -92,42 +94,49 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
         for (int v = 0; v < 16; ++v)
           if (k0 + 16 * NT * h + 16 * t + v > last) s[t][v] = -INFINITY;
     }
-    float top = s[0][0];
+    // The weights against the level so far.  It is raised only where they would pass 2^14 in sum (and by the first
+    // tile), so that most tiles need no maximum.
+    Operand<T> w[NT][2];
+    float with = sum;
+    auto weigh = [&] {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) top = fmaxf(top, s[t][v]);
-    top = max_halves(top);
-    if (__any((top - level) * a.scale2 > kBehind || (level == -INFINITY && top > level))) {
-      const float grown = fmaxf(top, level);
+        for (int half = 0; half < 2; ++half) {
+          float p[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * half + i], a.scale2, -off));
+          w[t][half] = rounded<T>(p);
+          with = add_weights<T>(w[t][half], p, with);
+        }
+    };
+    if (!first_tile) weigh();
+    if (first_tile || __any(with - sum > 0x1p14f)) {
+      float top = s[0][0];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) top = fmaxf(top, s[t][v]);
+      const float grown = fmaxf(max_halves(top), level);
       const float by = grown == -INFINITY ? 1.f : exp2f((level - grown) * a.scale2);
       level = grown;
       off = grown == -INFINITY ? 0.f : grown * a.scale2;
+      first_tile = __any(grown == -INFINITY);   // a query without pairs so far has no level yet
       sum *= by;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[d][v] *= by;
+      with = sum;
+      weigh();
     }
+    sum = with;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      Operand<T> w[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * half + i], a.scale2, -off));
-        w[half] = rounded<T>(p);
-        sum = add_weights<T>(w[half], p, sum);
-      }
-      add_columns<T>(o, value_view, t, w);
-    }
+    for (int t = 0; t < NT; ++t) add_columns<T>(o, value_view, t, w[t]);
     if (BUFFERS == 2) {
       now_in ^= 1;
-      if (more) {
-        next_k.store(keys[now_in]);
-        next_v.store(values[now_in]);
-      }
+      next_k.store(keys[now_in]);
+      next_v.store(values[now_in]);
       __syncthreads();
     }
   }
@@ -342,11 +351,11 @@ __global__ __launch_bounds__(256) void join(const Attention a, int splits, const
 
 bool few_rows(const sdk_bucket_attention* a) { return a->heads / a->key_heads * a->queries <= 32; }
 
-// Parts that the keys are dealt to: enough workgroups for the 256 CUs, at least 256 keys each.
+// Parts that the keys are dealt to: two workgroups for each of the 256 CUs, at least 256 keys each.
 int forward_splits(const sdk_bucket_attention* a) {
   const bool few = few_rows(a);
   const int64_t groups = few ? a->batch * a->key_heads : a->batch * a->heads * ceil_div(a->queries, 32 * kWaves);
-  if (groups >= (few ? 512 : 256) || groups == 0) return 1;
+  if (groups >= 512 || groups == 0) return 1;
   return (int)std::max<int64_t>(1, std::min(ceil_div(512, groups), a->keys / 256));
 }
 
