@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
   const auto key_view = keys.view(lane), value_view = values.view(lane);
   if (from < to) request(from);
   landed();
-  for (int k0 = from; k0 < to; k0 += KEYS) {
+  auto step = [&](int k0, auto edge) {   // edge: some key may be beyond a lane's last
     __syncthreads();
     next_k.store(keys);
     next_v.store(values);
@@ -199,11 +199,12 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
     for (int t = 0; t < NT; ++t) {
       floatx16 s = dot_tile<T, DP>(key_view, t, q, [&](int v) { return table[bucket[t][v]]; });
       const floatx16 e = dot_tile<T, DP>(value_view, t, g, [&](int) { return -my_delta; });
-      if (k0 + KEYS > last + 1) {
+      if constexpr (edge)
+        if (k0 + KEYS > last + 1) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (k0 + 16 * NT * h + 16 * t + v > last) s[v] = -INFINITY;
-      }
+          for (int v = 0; v < 16; ++v)
+            if (k0 + 16 * NT * h + 16 * t + v > last) s[v] = -INFINITY;
+        }
       float ds[16];
 #pragma unroll
       for (int v = 0; v < 16; ++v) ds[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -my_lse)) * e[v];
@@ -217,7 +218,13 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
       const Operand<T> w[2] = {rounded<T>(ds), rounded<T>(ds + 8)};
       add_columns<T>(dq, key_view, t, w);
     }
-  }
+  };
+  // whole tiles that every query of the workgroup sees, in a loop without branches
+  const int whole = (a.causal ? std::max(0, std::min(len, first + shift + 1)) : len) / KEYS * KEYS;
+  int k0 = from;
+  if constexpr (sizeof(T) == 2)   // float32: the registers do not hold two loops (170 us for 149 with one)
+    for (; k0 < std::min(to, whole); k0 += KEYS) step(k0, std::false_type());
+  for (; k0 < to; k0 += KEYS) step(k0, std::true_type());
   const float back = exp2f(-kLift<T>) / held;
   if (in && splits > 1)
     store_columns<float, DP>(part + ((int64_t)work.split * a.batch * a.heads * a.queries + row) * a.dim, a.dim, 0, a.dim,
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(256) void join_table(const Attention a, int each, c
 // tiles): S = Q K^T has the keys in columns.  The next tile is requested while this one is worked on, into the
 // other buffer.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 32 ? 1 : kBackwardWaves<DP>) void grad_keys(
     const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top,
     const uint8_t* turned, int pitch, float* part) {
   constexpr int NT = kParts<T>, ROWS = 32 * NT;
@@ -345,7 +352,7 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_keys(
     const bool more = unit + 1 < stop;
 #pragma unroll
     for (int t = 0; t < NT; ++t) bucket[t] = next_bucket[t];
-    if (more) request(unit + 1);   // everything in it has landed by `put`: until then no load is waited for
+    request(more ? unit + 1 : unit);   // it has landed by `put`: until then no load is waited for
     const auto query_view = queries[now].view(lane), grad_view = grads[now].view(lane);
     const float *now_lse = row_lse[now] + 16 * NT * h, *now_delta = row_delta[now] + 16 * NT * h;
 #pragma unroll
@@ -415,11 +422,10 @@ __global__ __launch_bounds__(256) void join_splits(const float* part, int64_t pi
   store_pack<T, 4>(out + bh / heads * s0 + bh % heads * s1 + token * s2 + d, x);
 }
 
-// Parts that a walk of `steps` tiles is dealt to, for `groups` workgroups without: two workgroups a CU, in causal
-// calls, whose tiles differ in work, four; at least four tiles each.  (256 workgroups of dk and dv, 8192 x 8192 pairs
-// of 16 heads: 967 us as they are, 640 as two parts each and a join.)
-int splits_for(int64_t groups, int64_t steps, bool causal) {
-  const int64_t wanted = causal ? 1024 : 512;
+// Parts that a walk of `steps` tiles is dealt to, for `groups` workgroups without: two workgroups a CU, for the keys of
+// causal calls, whose tiles differ most, four; at least four tiles each.  (256 workgroups of dk and dv, 8192 x 8192 pairs
+// of 16 heads: 967 us as they are, 730 as two parts each and a join.)
+int splits_for(int64_t groups, int64_t steps, int64_t wanted) {
   if (groups >= wanted || groups == 0) return 1;
   return (int)std::max<int64_t>(1, std::min(ceil_div(wanted, groups), steps / 4));
 }
@@ -434,9 +440,9 @@ Space space_of(const sdk_bucket_attention* a) {
   const int64_t tile = 32 * (a->dtype == SDK_F32 ? kParts<float> : kParts<bf16>), rows = 32 * kWaves;
   const int64_t q_rows = a->batch * a->heads * a->queries, k_rows = a->batch * a->key_heads * a->keys;
   const int64_t q_groups = a->batch * a->heads * ceil_div(a->queries, rows);
-  w.query_splits = splits_for(q_groups, ceil_div(a->keys, tile), a->causal);
+  w.query_splits = splits_for(q_groups, ceil_div(a->keys, tile), 512);
   w.key_splits = splits_for(a->batch * a->key_heads * ceil_div(a->keys, rows),
-                            a->heads / a->key_heads * ceil_div(a->queries, tile), a->causal);
+                            a->heads / a->key_heads * ceil_div(a->queries, tile), a->causal ? 1024 : 512);
   w.pitch = (int)ceil_div(a->queries, 64) * 64;
   w.top = 0;
   w.delta = 256;
