@@ -88,8 +88,9 @@ using namespace sdk::token;
 extern "C" {
 
 size_t sdk_bucket_attention_workspace_bytes(const sdk_bucket_attention* a, int32_t backward) {
-  if (check(a) != SDK_OK || a->batch == 0 || a->queries == 0) return 0;
+  if (check(a) != SDK_OK || a->batch == 0) return 0;
   if (backward) return backward_bytes(a);
+  if (a->queries == 0) return 0;
   const int splits = forward_splits(a);
   return splits == 1 ? 0 : (size_t)splits * a->batch * a->heads * a->queries * (a->dim + 1) * sizeof(float);
 }

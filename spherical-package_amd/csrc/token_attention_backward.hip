@@ -489,9 +489,10 @@ int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t
   float *delta = (float*)(ws + w.delta), *lse2 = (float*)(ws + w.lse2), *part = (float*)(ws + w.part);
   unsigned* top = (unsigned*)(ws + w.top);
   const int columns = !a->grad_table ? 0 : a->buckets <= 64 ? 64 : a->buckets <= 128 ? 32 : 16;
+  // read by every kernel of float16 gradients, queries or not
+  if (__is_same(T, f16) && a->batch > 0) launch(clear_word, dim3(1), dim3(1), s, top);
   if (any) {
     constexpr int LANES = 128 / kWide<T>;
-    if (__is_same(T, f16)) launch(clear_word, dim3(1), dim3(1), s, top);
     // few workgroups where each ends with an atomic: 16384 of them took 190 us
     const int64_t groups = std::min<int64_t>(ceil_div(rows, 256 / LANES), __is_same(T, f16) ? 1024 : 1 << 30);
     launch(row_terms<T, LANES>, dim3((unsigned)groups), dim3(256), s, d, delta, lse2, top);

@@ -237,19 +237,37 @@ __global__ __launch_bounds__(1024) void norm_weight_grad(const float* parts, int
   }
 }
 
-// out = codes * scale of the row, a chunk of V codes a thread.
-template <typename T, int V>
-__global__ __launch_bounds__(256) void dequantize(const unsigned char* codes, const float* scales, T* out,
-                                                  int64_t chunks, int per_row, int fp8) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= chunks) return;
-  const float s = scales[c / per_row];
-  const Pack<unsigned char, V> q = reinterpret_cast<const Pack<unsigned char, V>*>(codes)[c];
-  float f[V];
+// out = codes * scale of the row, eight codes a thread; rows whose width is no multiple of eight end inside a thread's
+// eight.
+template <typename T>
+__global__ __launch_bounds__(256) void dequantize(const unsigned char* codes, const float* scales, T* out, int64_t size,
+                                                  int width, int fp8, int wide) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at >= size) return;
+  int64_t row = at / width;
+  int left = (int)(width - (at - row * width));   // codes of this row from the thread's first on
+  float s = scales[row];
+  auto value = [&](unsigned char c) {
+    return (fp8 ? __builtin_amdgcn_cvt_f32_fp8((int)c, 0) : (float)(signed char)c) * s;
+  };
+  if (wide && at + 8 <= size) {
+    const Pack<unsigned char, 8> q = *reinterpret_cast<const Pack<unsigned char, 8>*>(codes + at);
+    float f[8];
 #pragma unroll
-  for (int e = 0; e < V; ++e)
-    f[e] = (fp8 ? __builtin_amdgcn_cvt_f32_fp8((int)q.v[e], 0) : (float)(signed char)q.v[e]) * s;
-  store_pack<T, V>(out + c * V, f);
+    for (int e = 0; e < 8; ++e) {
+      if (left == 0) s = scales[++row], left = width;
+      f[e] = value(q.v[e]);
+      --left;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += kWide<T>) store_pack<T, kWide<T>>(out + at + e, *reinterpret_cast<float(*)[kWide<T>]>(f + e));
+  } else {
+    for (int e = 0; e < 8 && at + e < size; ++e) {
+      if (left == 0) s = scales[++row], left = width;
+      out[at + e] = (T)value(codes[at + e]);
+      --left;
+    }
+  }
 }
 
 // Threads of a row: at most 16 elements a thread.
@@ -287,7 +305,7 @@ int64_t backward_groups(int64_t rows, int64_t width) {
 }
 
 int check(int64_t rows, int64_t width, int dtype, int weight_dtype) {
-  SDK_REQUIRE(rows >= 0, "rows = %lld must not be negative", (long long)rows);
+  SDK_REQUIRE(rows >= 0 && rows < (int64_t)1 << 31, "rows = %lld must be between 0 and 2^31", (long long)rows);
   SDK_REQUIRE(width >= 1 && width <= kMostWidth, "width = %lld must be between 1 and %lld",
               (long long)width, (long long)kMostWidth);
   SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
@@ -362,7 +380,7 @@ int sdk_add_rms_norm_backward(const void* grad, const void* grad_sum, const void
 
 int sdk_dequantize_rows(const void* codes, const float* scales, void* out, int64_t rows, int64_t width,
                         int32_t codes_kind, int32_t dtype, sdk_stream_t stream) {
-  SDK_REQUIRE(rows >= 0 && width >= 1 && width < (int64_t)1 << 31, "rows %lld of width %lld", (long long)rows,
+  SDK_REQUIRE(rows >= 0 && rows < (int64_t)1 << 31 && width >= 1 && width < (int64_t)1 << 31, "rows %lld of width %lld", (long long)rows,
               (long long)width);
   SDK_REQUIRE(codes_kind == kInt8 || codes_kind == kFp8, "codes = %d must be 1 (int8) or 2 (float8 e4m3)",
               codes_kind);
@@ -370,18 +388,12 @@ int sdk_dequantize_rows(const void* codes, const float* scales, void* out, int64
   if (rows == 0) return SDK_OK;
   SDK_REQUIRE(codes && scales && out, "codes, scales and out must not be NULL");
   hipStream_t s = (hipStream_t)stream;
-  const bool wide = width % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)out & 31) == 0;
-  const int64_t chunks = rows * width / (wide ? 8 : 1);
-  SDK_REQUIRE(ceil_div(chunks, 256) < (int64_t)1 << 31, "%lld rows of width %lld are too many",
-              (long long)rows, (long long)width);
-  SDK_DISPATCH_TOKEN_DTYPE(dtype, {
-    if (wide)
-      launch(dequantize<T, 8>, dim3((unsigned)ceil_div(chunks, 256)), dim3(256), s,
-             (const unsigned char*)codes, scales, (T*)out, chunks, (int)(width / 8), (int)(codes_kind == kFp8));
-    else
-      launch(dequantize<T, 1>, dim3((unsigned)ceil_div(chunks, 256)), dim3(256), s,
-             (const unsigned char*)codes, scales, (T*)out, chunks, (int)width, (int)(codes_kind == kFp8));
-  });
+  const int wide = ((uintptr_t)codes & 7) == 0 && aligned16(out);
+  const int64_t size = rows * width, groups = ceil_div(size, 2048);
+  SDK_REQUIRE(groups < (int64_t)1 << 31, "%lld rows of width %lld are too many", (long long)rows, (long long)width);
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(dequantize<T>, dim3((unsigned)groups), dim3(256), s,
+                                         (const unsigned char*)codes, scales, (T*)out, size, (int)width,
+                                         (int)(codes_kind == kFp8), wide));
   SDK_LAUNCH_CHECK("dequantize_rows");
   return SDK_OK;
 }

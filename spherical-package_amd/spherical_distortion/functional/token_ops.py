@@ -8,6 +8,7 @@ float32, bfloat16 and float16; sums, softmax statistics and norms are float32.
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from _spherical_distortion_ext import _token_ops
 from _spherical_distortion_ext._ops import ops as _sdk_ops
@@ -23,6 +24,7 @@ class BucketAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output):
         query, key, value, bias_table, bucket_map, key_lengths, out, lse = ctx.saved_tensors
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
@@ -66,6 +68,7 @@ class AddRMSNormFunction(torch.autograd.Function):
         return (out, x.view_as(x)) if ctx.alone else (out, summed)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad, grad_sum):
         summed, weight, inverse = ctx.saved_tensors
         need_x, need_r, need_w, _ = ctx.needs_input_grad

@@ -250,10 +250,11 @@ def test_gradients_that_are_not_wanted_and_repeated_runs():
         assert torch.equal(got, full[i])
 
 
-def test_empty_sizes():
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_empty_sizes(dtype):
     from spherical_distortion import functional as F
     for B, Lq, Lk in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
-        q, k, v, table, bmap, do = _inputs(B, 2, 1, Lq, Lk, 16, 3, torch.float32, seed=1)
+        q, k, v, table, bmap, do = _inputs(B, 2, 1, Lq, Lk, 16, 3, dtype, seed=1)
         leaves = [t.requires_grad_() for t in (q, k, v, table)]
         out = F.bucket_attention(*leaves, bmap)
         assert out.shape == (B, 2, Lq, 16) and not bool(out.any())
@@ -282,6 +283,59 @@ def test_another_stream_and_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(captured, F.bucket_attention(q, k, v, table, bmap))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_expanded_keys(dtype):
+    """One key head expanded over all heads, one token expanded over all positions: the bits of the same keys laid
+    out."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(2, 4, 1, 90, 100, 32, 7, dtype, seed=14)
+    for kk in (k.expand(2, 4, 100, 32), k[:, :, :1].expand(2, 1, 100, 32)):
+        vv = v.expand(2, kk.shape[1], 100, 32)
+        results = []
+        for pair in ((kk, vv), (kk.contiguous(), vv.contiguous())):
+            leaves = [t.detach().requires_grad_() for t in (q, *pair, table)]
+            out = F.bucket_attention(*leaves, bmap)
+            results.append((out, *torch.autograd.grad(out, leaves, do)))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradients_in_a_graph(dtype):
+    """Forward and backward captured, replayed with new inputs between eager calls: the same bits."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 4, 2, 150, 170, 64, 30, dtype, seed=15)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+
+    def run():
+        out = F.bucket_attention(*leaves, bmap)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for seed in (30, 31, 32):
+        fresh = _inputs(1, 4, 2, 150, 170, 64, 30, dtype, seed=seed)
+        with torch.no_grad():
+            for old, new in zip((q, k, v, table, bmap, do), fresh):
+                old.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, run()))
+
+
+def test_no_second_derivative():
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 1, 1, 4, 5, 8, 2, torch.float32, seed=1)
+    q.requires_grad_()
+    first, = torch.autograd.grad(F.bucket_attention(q, k, v, table, bmap), [q], do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), [q])
 
 
 def test_refusals():
