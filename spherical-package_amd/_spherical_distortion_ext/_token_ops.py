@@ -314,9 +314,24 @@ def adamw_moment_values(codes, scales, dtype):
     return out
 
 
+# --------------------------------------------------------------------------- forms with gradients
+# Registered with autograd by the compiled layer alone; without it functional/token_ops.py's autograd functions serve.
+def bucket_attention(query, key, value, bias_table, bucket_map, key_lengths, causal, scale):
+    return bucket_attention_forward(query, key, value, bias_table, bucket_map, key_lengths, causal, scale)[0]
+
+
+def rms_norm_pair(x, residual, weight, eps):
+    """-> [norm, x + residual], or [norm] without a residual."""
+    return list(add_rms_norm(x, residual, weight, eps)[:1 if residual is None else 2])
+
+
 # --------------------------------------------------------------------------- registration
 _SETTINGS = " float lr, float beta1, float beta2, float eps, float weight_decay, int step) -> ()"
 _SCHEMAS = (
+    ("bucket_attention",
+     "(Tensor query, Tensor key, Tensor value, Tensor bias_table, Tensor bucket_map, Tensor? key_lengths,"
+     " bool causal, float scale) -> Tensor", bucket_attention),
+    ("rms_norm_pair", "(Tensor x, Tensor? residual, Tensor weight, float eps) -> Tensor[]", rms_norm_pair),
     ("bucket_attention_forward",
      "(Tensor query, Tensor key, Tensor value, Tensor bias_table, Tensor bucket_map, Tensor? key_lengths,"
      " bool causal, float scale) -> (Tensor, Tensor)", bucket_attention_forward),

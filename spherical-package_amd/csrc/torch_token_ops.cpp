@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <cmath>
@@ -339,9 +340,106 @@ Tensor adamw_moment_values(const Tensor& codes, const Tensor& scales, at::Scalar
   return out;
 }
 
+// ------------------------------------------------------------------------------------------ autograd
+// The differentiable forms: what functional/token_ops.py's autograd functions do, without an interpreter in the
+// backward.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+struct BucketAttention : torch::autograd::Function<BucketAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,
+                        const Tensor& map, const OptTensor& lengths, bool causal, double scale) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [out, lse] = bucket_attention_forward(q, k, v, table, map, lengths, causal, scale);
+    ctx->save_for_backward({q, k, v, table, map, has(lengths) ? *lengths : Tensor(), out, lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const OptTensor n = saved[5].defined() ? OptTensor(saved[5]) : OptTensor();
+    const bool need_q = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2),
+               need_t = ctx->needs_input_grad(3);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [dq, dk, dv, dt] = bucket_attention_backward(
+        grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], n, saved[6], saved[7],
+        ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), need_q, need_k || need_v, need_t);
+    return {need_q ? dq : Tensor(), need_k ? dk : Tensor(), need_v ? dv : Tensor(), need_t ? dt : Tensor(),
+            Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor bucket_attention_only(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& map,
+                             const OptTensor& lengths, bool causal, double scale) {
+  return std::get<0>(bucket_attention_forward(q, k, v, table, map, lengths, causal, scale));
+}
+
+Tensor bucket_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,
+                                 const Tensor& map, const OptTensor& lengths, bool causal, double scale) {
+  if (wants_gradient({&q, &k, &v, &table}))
+    return BucketAttention::apply(q, k, v, table, map, lengths, causal, scale);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return bucket_attention_only(q, k, v, table, map, lengths, causal, scale);
+}
+
+struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
+  // x and weight first: gradients are counted over the tensors that are there
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                               double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const bool alone = !has(residual);
+    auto [out, summed, inverse] = add_rms_norm(x, residual, weight, eps);
+    ctx->saved_data["alone"] = alone;
+    ctx->save_for_backward({alone ? x : summed, weight, inverse});
+    ctx->set_materialize_grads(false);
+    return alone ? variable_list{out} : variable_list{out, summed};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool alone = ctx->saved_data["alone"].toBool();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+               need_r = !alone && ctx->needs_input_grad(2);
+    const Tensor sum = grads.size() > 1 ? grads[1] : Tensor();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    if (!grads[0].defined())   // only the sum was used, or nothing
+      return {need_x ? sum : Tensor(), need_w ? at::zeros_like(saved[1]) : Tensor(), need_r ? sum : Tensor(), Tensor()};
+    auto [dx, dw] = add_rms_norm_backward(grads[0].contiguous(), sum.defined() ? OptTensor(sum.contiguous()) : OptTensor(),
+                                          saved[0], saved[1], saved[2], need_x || need_r, need_w);
+    return {need_x ? dx : Tensor(), need_w ? dw : Tensor(), need_r ? dx : Tensor(), Tensor()};
+  }
+};
+
+std::vector<Tensor> rms_norm_pair(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps) {
+  auto [out, summed, inverse] = add_rms_norm(x, residual, weight, eps);
+  return has(residual) ? std::vector<Tensor>{out, summed} : std::vector<Tensor>{out};
+}
+
+std::vector<Tensor> rms_norm_pair_autograd(const Tensor& x, const OptTensor& residual, const Tensor& weight,
+                                           double eps) {
+  if (wants_gradient({&x, &weight}) || (has(residual) && wants_gradient({&*residual})))
+    return AddRmsNorm::apply(x, weight, residual, eps);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rms_norm_pair(x, residual, weight, eps);
+}
+
 }  // namespace
 
+TORCH_LIBRARY_IMPL(sdk_mapped_ops, AutogradCUDA, m) {
+  m.impl("bucket_attention", &bucket_attention_autograd);
+  m.impl("rms_norm_pair", &rms_norm_pair_autograd);
+}
+
 TORCH_LIBRARY_IMPL(sdk_mapped_ops, CUDA, m) {
+  m.impl("bucket_attention", &bucket_attention_only);
+  m.impl("rms_norm_pair", &rms_norm_pair);
   m.impl("bucket_attention_forward", &bucket_attention_forward);
   m.impl("bucket_attention_backward", &bucket_attention_backward);
   m.impl("add_rms_norm", &add_rms_norm);
@@ -355,6 +453,6 @@ TORCH_LIBRARY_IMPL(sdk_mapped_ops, CUDA, m) {
 
 // Names of the operators above, for the Python side (which implements those that are missing here).
 extern "C" const char* sdk_torch_token_ops(void) {
-  return "bucket_attention_forward,bucket_attention_backward,add_rms_norm,add_rms_norm_quantized,"
+  return "bucket_attention,rms_norm_pair,bucket_attention_forward,bucket_attention_backward,add_rms_norm,add_rms_norm_quantized,"
          "add_rms_norm_backward,dequantize_rows,adamw_step,adamw_step_8bit,adamw_moment_values";
 }

@@ -50,6 +50,8 @@ def bucket_attention(query, key, value, bias_table, bucket_map, key_lengths=None
     With gradients for query, key, value and bias_table.  A few queries against many keys (one new
     token and its cache) are dealt to the GPU along the keys."""
     scale = 1.0 / math.sqrt(query.shape[-1]) if scale is None else float(scale)
+    if "bucket_attention" in _token_ops.NATIVE_OPS:
+        return _sdk_ops.bucket_attention(query, key, value, bias_table, bucket_map, key_lengths, bool(causal), scale)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad
                                     or bias_table.requires_grad):
         return BucketAttentionFunction.apply(query, key, value, bias_table, bucket_map, key_lengths, bool(causal),
@@ -84,6 +86,9 @@ def add_rms_norm(input, residual, weight, eps=1e-6):
     """(weight * h / sqrt(mean(h ** 2) + eps), h) with h = input + residual, over the last axis; a
     residual of None adds nothing.  weight: one value for each of the last axis (up to 16384), of the
     input's type or float32.  The sum is normalised before it is rounded to the input's type."""
+    if "rms_norm_pair" in _token_ops.NATIVE_OPS:
+        both = _sdk_ops.rms_norm_pair(input, residual, weight, float(eps))
+        return (both[0], input) if residual is None else (both[0], both[1])
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         return AddRMSNormFunction.apply(input, residual, weight, float(eps))

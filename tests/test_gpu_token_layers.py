@@ -67,6 +67,43 @@ def test_compiled_and_python_operators_agree():
     _both("adamw_moment_values", vc[1], vs[1], torch.float16)
 
 
+def test_compiled_and_python_gradients_agree():
+    """The compiled autograd functions and the Python ones: the same bits, and gradients only where wanted."""
+    from _spherical_distortion_ext import _token_ops
+    from spherical_distortion import functional as F
+    torch.manual_seed(4)
+    q = torch.randn(2, 4, 40, 16, device=DEV)
+    k, v = (torch.randn(2, 2, 50, 16, device=DEV) for _ in range(2))
+    table = torch.randn(4, 6, device=DEV)
+    bmap = torch.randint(0, 7, (40, 50), device=DEV).to(torch.uint8)
+    do = torch.randn_like(q)
+    for wanted in ((1, 1, 1, 1), (1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 1), (0, 0, 0, 1)):
+        results = []
+        for fn in (_token_ops.ops.bucket_attention, F.BucketAttentionFunction.apply):
+            leaves = [t.detach().requires_grad_(bool(w)) for t, w in zip((q, k, v, table), wanted)]
+            out = fn(*leaves, bmap, None, True, 0.3)
+            out.backward(do)
+            results.append([out.detach()] + [t.grad for t in leaves])
+        for a, b, w in zip(*results, (1,) + wanted):
+            assert (a is None and b is None) if not w else torch.equal(a, b)
+    x, r, dy, ds = (torch.randn(30, 70, device=DEV) for _ in range(4))
+    w = torch.rand(70, device=DEV)
+    for use in ((dy, ds), (dy, None), (None, ds)):
+        for residual in (r, None):
+            results = []
+            for fn in (_token_ops.ops.rms_norm_pair, F.AddRMSNormFunction.apply):
+                leaves = [t.detach().requires_grad_() for t in ((x, w) if residual is None else (x, residual, w))]
+                both = fn(leaves[0], None if residual is None else leaves[1], leaves[-1], 1e-6)
+                both = list(both)[:1 if residual is None else 2]
+                pairs = [(o, g) for o, g in zip(both, use) if g is not None]
+                if not pairs:
+                    continue
+                grads = torch.autograd.grad([o for o, _ in pairs], leaves, [g for _, g in pairs], allow_unused=True)
+                results.append([o.detach() for o in both] + [torch.zeros(()) if g is None else g for g in grads])
+            if results:
+                assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(*results))
+
+
 def test_python_operators_refuse_what_the_compiled_ones_refuse():
     from _spherical_distortion_ext import _token_ops
     q = torch.randn(1, 2, 4, 16, device=DEV)
