@@ -809,14 +809,15 @@ int sdk_mapped_max_unpool_planned_bands(const void* grad_output, const int64_t* 
  * `causal`, if j > i + key_lengths[b] - queries (the last query sees every key).  A query without
  * pairs gets zeros, and -inf as its lse.  Keys and values at or beyond key_lengths[b] are not read;
  * those of pairs that the map leaves out are, and have to be finite.
- * A bias of -inf leaves its bucket out; finite ones beyond 2^100 / max(scale, 1 / scale) count as that.
+ * A bias of -inf leaves its bucket out; finite ones beyond 2^20 log(2) in magnitude count as one value, so that
+ * pairs masked by a type's lowest value weigh nothing beside others and the same among themselves.
  *
  * query, output [batch, heads, queries, dim]; key, value [batch, key_heads, keys, dim], heads a
  * multiple of key_heads (head h reads key head h / (heads / key_heads)); bias_table [heads, buckets]
  * dense, of `dtype` or float32 (table_dtype); bucket_map [queries, keys] bytes, or one such map for
  * each batch element; key_lengths [batch] or NULL (every key counts).  Strides in elements, of the
  * batch, head and token axes; the last axis is dense.  dim: a multiple of 8 up to 128, rows of every
- * tensor 16-byte aligned; buckets: 1 .. 256; scale > 0.
+ * tensor 16-byte aligned; buckets: 1 .. 256; scale: 2^-32 .. 2^32.
  * Backward: gradients that are NULL are not formed; grad_table [heads, buckets] of table_dtype.
  * Every sum is formed in an order that depends on the sizes alone. */
 typedef struct sdk_bucket_attention {
@@ -827,7 +828,8 @@ typedef struct sdk_bucket_attention {
   const uint8_t* bucket_map;
   const int32_t* key_lengths;
   void* output;             /* written by the forward, read by the backward */
-  float* lse;               /* [batch, heads, queries]: log2 of the sum of exp(s); forward: may be NULL */
+  float* lse;               /* [2, batch, heads, queries], of which the sum is log2 of the sum of exp(s) (the
+                               second is 0 for ordinary levels); forward: may be NULL */
   const void* grad_output;
   void* grad_query;
   void* grad_key;

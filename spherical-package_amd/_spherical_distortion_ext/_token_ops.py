@@ -82,8 +82,8 @@ def _check_attention(query, key, value, bias_table, bucket_map, key_lengths, sca
         raise RuntimeError("key_lengths must be int32 of shape [%d], got %s %s"
                            % (B, key_lengths.dtype, tuple(key_lengths.shape)))
     _dense(key_lengths=key_lengths)
-    if not scale > 0 or scale == float("inf"):
-        raise RuntimeError("scale must be positive and finite, got %s" % scale)
+    if not 2.0 ** -32 <= scale <= 2.0 ** 32:
+        raise RuntimeError("scale must be between 2^-32 and 2^32, got %s" % scale)
 
 
 def _args(query, key, value, bias_table, bucket_map, key_lengths, causal, scale):
@@ -113,12 +113,13 @@ def _run(name, a, backward, ref):
 
 
 def bucket_attention_forward(query, key, value, bias_table, bucket_map, key_lengths, causal, scale):
-    """-> (output like query, lse [batch, heads, queries] float32)."""
+    """-> (output like query, lse [2, batch, heads, queries] float32: two numbers whose sum is log2 of the row's sum of
+    exponentials)."""
     _check_attention(query, key, value, bias_table, bucket_map, key_lengths, scale)
     with torch.cuda.device(query.device):
         a, keep = _args(query, key, value, bias_table, bucket_map, key_lengths, causal, scale)
         out = torch.empty_like(keep[0])
-        lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device)
+        lse = torch.empty((2,) + tuple(query.shape[:3]), dtype=torch.float32, device=query.device)
         a.output, a.output_strides, a.lse = out.data_ptr(), _strides(out), lse.data_ptr()
         _run("sdk_bucket_attention_forward", a, 0, query)
     return out, lse
@@ -129,7 +130,7 @@ def bucket_attention_backward(grad_output, query, key, value, bias_table, bucket
     """-> gradients of query, key, value and bias_table; those not asked for are empty tensors."""
     _check_attention(query, key, value, bias_table, bucket_map, key_lengths, scale)
     _on_gpu(query, grad_output=grad_output, output=output, lse=lse)
-    if grad_output.shape != query.shape or output.shape != query.shape or lse.shape != query.shape[:3]:
+    if grad_output.shape != query.shape or output.shape != query.shape or tuple(lse.shape) != (2,) + tuple(query.shape[:3]):
         raise RuntimeError("grad_output, output and lse must have the shapes of the forward's results")
     if grad_output.dtype != query.dtype or output.dtype != query.dtype or lse.dtype != torch.float32:
         raise RuntimeError("grad_output and output must have dtype %s, lse float32" % query.dtype)

@@ -22,7 +22,7 @@ Attention on_device(const sdk_bucket_attention* a) {
   d.key_heads = (int)a->key_heads, d.dim = (int)a->dim, d.buckets = (int)a->buckets, d.causal = a->causal != 0;
   d.table_float = a->table_dtype == SDK_F32;
   d.scale = (float)a->scale, d.scale2 = (float)(a->scale * 1.4426950408889634);
-  d.limit = (float)(0x1p100 / std::max(1.0, a->scale));
+  d.limit = (float)std::ldexp(1.0, 90 - std::ilogb(a->scale));
   return d;
 }
 
@@ -40,8 +40,7 @@ int check(const sdk_bucket_attention* a) {
               (long long)a->dim);
   SDK_REQUIRE(a->buckets >= 1 && a->buckets <= 256, "buckets = %lld must be between 1 and 256",
               (long long)a->buckets);
-  SDK_REQUIRE(a->scale > 0 && std::isfinite(a->scale) && std::isfinite((float)a->scale) && (float)a->scale > 0,
-              "scale must be positive and finite");
+  SDK_REQUIRE(a->scale >= 0x1p-32 && a->scale <= 0x1p32, "scale must be between 2^-32 and 2^32");
   // tokens are counted in 32 bits, with room for a tile beyond the last one
   SDK_REQUIRE(a->batch < 65536 && a->heads < 1 << 20 && a->queries < 1 << 30 && a->keys < 1 << 30,
               "a batch of 65536 or more, 2^20 heads or 2^30 tokens");
@@ -92,7 +91,7 @@ size_t sdk_bucket_attention_workspace_bytes(const sdk_bucket_attention* a, int32
   if (backward) return backward_bytes(a);
   if (a->queries == 0) return 0;
   const int splits = forward_splits(a);
-  return splits == 1 ? 0 : (size_t)splits * a->batch * a->heads * a->queries * (a->dim + 1) * sizeof(float);
+  return splits == 1 ? 0 : (size_t)splits * a->batch * a->heads * a->queries * (a->dim + 2) * sizeof(float);
 }
 
 int sdk_bucket_attention_forward(const sdk_bucket_attention* a, void* workspace, size_t workspace_bytes,

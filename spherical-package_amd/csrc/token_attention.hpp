@@ -266,14 +266,13 @@ struct Carry {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) v[n] = __builtin_amdgcn_raw_buffer_load_b128(all, at[n], 0, 0);
   }
-  __device__ __forceinline__ void scale(float by) {
+  // the tile's token that vector n belongs to
+  __device__ __forceinline__ int token(int n) const { return (n * THREADS + (int)threadIdx.x) / kVectors; }
+  __device__ __forceinline__ void scale(int n, float by) {
+    Pack<T, kWide<T>> x = __builtin_bit_cast(Pack<T, kWide<T>>, v[n]);
 #pragma unroll
-    for (int n = 0; n < kCount; ++n) {
-      Pack<T, kWide<T>> x = __builtin_bit_cast(Pack<T, kWide<T>>, v[n]);
-#pragma unroll
-      for (int e = 0; e < kWide<T>; ++e) x.v[e] = (T)((float)x.v[e] * by);
-      v[n] = __builtin_bit_cast(u32x4, x);
-    }
+    for (int e = 0; e < kWide<T>; ++e) x.v[e] = (T)((float)x.v[e] * by);
+    v[n] = __builtin_bit_cast(u32x4, x);
   }
   __device__ __forceinline__ void store(Tile<T, DP, NT>& tile) const {
 #pragma unroll
@@ -347,9 +346,13 @@ __device__ __forceinline__ float add_weights(const Operand<T>& w, const float* f
   return sum;
 }
 
-// A query's running maximum may fall behind by this much (a factor of 2^8 of the weights) before its sums are
-// brought to a new one.
-constexpr float kBehind = 8.f;
+// log2 of a row's sum of exponentials, 2^level * sum, as two numbers: one that carries it and a rest of zero, or, where
+// the level is so large that it would swallow the sum's part, the level and that part.  A row without pairs: -inf, 0.
+__device__ __forceinline__ float2 lse_of(float level, float sum) {
+  if (!(sum > 0.f || sum != sum)) return make_float2(-INFINITY, 0.f);
+  const float part = log2f(sum);
+  return fabsf(level) > 1024.f ? make_float2(level, part) : make_float2(level + part, 0.f);
+}
 
 // Workgroups follow each other round the eight dies; consecutive tiles of one head share its keys and values, so
 // each die gets a consecutive range of tiles.
@@ -374,14 +377,16 @@ struct Attention {
     const int n = __builtin_amdgcn_readfirstlane(lengths[b]);
     return n < 0 ? 0 : n > keys ? keys : n;
   }
-  // bias / scale of a bucket: scores enter the softmax as scale2 * (q k + bias / scale)
+  // bias / scale of a bucket: scores enter the softmax as scale2 * (q k + bias / scale).  Finite biases of 2^20 powers
+  // of two or more, as masks have them, become one value +-limit, a power of two: limit * scale2 is exact, so that
+  // the level of a row of nothing else is too, and its pairs weigh the same.
   __device__ __forceinline__ float bias(int head, int bucket, bool half_is_bf16) const {
     if (bucket >= buckets) return -INFINITY;
     const int64_t at = (int64_t)head * buckets + bucket;
     const float x = table_float ? ((const float*)table)[at]
                                 : half_is_bf16 ? (float)((const bf16*)table)[at] : (float)((const f16*)table)[at];
-    const float y = x / scale;
-    return fabsf(x) < INFINITY ? fminf(fmaxf(y, -limit), limit) : x;
+    if (fabsf(x) < INFINITY && fabsf(x) > 0x1p20f * 0.6931472f) return x < 0.f ? -limit : limit;
+    return x / scale;
   }
 };
 
@@ -466,6 +471,21 @@ struct Work {
 };
 
 // host
+// Parts that a walk of `steps` tiles is dealt to, for `groups` workgroups without and `slots` that run at once: the
+// fewest rounds of workgroups times the tiles of a round; a part costs about four tiles more (its operands, its sums
+// in memory), and has four at least.  More workgroups than that stay whole: 1152 of the forward at 4608 x 4608 pairs
+// as two parts each took 284 us and a join for 265.  balance: two parts at least where all run at once (causal walks
+// differ in length: 256 workgroups of dk and dv, 228 us whole, 148 as two parts, 170 as four).
+inline int parts_of(int64_t groups, int64_t steps, int64_t slots, bool balance) {
+  if (groups == 0 || groups > slots || (groups == slots && !balance)) return 1;
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t s = balance && steps >= 8 ? 2 : 1; s <= 16 && (s <= 2 || s * 4 <= steps); ++s) {
+    const int64_t cost = ceil_div(groups * s, slots) * (ceil_div(steps, s) + 4);
+    if (cost < least) least = cost, best = s;
+  }
+  return (int)best;
+}
+
 Attention on_device(const sdk_bucket_attention* a);
 bool few_rows(const sdk_bucket_attention* a);       // whether a key head's rows go to the kernel of few queries
 int forward_splits(const sdk_bucket_attention* a);

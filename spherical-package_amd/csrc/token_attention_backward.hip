@@ -32,6 +32,21 @@ __device__ __forceinline__ float gradient_scale(const unsigned* top) {
   return exponent == 0 || exponent >= 255 ? 1.f : __uint_as_float((247 - exponent) << 23);
 }
 
+// The two numbers of a row's lse as p = 2^(scale2 s - off) * factor, lifted.  The factor is not 1 for levels alone that
+// would swallow what is added to them.
+template <typename T>
+struct Lse {
+  float off, factor = 1.f;
+  bool far;
+  __device__ __forceinline__ Lse(float level, float part) : off(level) {
+    far = fabsf(level) > 1024.f && fabsf(level) < INFINITY;
+    if (far)
+      factor = __builtin_amdgcn_exp2f(kLift<T> - part);
+    else
+      off -= kLift<T>;
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void flip(Operand<T>& x, bool odd) {
   if constexpr (sizeof(T) == 4) {
@@ -46,7 +61,7 @@ __device__ __forceinline__ void flip(Operand<T>& x, bool odd) {
 // ------------------------------------------------------------------------------------------ terms of a row
 __global__ void clear_word(unsigned* word) { *word = 0; }
 
-// D_i and log2 of the softmax's sum (+inf for a query without pairs: its p are zeros); float16: the largest |do|.
+// D_i and the first number of the lse (+inf for a query without pairs: its p are zeros); float16: the largest |do|.
 // A row is read by LANES lanes, 16 bytes each.
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta, float* lse2, unsigned* top) {
@@ -153,7 +168,8 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
   const int last = a.causal ? std::min(len - 1, clamped + shift) : len - 1;
   const bool in = query < a.queries;
   const float held = gradient_scale<T>(top);
-  const float my_lse = in ? lse2[row] - kLift<T> : INFINITY;
+  const Lse<T> lse(in ? lse2[row] : INFINITY, in ? a.lse[(int64_t)a.batch * a.heads * a.queries + row] : 0.f);
+  const float my_lse = lse.off, rest = lse.factor;   // rest: a factor of everything this lane sums
   float my_delta = in ? delta[row] * held : 0.f;
 
   Operand<T> q[DP / 16], g[DP / 16];
@@ -208,6 +224,10 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
       float ds[16];
 #pragma unroll
       for (int v = 0; v < 16; ++v) ds[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -my_lse)) * e[v];
+      if constexpr (COLUMNS == 16) {   // two queries to a column
+#pragma unroll
+        for (int v = 0; v < 16; ++v) ds[v] *= rest;
+      }
       if constexpr (COLUMNS > 0) {
 #pragma unroll
         for (int turn = 0; turn < 64 / COLUMNS; ++turn) {
@@ -225,24 +245,26 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
   if constexpr (sizeof(T) == 2)   // float32: the registers do not hold two loops (170 us for 149 with one)
     for (; k0 < std::min(to, whole); k0 += KEYS) step(k0, std::false_type());
   for (; k0 < to; k0 += KEYS) step(k0, std::true_type());
-  const float back = exp2f(-kLift<T>) / held;
+  const float back = exp2f(-kLift<T>) / held, mine_back = back * sign * (COLUMNS == 16 ? 1.f : rest);
   if (in && splits > 1)
     store_columns<float, DP>(part + ((int64_t)work.split * a.batch * a.heads * a.queries + row) * a.dim, a.dim, 0, a.dim,
-                             lane, dq, a.scale * back * sign);
+                             lane, dq, a.scale * mine_back);
   else if (in && a.dq)
     store_columns<T, DP>((T*)a.dq + b * a.dqs[0] + head * a.dqs[1], a.dqs[2], query, a.dim, lane, dq,
-                         a.scale * back * sign);
+                         a.scale * mine_back);
   if constexpr (COLUMNS > 0) {
+    __shared__ float column_back[kWaves][COLUMNS];
+    if (lane < COLUMNS) column_back[wave][lane] = mine_back;
     __syncthreads();
     for (int i = threadIdx.x; i < a.buckets; i += kThreads) {
       float x = 0.f;
       for (int w = 0; w < kWaves; ++w)
+#pragma unroll 4
         for (int c = 0; c < COLUMNS; ++c) {   // begun at the bucket's own column: other banks for other lanes
           const int column = (c + i) % COLUMNS;
-          const float y = sums[(w * (a.buckets + 1) + i) * COLUMNS + column];
-          x += column % 2 ? -y : y;
+          x += sums[(w * (a.buckets + 1) + i) * COLUMNS + column] * column_back[w][column];
         }
-      table_parts[(((int64_t)work.head * tiles + work.tile) * splits + work.split) * a.buckets + i] = x * back;
+      table_parts[(((int64_t)work.head * tiles + work.tile) * splits + work.split) * a.buckets + i] = x;
     }
   }
 }
@@ -313,7 +335,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 32 ? 1 : kBackward
 
   Carry<T, DP, NT, kThreads> next_q(a.qs[2], a.dim), next_g(a.gs[2], a.dim);
   Buckets bucket[NT], next_bucket[NT];
-  float next_lse = 0.f, next_delta = 0.f;
+  float next_lse = 0.f, next_delta = 0.f, next_rest = 0.f, next_level[decltype(next_g)::kCount];
+  int64_t next_row = 0;
+  const float* rests = a.lse + (int64_t)a.batch * a.heads * a.queries;
   auto request = [&](int unit) {
     const int head = shared_head * group + unit / each, q0 = from + unit % each * ROWS;
     next_q.load((const T*)a.q + b * a.qs[0] + head * a.qs[1] + q0 * a.qs[2], a.qs[2], a.queries - q0, a.dim);
@@ -321,20 +345,33 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 32 ? 1 : kBackward
 #pragma unroll
     for (int t = 0; t < NT; ++t)   // rows of the turned map are padded to whole tiles
       next_bucket[t].load(map + q0 + 16 * NT * h + 16 * t);
+    next_row = ((int64_t)b * a.heads + head) * a.queries + q0;
+#pragma unroll
+    for (int n = 0; n < next_g.kCount; ++n)
+      next_level[n] = lse2[next_row + std::min(next_g.token(n), a.queries - 1 - q0)];
     if (threadIdx.x < ROWS) {
       const int q = q0 + threadIdx.x;
-      const int64_t row = ((int64_t)b * a.heads + head) * a.queries + q;
-      next_lse = INFINITY, next_delta = 0.f;
-      if (q < a.queries) next_lse = lse2[row], next_delta = delta[row];   // worked on in put: nothing waits here
+      const int64_t row = next_row + threadIdx.x;
+      next_lse = INFINITY, next_delta = 0.f, next_rest = 0.f;
+      // worked on in put: nothing waits here
+      if (q < a.queries) next_lse = lse2[row], next_delta = delta[row], next_rest = rests[row];
     }
   };
   auto put = [&](int buffer) {
     next_q.store(queries[buffer]);
-    if constexpr (__is_same(T, f16)) next_g.scale(held);
+    // a row's factor belongs to p: do and D take it instead (the rows that have one are rare)
+#pragma unroll
+    for (int n = 0; n < next_g.kCount; ++n) {
+      const Lse<T> lse(next_level[n], 0.f);
+      float by = held;
+      if (__any(lse.far)) by *= Lse<T>(next_level[n], lse.far ? rests[next_row + next_g.token(n)] : 0.f).factor;
+      if (__is_same(T, f16) || __any(lse.far)) next_g.scale(n, by);
+    }
     next_g.store(grads[buffer]);
     if (threadIdx.x < ROWS) {
-      row_lse[buffer][threadIdx.x] = kLift<T> - next_lse;
-      row_delta[buffer][threadIdx.x] = -next_delta * held;
+      const Lse<T> lse(next_lse, next_rest);
+      row_lse[buffer][threadIdx.x] = -lse.off;
+      row_delta[buffer][threadIdx.x] = -next_delta * held * lse.factor;
     }
   };
   auto put_bias = [&](int unit) {
@@ -422,14 +459,6 @@ __global__ __launch_bounds__(256) void join_splits(const float* part, int64_t pi
   store_pack<T, 4>(out + bh / heads * s0 + bh % heads * s1 + token * s2 + d, x);
 }
 
-// Parts that a walk of `steps` tiles is dealt to, for `groups` workgroups without: two workgroups a CU, for the keys of
-// causal calls, whose tiles differ most, four; at least four tiles each.  (256 workgroups of dk and dv, 8192 x 8192 pairs
-// of 16 heads: 967 us as they are, 730 as two parts each and a join.)
-int splits_for(int64_t groups, int64_t steps, int64_t wanted) {
-  if (groups >= wanted || groups == 0) return 1;
-  return (int)std::max<int64_t>(1, std::min(ceil_div(wanted, groups), steps / 4));
-}
-
 struct Space {
   int query_splits, key_splits, pitch;
   int64_t top, delta, lse2, parts, turned, part, total;
@@ -440,9 +469,11 @@ Space space_of(const sdk_bucket_attention* a) {
   const int64_t tile = 32 * (a->dtype == SDK_F32 ? kParts<float> : kParts<bf16>), rows = 32 * kWaves;
   const int64_t q_rows = a->batch * a->heads * a->queries, k_rows = a->batch * a->key_heads * a->keys;
   const int64_t q_groups = a->batch * a->heads * ceil_div(a->queries, rows);
-  w.query_splits = splits_for(q_groups, ceil_div(a->keys, tile), 512);
-  w.key_splits = splits_for(a->batch * a->key_heads * ceil_div(a->keys, rows),
-                            a->heads / a->key_heads * ceil_div(a->queries, tile), a->causal ? 1024 : 512);
+  // workgroups that run at once, by the registers of their waves
+  const int64_t slots = a->dim <= 64 ? 512 : 256, key_slots = a->dtype == SDK_F32 && a->dim > 32 ? 256 : slots;
+  w.query_splits = parts_of(q_groups, ceil_div(a->keys, tile), slots, false);
+  w.key_splits = parts_of(a->batch * a->key_heads * ceil_div(a->keys, rows),
+                          a->heads / a->key_heads * ceil_div(a->queries, tile), key_slots, a->causal);
   w.pitch = (int)ceil_div(a->queries, 64) * 64;
   w.top = 0;
   w.delta = 256;

@@ -10,11 +10,16 @@ namespace sdk {
 namespace token {
 namespace {
 
+__device__ __forceinline__ void put_lse(float* to, int64_t rows, int64_t row, float2 lse) {
+  to[row] = lse.x;
+  to[rows + row] = lse.y;
+}
+
 // ------------------------------------------------------------------------------------------ many queries
 // A workgroup takes 128 queries of a head and walks the keys, 32 queries a wave: S^T = K Q^T has the queries in
 // columns, so a query's maximum and sum are one lane's (and the lane's 32 further on).  The next tile is requested
 // while this one is worked on; with two buffers a step has one barrier.
-// splits > 1: each takes a part of the keys and leaves its normalised output and log2 of its sum for `join`.
+// splits > 1: each takes a part of the keys and leaves its normalised output and log2 of its sum (two numbers) for `join`.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int splits, int tiles, float* part_out,
                                                       float* part_lse) {
@@ -143,16 +148,16 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
   sum += other_half(sum);
   if (query >= a.queries) return;
   const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  const float lse2 = sum > 0.f || sum != sum ? off + log2f(sum) : -INFINITY;
+  const float2 lse = lse_of(off, sum);
   const int64_t row = (int64_t)work.head * a.queries + query;
   if (splits > 1) {
     const int64_t rows = (int64_t)a.batch * a.heads * a.queries;
     store_columns<float, DP>(part_out + work.split * rows * a.dim, a.dim, row, a.dim, lane, o, by);
-    if (h == 0) part_lse[work.split * rows + row] = lse2;
+    if (h == 0) put_lse(part_lse + work.split * 2 * rows, rows, row, lse);
     return;
   }
   store_columns<T, DP>((T*)a.out + b * a.os[0] + head * a.os[1], a.os[2], query, a.dim, lane, o, by);
-  if (a.lse && h == 0) a.lse[row] = lse2;
+  if (a.lse && h == 0) put_lse(a.lse, (int64_t)a.batch * a.heads * a.queries, row, lse);
 }
 
 // ------------------------------------------------------------------------------------------ few queries
@@ -303,60 +308,63 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
   }
   if (wave != 0 || lane % 32 >= rows) return;
   const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  const float lse2 = sum > 0.f || sum != sum ? fmaf(most, a.scale2, log2f(sum)) : -INFINITY;
+  const float2 lse = lse_of(most == -INFINITY ? 0.f : most * a.scale2, sum);
   const int64_t row = ((int64_t)b * a.heads + head) * a.queries + query;
   if (splits > 1) {
     const int64_t all = (int64_t)a.batch * a.heads * a.queries;
     store_columns<float, DP>(part_out + split * all * a.dim, a.dim, row, a.dim, lane, o, by);
-    if (h == 0) part_lse[split * all + row] = lse2;
+    if (h == 0) put_lse(part_lse + split * 2 * all, all, row, lse);
     return;
   }
   store_columns<T, DP>((T*)a.out + b * a.os[0] + head * a.os[1], a.os[2], query, a.dim, lane, o, by);
-  if (a.lse && h == 0) a.lse[row] = lse2;
+  if (a.lse && h == 0) put_lse(a.lse, (int64_t)a.batch * a.heads * a.queries, row, lse);
 }
 
-// The splits of a row: weights 2^(lse2 - largest), a wave a row.
+// The splits of a row: weights 2^(lse2 - largest); four values a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void join(const Attention a, int splits, const float* part_out,
                                             const float* part_lse) {
-  const int lane = threadIdx.x % 64;
-  const int64_t rows = (int64_t)a.batch * a.heads * a.queries, row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const int per_row = a.dim / 4;
+  const int64_t rows = (int64_t)a.batch * a.heads * a.queries, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / per_row;
   if (row >= rows) return;
+  const int d = (int)(i % per_row) * 4;
   float most = -INFINITY;
-  for (int s = lane; s < splits; s += 64) most = fmaxf(most, part_lse[s * rows + row]);
-  most = over_wave<Largest>(most);
+  for (int s = 0; s < splits; ++s) most = Largest::of(most, part_lse[s * 2 * rows + row]);
   const float off = most == -INFINITY ? 0.f : most;
-  float sum = 0.f, x[2] = {0.f, 0.f};
-  const int d = 2 * lane;
+  float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < splits; ++s) {
-    const float w = __builtin_amdgcn_exp2f(part_lse[s * rows + row] - off);
+    const float* lse = part_lse + s * 2 * rows + row;
+    const float w = __builtin_amdgcn_exp2f((lse[0] - off) + lse[rows]);
+    float y[4];
+    load_pack<float, 4>(part_out + (s * rows + row) * a.dim + d, y);
     sum += w;
-    if (d < a.dim) {
-      const float2 f = *reinterpret_cast<const float2*>(part_out + (s * rows + row) * a.dim + d);
-      x[0] += w * f.x;
-      x[1] += w * f.y;
-    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += w * y[e];
   }
   const int64_t query = row % a.queries, bh = row / a.queries;
   const int head = (int)(bh % a.heads), b = (int)(bh / a.heads);
   const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  if (d < a.dim) {
-    const float f[2] = {x[0] * by, x[1] * by};
-    store_pack<T, 2>((T*)a.out + b * a.os[0] + head * a.os[1] + query * a.os[2] + d, f);
-  }
-  if (a.lse && lane == 0) a.lse[row] = off + log2f(sum);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] *= by;
+  store_pack<T, 4>((T*)a.out + b * a.os[0] + head * a.os[1] + query * a.os[2] + d, x);
+  if (a.lse && d == 0) put_lse(a.lse, rows, row, lse_of(off, sum));
 }
 
 }  // namespace
 
 bool few_rows(const sdk_bucket_attention* a) { return a->heads / a->key_heads * a->queries <= 32; }
 
-// Parts that the keys are dealt to: two workgroups for each of the 256 CUs, at least 256 keys each.
+// Parts that the keys are dealt to.  Few queries: two workgroups a CU, at least 256 keys each.
 int forward_splits(const sdk_bucket_attention* a) {
-  const bool few = few_rows(a);
-  const int64_t groups = few ? a->batch * a->key_heads : a->batch * a->heads * ceil_div(a->queries, 32 * kWaves);
-  if (groups >= 512 || groups == 0) return 1;
-  return (int)std::max<int64_t>(1, std::min(ceil_div(512, groups), a->keys / 256));
+  if (few_rows(a)) {
+    const int64_t groups = a->batch * a->key_heads;
+    if (groups >= 512 || groups == 0) return 1;
+    return (int)std::max<int64_t>(1, std::min(ceil_div(512, groups), a->keys / 256));
+  }
+  const int64_t groups = a->batch * a->heads * ceil_div(a->queries, 32 * kWaves);
+  const int64_t slots = a->dim <= 64 && a->dtype != SDK_F32 ? 768 : 512;   // by the registers of their waves
+  return parts_of(groups, ceil_div(a->keys, 32 * (a->dtype == SDK_F32 ? kParts<float> : kParts<bf16>)), slots, false);
 }
 
 int run_forward(const sdk_bucket_attention* a, void* workspace, hipStream_t s) {
@@ -376,7 +384,7 @@ int run_forward(const sdk_bucket_attention* a, void* workspace, hipStream_t s) {
       ATTENTION_DIM(a->dim, launch(attend<T, DP>, dim3((unsigned)(tiles * a->batch * a->heads) * splits),
                                    dim3(kThreads), s, d, splits, tiles, part_out, part_lse));
     if (splits > 1)
-      launch(join<T>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), s, d, splits, (const float*)part_out,
+      launch(join<T>, dim3((unsigned)ceil_div(rows * (a->dim / 4), 256)), dim3(256), s, d, splits, (const float*)part_out,
              (const float*)part_lse);
   });
   SDK_LAUNCH_CHECK("bucket_attention_forward");

@@ -8,7 +8,6 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
-#include <cmath>
 #include <cstdint>
 #include <optional>
 #include <vector>
@@ -102,7 +101,7 @@ void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
                 "key_lengths must be int32 of shape [", B, "], got ", lengths->scalar_type(), " ", lengths->sizes());
     dense("key_lengths", lengths);
   }
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite, got ", scale);
+  TORCH_CHECK(scale >= 0x1p-32 && scale <= 0x1p32, "scale must be between 2^-32 and 2^32, got ", scale);
 }
 
 // The argument block; the tensors may be replaced by dense copies, which the caller keeps.
@@ -131,7 +130,7 @@ std::tuple<Tensor, Tensor> bucket_attention_forward(Tensor q, Tensor k, Tensor v
   check_attention(q, k, v, table, map, lengths, scale);
   c10::DeviceGuard guard(q.device());
   sdk_bucket_attention a = attention_args(q, k, v, table, map, lengths, causal, scale);
-  Tensor out = at::empty_like(q), lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
+  Tensor out = at::empty_like(q), lse = at::empty({2, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
   a.output = ptr(out), a.lse = (float*)ptr(lse);
   strides(out, a.output_strides);
   const size_t need = sdk_bucket_attention_workspace_bytes(&a, 0);
@@ -145,7 +144,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> bucket_attention_backward(
     Tensor lse, bool causal, double scale, bool need_query, bool need_keys, bool need_table) {
   check_attention(q, k, v, table, map, lengths, scale);
   beside(q, "grad_output", grad), beside(q, "output", out), beside(q, "lse", lse);
-  TORCH_CHECK(grad.sizes() == q.sizes() && out.sizes() == q.sizes() && lse.sizes() == q.sizes().slice(0, 3),
+  TORCH_CHECK(grad.sizes() == q.sizes() && out.sizes() == q.sizes() && lse.dim() == 4 && lse.size(0) == 2 &&
+                  lse.sizes().slice(1) == q.sizes().slice(0, 3),
               "grad_output, output and lse must have the shapes of the forward's results");
   TORCH_CHECK(grad.scalar_type() == q.scalar_type() && out.scalar_type() == q.scalar_type() &&
                   lse.scalar_type() == at::kFloat,

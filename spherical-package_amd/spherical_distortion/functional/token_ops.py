@@ -45,7 +45,9 @@ def bucket_attention(query, key, value, bias_table, bucket_map, key_lengths=None
     own.  A pair whose bucket is not below `buckets` does not count; nor do keys from key_lengths[b] on
     (int32 [B]; keys and values there are not read), nor, with `causal`, key j of query i where
     j > i + key_lengths[b] - queries: the last query sees every key.  A query without pairs gives
-    zeros.  scale: dim ** -0.5 if None.
+    zeros.  A bias of -inf leaves its bucket out; finite biases beyond 7e5 in magnitude count as one value: a
+    mask by the type's lowest weighs nothing beside others, and the same among themselves.  scale: dim ** -0.5
+    if None.
 
     With gradients for query, key, value and bias_table.  A few queries against many keys (one new
     token and its cache) are dealt to the GPU along the keys."""

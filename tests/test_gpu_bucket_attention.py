@@ -165,6 +165,27 @@ def test_biases_that_mask(lowest):
     _close(out, want, TOL[torch.float32])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lowest", [torch.finfo(torch.float32).min, -1e30])
+@pytest.mark.parametrize("buckets", [6, 40, 200])
+@pytest.mark.parametrize("lq,lk", [(70, 90), (150, 700), (3, 700)])
+def test_gradients_of_rows_that_biases_mask(lq, lk, buckets, lowest, dtype):
+    """Rows all of whose biases are one lowest value (beside ordinary rows): equal weights, forward and backward,
+    whatever part of the keys a workgroup takes."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(2, 4, 2, lq, lk, 64, buckets, dtype, seed=16 + lk)
+    table[1] = lowest
+    table[:, 2] = lowest
+    bmap[1::5] = 2
+    bmap[2] = 255
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = F.bucket_attention(*leaves, bmap)
+    grads = torch.autograd.grad(out, leaves, do)
+    want = _exact(q, k, v, table, bmap, grad=do)
+    for got, ref, terms in zip((out, *grads), want, _terms(q, k, v, do)):
+        _close(got, ref, TOL[dtype], terms)
+
+
 @pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** 12])
 def test_small_and_large_gradients_of_float16(size):
     """Gradients as a loss scale leaves them: weights of 1 / 600 times gradients of 2^-12 lie far below float16's
