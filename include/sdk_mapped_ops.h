@@ -828,8 +828,10 @@ typedef struct sdk_bucket_attention {
   const uint8_t* bucket_map;
   const int32_t* key_lengths;
   void* output;             /* written by the forward, read by the backward */
-  float* lse;               /* [2, batch, heads, queries], of which the sum is log2 of the sum of exp(s) (the
-                               second is 0 for ordinary levels); forward: may be NULL */
+  void* output_rest;        /* 16-bit types, strides of output: what rounding took from it, of the same type; the
+                               backward's <grad_output, output> cancels against sums of its terms.  May be NULL */
+  float* lse;               /* [2, batch, heads, queries]: a whole number and a rest, of which the sum is log2 of
+                               the sum of exp(s); forward: may be NULL */
   const void* grad_output;
   void* grad_query;
   void* grad_key;

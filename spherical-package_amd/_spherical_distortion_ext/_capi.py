@@ -19,7 +19,7 @@ _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c
 class BucketAttention(ctypes.Structure):
     """sdk_bucket_attention."""
     _fields_ = ([(n, _vp) for n in ("query", "key", "value", "bias_table", "bucket_map", "key_lengths", "output",
-                                    "lse", "grad_output", "grad_query", "grad_key", "grad_value", "grad_table")]
+                                    "output_rest", "lse", "grad_output", "grad_query", "grad_key", "grad_value", "grad_table")]
                 + [(n, _i64) for n in ("batch", "heads", "key_heads", "queries", "keys", "dim", "buckets")]
                 + [(n + "_strides", _i64 * 3) for n in ("query", "key", "value", "output", "grad_output",
                                                         "grad_query", "grad_key", "grad_value")]

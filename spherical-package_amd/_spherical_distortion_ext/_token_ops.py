@@ -113,30 +113,37 @@ def _run(name, a, backward, ref):
 
 
 def bucket_attention_forward(query, key, value, bias_table, bucket_map, key_lengths, causal, scale):
-    """-> (output like query, lse [2, batch, heads, queries] float32: two numbers whose sum is log2 of the row's sum of
-    exponentials)."""
+    """-> (output like query, what rounding took from it (float32: an empty tensor), lse [2, batch, heads, queries]
+    float32: two numbers whose sum is log2 of the row's sum of exponentials)."""
     _check_attention(query, key, value, bias_table, bucket_map, key_lengths, scale)
     with torch.cuda.device(query.device):
         a, keep = _args(query, key, value, bias_table, bucket_map, key_lengths, causal, scale)
         out = torch.empty_like(keep[0])
         lse = torch.empty((2,) + tuple(query.shape[:3]), dtype=torch.float32, device=query.device)
+        rest = out.new_empty(0) if out.dtype == torch.float32 else torch.empty_like(out)
         a.output, a.output_strides, a.lse = out.data_ptr(), _strides(out), lse.data_ptr()
+        a.output_rest = 0 if out.dtype == torch.float32 else rest.data_ptr()
         _run("sdk_bucket_attention_forward", a, 0, query)
-    return out, lse
+    return out, rest, lse
 
 
-def bucket_attention_backward(grad_output, query, key, value, bias_table, bucket_map, key_lengths, output, lse,
-                              causal, scale, need_query, need_keys, need_table):
+def bucket_attention_backward(grad_output, query, key, value, bias_table, bucket_map, key_lengths, output, rest,
+                              lse, causal, scale, need_query, need_keys, need_table):
     """-> gradients of query, key, value and bias_table; those not asked for are empty tensors."""
     _check_attention(query, key, value, bias_table, bucket_map, key_lengths, scale)
-    _on_gpu(query, grad_output=grad_output, output=output, lse=lse)
+    _on_gpu(query, grad_output=grad_output, output=output, rest=rest, lse=lse)
     if grad_output.shape != query.shape or output.shape != query.shape or tuple(lse.shape) != (2,) + tuple(query.shape[:3]):
         raise RuntimeError("grad_output, output and lse must have the shapes of the forward's results")
     if grad_output.dtype != query.dtype or output.dtype != query.dtype or lse.dtype != torch.float32:
         raise RuntimeError("grad_output and output must have dtype %s, lse float32" % query.dtype)
+    if rest.numel() and (rest.shape != output.shape or rest.dtype != output.dtype or rest.stride() != output.stride()):
+        raise RuntimeError("the output's rest must be like the output, or empty")
     with torch.cuda.device(query.device):
         a, keep = _args(query, key, value, bias_table, bucket_map, key_lengths, causal, scale)
         grad_output, output, lse = _rows_ready(grad_output), _rows_ready(output), lse.contiguous()
+        if rest.numel():
+            rest = _rows_ready(rest)
+            a.output_rest = rest.data_ptr()
         a.grad_output, a.grad_output_strides = grad_output.data_ptr(), _strides(grad_output)
         a.output, a.output_strides, a.lse = output.data_ptr(), _strides(output), lse.data_ptr()
         dq, dk, dv = (torch.empty_like(t) if need else t.new_empty(0)
@@ -335,10 +342,10 @@ _SCHEMAS = (
     ("rms_norm_pair", "(Tensor x, Tensor? residual, Tensor weight, float eps) -> Tensor[]", rms_norm_pair),
     ("bucket_attention_forward",
      "(Tensor query, Tensor key, Tensor value, Tensor bias_table, Tensor bucket_map, Tensor? key_lengths,"
-     " bool causal, float scale) -> (Tensor, Tensor)", bucket_attention_forward),
+     " bool causal, float scale) -> (Tensor, Tensor, Tensor)", bucket_attention_forward),
     ("bucket_attention_backward",
      "(Tensor grad_output, Tensor query, Tensor key, Tensor value, Tensor bias_table, Tensor bucket_map,"
-     " Tensor? key_lengths, Tensor output, Tensor lse, bool causal, float scale, bool need_query, bool need_keys,"
+     " Tensor? key_lengths, Tensor output, Tensor rest, Tensor lse, bool causal, float scale, bool need_query, bool need_keys,"
      " bool need_table) -> (Tensor, Tensor, Tensor, Tensor)", bucket_attention_backward),
     ("add_rms_norm", "(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)",
      add_rms_norm),

@@ -10,7 +10,7 @@ namespace token {
 Attention on_device(const sdk_bucket_attention* a) {
   Attention d = {};
   d.q = a->query, d.k = a->key, d.v = a->value, d.table = a->bias_table, d.out = a->output, d.grad = a->grad_output;
-  d.map = a->bucket_map, d.lengths = a->key_lengths;
+  d.map = a->bucket_map, d.lengths = a->key_lengths, d.rest = a->dtype == SDK_F32 ? nullptr : a->output_rest;
   d.dq = a->grad_query, d.dk = a->grad_key, d.dv = a->grad_value, d.dtable = a->grad_table, d.lse = a->lse;
   for (int i = 0; i < 3; ++i) {
     d.qs[i] = a->query_strides[i], d.ks[i] = a->key_strides[i], d.vs[i] = a->value_strides[i];
@@ -63,6 +63,8 @@ int check_rows(const char* name, const void* p, const int64_t* strides, int dtyp
 int check_inputs(const sdk_bucket_attention* a) {
   if (int rc = check_rows("query", a->query, a->query_strides, a->dtype)) return rc;
   if (int rc = check_rows("output", a->output, a->output_strides, a->dtype)) return rc;
+  if (a->output_rest)
+    if (int rc = check_rows("output_rest", a->output_rest, a->output_strides, a->dtype)) return rc;
   SDK_REQUIRE(a->bias_table, "bias_table must not be NULL");
   if (a->keys == 0) return SDK_OK;
   if (int rc = check_rows("key", a->key, a->key_strides, a->dtype)) return rc;

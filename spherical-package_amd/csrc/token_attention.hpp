@@ -346,12 +346,33 @@ __device__ __forceinline__ float add_weights(const Operand<T>& w, const float* f
   return sum;
 }
 
-// log2 of a row's sum of exponentials, 2^level * sum, as two numbers: one that carries it and a rest of zero, or, where
-// the level is so large that it would swallow the sum's part, the level and that part.  A row without pairs: -inf, 0.
+// A row's sum of exponentials is 2^level * sum.  The level is a whole number at or above (or little below) the largest
+// score in powers of two: weights against two levels differ by a power of two, so that they round to 16 bits alike in
+// every part of the keys and in the backward.  Kept as (level, log2 sum); a row without pairs: (-inf, 0).
 __device__ __forceinline__ float2 lse_of(float level, float sum) {
-  if (!(sum > 0.f || sum != sum)) return make_float2(-INFINITY, 0.f);
-  const float part = log2f(sum);
-  return fabsf(level) > 1024.f ? make_float2(level, part) : make_float2(level + part, 0.f);
+  return sum > 0.f || sum != sum ? make_float2(level, log2f(sum)) : make_float2(-INFINITY, 0.f);
+}
+
+// The weights of a row as the product takes them, as floats again.
+template <typename T>
+__device__ __forceinline__ void as_rounded(float (&p)[16]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const Operand<T> w = rounded<T>(p + 8 * half);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (__is_same(T, bf16)) {
+          p[8 * half + 2 * i] = __uint_as_float(w.u[i] << 16);
+          p[8 * half + 2 * i + 1] = __uint_as_float(w.u[i] & 0xffff0000u);
+        } else {
+          const f16x2 x = __builtin_bit_cast(f16x2, w.u[i]);
+          p[8 * half + 2 * i] = (float)x[0];
+          p[8 * half + 2 * i + 1] = (float)x[1];
+        }
+      }
+    }
+  }
 }
 
 // Workgroups follow each other round the eight dies; consecutive tiles of one head share its keys and values, so
@@ -364,6 +385,7 @@ __device__ __forceinline__ unsigned by_die(unsigned id, unsigned count) {
 // What the kernels take of sdk_bucket_attention; scale2 = scale * log2(e).
 struct Attention {
   const void *q, *k, *v, *table, *out, *grad;
+  void* rest;
   const uint8_t* map;
   const int32_t* lengths;
   void *dq, *dk, *dv, *dtable;
@@ -421,6 +443,24 @@ __device__ __forceinline__ void store_columns(T* base, int64_t stride, int64_t r
                             acc[d][4 * a + 3] * by};
         store_pack<T, 4>(base + row * stride + at, f);
       }
+    }
+}
+
+// The same for the output: rounded, and, where `rest` is not NULL, what the rounding took.
+template <typename T, int DP>
+__device__ __forceinline__ void store_output(T* base, T* rest, int64_t stride, int64_t row, int dim, int lane,
+                                             floatx16 (&acc)[DP / 32], float by) {
+  store_columns<T, DP>(base, stride, row, dim, lane, acc, by);
+  if constexpr (sizeof(T) == 2)
+    if (rest) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float x = acc[d][v] * by;
+          acc[d][v] = x - (float)(T)x;
+        }
+      store_columns<T, DP>(rest, stride, row, dim, lane, acc, 1.f);
     }
 }
 

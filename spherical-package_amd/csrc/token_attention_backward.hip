@@ -32,18 +32,20 @@ __device__ __forceinline__ float gradient_scale(const unsigned* top) {
   return exponent == 0 || exponent >= 255 ? 1.f : __uint_as_float((247 - exponent) << 23);
 }
 
-// The two numbers of a row's lse as p = 2^(scale2 s - off) * factor, lifted.  The factor is not 1 for levels alone that
-// would swallow what is added to them.
+// A row's level and log2 of its sum as p = 2^(scale2 s - off) * factor, lifted.  whole: off is a whole number, for
+// weights that round as the forward's did; the factor is then between 1 and 2.  Else it is 1, but for levels (of rows
+// that biases mask) that would swallow what is added to them.
 template <typename T>
 struct Lse {
   float off, factor = 1.f;
   bool far;
-  __device__ __forceinline__ Lse(float level, float part) : off(level) {
+  __device__ __forceinline__ Lse(float level, float part, bool whole) : off(level) {
     far = fabsf(level) > 1024.f && fabsf(level) < INFINITY;
+    const float up = whole ? ceilf(part) : part;
     if (far)
       factor = __builtin_amdgcn_exp2f(kLift<T> - part);
     else
-      off -= kLift<T>;
+      off += up - kLift<T>, factor = __builtin_amdgcn_exp2f(up - part);
   }
 };
 
@@ -61,7 +63,7 @@ __device__ __forceinline__ void flip(Operand<T>& x, bool odd) {
 // ------------------------------------------------------------------------------------------ terms of a row
 __global__ void clear_word(unsigned* word) { *word = 0; }
 
-// D_i and the first number of the lse (+inf for a query without pairs: its p are zeros); float16: the largest |do|.
+// D_i and the row's level (+inf for a query without pairs: its p are zeros); float16: the largest |do|.
 // A row is read by LANES lanes, 16 bytes each.
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta, float* lse2, unsigned* top) {
@@ -77,7 +79,13 @@ __global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta
       const int head = (int)(bh % a.heads), b = (int)(bh / a.heads);
       if (d < a.dim) {
         float x[kWide<T>], y[kWide<T>];
-        load_pack<T, kWide<T>>((const T*)a.out + b * a.os[0] + head * a.os[1] + query * a.os[2] + d, x);
+        const int64_t at = b * a.os[0] + head * a.os[1] + query * a.os[2] + d;
+        load_pack<T, kWide<T>>((const T*)a.out + at, x);
+        if (a.rest) {
+          load_pack<T, kWide<T>>((const T*)a.rest + at, y);
+#pragma unroll
+          for (int e = 0; e < kWide<T>; ++e) x[e] += y[e];
+        }
         load_pack<T, kWide<T>>((const T*)a.grad + b * a.gs[0] + head * a.gs[1] + query * a.gs[2] + d, y);
 #pragma unroll
         for (int e = 0; e < kWide<T>; ++e) {
@@ -168,7 +176,7 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
   const int last = a.causal ? std::min(len - 1, clamped + shift) : len - 1;
   const bool in = query < a.queries;
   const float held = gradient_scale<T>(top);
-  const Lse<T> lse(in ? lse2[row] : INFINITY, in ? a.lse[(int64_t)a.batch * a.heads * a.queries + row] : 0.f);
+  const Lse<T> lse(in ? lse2[row] : INFINITY, in ? a.lse[(int64_t)a.batch * a.heads * a.queries + row] : 0.f, true);
   const float my_lse = lse.off, rest = lse.factor;   // rest: a factor of everything this lane sums
   float my_delta = in ? delta[row] * held : 0.f;
 
@@ -221,9 +229,15 @@ __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
           for (int v = 0; v < 16; ++v)
             if (k0 + 16 * NT * h + 16 * t + v > last) s[v] = -INFINITY;
         }
+      // The forward's own weights, rounded as they were: D is the mean of do v^T under these, so that a row's ds add up
+      // to zero.  Unrounded ones miss it by 2^-9 of a weight, which a sum over many keys shows where the table's
+      // entries, or keys with much in common, cancel.
       float ds[16];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) ds[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -my_lse)) * e[v];
+      for (int v = 0; v < 16; ++v) ds[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -my_lse));
+      as_rounded<T>(ds);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) ds[v] *= e[v];
       if constexpr (COLUMNS == 16) {   // two queries to a column
 #pragma unroll
         for (int v = 0; v < 16; ++v) ds[v] *= rest;
@@ -362,14 +376,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 32 ? 1 : kBackward
     // a row's factor belongs to p: do and D take it instead (the rows that have one are rare)
 #pragma unroll
     for (int n = 0; n < next_g.kCount; ++n) {
-      const Lse<T> lse(next_level[n], 0.f);
+      const Lse<T> lse(next_level[n], 0.f, false);
       float by = held;
-      if (__any(lse.far)) by *= Lse<T>(next_level[n], lse.far ? rests[next_row + next_g.token(n)] : 0.f).factor;
+      if (__any(lse.far)) by *= Lse<T>(next_level[n], lse.far ? rests[next_row + next_g.token(n)] : 0.f, false).factor;
       if (__is_same(T, f16) || __any(lse.far)) next_g.scale(n, by);
     }
     next_g.store(grads[buffer]);
     if (threadIdx.x < ROWS) {
-      const Lse<T> lse(next_lse, next_rest);
+      const Lse<T> lse(next_lse, next_rest, false);
       row_lse[buffer][threadIdx.x] = -lse.off;
       row_delta[buffer][threadIdx.x] = -next_delta * held * lse.factor;
     }

@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
   load_columns<T, DP>(q, (const T*)a.q + b * a.qs[0] + head * a.qs[1], a.qs[2], query, query < a.queries, a.dim, lane);
   floatx16 o[DP / 32];
   clear(o);
-  // `level`: a score near the largest so far, common to both halves; sum: of 2^(score - level), of this lane's keys
+  // level (lse_of): common to both halves, off: the same, 0 where there is none; sum: of this lane's keys
   float level = -INFINITY, off = 0.f, sum = 0.f;
 
   Carry<T, DP, NT, kThreads> next_k(a.ks[2], a.dim), next_v(a.vs[2], a.dim);
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
         for (int v = 0; v < 16; ++v)
           if (k0 + 16 * NT * h + 16 * t + v > last) s[t][v] = -INFINITY;
     }
-    // The weights against the level so far.  It is raised only where they would pass 2^14 in sum (and by the first
+    // The weights against the level so far.  It is raised only where they would pass 2^10 in sum (and by the first
     // tile), so that most tiles need no maximum.
     Operand<T> w[NT][2];
     float with = sum;
@@ -116,16 +116,16 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
         }
     };
     if (!first_tile) weigh();
-    if (first_tile || __any(with - sum > 0x1p14f)) {
+    if (first_tile || __any(with - sum > 0x1p10f)) {
       float top = s[0][0];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int v = 0; v < 16; ++v) top = fmaxf(top, s[t][v]);
-      const float grown = fmaxf(max_halves(top), level);
-      const float by = grown == -INFINITY ? 1.f : exp2f((level - grown) * a.scale2);
+      const float grown = fmaxf(ceilf(max_halves(top) * a.scale2), level);
+      const float by = grown == -INFINITY ? 1.f : exp2f(level - grown);
       level = grown;
-      off = grown == -INFINITY ? 0.f : grown * a.scale2;
+      off = grown == -INFINITY ? 0.f : grown;
       first_tile = __any(grown == -INFINITY);   // a query without pairs so far has no level yet
       sum *= by;
 #pragma unroll
@@ -156,7 +156,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const Attention a, int spl
     if (h == 0) put_lse(part_lse + work.split * 2 * rows, rows, row, lse);
     return;
   }
-  store_columns<T, DP>((T*)a.out + b * a.os[0] + head * a.os[1], a.os[2], query, a.dim, lane, o, by);
+  const int64_t at = b * a.os[0] + head * a.os[1];
+  store_output<T, DP>((T*)a.out + at, a.rest ? (T*)a.rest + at : nullptr, a.os[2], query, a.dim, lane, o, by);
   if (a.lse && h == 0) put_lse(a.lse, (int64_t)a.batch * a.heads * a.queries, row, lse);
 }
 
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
   load_columns<T, DP>(q, (const T*)a.q + b * a.qs[0] + head * a.qs[1], a.qs[2], query, true, a.dim, lane);
   floatx16 o[DP / 32];
   clear(o);
-  float most = -INFINITY, sum = 0.f;
+  float most = -INFINITY, sum = 0.f;   // level and sum (lse_of)
   __syncthreads();
 
   // the keys in registers as dot_tile asks for them
@@ -255,9 +256,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
 #pragma unroll
     for (int v = 1; v < 16; ++v) now = fmaxf(now, s[v]);
     now = max_halves(now);
+    now = ceilf(now * a.scale2);
     if (__any(now > most)) {
       const float grown = fmaxf(now, most);
-      const float by = grown == -INFINITY ? 1.f : exp2f((most - grown) * a.scale2);
+      const float by = grown == -INFINITY ? 1.f : exp2f(most - grown);
       most = grown;
       sum *= by;
 #pragma unroll
@@ -265,15 +267,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[d][v] *= by;
     }
-    const float off = most == -INFINITY ? 0.f : most * a.scale2;
+    const float off = most == -INFINITY ? 0.f : most;
     float p[16];
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      p[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -off));
-      sum += p[v];
-    }
+    for (int v = 0; v < 16; ++v) p[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -off));
     wave_order();
     const Operand<T> w[2] = {rounded<T>(p), rounded<T>(p + 8)};
+    sum = add_weights<T>(w[1], p + 8, add_weights<T>(w[0], p, sum));
     add_columns<T>(o, value_view, 0, w);
     wave_order();
   }
@@ -295,8 +295,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
     __syncthreads();
     if (wave < step) {
       const float other = level[slot][0][lane % 32], grown = fmaxf(most, other);
-      const float mine = grown == -INFINITY ? 1.f : exp2f((most - grown) * a.scale2);
-      const float theirs = grown == -INFINITY ? 1.f : exp2f((other - grown) * a.scale2);
+      const float mine = grown == -INFINITY ? 1.f : exp2f(most - grown);
+      const float theirs = grown == -INFINITY ? 1.f : exp2f(other - grown);
       most = grown;
       sum = sum * mine + level[slot][1][lane % 32] * theirs;
 #pragma unroll
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
   }
   if (wave != 0 || lane % 32 >= rows) return;
   const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  const float2 lse = lse_of(most == -INFINITY ? 0.f : most * a.scale2, sum);
+  const float2 lse = lse_of(most, sum);
   const int64_t row = ((int64_t)b * a.heads + head) * a.queries + query;
   if (splits > 1) {
     const int64_t all = (int64_t)a.batch * a.heads * a.queries;
@@ -316,7 +316,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
     if (h == 0) put_lse(part_lse + split * 2 * all, all, row, lse);
     return;
   }
-  store_columns<T, DP>((T*)a.out + b * a.os[0] + head * a.os[1], a.os[2], query, a.dim, lane, o, by);
+  const int64_t at = b * a.os[0] + head * a.os[1];
+  store_output<T, DP>((T*)a.out + at, a.rest ? (T*)a.rest + at : nullptr, a.os[2], query, a.dim, lane, o, by);
   if (a.lse && h == 0) put_lse(a.lse, (int64_t)a.batch * a.heads * a.queries, row, lse);
 }
 
@@ -347,7 +348,13 @@ __global__ __launch_bounds__(256) void join(const Attention a, int splits, const
   const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] *= by;
-  store_pack<T, 4>((T*)a.out + b * a.os[0] + head * a.os[1] + query * a.os[2] + d, x);
+  const int64_t at = b * a.os[0] + head * a.os[1] + query * a.os[2] + d;
+  store_pack<T, 4>((T*)a.out + at, x);
+  if (a.rest) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] -= (float)(T)x[e];
+    store_pack<T, 4>((T*)a.rest + at, x);
+  }
   if (a.lse && d == 0) put_lse(a.lse, rows, row, lse_of(off, sum));
 }
 

@@ -125,36 +125,56 @@ Tensor workspace(const Tensor& ref, size_t bytes) {
   return bytes ? at::empty({(int64_t)bytes}, ref.options().dtype(at::kByte)) : Tensor();
 }
 
-std::tuple<Tensor, Tensor> bucket_attention_forward(Tensor q, Tensor k, Tensor v, Tensor table, Tensor map,
-                                                    const OptTensor& lengths, bool causal, double scale) {
+// for_backward: with the lse and, of 16-bit types, what rounding took from the output.
+std::tuple<Tensor, Tensor, Tensor> attend(Tensor q, Tensor k, Tensor v, Tensor table, Tensor map,
+                                          const OptTensor& lengths, bool causal, double scale, bool for_backward) {
   check_attention(q, k, v, table, map, lengths, scale);
   c10::DeviceGuard guard(q.device());
   sdk_bucket_attention a = attention_args(q, k, v, table, map, lengths, causal, scale);
-  Tensor out = at::empty_like(q), lse = at::empty({2, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-  a.output = ptr(out), a.lse = (float*)ptr(lse);
+  Tensor out = at::empty_like(q), rest, lse;
+  a.output = ptr(out);
+  if (for_backward) {
+    lse = at::empty({2, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    a.lse = (float*)ptr(lse);
+    rest = q.scalar_type() == at::kFloat ? nothing(q) : at::empty_like(out);
+    if (rest.numel()) a.output_rest = ptr(rest);
+  }
   strides(out, a.output_strides);
   const size_t need = sdk_bucket_attention_workspace_bytes(&a, 0);
   Tensor ws = workspace(q, need);
   TOKEN_CALL(sdk_bucket_attention_forward, &a, need ? ptr(ws) : nullptr, need, stream_of(q));
-  return {out, lse};
+  return {out, rest, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> bucket_attention_forward(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                            const Tensor& table, const Tensor& map,
+                                                            const OptTensor& lengths, bool causal, double scale) {
+  return attend(q, k, v, table, map, lengths, causal, scale, true);
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> bucket_attention_backward(
     Tensor grad, Tensor q, Tensor k, Tensor v, Tensor table, Tensor map, const OptTensor& lengths, Tensor out,
-    Tensor lse, bool causal, double scale, bool need_query, bool need_keys, bool need_table) {
+    Tensor rest, Tensor lse, bool causal, double scale, bool need_query, bool need_keys, bool need_table) {
   check_attention(q, k, v, table, map, lengths, scale);
-  beside(q, "grad_output", grad), beside(q, "output", out), beside(q, "lse", lse);
+  beside(q, "grad_output", grad), beside(q, "output", out), beside(q, "rest", rest), beside(q, "lse", lse);
   TORCH_CHECK(grad.sizes() == q.sizes() && out.sizes() == q.sizes() && lse.dim() == 4 && lse.size(0) == 2 &&
                   lse.sizes().slice(1) == q.sizes().slice(0, 3),
               "grad_output, output and lse must have the shapes of the forward's results");
   TORCH_CHECK(grad.scalar_type() == q.scalar_type() && out.scalar_type() == q.scalar_type() &&
                   lse.scalar_type() == at::kFloat,
               "grad_output and output must have dtype ", q.scalar_type(), ", lse float32");
+  TORCH_CHECK(rest.numel() == 0 || (rest.sizes() == out.sizes() && rest.strides() == out.strides() &&
+                                    rest.scalar_type() == out.scalar_type()),
+              "the output's rest must be like the output, or empty");
   c10::DeviceGuard guard(q.device());
   sdk_bucket_attention a = attention_args(q, k, v, table, map, lengths, causal, scale);
   grad = rows_ready(grad), out = rows_ready(out), lse = lse.contiguous();
   a.grad_output = ptr(grad), a.output = ptr(out), a.lse = (float*)ptr(lse);
   strides(grad, a.grad_output_strides), strides(out, a.output_strides);
+  if (rest.numel()) {
+    rest = rows_ready(rest);
+    a.output_rest = ptr(rest);
+  }
   Tensor dq = need_query ? at::empty_like(q) : nothing(q);
   Tensor dk = need_keys ? at::empty_like(k) : nothing(k), dv = need_keys ? at::empty_like(v) : nothing(v);
   Tensor dt = need_table ? at::empty_like(table) : nothing(table);
@@ -357,8 +377,8 @@ struct BucketAttention : torch::autograd::Function<BucketAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,
                         const Tensor& map, const OptTensor& lengths, bool causal, double scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [out, lse] = bucket_attention_forward(q, k, v, table, map, lengths, causal, scale);
-    ctx->save_for_backward({q, k, v, table, map, has(lengths) ? *lengths : Tensor(), out, lse});
+    auto [out, rest, lse] = bucket_attention_forward(q, k, v, table, map, lengths, causal, scale);
+    ctx->save_for_backward({q, k, v, table, map, has(lengths) ? *lengths : Tensor(), out, rest, lse});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return out;
@@ -370,7 +390,7 @@ struct BucketAttention : torch::autograd::Function<BucketAttention> {
                need_t = ctx->needs_input_grad(3);
     at::AutoDispatchBelowADInplaceOrView guard;
     auto [dq, dk, dv, dt] = bucket_attention_backward(
-        grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], n, saved[6], saved[7],
+        grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], n, saved[6], saved[7], saved[8],
         ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), need_q, need_k || need_v, need_t);
     return {need_q ? dq : Tensor(), need_k ? dk : Tensor(), need_v ? dv : Tensor(), need_t ? dt : Tensor(),
             Tensor(), Tensor(), Tensor(), Tensor()};
@@ -379,7 +399,7 @@ struct BucketAttention : torch::autograd::Function<BucketAttention> {
 
 Tensor bucket_attention_only(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& map,
                              const OptTensor& lengths, bool causal, double scale) {
-  return std::get<0>(bucket_attention_forward(q, k, v, table, map, lengths, causal, scale));
+  return std::get<0>(attend(q, k, v, table, map, lengths, causal, scale, false));
 }
 
 Tensor bucket_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,

@@ -17,19 +17,19 @@ from _spherical_distortion_ext._ops import ops as _sdk_ops
 class BucketAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, bias_table, bucket_map, key_lengths, causal, scale):
-        out, lse = _sdk_ops.bucket_attention_forward(query, key, value, bias_table, bucket_map, key_lengths, causal,
-                                                     scale)
-        ctx.save_for_backward(query, key, value, bias_table, bucket_map, key_lengths, out, lse)
+        out, rest, lse = _sdk_ops.bucket_attention_forward(query, key, value, bias_table, bucket_map, key_lengths,
+                                                           causal, scale)
+        ctx.save_for_backward(query, key, value, bias_table, bucket_map, key_lengths, out, rest, lse)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        query, key, value, bias_table, bucket_map, key_lengths, out, lse = ctx.saved_tensors
+        query, key, value, bias_table, bucket_map, key_lengths, out, rest, lse = ctx.saved_tensors
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
         dq, dk, dv, dt = _sdk_ops.bucket_attention_backward(
-            grad_output, query, key, value, bias_table, bucket_map, key_lengths, out, lse, ctx.causal, ctx.scale,
+            grad_output, query, key, value, bias_table, bucket_map, key_lengths, out, rest, lse, ctx.causal, ctx.scale,
             need_q, need_k or need_v, need_t)
         return (dq if need_q else None, dk if need_k else None, dv if need_v else None, dt if need_t else None,
                 None, None, None, None)

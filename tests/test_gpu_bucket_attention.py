@@ -199,6 +199,19 @@ def test_small_and_large_gradients_of_float16(size):
         assert float((got.double().cpu() - ref).abs().max()) <= TOL[torch.float16] * float(ref.abs().max()) + 2.0 ** -25
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_table_gradients_that_cancel(dtype):
+    """Two buckets: one key of each row, and all others.  Their gradients are opposite and small beside the terms
+    summed: what one rounding of the output to 16 bits does to D (2^-9 or 2^-12 of about 0.3 a row) would show."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 4, 2, 24, 1500, 112, 2, dtype, seed=19)
+    bmap.fill_(1)
+    bmap[torch.arange(24), torch.arange(24)] = 0
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    got, = torch.autograd.grad(F.bucket_attention(*leaves, bmap), leaves[3:], do)
+    _close(got, _exact(q, k, v, table, bmap, grad=do)[4], TOL[dtype])
+
+
 def test_bias_table_of_the_queries_type_and_scale():
     from spherical_distortion import functional as F
     q, k, v, table, bmap, do = _inputs(2, 4, 2, 90, 110, 64, 30, torch.bfloat16, seed=6)

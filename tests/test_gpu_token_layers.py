@@ -33,10 +33,10 @@ def test_compiled_and_python_operators_agree():
     table = torch.randn(4, 9, device=DEV)
     bmap = torch.randint(0, 10, (70, 90), device=DEV).to(torch.uint8)
     n = torch.tensor([90, 41], dtype=torch.int32, device=DEV)
-    out, lse = _both("bucket_attention_forward", q, k, v, table, bmap, n, True, 0.2)
+    out, rest, lse = _both("bucket_attention_forward", q, k, v, table, bmap, n, True, 0.2)
     do = torch.randn_like(q)
     for needs in ((True, True, True), (False, True, False), (True, False, False), (False, False, True)):
-        _both("bucket_attention_backward", do, q, k, v, table, bmap, n, out, lse, True, 0.2, *needs)
+        _both("bucket_attention_backward", do, q, k, v, table, bmap, n, out, rest, lse, True, 0.2, *needs)
     x, r, w = torch.randn(20, 100, device=DEV), torch.randn(20, 100, device=DEV), torch.rand(100, device=DEV)
     for residual in (r, None):
         y, s, inv = _both("add_rms_norm", x, residual, w, 1e-6)
