@@ -281,23 +281,24 @@ int deal(int64_t count, const int64_t* sizes, int64_t per_group, Put put, Run ru
   int64_t groups = 0;
   auto flush = [&] {
     for (int k = used; k < kTensors; ++k) t.start[k] = 0xffffffffu;
-    run(t, (unsigned)groups);
+    const int rc = run(t, (unsigned)groups);
     used = 0;
     groups = 0;
+    return rc;
   };
   for (int64_t i = 0; i < count; ++i) {
     if (sizes[i] == 0) continue;
     const int64_t mine = ceil_div(sizes[i], per_group);
     SDK_REQUIRE(mine < (int64_t)1 << 31, "tensor %lld of %lld values is too large", (long long)i,
                 (long long)sizes[i]);
-    if (used == kTensors || groups + mine >= (int64_t)1 << 31) flush();
+    if (used == kTensors || groups + mine >= (int64_t)1 << 31)
+      if (int rc = flush()) return rc;
     put(t, used, i);
     t.n[used] = sizes[i];
     t.start[used++] = (unsigned)groups;
     groups += mine;
   }
-  if (used) flush();
-  return SDK_OK;
+  return used ? flush() : SDK_OK;
 }
 
 }  // namespace
@@ -318,20 +319,19 @@ int sdk_adamw_step(void* const* params, const void* const* grads, float* const* 
     SDK_REQUIRE(sizes[i] == 0 || (sizes[i] > 0 && params[i] && grads[i] && avgs[i] && sqs[i]),
                 "tensor %lld: NULL pointer or negative size", (long long)i);
   const Settings s = settings_of(lr, beta1, beta2, eps, weight_decay, step);
-  if (int rc = deal<Tensors32>(
-          count, sizes, kPerGroup32,
-          [&](Tensors32& t, int k, int64_t i) {
-            t.p[k] = params[i];
-            t.g[k] = grads[i];
-            t.m[k] = avgs[i];
-            t.v[k] = sqs[i];
-          },
-          [&](const Tensors32& t, unsigned groups) {
-            SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(adamw32<T>, dim3(groups), dim3(256), (hipStream_t)stream, t, s));
-          }))
-    return rc;
-  SDK_LAUNCH_CHECK("adamw_step");
-  return SDK_OK;
+  return deal<Tensors32>(
+      count, sizes, kPerGroup32,
+      [&](Tensors32& t, int k, int64_t i) {
+        t.p[k] = params[i];
+        t.g[k] = grads[i];
+        t.m[k] = avgs[i];
+        t.v[k] = sqs[i];
+      },
+      [&](const Tensors32& t, unsigned groups) -> int {
+        SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(adamw32<T>, dim3(groups), dim3(256), (hipStream_t)stream, t, s));
+        SDK_LAUNCH_CHECK("adamw_step");
+        return SDK_OK;
+      });
 }
 
 int sdk_adamw_step_8bit(void* const* params, const void* const* grads, int8_t* const* avg_codes,
@@ -346,22 +346,21 @@ int sdk_adamw_step_8bit(void* const* params, const void* const* grads, int8_t* c
                                   sq_codes[i] && sq_scales[i]),
                 "tensor %lld: NULL pointer or negative size", (long long)i);
   const Settings s = settings_of(lr, beta1, beta2, eps, weight_decay, step);
-  if (int rc = deal<Tensors8>(
-          count, sizes, kPerGroup8,
-          [&](Tensors8& t, int k, int64_t i) {
-            t.p[k] = params[i];
-            t.g[k] = grads[i];
-            t.mc[k] = (signed char*)avg_codes[i];
-            t.ms[k] = avg_scales[i];
-            t.vc[k] = sq_codes[i];
-            t.vs[k] = sq_scales[i];
-          },
-          [&](const Tensors8& t, unsigned groups) {
-            SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(adamw8<T>, dim3(groups), dim3(256), (hipStream_t)stream, t, s));
-          }))
-    return rc;
-  SDK_LAUNCH_CHECK("adamw_step_8bit");
-  return SDK_OK;
+  return deal<Tensors8>(
+      count, sizes, kPerGroup8,
+      [&](Tensors8& t, int k, int64_t i) {
+        t.p[k] = params[i];
+        t.g[k] = grads[i];
+        t.mc[k] = (signed char*)avg_codes[i];
+        t.ms[k] = avg_scales[i];
+        t.vc[k] = sq_codes[i];
+        t.vs[k] = sq_scales[i];
+      },
+      [&](const Tensors8& t, unsigned groups) -> int {
+        SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(adamw8<T>, dim3(groups), dim3(256), (hipStream_t)stream, t, s));
+        SDK_LAUNCH_CHECK("adamw_step_8bit");
+        return SDK_OK;
+      });
 }
 
 int sdk_adamw_moment_values(const void* codes, const float* scales, void* out, int64_t size, int32_t second,

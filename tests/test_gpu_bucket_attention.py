@@ -372,6 +372,49 @@ def test_no_second_derivative():
         torch.autograd.grad(first.sum(), [q])
 
 
+@pytest.mark.parametrize("queries", [2, 200])
+def test_offsets_beyond_32_bits(queries):
+    """Keys and values whose tokens lie 2^22 elements apart, in 5.9 GB: the bits of dense ones, forward and backward."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 2, 1, queries, 700, 64, 20, torch.bfloat16, seed=17)
+    apart = 1 << 22
+    memory = torch.empty(700 * apart, dtype=torch.bfloat16, device=DEV)
+    results = []
+    for far in (False, True):
+        pair = []
+        for i, t in enumerate((k, v)):
+            if far:
+                view = memory[64 * i:].as_strided((1, 1, 700, 64), (apart, apart, apart, 1), storage_offset=64 * i)
+                view.copy_(t)
+                t = view
+            pair.append(t)
+        leaves = [t.detach().requires_grad_() for t in (q, *pair, table)]
+        out = F.bucket_attention(*leaves, bmap)
+        results.append((out, *torch.autograd.grad(out, leaves, do)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_a_map_of_more_than_4_gb():
+    """66000 x 66000 pairs: the last queries against a call of their own, forward and gradient."""
+    from spherical_distortion import functional as F
+    n, last = 66000, 300
+    g = torch.Generator(device=DEV).manual_seed(18)
+    q, k, v = (torch.randn(1, 1, n, 8, generator=g, device=DEV).to(torch.bfloat16) for _ in range(3))
+    table = torch.randn(1, 40, generator=g, device=DEV)
+    bmap = torch.randint(0, 40, (n, n), generator=g, device=DEV, dtype=torch.uint8)
+    do = torch.zeros_like(q)
+    do[:, :, -last:] = torch.randn(1, 1, last, 8, generator=g, device=DEV).to(torch.bfloat16)
+    results = []
+    for first in (0, n - last):
+        leaves = [t.detach().requires_grad_() for t in (q[:, :, first:], k, v, table)]
+        out = F.bucket_attention(*leaves, bmap[first:])
+        grads = torch.autograd.grad(out, leaves, do[:, :, first:])
+        results.append([t.detach().double().cpu() for t in (out[:, :, -last:], grads[0][:, :, -last:], *grads[1:])])
+    for a, b in zip(*results):   # sums over 66000 keys in other parts: each within the type's bound of the exact one
+        assert float((a - b).abs().max()) <= 2 * TOL[torch.bfloat16] * float(b.abs().max())
+
+
 def test_refusals():
     from spherical_distortion import functional as F
     q, k, v, table, bmap, do = _inputs(2, 4, 2, 8, 9, 16, 3, torch.float32, seed=1)
