@@ -90,6 +90,9 @@ SHAPES = [  # B, H, Hk, Lq, Lk, D, buckets
     (1, 3, 3, 200, 130, 128, 129),
     (1, 2, 2, 33, 700, 96, 250),
     (1, 8, 1, 5, 600, 128, 256),
+    (2, 2, 1, 9, 300, 88, 12),
+    (1, 2, 2, 40, 90, 112, 17),
+    (1, 4, 1, 150, 140, 96, 40),
 ]
 
 
