@@ -534,7 +534,7 @@ int run_forward(const sdk_bucket_attention* a, void* workspace, hipStream_t s);
 int run_backward(const sdk_bucket_attention* a, void* workspace, hipStream_t s);
 
 // Runs the statement with DP, the padded dim, a multiple of the products' 32 columns.  96 beside 128: 2 x 16 heads of 80,
-// 2048 tokens, 75 us for 93 forward and 461 for 525 with gradients in bfloat16; 1024 tokens in float32 411 for 617, whose
+// 2048 tokens, 75 us for 93 forward and 398 for 525 with gradients in bfloat16; 1024 tokens in float32 411 for 617, whose
 // registers of three pieces then fit.
 #define ATTENTION_DIM(dim, ...)                                  \
   do {                                                           \

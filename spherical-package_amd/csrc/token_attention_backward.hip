@@ -16,9 +16,13 @@ namespace sdk {
 namespace token {
 namespace {
 
-// Waves of a SIMD: with two, accumulators lie among the 256 registers of a wave.
-template <int DP>
-constexpr int kBackwardWaves = DP <= 64 ? 2 : 1;
+// Waves of a SIMD: with two, accumulators lie among the 256 registers of a wave.  Heads of 96 in 16 bits spill 12 to 24
+// bytes for it in grad_queries, once: 2 x 16 heads of 80, 2048 tokens, forward and backward 398 us for 460; heads of 128
+// would spill 200 to 440.
+template <typename T, int DP>
+constexpr int kQueryWaves = DP <= (sizeof(T) == 2 ? 96 : 64) ? 2 : 1;
+template <typename T, int DP>
+constexpr int kKeyWaves = DP <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1;
 
 template <typename T>
 constexpr float kLift = __is_same(T, f16) ? 8.f : 0.f;   // log2 of what p is held times
@@ -103,7 +107,9 @@ __global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta
   }
   if constexpr (__is_same(T, f16)) {   // the order of a maximum does not matter
     most = over_group<Largest, 256>(most, slots);
-    if (threadIdx.x == 0) atomicMax(top, __float_as_uint(most) & 0x7fffffffu);
+    const unsigned mine = __float_as_uint(most) & 0x7fffffffu;
+    // most groups see a larger one there already: 18 us for 21 over 65536 rows of 128
+    if (threadIdx.x == 0 && mine > __hip_atomic_load(top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(top, mine);
   }
 }
 
@@ -144,7 +150,7 @@ __device__ __forceinline__ void add_by_bucket(float* column, const Buckets& buck
 // the rounding of the weights is 40.
 // part: splits > 1: float32 sums of the splits, [split][row][dim].
 template <typename T, int DP, int COLUMNS>
-__global__ __launch_bounds__(kThreads, kBackwardWaves<DP>) void grad_queries(
+__global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
     const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top, float* part,
     float* table_parts) {
   constexpr int NT = kParts<T>, KEYS = 32 * NT;
@@ -315,7 +321,7 @@ __global__ __launch_bounds__(256) void join_table(const Attention a, int each, c
 // other buffer.  Bound by LDS (both operands straight and turned) and what it does not overlap: 4 key heads of 16 heads
 // of 64, 8192 x 8192 pairs in bfloat16 take 755 us, 730 TFLOP/s.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 32 ? 1 : kBackwardWaves<DP>) void grad_keys(
+__global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
     const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top,
     const uint8_t* turned, int pitch, float* part) {
   constexpr int NT = kParts<T>, ROWS = 32 * NT;
@@ -486,8 +492,9 @@ Space space_of(const sdk_bucket_attention* a) {
   const int64_t q_rows = a->batch * a->heads * a->queries, k_rows = a->batch * a->key_heads * a->keys;
   const int64_t q_groups = a->batch * a->heads * ceil_div(a->queries, rows);
   // workgroups that run at once, by the registers of their waves
-  const int64_t slots = a->dim <= 64 ? 512 : 256, key_slots = a->dtype == SDK_F32 && a->dim > 32 ? 256 : slots;
-  w.query_splits = parts_of(q_groups, ceil_div(a->keys, tile), slots, false);
+  const bool wide = a->dtype == SDK_F32;
+  const int64_t query_slots = a->dim <= (wide ? 64 : 96) ? 512 : 256, key_slots = a->dim <= (wide ? 32 : 64) ? 512 : 256;
+  w.query_splits = parts_of(q_groups, ceil_div(a->keys, tile), query_slots, false);
   w.key_splits = parts_of(a->batch * a->key_heads * ceil_div(a->keys, rows),
                           a->heads / a->key_heads * ceil_div(a->queries, tile), key_slots, a->causal);
   w.pitch = (int)ceil_div(a->queries, 64) * 64;
@@ -540,7 +547,7 @@ int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t
   if (__is_same(T, f16) && a->batch > 0) launch(clear_word, dim3(1), dim3(1), s, top);
   if (any) {
     constexpr int LANES = 128 / kWide<T>;
-    // few workgroups where each ends with an atomic: 16384 of them took 190 us
+    // few workgroups where each ends with an atomic: 16384 of them took 190 us, 2048 took 21 for 18
     const int64_t groups = std::min<int64_t>(ceil_div(rows, 256 / LANES), __is_same(T, f16) ? 1024 : 1 << 30);
     launch(row_terms<T, LANES>, dim3((unsigned)groups), dim3(256), s, d, delta, lse2, top);
     if (a->grad_query || a->grad_table) {
