@@ -266,8 +266,6 @@ struct Carry {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) v[n] = __builtin_amdgcn_raw_buffer_load_b128(all, at[n], 0, 0);
   }
-  // the tile's token that vector n belongs to
-  __device__ __forceinline__ int token(int n) const { return (n * THREADS + (int)threadIdx.x) / kVectors; }
   __device__ __forceinline__ void scale(int n, float by) {
     Pack<T, kWide<T>> x = __builtin_bit_cast(Pack<T, kWide<T>>, v[n]);
 #pragma unroll

@@ -327,11 +327,12 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
   constexpr int NT = kParts<T>, ROWS = 32 * NT;
   __shared__ __attribute__((aligned(16))) struct {
     float table[kTable];
-    float row_lse[2][ROWS], row_delta[2][ROWS];
-    Tile<T, DP, NT> queries[2], grads[2];
+    float row_lse[2][ROWS], row_delta[2][ROWS], row_factor[2][ROWS];
+    Tile<T, DP, NT> queries[2], grads[2];   // 16-byte aligned
+    int far[2];                             // whether some row of the tile has a factor
   } lds;
   auto& table = lds.table;
-  auto &row_lse = lds.row_lse, &row_delta = lds.row_delta;
+  auto &row_lse = lds.row_lse, &row_delta = lds.row_delta, &row_factor = lds.row_factor;
   auto &queries = lds.queries, &grads = lds.grads;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, h = lane / 32;
   const Work work(tiles, a.batch * a.key_heads, splits, a.causal, true);
@@ -357,8 +358,7 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
 
   Carry<T, DP, NT, kThreads> next_q(a.qs[2], a.dim), next_g(a.gs[2], a.dim);
   Buckets bucket[NT], next_bucket[NT];
-  float next_lse = 0.f, next_delta = 0.f, next_rest = 0.f, next_level[decltype(next_g)::kCount];
-  int64_t next_row = 0;
+  float next_lse = 0.f, next_delta = 0.f, next_rest = 0.f;
   const float* rests = a.lse + (int64_t)a.batch * a.heads * a.queries;
   auto request = [&](int unit) {
     const int head = shared_head * group + unit / each, q0 = from + unit % each * ROWS;
@@ -367,13 +367,9 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
 #pragma unroll
     for (int t = 0; t < NT; ++t)   // rows of the turned map are padded to whole tiles
       next_bucket[t].load(map + q0 + 16 * NT * h + 16 * t);
-    next_row = ((int64_t)b * a.heads + head) * a.queries + q0;
-#pragma unroll
-    for (int n = 0; n < next_g.kCount; ++n)
-      next_level[n] = lse2[next_row + std::min(next_g.token(n), a.queries - 1 - q0)];
     if (threadIdx.x < ROWS) {
       const int q = q0 + threadIdx.x;
-      const int64_t row = next_row + threadIdx.x;
+      const int64_t row = ((int64_t)b * a.heads + head) * a.queries + q;
       next_lse = INFINITY, next_delta = 0.f, next_rest = 0.f;
       // worked on in put: nothing waits here
       if (q < a.queries) next_lse = lse2[row], next_delta = delta[row], next_rest = rests[row];
@@ -381,19 +377,18 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
   };
   auto put = [&](int buffer) {
     next_q.store(queries[buffer]);
-    // a row's factor belongs to p: do and D take it instead (the rows that have one are rare)
+    if constexpr (__is_same(T, f16)) {
 #pragma unroll
-    for (int n = 0; n < next_g.kCount; ++n) {
-      const Lse<T> lse(next_level[n], 0.f, false);
-      float by = held;
-      if (__any(lse.far)) by *= Lse<T>(next_level[n], lse.far ? rests[next_row + next_g.token(n)] : 0.f, false).factor;
-      if (__is_same(T, f16) || __any(lse.far)) next_g.scale(n, by);
+      for (int n = 0; n < next_g.kCount; ++n) next_g.scale(n, held);
     }
     next_g.store(grads[buffer]);
-    if (threadIdx.x < ROWS) {
+    if (threadIdx.x < ROWS) {   // lanes of the first wave
       const Lse<T> lse(next_lse, next_rest, false);
       row_lse[buffer][threadIdx.x] = -lse.off;
-      row_delta[buffer][threadIdx.x] = -next_delta * held * lse.factor;
+      row_delta[buffer][threadIdx.x] = -next_delta * held;
+      row_factor[buffer][threadIdx.x] = lse.factor;
+      const unsigned long long some = __ballot(lse.far);
+      if (threadIdx.x == 0) lds.far[buffer] = some != 0;
     }
   };
   auto put_bias = [&](int unit) {
@@ -414,6 +409,8 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
     request(more ? unit + 1 : unit);   // it has landed by `put`: until then no load is waited for
     const auto query_view = queries[now].view(lane), grad_view = grads[now].view(lane);
     const float *now_lse = row_lse[now] + 16 * NT * h, *now_delta = row_delta[now] + 16 * NT * h;
+    const float* now_factor = row_factor[now] + 16 * NT * h;
+    const bool some_far = __builtin_amdgcn_readfirstlane(lds.far[now]) != 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       floatx16 s = dot_tile<T, DP>(query_view, t, k, [&](int i) { return table[bucket[t][i]]; });
@@ -426,6 +423,10 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
       float p[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, now_lse[16 * t + i]));
+      if (some_far) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] *= now_factor[16 * t + i];
+      }
       {
         const Operand<T> w[2] = {rounded<T>(p), rounded<T>(p + 8)};
         add_columns<T>(dv, grad_view, t, w);

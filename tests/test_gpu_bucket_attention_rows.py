@@ -1,0 +1,31 @@
+"""Rows that stand apart in the backward of attention with a bias for each bucket: those whose level lies beyond what a
+sum can be added to.  Inputs, definition and bounds are those of test_gpu_bucket_attention."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_bucket_attention import DEV, TOL, _close, _exact, _inputs, _terms
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [1, 33, 65, 70])
+def test_a_masked_last_row_reads_nothing_behind_it(queries, dtype):
+    """The last query of the last head has nothing but the lowest bias, and its tile ends behind it: what lies behind
+    the rows' sums in memory (here NaN, in memory of this test) plays no part."""
+    from _spherical_distortion_ext._token_ops import ops
+    q, k, v, table, bmap, do = _inputs(2, 4, 2, queries, 90, 64, 6, dtype, seed=40 + queries)
+    table[-1, 2] = torch.finfo(torch.float32).min
+    bmap[-1] = 2
+    scale = 64 ** -0.5
+    out, rest, lse = ops.bucket_attention_forward(q, k, v, table, bmap, None, False, scale)
+    memory = torch.full((lse.numel() + 256,), math.nan, device=DEV)
+    held = memory[:lse.numel()].view(lse.shape)
+    held.copy_(lse)
+    grads = ops.bucket_attention_backward(do, q, k, v, table, bmap, None, out, rest, held, False, scale, True, True, True)
+    want = _exact(q, k, v, table, bmap, grad=do)
+    for got, ref, terms in zip((out, *grads), want, _terms(q, k, v, do)):
+        _close(got, ref, TOL[dtype], terms)
