@@ -3,9 +3,11 @@
 // implementation of each) in C++, where a call of a few microseconds on the GPU is not bound by its host side.
 // Part of libsdk_torch_ops.so; no device code here.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <cstdint>
@@ -366,11 +368,31 @@ Tensor adamw_moment_values(const Tensor& codes, const Tensor& scales, at::Scalar
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// Below autograd a tangent would be left out.
+void no_tangent(std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                "forward-mode derivatives of this operator are not implemented");
+}
+
 bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
+  no_tangent(tensors);
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Gradients of a backward that is itself recorded (create_graph): they ask for a gradient, and raise when it is formed.
+// Plain tensors would be constants to whatever is differentiated beside them.
+variable_list only_first(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  const auto node = std::make_shared<torch::autograd::DelayedError>(
+      "second derivatives of this operator are not implemented", (int64_t)grads.size());
+  return (*node)(std::move(grads));
 }
 
 struct BucketAttention : torch::autograd::Function<BucketAttention> {
@@ -383,7 +405,8 @@ struct BucketAttention : torch::autograd::Function<BucketAttention> {
     ctx->saved_data["scale"] = scale;
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  static variable_list backward(AutogradContext* ctx, variable_list grads) { return only_first(gradients(ctx, grads)); }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
     const OptTensor n = saved[5].defined() ? OptTensor(saved[5]) : OptTensor();
     const bool need_q = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2),
@@ -422,7 +445,8 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     ctx->set_materialize_grads(false);
     return alone ? variable_list{out} : variable_list{out, summed};
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  static variable_list backward(AutogradContext* ctx, variable_list grads) { return only_first(gradients(ctx, grads)); }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
     const bool alone = ctx->saved_data["alone"].toBool();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
@@ -444,8 +468,8 @@ std::vector<Tensor> rms_norm_pair(const Tensor& x, const OptTensor& residual, co
 
 std::vector<Tensor> rms_norm_pair_autograd(const Tensor& x, const OptTensor& residual, const Tensor& weight,
                                            double eps) {
-  if (wants_gradient({&x, &weight}) || (has(residual) && wants_gradient({&*residual})))
-    return AddRmsNorm::apply(x, weight, residual, eps);
+  const Tensor other = has(residual) ? *residual : Tensor();
+  if (wants_gradient({&x, &weight, &other})) return AddRmsNorm::apply(x, weight, residual, eps);
   at::AutoDispatchBelowADInplaceOrView guard;
   return rms_norm_pair(x, residual, weight, eps);
 }

@@ -5,13 +5,45 @@ tangent images): attention whose learned bias goes by the bucket of a pair's rel
 norm of a block with its residual, and the optimizer step.  The reference has none of them.
 float32, bfloat16 and float16; sums, softmax statistics and norms are float32.
 """
+import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
+from torch.autograd import forward_ad
 
 from _spherical_distortion_ext import _token_ops
 from _spherical_distortion_ext._ops import ops as _sdk_ops
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(g if g is None else g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("second derivatives of this operator are not implemented")
+
+
+def _only_first(backward):
+    """A backward whose gradients, where it is itself recorded (create_graph), ask for a gradient and raise when it is
+    formed.  Plain tensors would be constants to whatever is differentiated beside them."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        return _NoSecondDerivative.apply(*(g if g is None else g.detach().requires_grad_() for g in out))
+    return run
+
+
+def _wants_gradient(*tensors):
+    """Whether autograd is to see the call (of the Python functions; the compiled layer finds out by itself)."""
+    tensors = [t for t in tensors if t is not None]
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("forward-mode derivatives of this operator are not implemented")
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 class BucketAttentionFunction(torch.autograd.Function):
@@ -24,7 +56,7 @@ class BucketAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_only_first
     def backward(ctx, grad_output):
         query, key, value, bias_table, bucket_map, key_lengths, out, rest, lse = ctx.saved_tensors
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
@@ -49,13 +81,12 @@ def bucket_attention(query, key, value, bias_table, bucket_map, key_lengths=None
     mask by the type's lowest weighs nothing beside others, and the same among themselves.  scale: dim ** -0.5
     if None.
 
-    With gradients for query, key, value and bias_table.  A few queries against many keys (one new
-    token and its cache) are dealt to the GPU along the keys."""
+    With gradients for query, key, value and bias_table; second derivatives and forward mode raise.  A few
+    queries against many keys (one new token and its cache) are dealt to the GPU along the keys."""
     scale = 1.0 / math.sqrt(query.shape[-1]) if scale is None else float(scale)
     if "bucket_attention" in _token_ops.NATIVE_OPS:
         return _sdk_ops.bucket_attention(query, key, value, bias_table, bucket_map, key_lengths, bool(causal), scale)
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad
-                                    or bias_table.requires_grad):
+    if _wants_gradient(query, key, value, bias_table):
         return BucketAttentionFunction.apply(query, key, value, bias_table, bucket_map, key_lengths, bool(causal),
                                              scale)
     return _sdk_ops.bucket_attention_forward(query, key, value, bias_table, bucket_map, key_lengths, bool(causal),
@@ -72,7 +103,7 @@ class AddRMSNormFunction(torch.autograd.Function):
         return (out, x.view_as(x)) if ctx.alone else (out, summed)
 
     @staticmethod
-    @once_differentiable
+    @_only_first
     def backward(ctx, grad, grad_sum):
         summed, weight, inverse = ctx.saved_tensors
         need_x, need_r, need_w, _ = ctx.needs_input_grad
@@ -87,12 +118,12 @@ class AddRMSNormFunction(torch.autograd.Function):
 def add_rms_norm(input, residual, weight, eps=1e-6):
     """(weight * h / sqrt(mean(h ** 2) + eps), h) with h = input + residual, over the last axis; a
     residual of None adds nothing.  weight: one value for each of the last axis (up to 16384), of the
-    input's type or float32.  The sum is normalised before it is rounded to the input's type."""
+    input's type or float32.  The sum is normalised before it is rounded to the input's type.  Second
+    derivatives and forward mode raise."""
     if "rms_norm_pair" in _token_ops.NATIVE_OPS:
         both = _sdk_ops.rms_norm_pair(input, residual, weight, float(eps))
         return (both[0], input) if residual is None else (both[0], both[1])
-    if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
+    if _wants_gradient(input, residual, weight):
         return AddRMSNormFunction.apply(input, residual, weight, float(eps))
     out, summed, _ = _sdk_ops.add_rms_norm(input, residual, weight, float(eps))
     return out, input if residual is None else summed
