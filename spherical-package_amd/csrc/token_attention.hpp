@@ -266,12 +266,6 @@ struct Carry {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) v[n] = __builtin_amdgcn_raw_buffer_load_b128(all, at[n], 0, 0);
   }
-  __device__ __forceinline__ void scale(int n, float by) {
-    Pack<T, kWide<T>> x = __builtin_bit_cast(Pack<T, kWide<T>>, v[n]);
-#pragma unroll
-    for (int e = 0; e < kWide<T>; ++e) x.v[e] = (T)((float)x.v[e] * by);
-    v[n] = __builtin_bit_cast(u32x4, x);
-  }
   __device__ __forceinline__ void store(Tile<T, DP, NT>& tile) const {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {

@@ -7,9 +7,9 @@
 // The scores are formed again from the lse, once with the queries in registers (dq, dT) and once with the keys (dk,
 // dv): seven products instead of five, and no sum whose order depends on scheduling.
 //
-// float16 has few exponents: p (about 1 / keys) and ds would fall among its subnormal numbers.  There p is held times
-// 2^8, and do times a power of two that brings its largest magnitude to 2^-7 .. 2^-6 (ds then overflows beside values
-// beyond 128 alone); both are taken out of the sums, exactly.
+// float16 has few exponents: p (about 1 / keys) and ds would fall among its subnormal numbers, or beyond its largest.
+// There p is held times 2^8 and ds times a power of two of its own row (dq) or key (dk), so that rows and keys of any
+// size keep their precision beside others; they are taken out of the sums, exactly.  dv takes do as it is.
 #include "token_attention.hpp"
 
 namespace sdk {
@@ -27,28 +27,33 @@ constexpr int kKeyWaves = DP <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1;
 template <typename T>
 constexpr float kLift = __is_same(T, f16) ? 8.f : 0.f;   // log2 of what p is held times
 
-// What do is held times: from the bits of its largest magnitude.
-template <typename T>
-__device__ __forceinline__ float gradient_scale(const unsigned* top) {
-  if constexpr (!__is_same(T, f16)) return 1.f;
-  const unsigned exponent = *top >> 23;
-  return exponent == 0 || exponent >= 255 ? 1.f : __uint_as_float((247 - exponent) << 23);
-}
+// float16, dq: what p is held times (log2: lift) and what a row's do is (by).  With size = sum |do| of the row and value =
+// the largest |v|, |ds| is at most p 2 size value: below 2^15 as held.  Values beyond 2^9 lower the lift instead of
+// do, whose numbers would become subnormal.  p of far rows (Lse) reaches 2^10, not 2^lift.
+struct Hold {
+  float lift = kLift<f16>, by = 1.f;
+  __device__ __forceinline__ Hold(float size, float value, bool far) {
+    if (!(size > 0.f && size < INFINITY && value < INFINITY)) return;   // nothing to hold, or nothing finite
+    const int s = (int)(__float_as_uint(size) >> 23) - 126;             // size < 2^s
+    const int v = std::max((int)(__float_as_uint(value) >> 23) - 126, -8), up = 17 - std::max(v, 9);
+    lift = (float)up;
+    by = __uint_as_float((unsigned)(127 + 14 - (far ? 10 : up) - s - v) << 23);
+  }
+};
 
-// A row's level and log2 of its sum as p = 2^(scale2 s - off) * factor, lifted.  whole: off is a whole number, for
+// A row's level and log2 of its sum as p = 2^(scale2 s - off) * factor, times 2^lift.  whole: off is a whole number, for
 // weights that round as the forward's did; the factor is then between 1 and 2.  Else it is 1, but for levels (of rows
 // that biases mask) that would swallow what is added to them.
-template <typename T>
+__device__ __forceinline__ bool is_far(float level) { return fabsf(level) > 1024.f && fabsf(level) < INFINITY; }
 struct Lse {
   float off, factor = 1.f;
   bool far;
-  __device__ __forceinline__ Lse(float level, float part, bool whole) : off(level) {
-    far = fabsf(level) > 1024.f && fabsf(level) < INFINITY;
+  __device__ __forceinline__ Lse(float level, float part, bool whole, float lift) : off(level), far(is_far(level)) {
     const float up = whole ? ceilf(part) : part;
     if (far)
-      factor = __builtin_amdgcn_exp2f(kLift<T> - part);
+      factor = __builtin_amdgcn_exp2f(lift - part);
     else
-      off += up - kLift<T>, factor = __builtin_amdgcn_exp2f(up - part);
+      off += up - lift, factor = __builtin_amdgcn_exp2f(up - part);
   }
 };
 
@@ -64,16 +69,33 @@ __device__ __forceinline__ void flip(Operand<T>& x, bool odd) {
 }
 
 // ------------------------------------------------------------------------------------------ terms of a row
-__global__ void clear_word(unsigned* word) { *word = 0; }
-
-// D_i and the row's level (+inf for a query without pairs: its p are zeros); float16: the largest |do|.
-// A row is read by LANES lanes, 16 bytes each.
-template <typename T, int LANES>
-__global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta, float* lse2, unsigned* top) {
+// float16: the largest |v| among the keys that count of each key head, in `parts` parts of the keys.
+constexpr int kMostParts = 64;   // a lane each where they are read
+__global__ __launch_bounds__(256) void value_sizes(const Attention a, int parts, float* sizes) {
   __shared__ float slots[4];
+  const int part = (int)(blockIdx.x % (unsigned)parts), bh = (int)(blockIdx.x / (unsigned)parts);
+  const int head = bh % a.key_heads, b = bh / a.key_heads, d = 8 * (threadIdx.x % 16);
+  const int len = a.length(b), to = split_at(len, part + 1, parts);
+  const f16* v = (const f16*)a.v + b * a.vs[0] + head * a.vs[1] + d;
+  float most = 0.f;
+#pragma unroll 4
+  for (int key = split_at(len, part, parts) + threadIdx.x / 16; key < to; key += 16) {
+    if (d >= a.dim) continue;
+    float x[8];
+    load_pack<f16, 8>(v + key * a.vs[2], x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = Largest::of(most, fabsf(x[e]));
+  }
+  most = over_group<Largest, 256>(most, slots);
+  if (threadIdx.x == 0) sizes[blockIdx.x] = most;
+}
+
+// D_i and the row's level (+inf for a query without pairs: its p are zeros).  A row is read by LANES lanes, 16 bytes
+// each.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta, float* lse2) {
   const int lane = threadIdx.x % LANES, d = kWide<T> * lane;
   const int64_t rows = (int64_t)a.batch * a.heads * a.queries;
-  float most = 0.f;
   for (int64_t first = (int64_t)blockIdx.x * (256 / LANES); first < rows; first += (int64_t)gridDim.x * (256 / LANES)) {
     const int64_t row = first + threadIdx.x / LANES;
     float dot = 0.f;
@@ -91,10 +113,7 @@ __global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta
         }
         load_pack<T, kWide<T>>((const T*)a.grad + b * a.gs[0] + head * a.gs[1] + query * a.gs[2] + d, y);
 #pragma unroll
-        for (int e = 0; e < kWide<T>; ++e) {
-          dot = fmaf(x[e], y[e], dot);
-          if constexpr (__is_same(T, f16)) most = Largest::of(most, fabsf(y[e]));
-        }
+        for (int e = 0; e < kWide<T>; ++e) dot = fmaf(x[e], y[e], dot);
       }
     }
 #pragma unroll
@@ -104,12 +123,6 @@ __global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta
       delta[row] = dot;
       lse2[row] = l == -INFINITY ? INFINITY : l;
     }
-  }
-  if constexpr (__is_same(T, f16)) {   // the order of a maximum does not matter
-    most = over_group<Largest, 256>(most, slots);
-    const unsigned mine = __float_as_uint(most) & 0x7fffffffu;
-    // most groups see a larger one there already: 18 us for 21 over 65536 rows of 128
-    if (threadIdx.x == 0 && mine > __hip_atomic_load(top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(top, mine);
   }
 }
 
@@ -128,18 +141,19 @@ __global__ __launch_bounds__(256) void turn_map(const Attention a, uint8_t* turn
 }
 
 // ------------------------------------------------------------------------------------------ dq and the bias table
-// Adds x to the sums of its buckets in one lane's column, two at a time: read, add, write, and where the two meet the
+// Adds x * by to the sums of its buckets in one lane's column, two at a time: read, add, write, and where the two meet the
 // second takes the first's sum.  (An LDS float add of 64 lanes takes 193 cycles of a CU whatever its addresses, this
 // 13; by four or eight the comparisons cost more than the waits they save: 842 and 971 us of the kernel at 8192 x
 // 8192 pairs of 16 heads, 817 by two.)
 template <int COLUMNS>
-__device__ __forceinline__ void add_by_bucket(float* column, const Buckets& bucket, int buckets, const float* x) {
+__device__ __forceinline__ void add_by_bucket(float* column, const Buckets& bucket, int buckets, const float* x,
+                                              float by) {
 #pragma unroll
   for (int v = 0; v < 16; v += 2) {
     const int at = std::min((int)bucket[v], buckets) * COLUMNS, next = std::min((int)bucket[v + 1], buckets) * COLUMNS;
-    const float sum = column[at] + x[v], other = column[next];
+    const float sum = column[at] + x[v] * by, other = column[next];
     column[at] = sum;
-    column[next] = (next == at ? sum : other) + x[v + 1];
+    column[next] = (next == at ? sum : other) + x[v + 1] * by;
   }
 }
 
@@ -151,8 +165,8 @@ __device__ __forceinline__ void add_by_bucket(float* column, const Buckets& buck
 // part: splits > 1: float32 sums of the splits, [split][row][dim].
 template <typename T, int DP, int COLUMNS>
 __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
-    const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top, float* part,
-    float* table_parts) {
+    const Attention a, int splits, int tiles, const float* delta, const float* lse2, const float* sizes, int size_parts,
+    float* part, float* table_parts) {
   constexpr int NT = kParts<T>, KEYS = 32 * NT;
   __shared__ __attribute__((aligned(16))) struct {
     float table[kTable];   // at address zero: a lookup's address is four times the bucket
@@ -182,15 +196,24 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
   const uint8_t* map = a.map + b * a.ms[0] + clamped * a.ms[1];
   const int last = a.causal ? std::min(len - 1, clamped + shift) : len - 1;
   const bool in = query < a.queries;
-  const float held = gradient_scale<T>(top);
-  const Lse<T> lse(in ? lse2[row] : INFINITY, in ? a.lse[(int64_t)a.batch * a.heads * a.queries + row] : 0.f, true);
-  const float my_lse = lse.off, rest = lse.factor;   // rest: a factor of everything this lane sums
-  float my_delta = in ? delta[row] * held : 0.f;
+  const float level = in ? lse2[row] : INFINITY;
 
   Operand<T> q[DP / 16], g[DP / 16];
   load_columns<T, DP>(q, (const T*)a.q + b * a.qs[0] + head * a.qs[1], a.qs[2], query, in, a.dim, lane);
   load_columns<T, DP>(g, (const T*)a.grad + b * a.gs[0] + head * a.gs[1], a.gs[2], query, in, a.dim, lane);
+  float lift = kLift<T>, held = 1.f;
   if constexpr (__is_same(T, f16)) {
+    float size = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const f16x8 x = __builtin_bit_cast(f16x8, g[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) size += fabsf((float)x[e]);
+    }
+    const int64_t at = ((int64_t)b * a.key_heads + shared_head) * size_parts;
+    const float value = over_wave<Largest>(lane < size_parts ? sizes[at + lane] : 0.f);
+    const Hold hold(size + other_half(size), value, is_far(level));
+    lift = hold.lift, held = hold.by;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       f16x8 x = __builtin_bit_cast(f16x8, g[c]);
@@ -199,10 +222,17 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
       g[c] = __builtin_bit_cast(Operand<T>, x);
     }
   }
+  const Lse lse(level, in ? a.lse[(int64_t)a.batch * a.heads * a.queries + row] : 0.f, true, lift);
+  const float my_lse = lse.off;
+  float my_delta = in ? delta[row] * held : 0.f;
   // Odd lanes work with -do and -D, so that ds has the other sign: what the matrix unit's rounding leaves to one side
   // would add up in the table's sums, which cancel over many rows.  A lane's row and column are all of one sign.
   const float sign = lane % 2 ? -1.f : 1.f;
   my_delta *= sign;
+  // A factor of everything this lane sums.  16 columns hold two queries each, whose factors the table's sums take pair by
+  // pair: float16's, which have any size, beside ds, the others with it (15 registers fewer).
+  constexpr bool BESIDE = COLUMNS == 16 && __is_same(T, f16), WITHIN = COLUMNS == 16 && !BESIDE;
+  const float back = exp2f(-lift) / held * sign * (WITHIN ? 1.f : lse.factor);
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) flip(g[c], lane % 2);
   floatx16 dq[DP / 32];
@@ -245,14 +275,15 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
       as_rounded<T>(ds);
 #pragma unroll
       for (int v = 0; v < 16; ++v) ds[v] *= e[v];
-      if constexpr (COLUMNS == 16) {   // two queries to a column
+      if constexpr (WITHIN) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) ds[v] *= rest;
+        for (int v = 0; v < 16; ++v) ds[v] *= lse.factor;
       }
       if constexpr (COLUMNS > 0) {
 #pragma unroll
         for (int turn = 0; turn < 64 / COLUMNS; ++turn) {
-          if (lane / COLUMNS == turn) add_by_bucket<COLUMNS>(mine + lane % COLUMNS, bucket[t], a.buckets, ds);
+          if (lane / COLUMNS == turn)
+            add_by_bucket<COLUMNS>(mine + lane % COLUMNS, bucket[t], a.buckets, ds, BESIDE ? back : 1.f);
           if (COLUMNS < 64) wave_order();   // the next turn's lanes read what these wrote
         }
       }
@@ -266,16 +297,15 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
   if constexpr (sizeof(T) == 2)   // float32: the registers do not hold two loops (170 us for 149 with one)
     for (; k0 < std::min(to, whole); k0 += KEYS) step(k0, std::false_type());
   for (; k0 < to; k0 += KEYS) step(k0, std::true_type());
-  const float back = exp2f(-kLift<T>) / held, mine_back = back * sign * (COLUMNS == 16 ? 1.f : rest);
   if (in && splits > 1)
     store_columns<float, DP>(part + ((int64_t)work.split * a.batch * a.heads * a.queries + row) * a.dim, a.dim, 0, a.dim,
-                             lane, dq, a.scale * mine_back);
+                             lane, dq, a.scale * back);
   else if (in && a.dq)
     store_columns<T, DP>((T*)a.dq + b * a.dqs[0] + head * a.dqs[1], a.dqs[2], query, a.dim, lane, dq,
-                         a.scale * mine_back);
+                         a.scale * back);
   if constexpr (COLUMNS > 0) {
     __shared__ float column_back[kWaves][COLUMNS];
-    if (lane < COLUMNS) column_back[wave][lane] = mine_back;
+    if (lane < COLUMNS) column_back[wave][lane] = BESIDE ? 1.f : back;
     __syncthreads();
     for (int i = threadIdx.x; i < a.buckets; i += kThreads) {
       float x = 0.f;
@@ -322,8 +352,8 @@ __global__ __launch_bounds__(256) void join_table(const Attention a, int each, c
 // of 64, 8192 x 8192 pairs in bfloat16 take 755 us, 730 TFLOP/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
-    const Attention a, int splits, int tiles, const float* delta, const float* lse2, const unsigned* top,
-    const uint8_t* turned, int pitch, float* part) {
+    const Attention a, int splits, int tiles, const float* delta, const float* lse2, const uint8_t* turned,
+    int pitch, float* part) {
   constexpr int NT = kParts<T>, ROWS = 32 * NT;
   __shared__ __attribute__((aligned(16))) struct {
     float table[kTable];
@@ -341,7 +371,6 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
   const int first = work.tile * (32 * kWaves), key = first + wave * 32 + lane % 32;
   const int len = a.length(b), shift = len - a.queries;
   const uint8_t* map = turned + ((a.ms[0] ? (int64_t)b * a.keys : 0) + std::min(key, a.keys - 1)) * pitch;
-  const float held = gradient_scale<T>(top);
 
   Operand<T> k[DP / 16], v[DP / 16];
   load_columns<T, DP>(k, (const T*)a.k + b * a.ks[0] + shared_head * a.ks[1], a.ks[2], key, key < len, a.dim, lane);
@@ -349,6 +378,7 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
   floatx16 dk[DP / 32], dv[DP / 32];
   clear(dk);
   clear(dv);
+  float held = __is_same(T, f16) ? 0x1p100f : 1.f;   // what this key's ds are held times
 
   // tiles of queries that see some key of the workgroup, head after head
   const int from = a.causal ? std::max(0, first - shift) / ROWS * ROWS : 0;
@@ -377,15 +407,11 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
   };
   auto put = [&](int buffer) {
     next_q.store(queries[buffer]);
-    if constexpr (__is_same(T, f16)) {
-#pragma unroll
-      for (int n = 0; n < next_g.kCount; ++n) next_g.scale(n, held);
-    }
     next_g.store(grads[buffer]);
     if (threadIdx.x < ROWS) {   // lanes of the first wave
-      const Lse<T> lse(next_lse, next_rest, false);
+      const Lse lse(next_lse, next_rest, false, kLift<T>);
       row_lse[buffer][threadIdx.x] = -lse.off;
-      row_delta[buffer][threadIdx.x] = -next_delta * held;
+      row_delta[buffer][threadIdx.x] = -next_delta;
       row_factor[buffer][threadIdx.x] = lse.factor;
       const unsigned long long some = __ballot(lse.far);
       if (threadIdx.x == 0) lds.far[buffer] = some != 0;
@@ -433,6 +459,25 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] *= e[i];   // ds
+      if constexpr (__is_same(T, f16)) {
+        // Held below 2: where a larger one comes, from there on below 2^-3, so that the sums seldom change theirs.
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(p[i]));
+        if (__any(most * held >= 2.f)) {
+          most = max_halves(most);   // the halves share the sums
+          const unsigned exponent = std::min(__float_as_uint(most) >> 23, 240u);
+          const float next = most * held >= 2.f ? __uint_as_float((250 - exponent) << 23) : held;
+          const float by = next / held;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[d][i] *= by;
+          held = next;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] *= held;
+      }
       const Operand<T> w[2] = {rounded<T>(p), rounded<T>(p + 8)};
       add_columns<T>(dk, query_view, t, w);
     }
@@ -448,16 +493,16 @@ __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
     clear(dk);
     clear(dv);
   }
-  const float back = exp2f(-kLift<T>) / held;
+  const float back = exp2f(-kLift<T>), back_k = a.scale * (back / held);
   if (splits > 1) {
     const int64_t rows = (int64_t)a.batch * a.key_heads * a.keys, row = (int64_t)work.head * a.keys + key;
     float* to = part + ((int64_t)work.split * 2 * rows + row) * a.dim;
-    store_columns<float, DP>(to, a.dim, 0, a.dim, lane, dk, a.scale * back);
+    store_columns<float, DP>(to, a.dim, 0, a.dim, lane, dk, back_k);
     store_columns<float, DP>(to + rows * a.dim, a.dim, 0, a.dim, lane, dv, back);
     return;
   }
   if (a.dk)
-    store_columns<T, DP>((T*)a.dk + b * a.dks[0] + shared_head * a.dks[1], a.dks[2], key, a.dim, lane, dk, a.scale * back);
+    store_columns<T, DP>((T*)a.dk + b * a.dks[0] + shared_head * a.dks[1], a.dks[2], key, a.dim, lane, dk, back_k);
   if (a.dv) store_columns<T, DP>((T*)a.dv + b * a.dvs[0] + shared_head * a.dvs[1], a.dvs[2], key, a.dim, lane, dv, back);
 }
 
@@ -483,8 +528,8 @@ __global__ __launch_bounds__(256) void join_splits(const float* part, int64_t pi
 }
 
 struct Space {
-  int query_splits, key_splits, pitch;
-  int64_t top, delta, lse2, parts, turned, part, total;
+  int query_splits, key_splits, pitch, size_parts;
+  int64_t sizes, delta, lse2, parts, turned, part, total;
 };
 Space space_of(const sdk_bucket_attention* a) {
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
@@ -499,8 +544,9 @@ Space space_of(const sdk_bucket_attention* a) {
   w.key_splits = parts_of(a->batch * a->key_heads * ceil_div(a->keys, rows),
                           a->heads / a->key_heads * ceil_div(a->queries, tile), key_slots, a->causal);
   w.pitch = (int)ceil_div(a->queries, 64) * 64;
-  w.top = 0;
-  w.delta = 256;
+  w.size_parts = (int)std::min<int64_t>(kMostParts, std::max<int64_t>(1, ceil_div(a->keys, 128)));
+  w.sizes = 0;
+  w.delta = a->dtype == SDK_F16 ? up(a->batch * a->key_heads * w.size_parts * 4) : 0;
   w.lse2 = w.delta + up(q_rows * 4);
   w.parts = w.lse2 + up(q_rows * 4);
   w.turned = w.parts + up(q_groups * w.query_splits * a->buckets * 4);
@@ -524,7 +570,7 @@ int launch_grad_queries(const Attention& d, const Space& w, char* ws, hipStream_
   }
   kernel<<<dim3((unsigned)tiles * (unsigned)(d.batch * d.heads) * w.query_splits), dim3(kThreads), smem, s>>>(
       d, w.query_splits, tiles, (const float*)(ws + w.delta), (const float*)(ws + w.lse2),
-      (const unsigned*)(ws + w.top), (float*)(ws + w.part), (float*)(ws + w.parts));
+      (const float*)(ws + w.sizes), w.size_parts, (float*)(ws + w.part), (float*)(ws + w.parts));
   return SDK_OK;
 }
 
@@ -542,16 +588,15 @@ int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t
   const bool any = a->batch > 0 && a->queries > 0;
   const int64_t rows = a->batch * a->heads * a->queries;
   float *delta = (float*)(ws + w.delta), *lse2 = (float*)(ws + w.lse2), *part = (float*)(ws + w.part);
-  unsigned* top = (unsigned*)(ws + w.top);
   const int columns = !a->grad_table ? 0 : a->buckets <= 64 ? 64 : a->buckets <= 128 ? 32 : 16;
-  // read by every kernel of float16 gradients, queries or not
-  if (__is_same(T, f16) && a->batch > 0) launch(clear_word, dim3(1), dim3(1), s, top);
   if (any) {
     constexpr int LANES = 128 / kWide<T>;
-    // few workgroups where each ends with an atomic: 16384 of them took 190 us, 2048 took 21 for 18
-    const int64_t groups = std::min<int64_t>(ceil_div(rows, 256 / LANES), __is_same(T, f16) ? 1024 : 1 << 30);
-    launch(row_terms<T, LANES>, dim3((unsigned)groups), dim3(256), s, d, delta, lse2, top);
+    const int64_t groups = std::min<int64_t>(ceil_div(rows, 256 / LANES), 1 << 30);
+    launch(row_terms<T, LANES>, dim3((unsigned)groups), dim3(256), s, d, delta, lse2);
     if (a->grad_query || a->grad_table) {
+      if (__is_same(T, f16))
+        launch(value_sizes, dim3((unsigned)(a->batch * a->key_heads) * w.size_parts), dim3(256), s, d, w.size_parts,
+               (float*)(ws + w.sizes));
       int rc = SDK_OK;
       ATTENTION_DIM(a->dim, rc = columns == 0    ? launch_grad_queries<T, DP, 0>(d, w, ws, s)
                                  : columns == 64 ? launch_grad_queries<T, DP, 64>(d, w, ws, s)
@@ -573,7 +618,7 @@ int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t
              dim3(256), s, d, turned, w.pitch);
     ATTENTION_DIM(a->dim, launch(grad_keys<T, DP>, dim3((unsigned)(tiles * a->batch * a->key_heads) * w.key_splits),
                                  dim3(kThreads), s, d, w.key_splits, tiles, (const float*)delta, (const float*)lse2,
-                                 (const unsigned*)top, (const uint8_t*)turned, w.pitch, part));
+                                 (const uint8_t*)turned, w.pitch, part));
     if (w.key_splits > 1) {
       const int64_t values = a->batch * a->key_heads * a->keys * a->dim;
       if (a->grad_key) launch_join<T>(d, part, 2 * values, w.key_splits, d.dk, d.dks, d.keys, d.key_heads, s);
