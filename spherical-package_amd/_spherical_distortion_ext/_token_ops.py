@@ -284,6 +284,10 @@ def _step(name, params, lists, lr, beta1, beta2, eps, weight_decay, step):
     with torch.cuda.device(params[0].device):
         _capi.call(name, _pointers(params), *(_pointers(t) for t in lists), sizes, len(params), lr, beta1, beta2,
                    eps, weight_decay, step, _DTYPES[params[0].dtype], _ops._stream(params[0]))
+    # the kernels write through pointers: autograd has to learn of it to refuse a backward through the former values
+    for t in (t for tensors in (params, *lists[1:]) for t in tensors):
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, weight_decay, step):

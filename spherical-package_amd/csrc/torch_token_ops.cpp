@@ -309,6 +309,13 @@ std::vector<int64_t> sizes_of(at::TensorList params) {
   return n;
 }
 
+// The kernels write through pointers: autograd has to learn of it to refuse a backward through the former values.
+void changed(std::initializer_list<at::TensorList> lists) {
+  for (const at::TensorList& tensors : lists)
+    for (const Tensor& t : tensors)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList avgs, at::TensorList sqs, double lr,
                 double beta1, double beta2, double eps, double weight_decay, int64_t step) {
   if (params.empty()) return;
@@ -322,6 +329,7 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList avgs
   c10::DeviceGuard guard(params[0].device());
   TOKEN_CALL(sdk_adamw_step, p.data(), g.data(), (float* const*)m.data(), (float* const*)v.data(), n.data(),
              (int64_t)n.size(), lr, beta1, beta2, eps, weight_decay, step, dtype, stream_of(params[0]));
+  changed({params, avgs, sqs});
 }
 
 void adamw_step_8bit(at::TensorList params, at::TensorList grads, at::TensorList avg_codes, at::TensorList avg_scales,
@@ -341,6 +349,7 @@ void adamw_step_8bit(at::TensorList params, at::TensorList grads, at::TensorList
   TOKEN_CALL(sdk_adamw_step_8bit, p.data(), g.data(), (int8_t* const*)mc.data(), (float* const*)ms.data(),
              (uint8_t* const*)vc.data(), (float* const*)vs.data(), n.data(), (int64_t)n.size(), lr, beta1, beta2, eps,
              weight_decay, step, dtype, stream_of(params[0]));
+  changed({params, avg_codes, avg_scales, sq_codes, sq_scales});
 }
 
 Tensor adamw_moment_values(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
