@@ -126,18 +126,21 @@ __global__ __launch_bounds__(256) void row_terms(const Attention a, float* delta
   }
 }
 
-// map[query][key] to turned[key][query], rows of `pitch` bytes, 64 x 64 bytes a workgroup.
-__global__ __launch_bounds__(256) void turn_map(const Attention a, uint8_t* turned, int pitch) {
+// map[query][key] to turned[key][query], rows of `pitch` bytes, 64 x 64 bytes a workgroup at a time.
+__global__ __launch_bounds__(256) void turn_map(const Attention a, uint8_t* turned, int pitch, unsigned blocks) {
   __shared__ uint8_t block[64][65];
-  const int across = pitch / 64, q0 = (int)(blockIdx.x % across) * 64, k0 = (int)(blockIdx.x / across) * 64;
+  const int across = pitch / 64, x = threadIdx.x % 64;
   const uint8_t* map = a.map + (int64_t)blockIdx.y * a.ms[0];
-  const int x = threadIdx.x % 64;
-  for (int y = threadIdx.x / 64; y < 64; y += 4)
-    block[y][x] = q0 + y < a.queries && k0 + x < a.keys ? map[(q0 + y) * a.ms[1] + k0 + x] : 255;
-  __syncthreads();
   uint8_t* to = turned + (int64_t)blockIdx.y * a.keys * pitch;
-  for (int y = threadIdx.x / 64; y < 64; y += 4)
-    if (k0 + y < a.keys) to[(int64_t)(k0 + y) * pitch + q0 + x] = block[x][y];
+  for (unsigned i = blockIdx.x; i < blocks; i += gridDim.x) {
+    const int q0 = (int)(i % across) * 64, k0 = (int)(i / across) * 64;
+    for (int y = threadIdx.x / 64; y < 64; y += 4)
+      block[y][x] = q0 + y < a.queries && k0 + x < a.keys ? map[(q0 + y) * a.ms[1] + k0 + x] : 255;
+    __syncthreads();
+    for (int y = threadIdx.x / 64; y < 64; y += 4)
+      if (k0 + y < a.keys) to[(int64_t)(k0 + y) * pitch + q0 + x] = block[x][y];
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------------------------------ dq and the bias table
@@ -320,28 +323,29 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
   }
 }
 
-// dT[head][bucket]: a workgroup an entry; the `each` parts of every batch element are added in an order of their own,
+// dT[head][bucket]: a workgroup an entry at a time; the `each` parts of every batch element are added in an order of their own,
 // in double.
 template <typename T>
 __global__ __launch_bounds__(256) void join_table(const Attention a, int each, const float* parts) {
   __shared__ double sums[256];
-  const int head = blockIdx.x / a.buckets, bucket = blockIdx.x % a.buckets;
-  double x = 0;
   const int64_t count = (int64_t)a.batch * each;
-  for (int64_t i = threadIdx.x; i < count; i += 256)
-    x += parts[((i / each * a.heads + head) * each + i % each) * a.buckets + bucket];
-  sums[threadIdx.x] = x;
-  __syncthreads();
-  for (int n = 128; n > 0; n /= 2) {
-    if ((int)threadIdx.x < n) sums[threadIdx.x] += sums[threadIdx.x + n];
+  for (int at = blockIdx.x; at < a.heads * a.buckets; at += gridDim.x) {   // fewer than 2^28
+    const int head = at / a.buckets, bucket = at % a.buckets;
+    double x = 0;
+    for (int64_t i = threadIdx.x; i < count; i += 256)
+      x += parts[((i / each * a.heads + head) * each + i % each) * a.buckets + bucket];
+    sums[threadIdx.x] = x;
     __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    const int64_t at = (int64_t)head * a.buckets + bucket;
-    if (a.table_float)
-      ((float*)a.dtable)[at] = (float)sums[0];
-    else
-      ((T*)a.dtable)[at] = (T)(float)sums[0];
+    for (int n = 128; n > 0; n /= 2) {
+      if ((int)threadIdx.x < n) sums[threadIdx.x] += sums[threadIdx.x + n];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+      if (a.table_float)
+        ((float*)a.dtable)[at] = (float)sums[0];
+      else
+        ((T*)a.dtable)[at] = (T)(float)sums[0];
+    }
   }
 }
 
@@ -591,7 +595,7 @@ int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t
   const int columns = !a->grad_table ? 0 : a->buckets <= 64 ? 64 : a->buckets <= 128 ? 32 : 16;
   if (any) {
     constexpr int LANES = 128 / kWide<T>;
-    const int64_t groups = std::min<int64_t>(ceil_div(rows, 256 / LANES), 1 << 30);
+    const int64_t groups = std::min(ceil_div(rows, 256 / LANES), most_groups(256));
     launch(row_terms<T, LANES>, dim3((unsigned)groups), dim3(256), s, d, delta, lse2);
     if (a->grad_query || a->grad_table) {
       if (__is_same(T, f16))
@@ -608,14 +612,16 @@ int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t
     }
   }
   if (a->grad_table)
-    launch(join_table<T>, dim3((unsigned)(a->heads * a->buckets)), dim3(256), s, d,
+    launch(join_table<T>, dim3((unsigned)std::min(a->heads * a->buckets, most_groups(256))), dim3(256), s, d,
            any ? (int)ceil_div(a->queries, 32 * kWaves) * w.query_splits : 0, (const float*)(ws + w.parts));
   if ((a->grad_key || a->grad_value) && a->batch > 0 && a->keys > 0) {
     uint8_t* turned = (uint8_t*)(ws + w.turned);
     const int tiles = (int)ceil_div(a->keys, 32 * kWaves);
-    if (any)
-      launch(turn_map, dim3((unsigned)(w.pitch / 64 * ceil_div(a->keys, 64)), (unsigned)(a->map_strides[0] ? a->batch : 1)),
-             dim3(256), s, d, turned, w.pitch);
+    if (any) {
+      const int64_t blocks = w.pitch / 64 * ceil_div(a->keys, 64);   // fewer than 2^31
+      launch(turn_map, dim3((unsigned)std::min(blocks, most_groups(256)), (unsigned)(a->map_strides[0] ? a->batch : 1)),
+             dim3(256), s, d, turned, w.pitch, (unsigned)blocks);
+    }
     ATTENTION_DIM(a->dim, launch(grad_keys<T, DP>, dim3((unsigned)(tiles * a->batch * a->key_heads) * w.key_splits),
                                  dim3(kThreads), s, d, w.key_splits, tiles, (const float*)delta, (const float*)lse2,
                                  (const uint8_t*)turned, w.pitch, part));

@@ -302,27 +302,42 @@ constexpr int64_t kMostWidth = 16384;
 // Runs `CALL` with V, N, THREADS and ALIGNED for rows of `width`; `wide`: 16-byte vectors fit rows and pointers.  (Rows
 // that they do not fit are read by vectors all the same, at whatever address they begin: 41458 rows of 1235 float32
 // values to int8 and back 194 us, value by value 298.)
-#define NORM_SHAPE_N(NN, CALL)                                            \
+#define NORM_SHAPE_N(NN, ...)                                             \
   do {                                                                    \
     constexpr int N = NN;                                                 \
-    if (threads == 64) { constexpr int THREADS = 64; CALL; }              \
-    else if (threads == 256) { constexpr int THREADS = 256; CALL; }       \
-    else { constexpr int THREADS = 1024; CALL; }                          \
+    if (threads == 64) { constexpr int THREADS = 64; __VA_ARGS__; }       \
+    else if (threads == 256) { constexpr int THREADS = 256; __VA_ARGS__; } \
+    else { constexpr int THREADS = 1024; __VA_ARGS__; }                   \
   } while (0)
-#define NORM_SHAPE_V(CALL)                                                \
+#define NORM_SHAPE_V(...)                                                 \
   do {                                                                    \
     constexpr int V = kWide<T>;                                           \
     const int64_t n = ceil_div(width, (int64_t)threads * V);              \
-    if (n <= 1) NORM_SHAPE_N(1, CALL);                                    \
-    else if (n <= 2) NORM_SHAPE_N(2, CALL);                               \
-    else if constexpr (V <= 4) NORM_SHAPE_N(4, CALL);                     \
+    if (n <= 1) NORM_SHAPE_N(1, __VA_ARGS__);                             \
+    else if (n <= 2) NORM_SHAPE_N(2, __VA_ARGS__);                        \
+    else if constexpr (V <= 4) NORM_SHAPE_N(4, __VA_ARGS__);              \
   } while (0)
-#define NORM_SHAPE(CALL)                                                  \
+#define NORM_SHAPE(...)                                                   \
   do {                                                                    \
     const int threads = threads_of(width);                                \
-    if (wide) { constexpr bool ALIGNED = true; NORM_SHAPE_V(CALL); }      \
-    else { constexpr bool ALIGNED = false; NORM_SHAPE_V(CALL); }          \
+    if (wide) { constexpr bool ALIGNED = true; NORM_SHAPE_V(__VA_ARGS__); } \
+    else { constexpr bool ALIGNED = false; NORM_SHAPE_V(__VA_ARGS__); }   \
   } while (0)
+
+// The rows in launches of as many as one holds.
+template <typename T, int V, int N, int THREADS, bool ALIGNED>
+void run_forward(const T* x, const T* residual, const void* weight, int weight_float, void* out, float* scales, T* summed,
+                 float* inverse, int64_t rows, int width, float eps, int codes, hipStream_t s) {
+  constexpr int SHARE = kGroup<THREADS> / THREADS;
+  constexpr int64_t EACH = most_groups(kGroup<THREADS>) * SHARE;
+  for (int64_t row = 0; row < rows; row += EACH) {
+    const int64_t count = std::min(EACH, rows - row), at = row * width;
+    launch(norm_forward<T, V, N, THREADS, ALIGNED>, dim3((unsigned)ceil_div(count, SHARE)), dim3(kGroup<THREADS>), s, x + at,
+           residual ? residual + at : nullptr, weight, weight_float,
+           (void*)((char*)out + at * (codes == kPlain ? (int64_t)sizeof(T) : 1)), scales ? scales + row : nullptr,
+           summed ? summed + at : nullptr, inverse ? inverse + row : nullptr, count, width, eps, codes);
+  }
+}
 
 int64_t backward_groups(int64_t rows, int64_t width) {
   const int threads = threads_of(width), share = threads < 256 ? 256 / threads : 1;
@@ -362,10 +377,9 @@ int sdk_add_rms_norm(const void* x, const void* residual, const void* weight, vo
   SDK_DISPATCH_TOKEN_DTYPE(dtype, {
     const bool wide = width % kWide<T> == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) &&
                       aligned16(out) && aligned16(summed);
-    NORM_SHAPE(launch(norm_forward<T, V, N, THREADS, ALIGNED>,
-                      dim3((unsigned)ceil_div(rows, kGroup<THREADS> / THREADS)), dim3(kGroup<THREADS>), s,
-                      (const T*)x, (const T*)residual, weight, (int)(weight_dtype == SDK_F32), out, scales,
-                      (T*)summed, inverse, rows, (int)width, (float)eps, (int)codes));
+    NORM_SHAPE(run_forward<T, V, N, THREADS, ALIGNED>((const T*)x, (const T*)residual, weight, weight_dtype == SDK_F32, out,
+                                                      scales, (T*)summed, inverse, rows, (int)width, (float)eps,
+                                                      (int)codes, s));
   });
   SDK_LAUNCH_CHECK("add_rms_norm");
   return SDK_OK;
@@ -406,20 +420,23 @@ int sdk_add_rms_norm_backward(const void* grad, const void* grad_sum, const void
 
 int sdk_dequantize_rows(const void* codes, const float* scales, void* out, int64_t rows, int64_t width,
                         int32_t codes_kind, int32_t dtype, sdk_stream_t stream) {
-  SDK_REQUIRE(rows >= 0 && rows < (int64_t)1 << 31 && width >= 1 && width < (int64_t)1 << 31, "rows %lld of width %lld", (long long)rows,
-              (long long)width);
+  SDK_REQUIRE(rows >= 0 && rows < (int64_t)1 << 31 && width >= 1 && width < (int64_t)1 << 31,
+              "rows %lld of width %lld", (long long)rows, (long long)width);
   SDK_REQUIRE(codes_kind == kInt8 || codes_kind == kFp8, "codes = %d must be 1 (int8) or 2 (float8 e4m3)",
               codes_kind);
   SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
   if (rows == 0) return SDK_OK;
   SDK_REQUIRE(codes && scales && out, "codes, scales and out must not be NULL");
   hipStream_t s = (hipStream_t)stream;
-  const int wide = ((uintptr_t)codes & 7) == 0 && aligned16(out);
-  const int64_t size = rows * width, groups = ceil_div(size, 2048);
-  SDK_REQUIRE(groups < (int64_t)1 << 31, "%lld rows of width %lld are too many", (long long)rows, (long long)width);
-  SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(dequantize<T>, dim3((unsigned)groups), dim3(256), s,
-                                         (const unsigned char*)codes, scales, (T*)out, size, (int)width,
-                                         (int)(codes_kind == kFp8), wide));
+  const int64_t each = most_groups(256) * 2048 / width;   // rows of a launch: 16 at least
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, for (int64_t row = 0; row < rows; row += each) {
+    const unsigned char* from = (const unsigned char*)codes + row * width;
+    T* to = (T*)out + row * width;
+    const int64_t size = std::min(each, rows - row) * width;
+    const int wide = ((uintptr_t)from & 7) == 0 && aligned16(to);
+    launch(dequantize<T>, dim3((unsigned)ceil_div(size, 2048)), dim3(256), s, from, scales + row, to, size, (int)width,
+           (int)(codes_kind == kFp8), wide);
+  });
   SDK_LAUNCH_CHECK("dequantize_rows");
   return SDK_OK;
 }

@@ -273,7 +273,7 @@ int check(int64_t count, double lr, double b1, double b2, double eps, double wei
   return SDK_OK;
 }
 
-// Deals the tensors to launches of at most kTensors tensors and 2^31 - 1 workgroups.
+// Deals the tensors to launches of at most kTensors tensors and as many workgroups as one holds.
 template <typename Table, typename Put, typename Run>
 int deal(int64_t count, const int64_t* sizes, int64_t per_group, Put put, Run run) {
   Table t;
@@ -289,9 +289,9 @@ int deal(int64_t count, const int64_t* sizes, int64_t per_group, Put put, Run ru
   for (int64_t i = 0; i < count; ++i) {
     if (sizes[i] == 0) continue;
     const int64_t mine = ceil_div(sizes[i], per_group);
-    SDK_REQUIRE(mine < (int64_t)1 << 31, "tensor %lld of %lld values is too large", (long long)i,
+    SDK_REQUIRE(mine <= most_groups(256), "tensor %lld of %lld values is too large", (long long)i,
                 (long long)sizes[i]);
-    if (used == kTensors || groups + mine >= (int64_t)1 << 31)
+    if (used == kTensors || groups + mine > most_groups(256))
       if (int rc = flush()) return rc;
     put(t, used, i);
     t.n[used] = sizes[i];
@@ -370,9 +370,12 @@ int sdk_adamw_moment_values(const void* codes, const float* scales, void* out, i
   if (size == 0) return SDK_OK;
   SDK_REQUIRE(codes && scales && out, "codes, scales and out must not be NULL");
   const int wide = ((uintptr_t)codes & 15) == 0 && ((uintptr_t)out & 15) == 0;
-  SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(moment_values<T>, dim3((unsigned)ceil_div(size, 4096)), dim3(256),
-                                         (hipStream_t)stream, (const unsigned char*)codes, scales, (T*)out, size,
-                                         (int)(second != 0), wide));
+  constexpr int64_t EACH = most_groups(256) * 4096;   // of a launch: whole blocks
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, for (int64_t from = 0; from < size; from += EACH) {
+    const int64_t count = std::min(EACH, size - from);
+    launch(moment_values<T>, dim3((unsigned)ceil_div(count, 4096)), dim3(256), (hipStream_t)stream,
+           (const unsigned char*)codes + from, scales + from / kBlock, (T*)out + from, count, (int)(second != 0), wide);
+  });
   SDK_LAUNCH_CHECK("adamw_moment_values");
   return SDK_OK;
 }

@@ -97,6 +97,9 @@ __device__ __forceinline__ float over_group(float x, float* slots) {
   return x;
 }
 
+// Workgroups of `threads` that one launch holds along x: fewer than 2^32 threads.  A larger grid is cut without an error.
+constexpr int64_t most_groups(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
+
 inline bool known(int dtype) { return dtype == SDK_F32 || dtype == SDK_BF16 || dtype == SDK_F16; }
 inline size_t bytes_of(int dtype) { return dtype == SDK_F32 ? 4 : 2; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
