@@ -38,12 +38,21 @@ def _dense(**tensors):
 
 
 # --------------------------------------------------------------------------- attention
-def _rows_ready(t):
-    """`t`, or a dense copy where its rows are not 16-byte aligned or its last axis is not dense."""
+def _rows_fit(t):
+    """Whether the kernels read `t` where it lies: last axis dense, rows 16-byte aligned, 64 tokens within 2^31 bytes."""
     each = 16 // t.element_size()
-    ok = (t.data_ptr() % 16 == 0 and (t.shape[-1] == 1 or t.stride(-1) == 1)
-          and all(t.stride(i) % each == 0 or t.shape[i] == 1 for i in range(3)))
-    return t if ok else t.contiguous()
+    return (t.data_ptr() % 16 == 0 and (t.shape[-1] == 1 or t.stride(-1) == 1)
+            and all(t.stride(i) % each == 0 or t.shape[i] == 1 for i in range(3))
+            and (t.shape[2] == 1 or t.stride(2) < 2 ** 31 // (64 * t.element_size())))
+
+
+def _laid_out(t):
+    """A dense copy, of a dense tensor too (which may lie at any address)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _rows_ready(t):
+    return t if _rows_fit(t) else _laid_out(t)
 
 
 def _strides(t):
@@ -140,9 +149,10 @@ def bucket_attention_backward(grad_output, query, key, value, bias_table, bucket
         raise RuntimeError("the output's rest must be like the output, or empty")
     with torch.cuda.device(query.device):
         a, keep = _args(query, key, value, bias_table, bucket_map, key_lengths, causal, scale)
-        grad_output, output, lse = _rows_ready(grad_output), _rows_ready(output), lse.contiguous()
+        grad_output, lse = _rows_ready(grad_output), lse.contiguous()
+        if not _rows_fit(output) or (rest.numel() and not _rows_fit(rest)):   # both are read by the output's strides
+            output, rest = _laid_out(output), _laid_out(rest)
         if rest.numel():
-            rest = _rows_ready(rest)
             a.output_rest = rest.data_ptr()
         a.grad_output, a.grad_output_strides = grad_output.data_ptr(), _strides(grad_output)
         a.output, a.output_strides, a.lse = output.data_ptr(), _strides(output), lse.data_ptr()

@@ -61,13 +61,16 @@ hipStream_t stream_of(const Tensor& ref) {
 Tensor nothing(const Tensor& like) { return at::empty({0}, like.options()); }
 
 // ------------------------------------------------------------------------------------------ attention
-// `t`, or a dense copy where its rows are not 16-byte aligned or its last axis is not dense.
-Tensor rows_ready(const Tensor& t) {
+// Whether the kernels read `t` where it lies: last axis dense, rows 16-byte aligned, 64 tokens within 2^31 bytes.
+bool rows_fit(const Tensor& t) {
   const int64_t each = 16 / (int64_t)t.element_size();
   bool ok = (uintptr_t)t.data_ptr() % 16 == 0 && (t.size(-1) == 1 || t.stride(-1) == 1);
   for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % each == 0);
-  return ok ? t : t.contiguous();
+  return ok && (t.size(2) == 1 || t.stride(2) < ((int64_t)1 << 31) / (64 * (int64_t)t.element_size()));
 }
+// A dense copy, of a dense tensor too (which may lie at any address).
+Tensor laid_out(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+Tensor rows_ready(const Tensor& t) { return rows_fit(t) ? t : laid_out(t); }
 
 // Batch, head and token strides; those of axes of length one do not count.
 void strides(const Tensor& t, int64_t (&s)[3]) {
@@ -170,13 +173,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> bucket_attention_backward(
               "the output's rest must be like the output, or empty");
   c10::DeviceGuard guard(q.device());
   sdk_bucket_attention a = attention_args(q, k, v, table, map, lengths, causal, scale);
-  grad = rows_ready(grad), out = rows_ready(out), lse = lse.contiguous();
+  grad = rows_ready(grad), lse = lse.contiguous();
+  if (!rows_fit(out) || (rest.numel() && !rows_fit(rest)))   // both are read by the output's strides
+    out = laid_out(out), rest = laid_out(rest);
   a.grad_output = ptr(grad), a.output = ptr(out), a.lse = (float*)ptr(lse);
   strides(grad, a.grad_output_strides), strides(out, a.output_strides);
-  if (rest.numel()) {
-    rest = rows_ready(rest);
-    a.output_rest = ptr(rest);
-  }
+  if (rest.numel()) a.output_rest = ptr(rest);
   Tensor dq = need_query ? at::empty_like(q) : nothing(q);
   Tensor dk = need_keys ? at::empty_like(k) : nothing(k), dv = need_keys ? at::empty_like(v) : nothing(v);
   Tensor dt = need_table ? at::empty_like(table) : nothing(table);
