@@ -4,7 +4,25 @@ import torch
 from .. import functional as F
 
 _BLOCK = 256   # values that share a scale in 8 bits
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _MOMENTS = {32: ("exp_avg", "exp_avg_sq"), 8: ("avg_codes", "avg_scales", "sq_codes", "sq_scales")}
+
+
+def _on_gpu(p):
+    return p.is_cuda
+
+
+def _check(p):
+    """What the step refuses of a parameter with a gradient."""
+    if p.grad.is_sparse:
+        raise RuntimeError("AdamW does not take sparse gradients")
+    if not _on_gpu(p):
+        raise RuntimeError("this backend runs on the GPU only: parameters must be CUDA/HIP tensors")
+    if p.dtype not in _TYPES or p.grad.dtype != p.dtype:
+        raise RuntimeError("parameters must be float32, bfloat16 or float16 and their gradients alike, got %s and %s"
+                           % (p.dtype, p.grad.dtype))
+    if not p.is_contiguous():
+        raise RuntimeError("parameters must be contiguous, got strides %s of shape %s" % (p.stride(), tuple(p.shape)))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -13,7 +31,8 @@ class AdamW(torch.optim.Optimizer):
     params: float32, bfloat16 or float16 and contiguous.  moment_bits: 32, or 8 for moments held as codes
     with a scale for each 256 values (2 bytes a value instead of 8; functional.adamw_step_8bit says which
     values they stand for); parameters of fewer than `smallest_8bit` values keep 32 bits.  Each parameter
-    counts its own steps: one without a gradient is left as it is."""
+    counts its own steps: one without a gradient is left as it is.  A step checks every parameter before it
+    changes one, and counts for those whose call returned."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, moment_bits=32,
                  smallest_8bit=4096):
@@ -27,16 +46,17 @@ class AdamW(torch.optim.Optimizer):
                                       smallest_8bit=smallest_8bit))
 
     @staticmethod
-    def _begin(state, p, bits):
-        state["step"] = 0
+    def _begin(p, bits):
+        state = {"step": 0}
         if bits == 32:
             for name in _MOMENTS[32]:
                 state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            return
+            return state
         blocks = -(-p.numel() // _BLOCK)
         for kind, dtype in (("avg", torch.int8), ("sq", torch.uint8)):
             state[kind + "_codes"] = torch.zeros(p.shape, dtype=dtype, device=p.device)
             state[kind + "_scales"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        return state
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -45,28 +65,34 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None:
+                    _check(p)
+        for group in self.param_groups:
             settings = {k: group[k] for k in ("lr", "betas", "eps", "weight_decay")}
-            calls = {}   # (type, device, step, bits) -> lists
+            calls = {}   # (type, device, step, bits) -> lists of tensors, states
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                if p.grad.is_sparse:
-                    raise RuntimeError("AdamW does not take sparse gradients")
-                state = self.state[p]
+                state = self.state.get(p)
                 if not state:
                     eight = group["moment_bits"] == 8 and p.numel() >= group["smallest_8bit"]
-                    self._begin(state, p, 8 if eight else 32)
+                    state = self._begin(p, 8 if eight else 32)
                 bits = 32 if "exp_avg" in state else 8
-                state["step"] += 1
                 names = _MOMENTS[bits]
-                lists = calls.setdefault((p.dtype, p.device, state["step"], bits), [[] for _ in range(2 + len(names))])
+                lists, states = calls.setdefault((p.dtype, p.device, state["step"] + 1, bits),
+                                                 ([[] for _ in range(2 + len(names))], []))
                 lists[0].append(p)
                 lists[1].append(p.grad.contiguous())
                 for i, name in enumerate(names):
                     lists[2 + i].append(state[name])
-            for (_, _, step, bits), lists in calls.items():
+                states.append(state)
+            for (_, _, step, bits), (lists, states) in calls.items():
                 run = F.adamw_step if bits == 32 else F.adamw_step_8bit
                 run(*lists, step=step, **settings)
+                for p, state in zip(lists[0], states):
+                    state["step"] = step
+                    self.state[p] = state
         return loss
 
     def load_state_dict(self, state_dict):
