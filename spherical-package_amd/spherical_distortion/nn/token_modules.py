@@ -16,6 +16,11 @@ class BucketAttention(nn.Module):
         if width % num_heads or num_heads % num_key_heads:
             raise ValueError("width %d must divide into %d heads, and those into %d key heads"
                              % (width, num_heads, num_key_heads))
+        if width // num_heads % 8 or not 8 <= width // num_heads <= 128:
+            raise ValueError("width %d in %d heads: a head's values must be a multiple of 8 up to 128"
+                             % (width, num_heads))
+        if not 1 <= num_buckets <= 256:
+            raise ValueError("num_buckets must be between 1 and 256, got %s" % num_buckets)
         self.num_heads, self.num_key_heads, self.dim = num_heads, num_key_heads, width // num_heads
         self.query = nn.Linear(width, width, bias=False)
         self.key_value = nn.Linear(width, 2 * num_key_heads * self.dim, bias=False)
@@ -42,6 +47,8 @@ class AddRMSNorm(nn.Module):
 
     def __init__(self, width, eps=1e-6):
         super().__init__()
+        if not 1 <= width <= 16384:
+            raise ValueError("width must be between 1 and 16384, got %s" % width)
         self.eps = eps
         self.weight = nn.Parameter(torch.ones(width))
 

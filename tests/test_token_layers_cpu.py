@@ -81,3 +81,25 @@ def test_parameters_on_the_cpu_are_refused_before_any_state():
     with pytest.raises(RuntimeError, match="GPU"):
         optimizer.step()
     assert not optimizer.state
+
+
+@pytest.mark.parametrize("width,heads,buckets", [(96, 8, 9), (20, 5, 9), (1040, 8, 9), (64, 4, 0), (64, 4, 257)])
+def test_attention_modules_refuse_at_once_what_no_call_takes(width, heads, buckets):
+    """Heads of 12, 4 and 130 values, tables of 0 and 257 buckets."""
+    from spherical_distortion import nn as snn
+    with pytest.raises(ValueError):
+        snn.BucketAttention(width, heads, buckets)
+
+
+def test_attention_modules_take_every_size_of_a_call():
+    from spherical_distortion import nn as snn
+    for width, heads, buckets in ((8, 1, 1), (128, 1, 256), (1024, 8, 255)):
+        assert snn.BucketAttention(width, heads, buckets).bias_table.shape == (heads, buckets)
+
+
+@pytest.mark.parametrize("width", [0, -1, 16385])
+def test_norm_modules_refuse_at_once_what_no_call_takes(width):
+    from spherical_distortion import nn as snn
+    with pytest.raises(ValueError):
+        snn.AddRMSNorm(width)
+    assert snn.AddRMSNorm(16384).weight.shape == (16384,)
