@@ -29,3 +29,16 @@ def test_a_masked_last_row_reads_nothing_behind_it(queries, dtype):
     want = _exact(q, k, v, table, bmap, grad=do)
     for got, ref, terms in zip((out, *grads), want, _terms(q, k, v, do)):
         _close(got, ref, TOL[dtype], terms)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [104, 128])
+@pytest.mark.parametrize("heads,queries", [(32, 1), (8, 4)])
+def test_few_queries_of_wide_heads(heads, queries, dim, dtype):
+    """32 rows to one key head, the most that the kernel of few queries takes: in float32 its tiles, joined states and 32
+    tables are the largest LDS of all calls (137 KB)."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(2, heads, 1, queries, 700, dim, 200, dtype, seed=80 + dim + heads)
+    lengths = torch.tensor([700, 333], dtype=torch.int32)
+    out = F.bucket_attention(q, k, v, table, bmap, key_lengths=lengths.to(DEV))
+    _close(out, _exact(q, k, v, table, bmap, lengths), TOL[dtype])
