@@ -507,7 +507,7 @@ struct Work {
 // fewest rounds of workgroups times the tiles of a round; a part costs about four tiles more (its operands, its sums
 // in memory), and has four at least.  More workgroups than that stay whole: 1152 of the forward at 4608 x 4608 pairs
 // as two parts each took 284 us and a join for 265.  balance: two parts at least where all run at once (causal walks
-// differ in length: 256 workgroups of dk and dv, 228 us whole, 148 as two parts, 170 as four).
+// differ in length: 256 workgroups of dk and dv take 1.54 times as long whole as in two parts, in four 1.15 times).
 inline int parts_of(int64_t groups, int64_t steps, int64_t slots, bool balance) {
   if (groups == 0 || groups > slots || (groups == slots && !balance)) return 1;
   int64_t best = 1, least = INT64_MAX;

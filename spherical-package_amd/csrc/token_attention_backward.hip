@@ -146,8 +146,7 @@ __global__ __launch_bounds__(256) void turn_map(const Attention a, uint8_t* turn
 // ------------------------------------------------------------------------------------------ dq and the bias table
 // Adds x * by to the sums of its buckets in one lane's column, two at a time: read, add, write, and where the two meet the
 // second takes the first's sum.  (An LDS float add of 64 lanes takes 193 cycles of a CU whatever its addresses, this
-// 13; by four or eight the comparisons cost more than the waits they save: 842 and 971 us of the kernel at 8192 x
-// 8192 pairs of 16 heads, 817 by two.)
+// 13; by four or eight the comparisons cost more than the waits they save: 3 and 19 % more of the whole kernel.)
 template <int COLUMNS>
 __device__ __forceinline__ void add_by_bucket(float* column, const Buckets& bucket, int buckets, const float* x,
                                               float by) {
@@ -163,8 +162,8 @@ __device__ __forceinline__ void add_by_bucket(float* column, const Buckets& buck
 // As the forward, a workgroup walks the keys (or a split of them) with 128 queries.  Each lane adds its ds to the
 // bucket's sum in a column of its own (COLUMNS of them a wave: 64 up to 64 buckets, fewer beyond, then the lanes
 // that share one take turns; 0: no table gradient), so that every sum has one order.
-// Bound by vector instructions and LDS: 16 heads of 64, 8192 x 8192 pairs in bfloat16 take 860 us (480 TFLOP/s), of which
-// the rounding of the weights is 40.
+// Bound by vector instructions and LDS: 16 heads of 64, 8192 x 8192 pairs in bfloat16 take 704 us (585 TFLOP/s), 5 % of
+// it the rounding of the weights.
 // part: splits > 1: float32 sums of the splits, [split][row][dim].
 template <typename T, int DP, int COLUMNS>
 __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
@@ -271,7 +270,9 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
         }
       // The forward's own weights, rounded as they were: D is the mean of do v^T under these, so that a row's ds add up
       // to zero.  Unrounded ones miss it by 2^-9 of a weight, which a sum over many keys shows where the table's
-      // entries, or keys with much in common, cancel.
+      // entries, or keys with much in common, cancel.  ds then goes to the matrix unit in the inputs' type, here and for
+      // dk: gradients are off by 2.9e-3 of their size in bfloat16 (3.5e-4 in float16), 1.7e-3 (2.1e-4) of it their own
+      // rounding.  Weights and ds in two pieces everywhere leave that alone, and take 2241 us for a step of 1850.
       float ds[16];
 #pragma unroll
       for (int v = 0; v < 16; ++v) ds[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, -my_lse));
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
   // whole tiles that every query of the workgroup sees, in a loop without branches
   const int whole = (a.causal ? std::max(0, std::min(len, first + shift + 1)) : len) / KEYS * KEYS;
   int k0 = from;
-  if constexpr (sizeof(T) == 2)   // float32: the registers do not hold two loops (170 us for 149 with one)
+  if constexpr (sizeof(T) == 2)   // float32: the registers do not hold two loops (14 % more time than one)
     for (; k0 < std::min(to, whole); k0 += KEYS) step(k0, std::false_type());
   for (; k0 < to; k0 += KEYS) step(k0, std::true_type());
   if (in && splits > 1)
@@ -323,8 +324,8 @@ __global__ __launch_bounds__(kThreads, (kQueryWaves<T, DP>)) void grad_queries(
   }
 }
 
-// dT[head][bucket]: a workgroup an entry at a time; the `each` parts of every batch element are added in an order of their own,
-// in double.
+// dT[head][bucket]: a workgroup an entry at a time; the `each` parts of every batch element are added in an order of
+// their own, in double.
 template <typename T>
 __global__ __launch_bounds__(256) void join_table(const Attention a, int each, const float* parts) {
   __shared__ double sums[256];
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(256) void join_table(const Attention a, int each, c
 // A workgroup keeps 128 keys, 32 a wave, and walks the queries of every head that reads them (or a split of these
 // tiles): S = Q K^T has the keys in columns.  The next tile is requested while this one is worked on, into the
 // other buffer.  Bound by LDS (both operands straight and turned) and what it does not overlap: 4 key heads of 16 heads
-// of 64, 8192 x 8192 pairs in bfloat16 take 755 us, 730 TFLOP/s.
+// of 64, 8192 x 8192 pairs in bfloat16 take 651 us, 845 TFLOP/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, (kKeyWaves<T, DP>)) void grad_keys(
     const Attention a, int splits, int tiles, const float* delta, const float* lse2, const uint8_t* turned,
@@ -592,6 +593,11 @@ int run(const sdk_bucket_attention* a, const Attention& d, char* ws, hipStream_t
   const bool any = a->batch > 0 && a->queries > 0;
   const int64_t rows = a->batch * a->heads * a->queries;
   float *delta = (float*)(ws + w.delta), *lse2 = (float*)(ws + w.lse2), *part = (float*)(ws + w.part);
+  // As many columns as 66 KB hold.  Beside the tiles that leaves two workgroups a CU up to 59, 120 and 242 buckets with 64,
+  // 32 and 16 columns (heads of 64 in 16 bits; 51, 104 and 210 padded to 96, 50, 102 and 206 in float32), one beyond, which
+  // the slots that parts are planned with (space_of) do not know.  The backward of 16 heads of 64, 8192 x 8192 pairs: 48
+  // buckets 1472 us, 59 1467, 60 1784, 64 1788, 65 1705, 120 1742, 121 2279, 129 2200, 242 2242, 243 3113; without the table
+  // 1241 to 1345.
   const int columns = !a->grad_table ? 0 : a->buckets <= 64 ? 64 : a->buckets <= 128 ? 32 : 16;
   if (any) {
     constexpr int LANES = 128 / kWide<T>;

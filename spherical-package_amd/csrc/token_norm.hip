@@ -7,7 +7,8 @@
 //
 // All of it is bound by memory: a row is read once, held in registers, and every sum over it (squares,
 // largest magnitude, w g h) is formed there.  Sums are float32.  The forward normalises the sum before it is
-// rounded to the tensors' type; the backward reads the rounded h, which the forward wrote.
+// rounded to the tensors' type; the backward reads the rounded h, which the forward wrote (2 bytes a value less than
+// float32 sums): gradients are off by 2.5e-3 of their size in bfloat16, 1.7e-3 of it their own rounding.
 #include <algorithm>
 
 #include "token_types.hpp"
@@ -19,8 +20,9 @@ namespace {
 // A row is dealt to THREADS threads, N chunks of V elements each: chunk k of thread t begins at
 // (k * THREADS + t) * V, so that a wave reads consecutive memory.  Workgroups of at least 256 threads:
 // narrow rows share one.
-// 65536 rows of 1024 bfloat16 values: forward 88 us (6.1 TB/s of rows read and written), backward 110 us (4.9 TB/s), of
-// which the weight's sum over 1024 workgroups is 4.
+// 65536 rows of 1024 bfloat16 values: forward 87 us (6.2 TB/s of rows read and written), backward 110 us (4.9 TB/s), of
+// which the weight's sum over 1024 workgroups is 4.  Rows of fewer 16-byte vectors than 64 leave lanes without work: 2^26
+// bfloat16 values in rows of 64, 128 and 256 take 384, 211 and 126 us forward, of 512 90.
 template <int THREADS>
 constexpr int kGroup = THREADS < 256 ? 256 : THREADS;
 
