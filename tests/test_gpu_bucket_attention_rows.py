@@ -42,3 +42,24 @@ def test_few_queries_of_wide_heads(heads, queries, dim, dtype):
     lengths = torch.tensor([700, 333], dtype=torch.int32)
     out = F.bucket_attention(q, k, v, table, bmap, key_lengths=lengths.to(DEV))
     _close(out, _exact(q, k, v, table, bmap, lengths), TOL[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("buckets", [20, 200])
+@pytest.mark.parametrize("lq,lk", [(70, 90), (150, 700), (3, 700)])
+def test_rows_of_large_scores(lq, lk, buckets, dtype):
+    """A scale of 150: most rows' largest score lies beyond 1024 powers of two, some rows' below, with weights that differ.
+    A score of magnitude S is off by up to 2^-20 S (the order of its 64 float32 terms, exponent and level), and its weight
+    by as much of itself, twice in a gradient, whose terms have the scale as a factor."""
+    from spherical_distortion import functional as F
+    q, k, v, table, bmap, do = _inputs(1, 4, 2, lq, lk, 64, buckets, dtype, seed=90 + lk + buckets)
+    q[:, :, ::3] /= 64
+    scale = 150.0
+    size = scale * float((q.double().abs() @ k.double().abs().repeat_interleave(2, 1).transpose(2, 3).contiguous()).max())
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = F.bucket_attention(*leaves, bmap, scale=scale)
+    grads = torch.autograd.grad(out, leaves, do)
+    want = _exact(q, k, v, table, bmap, scale=scale, grad=do)
+    assert size > 5000
+    for got, ref, terms, factor in zip((out, *grads), want, _terms(q, k, v, do), (1, scale, scale, 1, 1)):
+        _close(got, ref, TOL[dtype] + 2.0 ** -19 * size, terms * factor)
