@@ -797,8 +797,8 @@ int sdk_mapped_max_unpool_planned_bands(const void* grad_output, const int64_t* 
 
 /* ------------------------------------------------------------------------- *
  * Operators on token sequences (spherical samples as tokens; not in the reference):
- * attention with a learned bias for each bucket of relative positions, residual
- * addition with root-mean-square norm, AdamW.  dtype: SDK_F32, SDK_BF16 or SDK_F16.
+ * attention with a learned bias for each bucket of relative positions, a gated linear
+ * recurrence, residual addition with root-mean-square and layer norm, AdamW, Muon.  dtype: SDK_F32, SDK_BF16 or SDK_F16.
  * Sums, softmax statistics and norms are float32.
  * ------------------------------------------------------------------------- */
 
@@ -888,6 +888,78 @@ int sdk_adamw_step_8bit(void* const* params, const void* const* grads, int8_t* c
 /* The values that the codes of a moment stand for (second: 0 first moment, 1 second). */
 int sdk_adamw_moment_values(const void* codes, const float* scales, void* out, int64_t size, int32_t second,
                             int32_t dtype, sdk_stream_t stream);
+
+/* Rows of h = x + residual (residual NULL: h = x) and their layer norm: out = weight * (h - mean(h)) /
+ * sqrt(mean((h - mean(h))^2) + eps) + bias (NULL: none).  summed (may be NULL): h, rounded to dtype; mean,
+ * inverse (may be NULL) [rows]: mean(h) and 1 / sqrt(..), for the backward.  width: up to 16384.
+ * weight_dtype, of weight and bias: dtype or SDK_F32.  Dense rows. */
+int sdk_add_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, void* out,
+                       void* summed, float* mean, float* inverse, int64_t rows, int64_t width, double eps,
+                       int32_t dtype, int32_t weight_dtype, sdk_stream_t stream);
+/* grad_x (the gradient of x and of residual): that of `grad` through the norm plus grad_sum (may be NULL).
+ * Gradients that are NULL are not formed; the workspace is needed for those of weight and bias. */
+size_t sdk_add_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const void* summed, const void* weight,
+                                const float* mean, const float* inverse, void* grad_x, void* grad_weight,
+                                void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t width,
+                                int32_t dtype, int32_t weight_dtype, sdk_stream_t stream);
+
+/* Gated linear recurrence along the tokens, each channel by itself:
+ *   f = sigmoid(gate)      h[t] = f[t] h[t-1] + (1 - f[t]) x[t]      output[t] = h[t], last = the last token's h
+ * x, gate [batch, tokens, width], strides in elements of the batch and token axes, last axis dense; output
+ * [batch, tokens, width] dense; state (h in front of the first token; NULL: zeros), last, and their gradients
+ * [batch, width] float32, dense.  lengths [batch] or NULL: tokens at and beyond lengths[b] are not read, their
+ * output and gradients are zeros.  reverse: from the last token that counts down to the first.
+ * Backward: grad_output (its strides) and grad_last may be NULL (zeros); gradients that are NULL are not formed;
+ * grad_x, grad_gate [batch, tokens, width] dense.  output is the forward's.
+ * width: up to 2^20.  Every sum is formed in an order that depends on the sizes alone. */
+typedef struct sdk_gated_scan {
+  const void* x;
+  const void* gate;
+  const float* state;
+  const int32_t* lengths;
+  void* output;
+  float* last;
+  const void* grad_output;
+  const float* grad_last;
+  void* grad_x;
+  void* grad_gate;
+  float* grad_state;
+  int64_t batch, tokens, width;
+  int64_t x_strides[2], gate_strides[2], grad_output_strides[2];
+  int32_t reverse, dtype;
+} sdk_gated_scan;
+
+size_t sdk_gated_scan_workspace_bytes(const sdk_gated_scan* a);
+int sdk_gated_scan_forward(const sdk_gated_scan* a, void* workspace, size_t workspace_bytes, sdk_stream_t stream);
+int sdk_gated_scan_backward(const sdk_gated_scan* a, void* workspace, size_t workspace_bytes, sdk_stream_t stream);
+/* One token of each sequence: state [batch, width] (states that do not overlap) is updated in place,
+ * output [batch, width] dense; x and gate [batch, width], strides of the batch axis in elements. */
+int sdk_gated_scan_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride, float* state,
+                        int64_t state_stride, void* output, int64_t batch, int64_t width, int32_t dtype,
+                        sdk_stream_t stream);
+
+/* `count` matrices [rows, columns] (dense, one behind the other) made orthogonal: X = x / (norm of x + eps), then
+ * `steps` (1 to 100) times
+ *   S = X X^T (of the smaller side)      X = a X + (b S + c S S) X        coefficients: a, b, c (host array)
+ * which brings the singular values towards one.  float32 and float16: products from two float16 pieces a value (22
+ * bits); bfloat16: from one (11 bits).  Sums are float32.  Singular values may pass 1 on the way but have to stay
+ * below 3.8: entries beyond 15 overflow and give NaN.  Sides up to 131072, matrices of up to 2^31 values; out may be x.
+ * eps: 2^-100 to 1.  The workspace begins at a multiple of 128. */
+size_t sdk_orthogonalize_workspace_bytes(int64_t rows, int64_t columns, int64_t count, int32_t dtype);
+int sdk_orthogonalize(const void* x, void* out, int64_t rows, int64_t columns, int64_t count, int32_t steps,
+                      const double* coefficients, double eps, void* workspace, size_t workspace_bytes, int32_t dtype,
+                      sdk_stream_t stream);
+/* One Muon step over `count` matrices, in place:
+ *   m = momentum m + (1 - momentum) g      u = momentum m + (1 - momentum) g with nesterov, or m
+ *   p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / columns)) orthogonalize(u)
+ * The lists are host arrays, read before the call returns; params and grads have `dtype`, momenta are float32.  No two
+ * tensors may overlap. */
+size_t sdk_muon_step_workspace_bytes(const int64_t* rows, const int64_t* columns, int64_t count, int32_t dtype);
+int sdk_muon_step(void* const* params, const void* const* grads, float* const* momenta, const int64_t* rows,
+                  const int64_t* columns, int64_t count, double lr, double momentum, int32_t nesterov,
+                  double weight_decay, int32_t steps, const double* coefficients, double eps, void* workspace,
+                  size_t workspace_bytes, int32_t dtype, sdk_stream_t stream);
 
 #ifdef __cplusplus
 }

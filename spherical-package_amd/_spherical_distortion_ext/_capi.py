@@ -27,7 +27,17 @@ class BucketAttention(ctypes.Structure):
                    ("table_dtype", _i32)])
 
 
+class GatedScan(ctypes.Structure):
+    """sdk_gated_scan."""
+    _fields_ = ([(n, _vp) for n in ("x", "gate", "state", "lengths", "output", "last", "grad_output", "grad_last",
+                                    "grad_x", "grad_gate", "grad_state")]
+                + [(n, _i64) for n in ("batch", "tokens", "width")]
+                + [(n + "_strides", _i64 * 2) for n in ("x", "gate", "grad_output")]
+                + [("reverse", _i32), ("dtype", _i32)])
+
+
 _attention = ctypes.POINTER(BucketAttention)
+_scan = ctypes.POINTER(GatedScan)
 _step_settings = [_i64] + [ctypes.c_double] * 5 + [_i64, _i32, _vp]
 # name -> argument types, in header order
 _CONV_DIMS = [_i64] * 8 + [_i32] * 4 + [_vp]
@@ -102,6 +112,14 @@ SIGNATURES = {
     "sdk_adamw_step": [_vp] * 5 + _step_settings,
     "sdk_adamw_step_8bit": [_vp] * 7 + _step_settings,
     "sdk_adamw_moment_values": [_vp] * 3 + [_i64] + [_i32] * 2 + [_vp],
+    "sdk_add_layer_norm": [_vp] * 8 + [_i64] * 2 + [ctypes.c_double] + [_i32] * 2 + [_vp],
+    "sdk_add_layer_norm_backward": [_vp] * 10 + [_sz] + [_i64] * 2 + [_i32] * 2 + [_vp],
+    "sdk_gated_scan_forward": [_scan, _vp, _sz, _vp],
+    "sdk_gated_scan_backward": [_scan, _vp, _sz, _vp],
+    "sdk_gated_scan_step": [_vp, _i64, _vp, _i64, _vp, _i64, _vp] + [_i64] * 2 + [_i32, _vp],
+    "sdk_orthogonalize": [_vp] * 2 + [_i64] * 3 + [_i32, _vp, ctypes.c_double, _vp, _sz, _i32, _vp],
+    "sdk_muon_step": [_vp] * 5 + [_i64] + [ctypes.c_double] * 2 + [_i32, ctypes.c_double, _i32, _vp, ctypes.c_double,
+                                                                    _vp, _sz, _i32, _vp],
 }
 OTHER_SYMBOLS = ("sdk_last_error", "sdk_version", "sdk_mapped_conv_workspace_bytes",
                  "sdk_resample_to_map_workspace_bytes", "sdk_mapped_max_unpool_workspace_bytes",
@@ -109,7 +127,9 @@ OTHER_SYMBOLS = ("sdk_last_error", "sdk_version", "sdk_mapped_conv_workspace_byt
                  "sdk_mapped_conv_plan_bytes", "sdk_mapped_conv_plan_bytes_columns",
                  "sdk_mapped_conv_columns_bytes",
                  "sdk_mapped_avg_unpool_lists_bytes", "sdk_bucket_attention_workspace_bytes",
-                 "sdk_add_rms_norm_backward_workspace_bytes")
+                 "sdk_add_rms_norm_backward_workspace_bytes", "sdk_add_layer_norm_backward_workspace_bytes",
+                 "sdk_gated_scan_workspace_bytes", "sdk_orthogonalize_workspace_bytes",
+                 "sdk_muon_step_workspace_bytes")
 
 _lib = None
 
@@ -154,6 +174,14 @@ def load():
     lib.sdk_bucket_attention_workspace_bytes.restype = _sz
     lib.sdk_add_rms_norm_backward_workspace_bytes.argtypes = [_i64] * 2
     lib.sdk_add_rms_norm_backward_workspace_bytes.restype = _sz
+    lib.sdk_add_layer_norm_backward_workspace_bytes.argtypes = [_i64] * 2
+    lib.sdk_add_layer_norm_backward_workspace_bytes.restype = _sz
+    lib.sdk_gated_scan_workspace_bytes.argtypes = [_scan]
+    lib.sdk_gated_scan_workspace_bytes.restype = _sz
+    lib.sdk_orthogonalize_workspace_bytes.argtypes = [_i64] * 3 + [_i32]
+    lib.sdk_orthogonalize_workspace_bytes.restype = _sz
+    lib.sdk_muon_step_workspace_bytes.argtypes = [_vp, _vp, _i64, _i32]
+    lib.sdk_muon_step_workspace_bytes.restype = _sz
     _lib = lib
     return lib
 

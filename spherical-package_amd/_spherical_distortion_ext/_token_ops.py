@@ -1,5 +1,6 @@
 """PyTorch-ROCm custom operators on token sequences over the C ABI: attention with a learned bias
-for each bucket of relative positions, residual addition with root-mean-square norm, AdamW.
+for each bucket of relative positions, a gated linear recurrence, residual addition with root-mean-square
+and layer norm, AdamW, Muon.
 
 Registered beside the mapped operators in ``torch.ops.sdk_mapped_ops``, for the CUDA (= HIP on
 ROCm) dispatch key only.  The reference has none of them.  Where libsdk_torch_ops.so is built, its
@@ -336,6 +337,225 @@ def adamw_moment_values(codes, scales, dtype):
     return out
 
 
+# --------------------------------------------------------------------------- layer norm
+def _check_layer_norm(x, residual, weight, bias):
+    _check_norm(x, residual, weight)
+    _on_gpu(x, bias=bias)
+    _dense(bias=bias)
+    if bias is not None and (bias.shape != weight.shape or bias.dtype != weight.dtype):
+        raise RuntimeError("bias must be like weight: %s %s, got %s %s"
+                           % (tuple(weight.shape), weight.dtype, tuple(bias.shape), bias.dtype))
+
+
+def add_layer_norm(x, residual, weight, bias, eps):
+    """-> (norm, x + residual, mean and reciprocal standard deviation of each row); without a residual the second
+    is an empty tensor."""
+    _check_layer_norm(x, residual, weight, bias)
+    out = torch.empty_like(x)
+    summed = x.new_empty(0) if residual is None else torch.empty_like(x)
+    mean, inverse = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    width = x.shape[-1]
+    with torch.cuda.device(x.device):
+        _capi.call("sdk_add_layer_norm", *(_ops._ptr(t) for t in (x, residual, weight, bias, out, None if residual is None
+                                                                  else summed, mean, inverse)),
+                   x.numel() // width, width, float(eps), _DTYPES[x.dtype], _DTYPES[weight.dtype], _ops._stream(x))
+    return out, summed, mean, inverse
+
+
+def add_layer_norm_backward(grad, grad_sum, summed, weight, mean, inverse, need_x, need_weight, need_bias):
+    """-> (gradient of x and of residual, of weight, of bias); those not asked for are empty tensors."""
+    _check_norm(summed, None, weight)
+    _on_gpu(summed, grad=grad, grad_sum=grad_sum, mean=mean, inverse=inverse)
+    for name, t in (("grad", grad), ("grad_sum", grad_sum)):
+        if t is not None and (t.shape != summed.shape or t.dtype != summed.dtype):
+            raise RuntimeError("%s must be like the sums: %s %s, got %s %s"
+                               % (name, tuple(summed.shape), summed.dtype, tuple(t.shape), t.dtype))
+    _dense(grad=grad, grad_sum=grad_sum, mean=mean, inverse=inverse)
+    width = summed.shape[-1]
+    rows = summed.numel() // width
+    for t in (mean, inverse):
+        if t.dtype != torch.float32 or t.numel() != rows:
+            raise RuntimeError("mean and inverse must be float32 with one value for each row")
+    dx = torch.empty_like(summed) if need_x else summed.new_empty(0)
+    dw, db = (torch.empty_like(weight) if need else weight.new_empty(0) for need in (need_weight, need_bias))
+    if not need_x and not need_weight and not need_bias:
+        return dx, dw, db
+    with torch.cuda.device(summed.device):
+        need = 0
+        if need_weight or need_bias:
+            need = _capi.load().sdk_add_layer_norm_backward_workspace_bytes(rows, width)
+        ws = torch.empty(need, dtype=torch.uint8, device=summed.device) if need else None
+        _capi.call("sdk_add_layer_norm_backward",
+                   *(_ops._ptr(t) for t in (grad, grad_sum, summed, weight, mean, inverse, dx if need_x else None,
+                                            dw if need_weight else None, db if need_bias else None, ws)), need,
+                   rows, width, _DTYPES[summed.dtype], _DTYPES[weight.dtype], _ops._stream(summed))
+    return dx, dw, db
+
+
+# --------------------------------------------------------------------------- gated scan
+def _check_scan(x, gate, state, lengths):
+    _on_gpu(x, gate=gate, state=state, lengths=lengths)
+    _dtype("x", x)
+    if x.dim() != 3:
+        raise RuntimeError("x must be [batch, tokens, width], got %s" % (tuple(x.shape),))
+    if gate.shape != x.shape or gate.dtype != x.dtype:
+        raise RuntimeError("gate must be like x: %s %s, got %s %s"
+                           % (tuple(x.shape), x.dtype, tuple(gate.shape), gate.dtype))
+    B, _, D = x.shape
+    if state is not None and (tuple(state.shape) != (B, D) or state.dtype != torch.float32):
+        raise RuntimeError("state must be float32 of shape [%d, %d], got %s %s"
+                           % (B, D, state.dtype, tuple(state.shape)))
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,)):
+        raise RuntimeError("lengths must be int32 of shape [%d], got %s %s" % (B, lengths.dtype, tuple(lengths.shape)))
+    _dense(lengths=lengths)
+
+
+def _tokens_ready(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else _laid_out(t)
+
+
+def _token_strides(t):
+    """Batch and token strides; those of axes of length one do not count."""
+    return (ctypes.c_int64 * 2)(*(t.stride(i) if t.shape[i] != 1 else 0 for i in range(2)))
+
+
+def _scan_args(x, gate, state, lengths, reverse):
+    """The argument block and the tensors whose memory it names."""
+    x, gate = _tokens_ready(x), _tokens_ready(gate)
+    state = None if state is None else state.contiguous()
+    a = _capi.GatedScan()
+    a.x, a.gate, a.state = x.data_ptr(), gate.data_ptr(), 0 if state is None else state.data_ptr()
+    a.lengths = 0 if lengths is None else lengths.data_ptr()
+    a.batch, a.tokens, a.width = x.shape
+    a.x_strides, a.gate_strides = _token_strides(x), _token_strides(gate)
+    a.reverse, a.dtype = int(reverse), _DTYPES[x.dtype]
+    return a, (x, gate, state, lengths)
+
+
+def _run_scan(name, a, ref):
+    need = _capi.load().sdk_gated_scan_workspace_bytes(ctypes.byref(a))
+    ws = torch.empty(need, dtype=torch.uint8, device=ref.device) if need else None
+    _capi.call(name, ctypes.byref(a), _ops._ptr(ws), need, _ops._stream(ref))
+
+
+def gated_scan_forward(x, gate, state, lengths, reverse):
+    """-> (output [batch, tokens, width], the last state [batch, width] float32)."""
+    _check_scan(x, gate, state, lengths)
+    with torch.cuda.device(x.device):
+        a, keep = _scan_args(x, gate, state, lengths, reverse)
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        last = torch.empty((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
+        a.output, a.last = out.data_ptr(), last.data_ptr()
+        _run_scan("sdk_gated_scan_forward", a, x)
+    return out, last
+
+
+def gated_scan_backward(grad_output, grad_last, x, gate, state, lengths, output, reverse, need_x, need_gate,
+                        need_state):
+    """-> gradients of x, gate and state; those not asked for are empty tensors."""
+    _check_scan(x, gate, state, lengths)
+    _on_gpu(x, grad_output=grad_output, grad_last=grad_last, output=output)
+    B, _, D = x.shape
+    for name, t in (("grad_output", grad_output), ("output", output)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise RuntimeError("%s must be like x: %s %s, got %s %s"
+                               % (name, tuple(x.shape), x.dtype, tuple(t.shape), t.dtype))
+    if grad_last is not None and (tuple(grad_last.shape) != (B, D) or grad_last.dtype != torch.float32):
+        raise RuntimeError("grad_last must be float32 of shape [%d, %d]" % (B, D))
+    dx, dgate = (torch.empty(x.shape if need else (0,), dtype=x.dtype, device=x.device) for need in (need_x, need_gate))
+    dstate = torch.empty((B, D) if need_state else (0,), dtype=torch.float32, device=x.device)
+    if not need_x and not need_gate and not need_state:
+        return dx, dgate, dstate
+    with torch.cuda.device(x.device):
+        a, keep = _scan_args(x, gate, state, lengths, reverse)
+        output = output.contiguous()
+        a.output = output.data_ptr()
+        if grad_output is not None:
+            grad_output = _tokens_ready(grad_output)
+            a.grad_output, a.grad_output_strides = grad_output.data_ptr(), _token_strides(grad_output)
+        if grad_last is not None:
+            grad_last = grad_last.contiguous()
+            a.grad_last = grad_last.data_ptr()
+        for name, t, need in (("grad_x", dx, need_x), ("grad_gate", dgate, need_gate), ("grad_state", dstate, need_state)):
+            if need:
+                setattr(a, name, t.data_ptr())
+        _run_scan("sdk_gated_scan_backward", a, x)
+    return dx, dgate, dstate
+
+
+def gated_scan_step(x, gate, state):
+    """One token of each sequence; state [batch, width] is updated in place. -> output like x, dense."""
+    _on_gpu(x, gate=gate, state=state)
+    _dtype("x", x)
+    if x.dim() != 2 or gate.shape != x.shape or gate.dtype != x.dtype:
+        raise RuntimeError("x and gate must be [batch, width] of one type, got %s %s and %s %s"
+                           % (tuple(x.shape), x.dtype, tuple(gate.shape), gate.dtype))
+    B, D = x.shape
+    if state.shape != x.shape or state.dtype != torch.float32:
+        raise RuntimeError("state must be float32 of shape [%d, %d], got %s %s"
+                           % (B, D, state.dtype, tuple(state.shape)))
+    if (D > 1 and state.stride(1) != 1) or (B > 1 and state.stride(0) < D):
+        raise RuntimeError("state must have dense rows that do not overlap (it is changed in place), got strides %s"
+                           % (state.stride(),))
+    x, gate = _tokens_ready(x), _tokens_ready(gate)
+    out = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        _capi.call("sdk_gated_scan_step", _ops._ptr(x), x.stride(0), _ops._ptr(gate), gate.stride(0), _ops._ptr(state),
+                   state.stride(0), _ops._ptr(out), B, D, _DTYPES[x.dtype], _ops._stream(x))
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
+    return out
+
+
+# --------------------------------------------------------------------------- matrices made orthogonal, Muon
+def _coefficients(values):
+    if len(values) != 3:
+        raise RuntimeError("coefficients must be three numbers, got %d" % len(values))
+    return (ctypes.c_double * 3)(*values)
+
+
+def orthogonalize(x, steps, coefficients, eps):
+    """-> a dense tensor like x [.., rows, columns]."""
+    _on_gpu(x)
+    dtype = _dtype("x", x)
+    if x.dim() < 2:
+        raise RuntimeError("x must be [.., rows, columns], got %s" % (tuple(x.shape),))
+    c = _coefficients(coefficients)
+    x = x.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rows, columns = x.shape[-2:]
+    count = x.numel() // (rows * columns) if x.numel() else 0
+    with torch.cuda.device(x.device):
+        need = _capi.load().sdk_orthogonalize_workspace_bytes(rows, columns, count, dtype)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        _capi.call("sdk_orthogonalize", _ops._ptr(x), _ops._ptr(out), rows, columns, count, steps, c, eps,
+                   _ops._ptr(ws), need, dtype, _ops._stream(x))
+    return out
+
+
+def muon_step(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, coefficients, eps):
+    _check_lists(params, {"params": (params, None, None), "grads": (grads, None, None),
+                          "momenta": (momenta, torch.float32, None)})
+    if not params:
+        return
+    for i, p in enumerate(params):
+        if p.dim() < 2:
+            raise RuntimeError("params[%d] must have two axes at least, got %s" % (i, tuple(p.shape)))
+    c, n = _coefficients(coefficients), len(params)
+    rows = (ctypes.c_int64 * n)(*(p.shape[0] for p in params))
+    columns = (ctypes.c_int64 * n)(*(p.numel() // p.shape[0] if p.shape[0] else 0 for p in params))
+    dtype = _DTYPES[params[0].dtype]
+    with torch.cuda.device(params[0].device):
+        need = _capi.load().sdk_muon_step_workspace_bytes(rows, columns, n, dtype)
+        ws = torch.empty(need, dtype=torch.uint8, device=params[0].device) if need else None
+        _capi.call("sdk_muon_step", _pointers(params), _pointers(grads), _pointers(momenta), rows, columns, n, lr,
+                   momentum, int(nesterov), weight_decay, steps, c, eps, _ops._ptr(ws), need, dtype,
+                   _ops._stream(params[0]))
+    for t in (*params, *momenta):
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 # --------------------------------------------------------------------------- forms with gradients
 # Registered with autograd by the compiled layer alone; without it functional/token_ops.py's autograd functions serve.
 def bucket_attention(query, key, value, bias_table, bucket_map, key_lengths, causal, scale):
@@ -345,6 +565,16 @@ def bucket_attention(query, key, value, bias_table, bucket_map, key_lengths, cau
 def rms_norm_pair(x, residual, weight, eps):
     """-> [norm, x + residual], or [norm] without a residual."""
     return list(add_rms_norm(x, residual, weight, eps)[:1 if residual is None else 2])
+
+
+def layer_norm_pair(x, residual, weight, bias, eps):
+    """-> [norm, x + residual], or [norm] without a residual."""
+    return list(add_layer_norm(x, residual, weight, bias, eps)[:1 if residual is None else 2])
+
+
+def gated_scan(x, gate, state, lengths, reverse):
+    """-> [output, last state]."""
+    return list(gated_scan_forward(x, gate, state, lengths, reverse))
 
 
 # --------------------------------------------------------------------------- registration
@@ -377,8 +607,26 @@ _SCHEMAS = (
      "(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] avg_codes, Tensor(c!)[] avg_scales,"
      " Tensor(d!)[] sq_codes, Tensor(e!)[] sq_scales," + _SETTINGS, adamw_step_8bit),
     ("adamw_moment_values", "(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor", adamw_moment_values),
+    ("layer_norm_pair", "(Tensor x, Tensor? residual, Tensor weight, Tensor? bias, float eps) -> Tensor[]",
+     layer_norm_pair),
+    ("add_layer_norm",
+     "(Tensor x, Tensor? residual, Tensor weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor, Tensor)",
+     add_layer_norm),
+    ("add_layer_norm_backward",
+     "(Tensor grad, Tensor? grad_sum, Tensor summed, Tensor weight, Tensor mean, Tensor inverse, bool need_x,"
+     " bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)", add_layer_norm_backward),
+    ("gated_scan", "(Tensor x, Tensor gate, Tensor? state, Tensor? lengths, bool reverse) -> Tensor[]", gated_scan),
+    ("gated_scan_forward", "(Tensor x, Tensor gate, Tensor? state, Tensor? lengths, bool reverse) -> (Tensor, Tensor)",
+     gated_scan_forward),
+    ("gated_scan_backward",
+     "(Tensor? grad_output, Tensor? grad_last, Tensor x, Tensor gate, Tensor? state, Tensor? lengths, Tensor output,"
+     " bool reverse, bool need_x, bool need_gate, bool need_state) -> (Tensor, Tensor, Tensor)", gated_scan_backward),
+    ("gated_scan_step", "(Tensor x, Tensor gate, Tensor(a!) state) -> Tensor", gated_scan_step),
+    ("orthogonalize", "(Tensor x, int steps, float[] coefficients, float eps) -> Tensor", orthogonalize),
+    ("muon_step",
+     "(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float lr, float momentum, bool nesterov,"
+     " float weight_decay, int steps, float[] coefficients, float eps) -> ()", muon_step),
 )
-
 
 
 def _native_names():

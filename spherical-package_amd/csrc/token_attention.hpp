@@ -367,13 +367,6 @@ __device__ __forceinline__ void as_rounded(float (&p)[16]) {
   }
 }
 
-// Workgroups follow each other round the eight dies; consecutive tiles of one head share its keys and values, so
-// each die gets a consecutive range of tiles.
-__device__ __forceinline__ unsigned by_die(unsigned id, unsigned count) {
-  const unsigned die = id % 8, each = count / 8, more = count % 8;
-  return die * each + (die < more ? die : more) + id / 8;
-}
-
 // What the kernels take of sdk_bucket_attention; scale2 = scale * log2(e).
 struct Attention {
   const void *q, *k, *v, *table, *out, *grad;

@@ -1,0 +1,354 @@
+// Addition of the residual and layer norm of rows, with the gradients of rows, weight and bias.
+//
+//   h = x + r     z_j = (h_j - mu) inv,  mu = mean_j h_j,  inv = 1 / sqrt(mean_j (h_j - mu)^2 + eps)
+//   y_j = w_j z_j + b_j
+//   dh_j = inv (q_j - mean_i q_i - z_j mean_i (q_i z_i)) + s_j,  q = w g     (g, s: the gradients of y and h)
+//   dw_j = sum over rows of g_j z_j,  db_j = sum over rows of g_j
+//
+// Bound by memory: a row is read once and held in registers, where the mean is formed first and the squares of the
+// distances from it after (their difference from sums of squares would lose a mean's square).  Sums are float32.  The
+// forward normalises the sum before it is rounded to the tensors' type; the backward reads the rounded h, which the
+// forward wrote.
+#include <algorithm>
+
+#include "token_types.hpp"
+
+namespace sdk {
+namespace token {
+namespace {
+
+// A row is dealt to THREADS threads (4 to 1024, the fewest that take it with 16 values each), in chunks of 16 bytes:
+// chunk k of thread t begins at (k * THREADS + t) * V.  Workgroups of at least 256 threads: narrow rows share one.
+template <int THREADS>
+constexpr int kGroup = THREADS < 256 ? 256 : THREADS;
+template <typename T>
+constexpr int kChunks = 16 / kWide<T>;
+constexpr int64_t kMostWidth = 16384;
+
+template <int THREADS>
+__device__ __forceinline__ float row_sum(float x, float* slots) {
+  if constexpr (THREADS < 64)
+    return over_lanes<Add, THREADS>(x);
+  else
+    return over_group<Add, THREADS>(x, slots);
+}
+
+template <typename T, int THREADS, bool ALIGNED>
+__global__ __launch_bounds__(kGroup<THREADS>) void layer_forward(const T* x, const T* residual, const void* weight,
+                                                                 const void* bias, int weight_float, T* out, T* summed,
+                                                                 float* mean, float* inverse, int64_t rows, int width,
+                                                                 float eps) {
+  constexpr int V = kWide<T>, N = kChunks<T>;
+  __shared__ float slots[kGroup<THREADS> / 64];
+  const int t = threadIdx.x % THREADS;
+  const int64_t row = (int64_t)blockIdx.x * (kGroup<THREADS> / THREADS) + threadIdx.x / THREADS;
+  const bool live = row < rows;
+  const int64_t base = row * width;
+  float h[N][V];
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[k][e] = 0.f;
+    if (live && j < width) {
+      get<T, V, ALIGNED>(x + base + j, h[k], width - j);
+      if (residual) {
+        float r[V];
+        get<T, V, ALIGNED>(residual + base + j, r, width - j);
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[k][e] += r[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum += h[k][e];
+  }
+  if (summed) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = (k * THREADS + t) * V;
+      if (live && j < width) put<T, V, ALIGNED>(summed + base + j, h[k], width - j);
+    }
+  }
+  const float mu = row_sum<THREADS>(sum, slots) / (float)width;
+  float sq = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int left = width - (k * THREADS + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      h[k][e] -= mu;
+      if (e < left) sq += h[k][e] * h[k][e];
+    }
+  }
+  const float inv = 1.f / sqrtf(row_sum<THREADS>(sq, slots) / (float)width + eps);
+  if (live && t == 0) {
+    if (mean) mean[row] = mu;
+    if (inverse) inverse[row] = inv;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+    if (live && j < width) {
+      float w[V], b[V];
+      load_weight<T, V, ALIGNED>(weight, weight_float, j, w, width - j);
+#pragma unroll
+      for (int e = 0; e < V; ++e) b[e] = 0.f;
+      if (bias) load_weight<T, V, ALIGNED>(bias, weight_float, j, b, width - j);
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[k][e] = h[k][e] * inv * w[e] + b[e];
+      put<T, V, ALIGNED>(out + base + j, h[k], width - j);
+    }
+  }
+}
+
+// Workgroup b takes rows b, b + gridDim.x, ... (times the rows that share a workgroup) and keeps its parts of dw and db
+// in registers; the parts [group][dw, db][width] are joined in their order by join_parts.
+template <typename T, int THREADS, bool ALIGNED>
+__global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad, const T* grad_sum, const T* h_in,
+                                                                  const void* weight, int weight_float,
+                                                                  const float* mean, const float* inverse, T* grad_x,
+                                                                  float* parts, int64_t rows, int width) {
+  constexpr int V = kWide<T>, N = kChunks<T>, SHARE = kGroup<THREADS> / THREADS;
+  __shared__ float slots[2][kGroup<THREADS> / 64];
+  const int t = threadIdx.x % THREADS, sub = threadIdx.x / THREADS;
+  float w[N][V], dw[N][V], db[N][V];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = (k * THREADS + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[k][e] = dw[k][e] = db[k][e] = 0.f;
+    if (j < width) load_weight<T, V, ALIGNED>(weight, weight_float, j, w[k], width - j);
+  }
+  for (int64_t first = (int64_t)blockIdx.x * SHARE; first < rows; first += (int64_t)gridDim.x * SHARE) {
+    const int64_t row = first + sub, base = row * width;
+    const bool live = row < rows;
+    const float inv = live ? inverse[row] : 0.f, mu = live ? mean[row] : 0.f;
+    float z[N][V], q[N][V], flat = 0.f, along = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = (k * THREADS + t) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[k][e] = q[k][e] = 0.f;
+      if (live && j < width) {
+        get<T, V, ALIGNED>(h_in + base + j, z[k], width - j);
+        get<T, V, ALIGNED>(grad + base + j, q[k], width - j);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        // beyond the row's end q and w are zeros: z counts nowhere
+        z[k][e] = (z[k][e] - mu) * inv;
+        dw[k][e] += q[k][e] * z[k][e];
+        db[k][e] += q[k][e];
+        q[k][e] *= w[k][e];
+        flat += q[k][e];
+        along += q[k][e] * z[k][e];
+      }
+    flat = row_sum<THREADS>(flat, slots[0]) / (float)width;
+    along = row_sum<THREADS>(along, slots[1]) / (float)width;
+    if (grad_x) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int j = (k * THREADS + t) * V;
+        if (live && j < width) {
+          float s[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[e] = 0.f;
+          if (grad_sum) get<T, V, ALIGNED>(grad_sum + base + j, s, width - j);
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[e] += inv * (q[k][e] - flat - z[k][e] * along);
+          put<T, V, ALIGNED>(grad_x + base + j, s, width - j);
+        }
+      }
+    }
+  }
+  if (!parts) return;
+  float* to = parts + (int64_t)blockIdx.x * 2 * width;
+  if constexpr (SHARE > 1) {   // the rows that share the workgroup are joined in LDS
+    __shared__ float joined[SHARE][THREADS * N * V];
+#pragma unroll
+    for (int which = 0; which < 2; ++which, to += width) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) joined[sub][(k * V + e) * THREADS + t] = which ? db[k][e] : dw[k][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < THREADS * N * V; i += kGroup<THREADS>) {
+        const int ke = i / THREADS, j = (ke / V * THREADS + i % THREADS) * V + ke % V;
+        float x = 0.f;
+#pragma unroll
+        for (int s = 0; s < SHARE; ++s) x += joined[s][i];
+        if (j < width) to[j] = x;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = (k * THREADS + t) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (j + e < width) to[j + e] = dw[k][e], to[width + j + e] = db[k][e];
+    }
+  }
+}
+
+// The sums over the parts: 64 of the 2 width columns a workgroup, a sixteenth of the parts a wave, eight at a time.
+template <typename T>
+__global__ __launch_bounds__(1024) void join_parts(const float* parts, int64_t count, int width, void* grad_weight,
+                                                   void* grad_bias, int is_float) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int j = blockIdx.x * 64 + lane;
+  const int64_t each = (count + 15) / 16, from = wave * each, to = from + each < count ? from + each : count;
+  float s = 0.f;
+  if (j < 2 * width) {
+    const int64_t step = 2 * (int64_t)width;
+    int64_t i = from;
+    for (; i + 8 <= to; i += 8) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = parts[(i + u) * step + j];
+      s += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    }
+    for (; i < to; ++i) s += parts[i * step + j];
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && j < 2 * width) {
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += sums[w][lane];
+    void* to_grad = j < width ? grad_weight : grad_bias;
+    const int at = j < width ? j : j - width;
+    if (!to_grad) return;
+    if (is_float)
+      ((float*)to_grad)[at] = s;
+    else
+      ((T*)to_grad)[at] = (T)s;
+  }
+}
+
+// Threads of a row: a power of two from 4 on, at most 16 values each.
+int threads_of(int64_t width) {
+  int threads = 4;
+  while (threads * 16 < width) threads *= 2;
+  return threads;
+}
+
+#define LAYER_THREADS(THREADS_, ...) \
+  case THREADS_: { constexpr int THREADS = THREADS_; __VA_ARGS__; break; }
+#define LAYER_SHAPE_OF(...)               \
+  switch (threads_of(width)) {            \
+    LAYER_THREADS(4, __VA_ARGS__)         \
+    LAYER_THREADS(8, __VA_ARGS__)         \
+    LAYER_THREADS(16, __VA_ARGS__)        \
+    LAYER_THREADS(32, __VA_ARGS__)        \
+    LAYER_THREADS(64, __VA_ARGS__)        \
+    LAYER_THREADS(128, __VA_ARGS__)       \
+    LAYER_THREADS(256, __VA_ARGS__)       \
+    LAYER_THREADS(512, __VA_ARGS__)       \
+    default: { constexpr int THREADS = 1024; __VA_ARGS__; } \
+  }
+// Runs the statement with THREADS and ALIGNED for rows of `width`; `wide`: 16-byte vectors fit rows and pointers.
+#define LAYER_SHAPE(...)                                                     \
+  do {                                                                       \
+    if (wide) { constexpr bool ALIGNED = true; LAYER_SHAPE_OF(__VA_ARGS__) }  \
+    else { constexpr bool ALIGNED = false; LAYER_SHAPE_OF(__VA_ARGS__) }      \
+  } while (0)
+
+// The rows in launches of as many as one holds.
+template <typename T, int THREADS, bool ALIGNED>
+void run_forward(const T* x, const T* residual, const void* weight, const void* bias, int weight_float, T* out, T* summed,
+                 float* mean, float* inverse, int64_t rows, int width, float eps, hipStream_t s) {
+  constexpr int SHARE = kGroup<THREADS> / THREADS;
+  constexpr int64_t EACH = most_groups(kGroup<THREADS>) * SHARE;
+  for (int64_t row = 0; row < rows; row += EACH) {
+    const int64_t count = std::min(EACH, rows - row), at = row * width;
+    launch(layer_forward<T, THREADS, ALIGNED>, dim3((unsigned)ceil_div(count, SHARE)), dim3(kGroup<THREADS>), s, x + at,
+           residual ? residual + at : nullptr, weight, bias, weight_float, out + at, summed ? summed + at : nullptr,
+           mean ? mean + row : nullptr, inverse ? inverse + row : nullptr, count, width, eps);
+  }
+}
+
+int64_t backward_groups(int64_t rows, int64_t width) {
+  const int threads = threads_of(width), share = threads < 256 ? 256 / threads : 1;
+  const int64_t groups = threads > 256 ? 512 : 1024;
+  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, share), groups));
+}
+
+int check(int64_t rows, int64_t width, int dtype, int weight_dtype) {
+  SDK_REQUIRE(rows >= 0 && rows < (int64_t)1 << 31, "rows = %lld must be between 0 and 2^31", (long long)rows);
+  SDK_REQUIRE(width >= 1 && width <= kMostWidth, "width = %lld must be between 1 and %lld",
+              (long long)width, (long long)kMostWidth);
+  SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
+  SDK_REQUIRE(weight_dtype == dtype || weight_dtype == SDK_F32,
+              "weight's dtype %d must be the rows' or float32", weight_dtype);
+  return SDK_OK;
+}
+
+}  // namespace
+}  // namespace token
+}  // namespace sdk
+
+using namespace sdk;
+using namespace sdk::token;
+
+extern "C" {
+
+int sdk_add_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, void* out,
+                       void* summed, float* mean, float* inverse, int64_t rows, int64_t width, double eps,
+                       int32_t dtype, int32_t weight_dtype, sdk_stream_t stream) {
+  if (int rc = check(rows, width, dtype, weight_dtype)) return rc;
+  SDK_REQUIRE(eps >= 0, "eps must not be negative");
+  if (rows == 0) return SDK_OK;
+  SDK_REQUIRE(x && weight && out, "x, weight and out must not be NULL");
+  hipStream_t s = (hipStream_t)stream;
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, {
+    const bool wide = width % kWide<T> == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) &&
+                      aligned16(bias) && aligned16(out) && aligned16(summed);
+    LAYER_SHAPE(run_forward<T, THREADS, ALIGNED>((const T*)x, (const T*)residual, weight, bias, weight_dtype == SDK_F32,
+                                                 (T*)out, (T*)summed, mean, inverse, rows, (int)width, (float)eps, s));
+  });
+  SDK_LAUNCH_CHECK("add_layer_norm");
+  return SDK_OK;
+}
+
+size_t sdk_add_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
+  if (rows < 1 || width < 1 || width > kMostWidth) return 0;
+  return (size_t)backward_groups(rows, width) * 2 * width * sizeof(float);
+}
+
+int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const void* summed, const void* weight,
+                                const float* mean, const float* inverse, void* grad_x, void* grad_weight,
+                                void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t width,
+                                int32_t dtype, int32_t weight_dtype, sdk_stream_t stream) {
+  if (int rc = check(rows, width, dtype, weight_dtype)) return rc;
+  SDK_REQUIRE(weight && (grad_x || grad_weight || grad_bias), "weight and one gradient at least must not be NULL");
+  SDK_REQUIRE(rows == 0 || (grad && summed && mean && inverse), "grad, summed, mean and inverse must not be NULL");
+  const bool sums = grad_weight || grad_bias;
+  const size_t need = sums ? sdk_add_layer_norm_backward_workspace_bytes(rows, width) : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SDK_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t groups = rows ? backward_groups(rows, width) : 0;
+  float* parts = sums ? (float*)workspace : nullptr;
+  SDK_DISPATCH_TOKEN_DTYPE(dtype, {
+    const bool wide = width % kWide<T> == 0 && aligned16(grad) && aligned16(grad_sum) && aligned16(summed) &&
+                      aligned16(weight) && aligned16(grad_x);
+    if (rows)
+      LAYER_SHAPE(launch(layer_backward<T, THREADS, ALIGNED>, dim3((unsigned)groups), dim3(kGroup<THREADS>), s,
+                         (const T*)grad, (const T*)grad_sum, (const T*)summed, weight,
+                         (int)(weight_dtype == SDK_F32), mean, inverse, (T*)grad_x, parts, rows, (int)width));
+    if (sums)
+      launch(join_parts<T>, dim3((unsigned)ceil_div(2 * width, 64)), dim3(1024), s, (const float*)parts, groups,
+             (int)width, grad_weight, grad_bias, (int)(weight_dtype == SDK_F32));
+  });
+  SDK_LAUNCH_CHECK("add_layer_norm_backward");
+  return SDK_OK;
+}
+
+}  // extern "C"

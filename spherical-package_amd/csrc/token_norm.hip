@@ -29,30 +29,6 @@ constexpr int kGroup = THREADS < 256 ? 256 : THREADS;
 constexpr int kPlain = 0, kInt8 = 1, kFp8 = 2;
 constexpr float kSmallestRow = 0x1p-100f;   // rows below it are zeros in 8 bits: 1 / scale stays finite
 
-// V values of a row, `left` of them in it; ALIGNED: rows and widths of whole vectors.
-template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ void get(const T* p, float (&f)[V], int left) {
-  if constexpr (ALIGNED)
-    load_pack<T, V>(p, f);
-  else
-    load_part<T, V>(p, f, left);
-}
-template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ void put(T* p, const float (&f)[V], int left) {
-  if constexpr (ALIGNED)
-    store_pack<T, V>(p, f);
-  else
-    store_part<T, V>(p, f, left);
-}
-
-template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ void load_weight(const void* w, int is_float, int64_t at, float (&f)[V], int left) {
-  if (is_float)
-    get<float, V, ALIGNED>((const float*)w + at, f, left);
-  else
-    get<T, V, ALIGNED>((const T*)w + at, f, left);
-}
-
 template <typename T, int V, int N, int THREADS, bool ALIGNED>
 __global__ __launch_bounds__(kGroup<THREADS>) void norm_forward(
     const T* x, const T* residual, const void* weight, int weight_float, void* out, float* scales,

@@ -64,6 +64,31 @@ __device__ __forceinline__ void store_part(T* p, const float (&f)[E], int left) 
   }
 }
 
+// V values of a row, `left` of them in it; ALIGNED: rows and widths of whole vectors.
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void get(const T* p, float (&f)[V], int left) {
+  if constexpr (ALIGNED)
+    load_pack<T, V>(p, f);
+  else
+    load_part<T, V>(p, f, left);
+}
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void put(T* p, const float (&f)[V], int left) {
+  if constexpr (ALIGNED)
+    store_pack<T, V>(p, f);
+  else
+    store_part<T, V>(p, f, left);
+}
+
+// V values of a weight that is held in the rows' type or in float32.
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void load_weight(const void* w, int is_float, int64_t at, float (&f)[V], int left) {
+  if (is_float)
+    get<float, V, ALIGNED>((const float*)w + at, f, left);
+  else
+    get<T, V, ALIGNED>((const T*)w + at, f, left);
+}
+
 struct Add {
   __device__ static float of(float a, float b) { return a + b; }
 };
@@ -76,6 +101,14 @@ template <typename Op>
 __device__ __forceinline__ float over_wave(float x) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) x = Op::of(x, __shfl_xor(x, d));
+  return x;
+}
+
+// Over the LANES (a power of two up to 64) consecutive lanes of a group that starts at a multiple of LANES.
+template <typename Op, int LANES>
+__device__ __forceinline__ float over_lanes(float x) {
+#pragma unroll
+  for (int d = LANES / 2; d > 0; d >>= 1) x = Op::of(x, __shfl_xor(x, d));
   return x;
 }
 
@@ -95,6 +128,13 @@ __device__ __forceinline__ float over_group(float x, float* slots) {
     for (int i = 1; i < THREADS / 64; ++i) x = Op::of(x, slots[first + i]);
   }
   return x;
+}
+
+// Workgroups follow each other round the eight dies; consecutive tiles of one head or matrix share its operands, so
+// each die gets a consecutive range of tiles.
+__device__ __forceinline__ unsigned by_die(unsigned id, unsigned count) {
+  const unsigned die = id % 8, each = count / 8, more = count % 8;
+  return die * each + (die < more ? die : more) + id / 8;
 }
 
 // Workgroups of `threads` that one launch holds along x: fewer than 2^32 threads.  A larger grid is cut without an error.

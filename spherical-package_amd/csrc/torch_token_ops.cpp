@@ -287,6 +287,161 @@ Tensor dequantize_rows(const Tensor& codes, const Tensor& scales, at::ScalarType
   return out;
 }
 
+// ------------------------------------------------------------------------------------------ layer norm
+void check_layer_norm(const Tensor& x, const OptTensor& residual, const Tensor& weight, const OptTensor& bias) {
+  check_norm(x, residual, weight);
+  beside(x, "bias", bias);
+  dense("bias", bias);
+  if (has(bias))
+    TORCH_CHECK(bias->sizes() == weight.sizes() && bias->scalar_type() == weight.scalar_type(),
+                "bias must be like weight: ", weight.sizes(), " ", weight.scalar_type(), ", got ", bias->sizes(), " ",
+                bias->scalar_type());
+}
+
+// for_backward: with each row's mean and reciprocal standard deviation.
+std::tuple<Tensor, Tensor, Tensor, Tensor> layer_norm(const Tensor& x, const OptTensor& residual, const Tensor& weight,
+                                                      const OptTensor& bias, double eps, bool for_backward) {
+  check_layer_norm(x, residual, weight, bias);
+  c10::DeviceGuard guard(x.device());
+  Tensor out = at::empty_like(x), summed = has(residual) ? at::empty_like(x) : nothing(x), mean, inverse;
+  if (for_backward) {
+    mean = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    inverse = at::empty_like(mean);
+  }
+  const int64_t width = x.size(-1);
+  TOKEN_CALL(sdk_add_layer_norm, ptr(x), ptr(residual), ptr(weight), ptr(bias), ptr(out),
+             has(residual) ? ptr(summed) : nullptr, for_backward ? (float*)ptr(mean) : nullptr,
+             for_backward ? (float*)ptr(inverse) : nullptr, x.numel() / width, width, eps,
+             dtype_of(x.scalar_type(), "x"), dtype_of(weight.scalar_type(), "weight"), stream_of(x));
+  return {out, summed, mean, inverse};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> add_layer_norm(const Tensor& x, const OptTensor& residual,
+                                                          const Tensor& weight, const OptTensor& bias, double eps) {
+  return layer_norm(x, residual, weight, bias, eps, true);
+}
+
+std::tuple<Tensor, Tensor, Tensor> add_layer_norm_backward(const Tensor& grad, const OptTensor& grad_sum,
+                                                           const Tensor& summed, const Tensor& weight,
+                                                           const Tensor& mean, const Tensor& inverse, bool need_x,
+                                                           bool need_weight, bool need_bias) {
+  check_norm(summed, OptTensor(), weight);
+  beside(summed, "grad", grad), beside(summed, "grad_sum", grad_sum);
+  beside(summed, "mean", mean), beside(summed, "inverse", inverse);
+  for (const auto& t : {std::pair<const char*, OptTensor>{"grad", grad}, {"grad_sum", grad_sum}})
+    if (has(t.second))
+      TORCH_CHECK(t.second->sizes() == summed.sizes() && t.second->scalar_type() == summed.scalar_type(), t.first,
+                  " must be like the sums: ", summed.sizes(), " ", summed.scalar_type(), ", got ", t.second->sizes(),
+                  " ", t.second->scalar_type());
+  dense("grad", grad), dense("grad_sum", grad_sum), dense("mean", mean), dense("inverse", inverse);
+  const int64_t width = summed.size(-1), rows = summed.numel() / width;
+  for (const Tensor& t : {mean, inverse})
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == rows,
+                "mean and inverse must be float32 with one value for each row");
+  c10::DeviceGuard guard(summed.device());
+  Tensor dx = need_x ? at::empty_like(summed) : nothing(summed);
+  Tensor dw = need_weight ? at::empty_like(weight) : nothing(weight);
+  Tensor db = need_bias ? at::empty_like(weight) : nothing(weight);
+  if (!need_x && !need_weight && !need_bias) return {dx, dw, db};
+  const size_t need = need_weight || need_bias ? sdk_add_layer_norm_backward_workspace_bytes(rows, width) : 0;
+  Tensor ws = workspace(summed, need);
+  TOKEN_CALL(sdk_add_layer_norm_backward, ptr(grad), ptr(grad_sum), ptr(summed), ptr(weight), (const float*)ptr(mean),
+             (const float*)ptr(inverse), need_x ? ptr(dx) : nullptr, need_weight ? ptr(dw) : nullptr,
+             need_bias ? ptr(db) : nullptr, need ? ptr(ws) : nullptr, need, rows, width,
+             dtype_of(summed.scalar_type(), "summed"), dtype_of(weight.scalar_type(), "weight"), stream_of(summed));
+  return {dx, dw, db};
+}
+
+// ------------------------------------------------------------------------------------------ gated scan
+void check_scan(const Tensor& x, const Tensor& gate, const OptTensor& state, const OptTensor& lengths) {
+  on_gpu(x);
+  beside(x, "gate", gate), beside(x, "state", state), beside(x, "lengths", lengths);
+  (void)dtype_of(x.scalar_type(), "x");
+  TORCH_CHECK(x.dim() == 3, "x must be [batch, tokens, width], got ", x.sizes());
+  TORCH_CHECK(gate.sizes() == x.sizes() && gate.scalar_type() == x.scalar_type(), "gate must be like x: ", x.sizes(), " ",
+              x.scalar_type(), ", got ", gate.sizes(), " ", gate.scalar_type());
+  const int64_t B = x.size(0), D = x.size(2);
+  if (has(state))
+    TORCH_CHECK(state->dim() == 2 && state->size(0) == B && state->size(1) == D && state->scalar_type() == at::kFloat,
+                "state must be float32 of shape [", B, ", ", D, "], got ", state->scalar_type(), " ", state->sizes());
+  if (has(lengths)) {
+    TORCH_CHECK(lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == B,
+                "lengths must be int32 of shape [", B, "], got ", lengths->scalar_type(), " ", lengths->sizes());
+    dense("lengths", lengths);
+  }
+}
+
+Tensor tokens_ready(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : laid_out(t); }
+
+// Batch and token strides; those of axes of length one do not count.
+void token_strides(const Tensor& t, int64_t (&s)[2]) {
+  for (int i = 0; i < 2; ++i) s[i] = t.size(i) == 1 ? 0 : t.stride(i);
+}
+
+// The argument block; the tensors may be replaced by dense copies, which the caller keeps.
+sdk_gated_scan scan_args(Tensor& x, Tensor& gate, OptTensor& state, const OptTensor& lengths, bool reverse) {
+  x = tokens_ready(x), gate = tokens_ready(gate);
+  if (has(state)) state = state->contiguous();
+  sdk_gated_scan a = {};
+  a.x = ptr(x), a.gate = ptr(gate), a.state = (const float*)ptr(state), a.lengths = (const int32_t*)ptr(lengths);
+  a.batch = x.size(0), a.tokens = x.size(1), a.width = x.size(2);
+  token_strides(x, a.x_strides), token_strides(gate, a.gate_strides);
+  a.reverse = reverse, a.dtype = dtype_of(x.scalar_type(), "x");
+  return a;
+}
+
+std::tuple<Tensor, Tensor> gated_scan_forward(Tensor x, Tensor gate, OptTensor state, const OptTensor& lengths,
+                                              bool reverse) {
+  check_scan(x, gate, state, lengths);
+  c10::DeviceGuard guard(x.device());
+  sdk_gated_scan a = scan_args(x, gate, state, lengths, reverse);
+  Tensor out = at::empty(x.sizes(), x.options());
+  Tensor last = at::empty({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
+  a.output = ptr(out), a.last = (float*)ptr(last);
+  const size_t need = sdk_gated_scan_workspace_bytes(&a);
+  Tensor ws = workspace(x, need);
+  TOKEN_CALL(sdk_gated_scan_forward, &a, need ? ptr(ws) : nullptr, need, stream_of(x));
+  return {out, last};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_scan_backward(OptTensor grad, OptTensor grad_last, Tensor x, Tensor gate,
+                                                       OptTensor state, const OptTensor& lengths, Tensor output,
+                                                       bool reverse, bool need_x, bool need_gate, bool need_state) {
+  check_scan(x, gate, state, lengths);
+  beside(x, "grad_output", grad), beside(x, "grad_last", grad_last), beside(x, "output", output);
+  const int64_t B = x.size(0), D = x.size(2);
+  for (const auto& t : {std::pair<const char*, OptTensor>{"grad_output", grad}, {"output", output}})
+    if (has(t.second))
+      TORCH_CHECK(t.second->sizes() == x.sizes() && t.second->scalar_type() == x.scalar_type(), t.first,
+                  " must be like x: ", x.sizes(), " ", x.scalar_type(), ", got ", t.second->sizes(), " ",
+                  t.second->scalar_type());
+  if (has(grad_last))
+    TORCH_CHECK(grad_last->dim() == 2 && grad_last->size(0) == B && grad_last->size(1) == D &&
+                    grad_last->scalar_type() == at::kFloat,
+                "grad_last must be float32 of shape [", B, ", ", D, "]");
+  c10::DeviceGuard guard(x.device());
+  Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : nothing(x);
+  Tensor dgate = need_gate ? at::empty(x.sizes(), x.options()) : nothing(x);
+  Tensor dstate = need_state ? at::empty({B, D}, x.options().dtype(at::kFloat))
+                             : at::empty({0}, x.options().dtype(at::kFloat));
+  if (!need_x && !need_gate && !need_state) return {dx, dgate, dstate};
+  sdk_gated_scan a = scan_args(x, gate, state, lengths, reverse);
+  output = output.contiguous();
+  a.output = ptr(output);
+  if (has(grad)) {
+    grad = tokens_ready(*grad);
+    a.grad_output = ptr(grad), token_strides(*grad, a.grad_output_strides);
+  }
+  if (has(grad_last)) grad_last = grad_last->contiguous(), a.grad_last = (const float*)ptr(grad_last);
+  if (need_x) a.grad_x = ptr(dx);
+  if (need_gate) a.grad_gate = ptr(dgate);
+  if (need_state) a.grad_state = (float*)ptr(dstate);
+  const size_t need = sdk_gated_scan_workspace_bytes(&a);
+  Tensor ws = workspace(x, need);
+  TOKEN_CALL(sdk_gated_scan_backward, &a, need ? ptr(ws) : nullptr, need, stream_of(x));
+  return {dx, dgate, dstate};
+}
+
 // ------------------------------------------------------------------------------------------ AdamW
 // The pointers of `tensors`, one for each parameter: like it, or `each` values to a scale.
 std::vector<void*> pointers(const char* name, at::TensorList params, at::TensorList tensors, at::ScalarType dtype,
@@ -371,6 +526,74 @@ Tensor adamw_moment_values(const Tensor& codes, const Tensor& scales, at::Scalar
   TOKEN_CALL(sdk_adamw_moment_values, ptr(codes), (const float*)ptr(scales), ptr(out), codes.numel(), (int)second, to,
              stream_of(codes));
   return out;
+}
+
+// One token of each sequence, the state in place.
+Tensor gated_scan_step(Tensor x, Tensor gate, const Tensor& state) {
+  on_gpu(x);
+  beside(x, "gate", gate), beside(x, "state", state);
+  const int dtype = dtype_of(x.scalar_type(), "x");
+  TORCH_CHECK(x.dim() == 2 && gate.sizes() == x.sizes() && gate.scalar_type() == x.scalar_type(),
+              "x and gate must be [batch, width] of one type, got ", x.sizes(), " ", x.scalar_type(), " and ",
+              gate.sizes(), " ", gate.scalar_type());
+  const int64_t B = x.size(0), D = x.size(1);
+  TORCH_CHECK(state.sizes() == x.sizes() && state.scalar_type() == at::kFloat, "state must be float32 of shape [", B,
+              ", ", D, "], got ", state.scalar_type(), " ", state.sizes());
+  TORCH_CHECK((D <= 1 || state.stride(1) == 1) && (B <= 1 || state.stride(0) >= D),
+              "state must have dense rows that do not overlap (it is changed in place), got strides ", state.strides());
+  c10::DeviceGuard guard(x.device());
+  x = tokens_ready(x), gate = tokens_ready(gate);
+  Tensor out = at::empty({B, D}, x.options());
+  TOKEN_CALL(sdk_gated_scan_step, ptr(x), x.stride(0), ptr(gate), gate.stride(0), (float*)ptr(state), state.stride(0),
+             ptr(out), B, D, dtype, stream_of(x));
+  changed({state});
+  return out;
+}
+
+// ------------------------------------------------------------------------------------------ Muon
+Tensor orthogonalize(Tensor x, int64_t steps, at::ArrayRef<double> coefficients, double eps) {
+  on_gpu(x);
+  const int dtype = dtype_of(x.scalar_type(), "x");
+  TORCH_CHECK(x.dim() >= 2, "x must be [.., rows, columns], got ", x.sizes());
+  TORCH_CHECK(coefficients.size() == 3, "coefficients must be three numbers, got ", coefficients.size());
+  TORCH_CHECK(steps >= 1 && steps <= 100, "steps = ", steps, " must be between 1 and 100");
+  c10::DeviceGuard guard(x.device());
+  x = x.contiguous();
+  Tensor out = at::empty(x.sizes(), x.options());
+  const int64_t rows = x.size(-2), columns = x.size(-1), count = x.numel() ? x.numel() / (rows * columns) : 0;
+  const size_t need = sdk_orthogonalize_workspace_bytes(rows, columns, count, dtype);
+  Tensor ws = workspace(x, need);
+  TOKEN_CALL(sdk_orthogonalize, ptr(x), ptr(out), rows, columns, count, (int)steps, coefficients.data(), eps,
+             need ? ptr(ws) : nullptr, need, dtype, stream_of(x));
+  return out;
+}
+
+void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momenta, double lr, double momentum,
+               bool nesterov, double weight_decay, int64_t steps, at::ArrayRef<double> coefficients, double eps) {
+  if (params.empty()) {
+    TORCH_CHECK(grads.empty() && momenta.empty(), "gradients or momenta without params");
+    return;
+  }
+  on_gpu(params[0]);
+  const at::ScalarType type = params[0].scalar_type();
+  const int dtype = dtype_of(type, "params");
+  const auto p = pointers("params", params, params, type, false), g = pointers("grads", params, grads, type, false);
+  const auto m = pointers("momenta", params, momenta, at::kFloat, false);
+  TORCH_CHECK(coefficients.size() == 3, "coefficients must be three numbers, got ", coefficients.size());
+  TORCH_CHECK(steps >= 1 && steps <= 100, "steps = ", steps, " must be between 1 and 100");
+  std::vector<int64_t> rows(params.size()), columns(params.size());
+  for (size_t i = 0; i < params.size(); ++i) {
+    TORCH_CHECK(params[i].dim() >= 2, "params[", i, "] must have two axes at least, got ", params[i].sizes());
+    rows[i] = params[i].size(0), columns[i] = rows[i] ? params[i].numel() / rows[i] : 0;
+  }
+  c10::DeviceGuard guard(params[0].device());
+  const int64_t n = (int64_t)params.size();
+  const size_t need = sdk_muon_step_workspace_bytes(rows.data(), columns.data(), n, dtype);
+  Tensor ws = workspace(params[0], need);
+  TOKEN_CALL(sdk_muon_step, p.data(), g.data(), (float* const*)m.data(), rows.data(), columns.data(), n, lr, momentum,
+             (int)nesterov, weight_decay, (int)steps, coefficients.data(), eps, need ? ptr(ws) : nullptr, need, dtype,
+             stream_of(params[0]));
+  changed({params, momenta});
 }
 
 // ------------------------------------------------------------------------------------------ autograd
@@ -485,9 +708,95 @@ std::vector<Tensor> rms_norm_pair_autograd(const Tensor& x, const OptTensor& res
   return rms_norm_pair(x, residual, weight, eps);
 }
 
+struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
+  // x and weight first: gradients are counted over the tensors that are there
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                               const OptTensor& bias, double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const bool alone = !has(residual);
+    auto [out, summed, mean, inverse] = add_layer_norm(x, residual, weight, bias, eps);
+    ctx->saved_data["alone"] = alone;
+    ctx->saved_data["bias"] = has(bias);
+    ctx->save_for_backward({alone ? x : summed, weight, mean, inverse});
+    ctx->set_materialize_grads(false);
+    return alone ? variable_list{out} : variable_list{out, summed};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) { return only_first(gradients(ctx, grads)); }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool alone = ctx->saved_data["alone"].toBool(), biased = ctx->saved_data["bias"].toBool();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+               need_r = !alone && ctx->needs_input_grad(2), need_b = biased && ctx->needs_input_grad(alone ? 2 : 3);
+    const Tensor sum = grads.size() > 1 ? grads[1] : Tensor();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    if (!grads[0].defined())   // only the sum was used, or nothing
+      return {need_x ? sum : Tensor(), need_w ? at::zeros_like(saved[1]) : Tensor(), need_r ? sum : Tensor(),
+              need_b ? at::zeros_like(saved[1]) : Tensor(), Tensor()};
+    auto [dx, dw, db] = add_layer_norm_backward(
+        grads[0].contiguous(), sum.defined() ? OptTensor(sum.contiguous()) : OptTensor(), saved[0], saved[1], saved[2],
+        saved[3], need_x || need_r, need_w, need_b);
+    return {need_x ? dx : Tensor(), need_w ? dw : Tensor(), need_r ? dx : Tensor(), need_b ? db : Tensor(), Tensor()};
+  }
+};
+
+std::vector<Tensor> layer_norm_pair(const Tensor& x, const OptTensor& residual, const Tensor& weight,
+                                    const OptTensor& bias, double eps) {
+  auto [out, summed, mean, inverse] = layer_norm(x, residual, weight, bias, eps, false);
+  return has(residual) ? std::vector<Tensor>{out, summed} : std::vector<Tensor>{out};
+}
+
+std::vector<Tensor> layer_norm_pair_autograd(const Tensor& x, const OptTensor& residual, const Tensor& weight,
+                                             const OptTensor& bias, double eps) {
+  const Tensor other = has(residual) ? *residual : Tensor(), more = has(bias) ? *bias : Tensor();
+  if (wants_gradient({&x, &weight, &other, &more})) return AddLayerNorm::apply(x, weight, residual, bias, eps);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return layer_norm_pair(x, residual, weight, bias, eps);
+}
+
+struct GatedScan : torch::autograd::Function<GatedScan> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const OptTensor& state,
+                               const OptTensor& lengths, bool reverse) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [out, last] = gated_scan_forward(x, gate, state, lengths, reverse);
+    ctx->saved_data["reverse"] = reverse;
+    ctx->saved_data["state"] = has(state);
+    ctx->save_for_backward({x, gate, has(state) ? *state : Tensor(), has(lengths) ? *lengths : Tensor(), out});
+    ctx->set_materialize_grads(false);
+    return {out, last};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) { return only_first(gradients(ctx, grads)); }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    auto optional = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    const bool need_x = ctx->needs_input_grad(0), need_gate = ctx->needs_input_grad(1),
+               need_state = ctx->saved_data["state"].toBool() && ctx->needs_input_grad(2);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [dx, dgate, dstate] = gated_scan_backward(
+        optional(grads[0]), optional(grads[1]), saved[0], saved[1], optional(saved[2]), optional(saved[3]), saved[4],
+        ctx->saved_data["reverse"].toBool(), need_x, need_gate, need_state);
+    return {need_x ? dx : Tensor(), need_gate ? dgate : Tensor(), need_state ? dstate : Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTensor& state, const OptTensor& lengths,
+                               bool reverse) {
+  auto [out, last] = gated_scan_forward(x, gate, state, lengths, reverse);
+  return {out, last};
+}
+
+std::vector<Tensor> gated_scan_autograd(const Tensor& x, const Tensor& gate, const OptTensor& state,
+                                        const OptTensor& lengths, bool reverse) {
+  const Tensor first = has(state) ? *state : Tensor();
+  if (wants_gradient({&x, &gate, &first})) return GatedScan::apply(x, gate, state, lengths, reverse);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return gated_scan(x, gate, state, lengths, reverse);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(sdk_mapped_ops, AutogradCUDA, m) {
+  m.impl("layer_norm_pair", &layer_norm_pair_autograd);
+  m.impl("gated_scan", &gated_scan_autograd);
   m.impl("bucket_attention", &bucket_attention_autograd);
   m.impl("rms_norm_pair", &rms_norm_pair_autograd);
 }
@@ -504,10 +813,20 @@ TORCH_LIBRARY_IMPL(sdk_mapped_ops, CUDA, m) {
   m.impl("adamw_step", &adamw_step);
   m.impl("adamw_step_8bit", &adamw_step_8bit);
   m.impl("adamw_moment_values", &adamw_moment_values);
+  m.impl("layer_norm_pair", &layer_norm_pair);
+  m.impl("add_layer_norm", &add_layer_norm);
+  m.impl("add_layer_norm_backward", &add_layer_norm_backward);
+  m.impl("gated_scan", &gated_scan);
+  m.impl("gated_scan_forward", &gated_scan_forward);
+  m.impl("gated_scan_backward", &gated_scan_backward);
+  m.impl("gated_scan_step", &gated_scan_step);
+  m.impl("orthogonalize", &orthogonalize);
+  m.impl("muon_step", &muon_step);
 }
 
 // Names of the operators above, for the Python side (which implements those that are missing here).
 extern "C" const char* sdk_torch_token_ops(void) {
   return "bucket_attention,rms_norm_pair,bucket_attention_forward,bucket_attention_backward,add_rms_norm,add_rms_norm_quantized,"
-         "add_rms_norm_backward,dequantize_rows,adamw_step,adamw_step_8bit,adamw_moment_values";
+         "add_rms_norm_backward,dequantize_rows,adamw_step,adamw_step_8bit,adamw_moment_values,layer_norm_pair,add_layer_norm,"
+         "add_layer_norm_backward,gated_scan,gated_scan_forward,gated_scan_backward,gated_scan_step,orthogonalize,muon_step";
 }

@@ -6,5 +6,6 @@ from .mapped_ops import (mapped_convolution, mapped_transposed_convolution,  # n
                          MappedAvgPoolFunction, MappedAvgUnpoolFunction, ResampleFunction,
                          UnresampleFunction, UVResampleFunction)
 from .token_ops import (bucket_attention, add_rms_norm, add_rms_norm_quantized, dequantize_rows,  # noqa: F401
-                        adamw_step, adamw_step_8bit, adamw_moment_values, BucketAttentionFunction,
-                        AddRMSNormFunction)
+                        adamw_step, adamw_step_8bit, adamw_moment_values, add_layer_norm, gated_scan,
+                        gated_scan_step, orthogonalize, muon_step, NEWTON_SCHULZ, BucketAttentionFunction,
+                        AddRMSNormFunction, AddLayerNormFunction, GatedScanFunction)

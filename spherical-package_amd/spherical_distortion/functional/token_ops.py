@@ -1,8 +1,8 @@
 """Functional entry points of the operators on token sequences.
 
 Spherical samples as tokens (the pixels of a coarse grid, the vertices of an icosphere, the patches of
-tangent images): attention whose learned bias goes by the bucket of a pair's relative position, the
-norm of a block with its residual, and the optimizer step.  The reference has none of them.
+tangent images): attention whose learned bias goes by the bucket of a pair's relative position, a gated
+recurrence along the tokens, the norms of a block with its residual, and the optimizers' steps.  The reference has none of them.
 float32, bfloat16 and float16; sums, softmax statistics and norms are float32.
 """
 import functools
@@ -146,6 +146,89 @@ def dequantize_rows(codes, scales, dtype=torch.float32):
     return _sdk_ops.dequantize_rows(codes, scales, dtype)
 
 
+class AddLayerNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        out, summed, mean, inverse = _sdk_ops.add_layer_norm(x, residual, weight, bias, eps)
+        ctx.save_for_backward(x if residual is None else summed, weight, mean, inverse)
+        ctx.alone = residual is None
+        ctx.set_materialize_grads(False)
+        return (out, x.view_as(x)) if ctx.alone else (out, summed)
+
+    @staticmethod
+    @_only_first
+    def backward(ctx, grad, grad_sum):
+        summed, weight, mean, inverse = ctx.saved_tensors
+        need_x, need_r, need_w, need_b, _ = ctx.needs_input_grad
+        if grad is None:   # only the sum was used
+            return (grad_sum if need_x else None, grad_sum if need_r else None,
+                    torch.zeros_like(weight) if need_w else None, torch.zeros_like(weight) if need_b else None, None)
+        dx, dw, db = _sdk_ops.add_layer_norm_backward(
+            grad.contiguous(), None if grad_sum is None else grad_sum.contiguous(), summed, weight, mean, inverse,
+            need_x or need_r, need_w, need_b)
+        return (dx if need_x else None, dx if need_r else None, dw if need_w else None, db if need_b else None, None)
+
+
+def add_layer_norm(input, residual, weight, bias=None, eps=1e-5):
+    """(weight * (h - mean(h)) / sqrt(var(h) + eps) + bias, h) with h = input + residual, over the last axis (var: mean
+    square of h - mean(h)); a residual of None adds nothing.  weight and bias (None: none): one value for each of the
+    last axis (up to 16384), both of the input's type or float32.  The sum is normalised before it is rounded to the
+    input's type.  Second derivatives and forward mode raise."""
+    if "layer_norm_pair" in _token_ops.NATIVE_OPS:
+        both = _sdk_ops.layer_norm_pair(input, residual, weight, bias, float(eps))
+        return (both[0], input) if residual is None else (both[0], both[1])
+    if _wants_gradient(input, residual, weight, bias):
+        return AddLayerNormFunction.apply(input, residual, weight, bias, float(eps))
+    out, summed = _sdk_ops.add_layer_norm(input, residual, weight, bias, float(eps))[:2]
+    return out, input if residual is None else summed
+
+
+class GatedScanFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, state, lengths, reverse):
+        out, last = _sdk_ops.gated_scan_forward(x, gate, state, lengths, reverse)
+        ctx.save_for_backward(x, gate, state, lengths, out)
+        ctx.reverse = reverse
+        ctx.set_materialize_grads(False)
+        return out, last
+
+    @staticmethod
+    @_only_first
+    def backward(ctx, grad_output, grad_last):
+        x, gate, state, lengths, out = ctx.saved_tensors
+        need_x, need_gate, need_state = ctx.needs_input_grad[:3]
+        dx, dgate, dstate = _sdk_ops.gated_scan_backward(grad_output, grad_last, x, gate, state, lengths, out, ctx.reverse,
+                                                         need_x, need_gate, need_state)
+        return dx if need_x else None, dgate if need_gate else None, dstate if need_state else None, None, None
+
+
+def gated_scan(input, gate, state=None, lengths=None, reverse=False):
+    """(h, last state) of h_t = f_t h_{t-1} + (1 - f_t) input_t, f = sigmoid(gate), each channel by itself.
+
+    input and gate [B, tokens, width] of one type (float32, bfloat16, float16), any strides whose last axis is dense
+    (others are copied); h like them, dense.  state: h in front of the first token, float32 [B, width] (None: zeros);
+    the last state, float32 too, is h behind the last token.  lengths (int32 [B]): tokens from lengths[b] on do not
+    count; input and gate are not read there, h and the gradients are zeros.  reverse: from the last token that counts
+    to the first.  The state is float32 throughout and h is rounded once; inputs or states that are not finite give NaN
+    from there on.  With gradients for input, gate and state; second derivatives and forward mode raise.
+
+    Long sequences of few channels are cut into segments that are worked on side by side."""
+    if "gated_scan" in _token_ops.NATIVE_OPS:
+        both = _sdk_ops.gated_scan(input, gate, state, lengths, bool(reverse))
+        return both[0], both[1]
+    if _wants_gradient(input, gate, state):
+        return GatedScanFunction.apply(input, gate, state, lengths, bool(reverse))
+    return _sdk_ops.gated_scan_forward(input, gate, state, lengths, bool(reverse))
+
+
+def gated_scan_step(input, gate, state):
+    """One token of each sequence: state (float32 [B, width]) = f state + (1 - f) input with f = sigmoid(gate), in place;
+    returns it in the input's type.  input and gate [B, width].  No gradients: raises where one would be wanted."""
+    if _wants_gradient(input, gate, state):
+        raise RuntimeError("gated_scan_step has no gradients: call it under torch.no_grad(), or gated_scan")
+    return _sdk_ops.gated_scan_step(input, gate, state)
+
+
 def _no_tensors(*lists):
     return not any(len(tensors) for tensors in lists)
 
@@ -181,3 +264,33 @@ def adamw_step_8bit(params, grads, avg_codes, avg_scales, sq_codes, sq_scales, *
 def adamw_moment_values(codes, scales, dtype=torch.float32):
     """The values that the codes of a first (int8) or second (uint8) moment stand for."""
     return _sdk_ops.adamw_moment_values(codes, scales, dtype)
+
+
+#: a, b, c of orthogonalize: steep at zero (3.4 times a step), so that five steps bring singular values from 0.002 of the
+#: norm on to between 0.68 and 1.14.
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(input, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """Matrices [.., rows, columns] with their singular values brought towards one by products alone: X = input / (its
+    Frobenius norm + eps), then `steps` times X = a X + (b S + c S S) X with S = X X^T of the smaller side.
+
+    float32 and float16 matrices are multiplied with 22 bits a value, bfloat16 with 11; sums are float32.  Singular
+    values have to stay below 3.8 on the way (entries beyond 15 overflow and give NaN), as with the coefficients given
+    here.  eps: 2 ** -100 to 1.  No gradients."""
+    with torch.no_grad():
+        return _sdk_ops.orthogonalize(input, steps, coefficients, eps)
+
+
+def muon_step(params, grads, momenta, *, lr=2e-2, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+              coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """One Muon step over lists of parameters, in place and in few launches (64 parameters at a time).
+
+    params and grads: float32, bfloat16 or float16, all of one type, two axes at least: [out, ..] counts as a matrix of
+    `out` rows (weights [out, in, taps] of mapped convolutions among them); momenta float32.  No two tensors may overlap.
+    m = momentum m + (1 - momentum) g;  u = momentum m + (1 - momentum) g with nesterov, else m;
+    p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / columns)) orthogonalize(u)."""
+    if _no_tensors(params, grads, momenta):
+        return
+    with torch.no_grad():
+        _sdk_ops.muon_step(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, coefficients, eps)

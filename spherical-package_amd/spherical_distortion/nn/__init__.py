@@ -2,4 +2,4 @@ from .modules import (MappedConvolution, MappedTransposedConvolution, MappedMaxP
                       MappedMaxUnpool,
                       MappedAvgPool, MappedAvgUnpool, Resample, Unresample, UVResample)
 from ..layer_utils import InterpolationType  # noqa: F401
-from .token_modules import BucketAttention, AddRMSNorm  # noqa: F401
+from .token_modules import BucketAttention, AddRMSNorm, AddLayerNorm, GatedScan  # noqa: F401

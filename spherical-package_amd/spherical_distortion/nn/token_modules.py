@@ -58,3 +58,64 @@ class AddRMSNorm(nn.Module):
     def quantized(self, x, residual=None, dtype=torch.int8):
         """(codes, scales, x + residual): the norm's rows in 8 bits, without gradients."""
         return F.add_rms_norm_quantized(x, residual, self.weight, self.eps, dtype)
+
+
+class AddLayerNorm(nn.Module):
+    """(layer norm of x + residual, x + residual); a residual of None adds nothing."""
+
+    def __init__(self, width, eps=1e-5, bias=True):
+        super().__init__()
+        if not 1 <= width <= 16384:
+            raise ValueError("width must be between 1 and 16384, got %s" % width)
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(width))
+        self.bias = nn.Parameter(torch.zeros(width)) if bias else None
+
+    def forward(self, x, residual=None):
+        return F.add_layer_norm(x, residual, self.weight, self.bias, self.eps)
+
+
+class GatedScan(nn.Module):
+    """Tokens [B, tokens, width] mixed along the sequence by a gated linear recurrence of `channels` (None: width)
+    channels, whose output is gated and projected back: linear in the number of tokens where attention is quadratic.
+    both_ways: the second half of the channels runs from the last token to the first, so that every token sees all.
+    The channels' gates begin with memories of two to about 400 tokens."""
+
+    def __init__(self, width, channels=None, both_ways=False):
+        super().__init__()
+        channels = width if channels is None else channels
+        if width < 1 or not 1 <= channels <= 1 << 20 or (both_ways and channels % 2):
+            raise ValueError("width %s and channels %s must be positive, channels at most 2^20 and even both ways"
+                             % (width, channels))
+        self.channels, self.both_ways = channels, both_ways
+        self.inputs = nn.Linear(width, 3 * channels)
+        self.out = nn.Linear(channels, width, bias=False)
+        with torch.no_grad():
+            ways = 2 if both_ways else 1
+            self.inputs.bias.zero_()
+            self.inputs.bias[channels:2 * channels] = torch.linspace(0, 6, channels // ways).repeat(ways)
+
+    def _out(self, h, z):
+        return self.out(h * nn.functional.silu(z))
+
+    def forward(self, x, state=None, lengths=None):
+        """(tokens like x, last state [B, channels] float32); the state goes in front of the next call's tokens.  Both
+        ways there is none: a state is refused, and None returned."""
+        x, gate, z = self.inputs(x).chunk(3, -1)
+        if not self.both_ways:
+            h, last = F.gated_scan(x, gate, state, lengths)
+            return self._out(h, z), last
+        if state is not None:
+            raise ValueError("a scan both ways begins with no state")
+        half = self.channels // 2
+        ahead, _ = F.gated_scan(x[..., :half], gate[..., :half], None, lengths)
+        back, _ = F.gated_scan(x[..., half:], gate[..., half:], None, lengths, reverse=True)
+        return self._out(torch.cat([ahead, back], -1), z), None
+
+    @torch.no_grad()
+    def step(self, x, state):
+        """One token [B, width] of each sequence; state (float32 [B, channels]) is updated in place."""
+        if self.both_ways:
+            raise ValueError("a scan both ways has no single tokens")
+        x, gate, z = self.inputs(x).chunk(3, -1)
+        return self._out(F.gated_scan_step(x, gate, state), z)

@@ -12,10 +12,10 @@ def _on_gpu(p):
     return p.is_cuda
 
 
-def _check(p):
-    """What the step refuses of a parameter with a gradient."""
+def check_parameter(optimizer, p):
+    """What a step refuses of a parameter with a gradient."""
     if p.grad.is_sparse:
-        raise RuntimeError("AdamW does not take sparse gradients")
+        raise RuntimeError("%s does not take sparse gradients" % optimizer)
     if not _on_gpu(p):
         raise RuntimeError("this backend runs on the GPU only: parameters must be CUDA/HIP tensors")
     if p.dtype not in _TYPES or p.grad.dtype != p.dtype:
@@ -67,7 +67,7 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             for p in group["params"]:
                 if p.grad is not None:
-                    _check(p)
+                    check_parameter("AdamW", p)
         for group in self.param_groups:
             settings = {k: group[k] for k in ("lr", "betas", "eps", "weight_decay")}
             calls = {}   # (type, device, step, bits) -> lists of tensors, states
