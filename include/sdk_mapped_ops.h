@@ -930,7 +930,7 @@ typedef struct sdk_gated_scan {
   int32_t reverse, dtype;
 } sdk_gated_scan;
 
-size_t sdk_gated_scan_workspace_bytes(const sdk_gated_scan* a);
+size_t sdk_gated_scan_workspace_bytes(const sdk_gated_scan* a, int32_t backward);
 int sdk_gated_scan_forward(const sdk_gated_scan* a, void* workspace, size_t workspace_bytes, sdk_stream_t stream);
 int sdk_gated_scan_backward(const sdk_gated_scan* a, void* workspace, size_t workspace_bytes, sdk_stream_t stream);
 /* One token of each sequence: state [batch, width] (states that do not overlap) is updated in place,

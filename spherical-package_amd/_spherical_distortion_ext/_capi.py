@@ -176,7 +176,7 @@ def load():
     lib.sdk_add_rms_norm_backward_workspace_bytes.restype = _sz
     lib.sdk_add_layer_norm_backward_workspace_bytes.argtypes = [_i64] * 2
     lib.sdk_add_layer_norm_backward_workspace_bytes.restype = _sz
-    lib.sdk_gated_scan_workspace_bytes.argtypes = [_scan]
+    lib.sdk_gated_scan_workspace_bytes.argtypes = [_scan, _i32]
     lib.sdk_gated_scan_workspace_bytes.restype = _sz
     lib.sdk_orthogonalize_workspace_bytes.argtypes = [_i64] * 3 + [_i32]
     lib.sdk_orthogonalize_workspace_bytes.restype = _sz

@@ -432,8 +432,8 @@ def _scan_args(x, gate, state, lengths, reverse):
     return a, (x, gate, state, lengths)
 
 
-def _run_scan(name, a, ref):
-    need = _capi.load().sdk_gated_scan_workspace_bytes(ctypes.byref(a))
+def _run_scan(name, a, backward, ref):
+    need = _capi.load().sdk_gated_scan_workspace_bytes(ctypes.byref(a), backward)
     ws = torch.empty(need, dtype=torch.uint8, device=ref.device) if need else None
     _capi.call(name, ctypes.byref(a), _ops._ptr(ws), need, _ops._stream(ref))
 
@@ -446,7 +446,7 @@ def gated_scan_forward(x, gate, state, lengths, reverse):
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         last = torch.empty((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
         a.output, a.last = out.data_ptr(), last.data_ptr()
-        _run_scan("sdk_gated_scan_forward", a, x)
+        _run_scan("sdk_gated_scan_forward", a, 0, x)
     return out, last
 
 
@@ -479,7 +479,7 @@ def gated_scan_backward(grad_output, grad_last, x, gate, state, lengths, output,
         for name, t, need in (("grad_x", dx, need_x), ("grad_gate", dgate, need_gate), ("grad_state", dstate, need_state)):
             if need:
                 setattr(a, name, t.data_ptr())
-        _run_scan("sdk_gated_scan_backward", a, x)
+        _run_scan("sdk_gated_scan_backward", a, 1, x)
     return dx, dgate, dstate
 
 

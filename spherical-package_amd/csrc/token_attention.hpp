@@ -457,13 +457,6 @@ __device__ __forceinline__ void clear(floatx16 (&x)[N]) {
     for (int v = 0; v < 16; ++v) x[d][v] = 0.f;
 }
 
-// Between a wave's writes to LDS and its other lanes' reads: LDS keeps a wave's order, so it is the compiler alone
-// that must not exchange them.
-__device__ __forceinline__ void wave_order() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // Waits for every load so far.  Before a loop: the compiler, which cannot tell a first step from a later one, would
 // otherwise wait in each step for what the loop uses of before it, and with it for the step's own requests.
 __device__ __forceinline__ void landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0) alone

@@ -1,7 +1,7 @@
 // Matrices made orthogonal by Newton-Schulz steps, alone and as the update of a Muon step over many parameters.
 //
 //   X_0 = U / (|U|_F + eps), smaller side first (k x l, k <= l)
-//   S = X X^T      P = b S + c S S^T      X' = a X + P X          (odd polynomial of the singular values, S = S^T)
+//   S = X X^T      P = a I + b S + c S S^T      X' = P X          (odd polynomial of the singular values, S = S^T)
 //   Muon: m = mu m + (1 - mu) g,  U = mu m + (1 - mu) g (nesterov) or m,
 //         p = p (1 - lr decay) - lr sqrt(max(1, rows / columns)) X_steps
 //
@@ -195,13 +195,103 @@ __device__ __forceinline__ void step_barrier() {
 
 constexpr int kGram = 0, kPolynomial = 1, kNext = 2, kLast = 3;
 
+// Waves of a workgroup, down and across, and 32 x 32 blocks of a wave.
+template <int TILE>
+struct Shape {
+  static constexpr int DOWN = 2, ACROSS = TILE == 256 ? 4 : 2, THREADS = 64 * DOWN * ACROSS;
+  static constexpr int Y = TILE / 32 / DOWN, X = TILE / 32 / ACROSS;
+  static constexpr int LOADS = 2 * TILE * 128 / 16 / THREADS;   // 16-byte requests of a thread and step
+};
+
+// A wave's 32 x 32 block on its way to memory: in LDS as rows of 128 bytes whose 16-byte chunks are exchanged by the row's
+// number, so that neither the lanes' columns nor the rows meet in one bank.
+__device__ __forceinline__ int chunk_at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) * 16); }
+
+// From the lanes (column lane % 32, rows 8 q + 4 (lane / 32) + e of value 4 q + e) to the lines of `rows` and `columns`
+// (NULL: not written), rows of the matrix in rows of operands and in columns of them.
+template <bool SPLIT>
+__device__ __forceinline__ void write_block(const floatx16& v, char* scratch, int lane, char* rows, int64_t rows_bytes,
+                                            char* columns, int64_t columns_bytes) {
+  constexpr int PIECES = SPLIT ? 2 : 1;
+  const int half = lane / 32, c = lane % 32;
+  f16 piece[2][16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    piece[0][e] = (f16)v[e];
+    piece[1][e] = (f16)(v[e] - (float)piece[0][e]);
+  }
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *(f16*)(scratch + chunk_at(8 * q + 4 * half + e, p * 4 + c / 8) + c % 8 * 2) = piece[p][4 * q + e];
+      if (columns) {
+        Pack<f16, 4> four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four.v[e] = piece[p][4 * q + e];
+        *reinterpret_cast<Pack<f16, 4>*>(scratch + 4096 + chunk_at(c, p * 4 + q) + half * 8) = four;
+      }
+    }
+  wave_order();
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  constexpr int CHUNKS = 4 * PIECES, ROWS = 64 / CHUNKS;   // chunks of a row; rows of a store
+#pragma unroll
+  for (int r = 0; r < 32; r += ROWS) {
+    const int row = r + lane / CHUNKS, chunk = lane % CHUNKS;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(scratch + chunk_at(row, chunk));
+    *reinterpret_cast<u32x4*>(rows + row * rows_bytes + chunk * 16) = x;
+    if (columns) {
+      const u32x4 y = *reinterpret_cast<const u32x4*>(scratch + 4096 + chunk_at(row, chunk));
+      *reinterpret_cast<u32x4*>(columns + row * columns_bytes + chunk * 16) = y;
+    }
+  }
+  wave_order();
+}
+
+// A block of the last product into the matrix: element (row, column) at p[row * stride + column]; `turned`: the block's
+// columns are the matrix's rows.
+template <typename T>
+__device__ __forceinline__ void write_result(const floatx16& v, char* scratch, int lane, T* p, int64_t stride, bool turned,
+                                             int64_t row0, int64_t column0, int64_t rows, int64_t columns, bool step,
+                                             float keep, float rate) {
+  const int half = lane / 32, c = lane % 32;
+  float x[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = v[e];
+  if (turned) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 four = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+      *reinterpret_cast<float4*>(scratch + chunk_at(c, 2 * q + half)) = four;
+    }
+    wave_order();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = *(const float*)(scratch + chunk_at(2 * e + half, c / 4) + c % 4 * 4);
+    wave_order();
+  }
+  T old[16];
+  bool there[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int row = turned ? 2 * e + half : 8 * (e / 4) + 4 * half + e % 4;
+    there[e] = row0 + row < rows && column0 + c < columns;
+    if (step && there[e]) old[e] = p[(row0 + row) * stride + column0 + c];
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int row = turned ? 2 * e + half : 8 * (e / 4) + 4 * half + e % 4;
+    if (there[e]) p[(row0 + row) * stride + column0 + c] = (T)(step ? (float)old[e] * keep - rate * x[e] : x[e]);
+  }
+}
+
 // One product of TILE x TILE values a workgroup, rows i of A with rows j of B, of which step k has 128 bytes each in LDS,
 // brought there without registers on the way while the step before is multiplied.  A row's eight 16-byte chunks are
 // exchanged by its number, so that the lanes of a read meet no bank twice.
 template <bool SPLIT, int TILE, int STAGE, typename T>
-__global__ __launch_bounds__(256) void product(const Table t, const Settings s, char* workspace, int turn) {
-  constexpr int SUB = TILE / 64;             // 32 x 32 blocks of a wave, each way
-  constexpr int LOADS = 2 * TILE / 32;       // 16-byte requests of a thread and step
+__global__ __launch_bounds__(Shape<TILE>::THREADS, TILE == 64 ? 4 : 2) void product(const Table t, const Settings s, char* workspace, int turn) {
+  using S = Shape<TILE>;
   __shared__ __attribute__((aligned(128))) char lds[2][2 * TILE * 128];
   const unsigned group = by_die(blockIdx.x, gridDim.x);
   const int i = matrix_of(t.start, group);
@@ -225,11 +315,11 @@ __global__ __launch_bounds__(256) void product(const Table t, const Settings s, 
   const int steps = (int)(row_bytes / 128);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const char* from[LOADS];
+  const char* from[S::LOADS];
 #pragma unroll
-  for (int r = 0; r < LOADS; ++r) {
-    const int row = r * 32 + wave * 8 + lane / 8;   // of A's rows, then B's
-    const bool second = r * 32 >= TILE;
+  for (int r = 0; r < S::LOADS; ++r) {
+    const int row = r * (S::THREADS / 8) + wave * 8 + lane / 8;   // of A's rows, then B's
+    const bool second = r >= S::LOADS / 2;
     int64_t global = second ? tj * TILE + row - TILE : ti * TILE + row;
     const int64_t most = (second ? b_rows : at.kp) - 1;
     global = global < most ? global : most;         // tiles that pass the end: their last rows again, not written
@@ -238,41 +328,39 @@ __global__ __launch_bounds__(256) void product(const Table t, const Settings s, 
   auto request = [&](int step) {
     char* to = lds[step & 1] + wave * 8 * 128;
 #pragma unroll
-    for (int r = 0; r < LOADS; ++r)
-      __builtin_amdgcn_global_load_lds((Global)(from[r] + (int64_t)step * 128), (Lds)(to + r * 32 * 128), 16, 0, 0);
+    for (int r = 0; r < S::LOADS; ++r)
+      __builtin_amdgcn_global_load_lds((Global)(from[r] + (int64_t)step * 128), (Lds)(to + r * S::THREADS * 16), 16, 0, 0);
   };
 
-  floatx16 acc[SUB][SUB];
+  floatx16 acc[S::Y][S::X];
 #pragma unroll
-  for (int y = 0; y < SUB; ++y)
+  for (int y = 0; y < S::Y; ++y)
 #pragma unroll
-    for (int x = 0; x < SUB; ++x)
+    for (int x = 0; x < S::X; ++x)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[y][x][v] = 0.f;
 
-  const int half = lane / 32, wy = wave / 2 * (TILE / 2), wx = wave % 2 * (TILE / 2);
+  const int half = lane / 32, wy = wave / S::ACROSS * S::Y * 32, wx = wave % S::ACROSS * S::X * 32;
   request(0);
   for (int step = 0; step < steps; ++step) {
     step_barrier();
     if (step + 1 < steps) request(step + 1);
     const char* buffer = lds[step & 1];
-    auto operand = [&](int row, int chunk) {
-      return *reinterpret_cast<const f16x8*>(buffer + row * 128 + ((chunk ^ (row & 7)) * 16));
-    };
+    auto operand = [&](int row, int chunk) { return *reinterpret_cast<const f16x8*>(buffer + chunk_at(row, chunk)); };
 #pragma unroll
     for (int kk = 0; kk < (SPLIT ? 2 : 4); ++kk) {
-      f16x8 a[SUB][2], b[SUB][2];
+      f16x8 a[S::Y][2], b[S::X][2];
 #pragma unroll
-      for (int y = 0; y < SUB; ++y)
+      for (int piece = 0; piece < (SPLIT ? 2 : 1); ++piece) {
 #pragma unroll
-        for (int piece = 0; piece < (SPLIT ? 2 : 1); ++piece) {
-          a[y][piece] = operand(wy + y * 32 + lane % 32, piece * 4 + kk * 2 + half);
-          b[y][piece] = operand(TILE + wx + y * 32 + lane % 32, piece * 4 + kk * 2 + half);
-        }
+        for (int x = 0; x < S::X; ++x) b[x][piece] = operand(TILE + wx + x * 32 + lane % 32, piece * 4 + kk * 2 + half);
 #pragma unroll
-      for (int y = 0; y < SUB; ++y)
+        for (int y = 0; y < S::Y; ++y) a[y][piece] = operand(wy + y * 32 + lane % 32, piece * 4 + kk * 2 + half);
+      }
 #pragma unroll
-        for (int x = 0; x < SUB; ++x) {
+      for (int y = 0; y < S::Y; ++y)
+#pragma unroll
+        for (int x = 0; x < S::X; ++x) {
           if constexpr (SPLIT) {
             acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[y][1], b[x][0], acc[y][x], 0, 0, 0);
             acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[y][0], b[x][1], acc[y][x], 0, 0, 0);
@@ -281,51 +369,41 @@ __global__ __launch_bounds__(256) void product(const Table t, const Settings s, 
         }
     }
   }
+  step_barrier();   // the buffers are free
 
-  // values v = 4 q .. 4 q + 3 of a lane: rows i0 + 8 q + 0 .. 3, column j
+  char* scratch = &lds[0][0] + wave * 8192;
   const bool mirrored = STAGE <= kPolynomial && ti == tj;
 #pragma unroll
-  for (int y = 0; y < SUB; ++y)
+  for (int y = 0; y < S::Y; ++y)
 #pragma unroll
-    for (int x = 0; x < SUB; ++x) {
-      const int64_t j = tj * TILE + wx + x * 32 + lane % 32, i0 = ti * TILE + wy + y * 32 + 4 * half;
-      if (j >= b_rows) continue;
+    for (int x = 0; x < S::X; ++x) {
+      const int64_t i0 = ti * TILE + wy + y * 32, j0 = tj * TILE + wx + x * 32;
+      if (i0 >= at.kp || j0 >= b_rows) continue;
+      floatx16 v;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t row = i0 + 8 * q;
-        if (row >= at.kp) continue;
-        float v[4];
+      for (int e = 0; e < 16; ++e) v[e] = acc[y][x][e] * (STAGE == kLast ? kDown * kDown : kDown);
+      if constexpr (STAGE == kPolynomial) {   // a I + b S + c S S; S is its own transpose
+        const int64_t j = j0 + lane % 32;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[y][x][4 * q + e] * kDown;
-        if constexpr (STAGE != kGram) {
+        for (int q = 0; q < 4; ++q) {
+          const int64_t row = i0 + 8 * q + 4 * half;
           float old[4];
-          read_values<SPLIT, 4>(STAGE == kPolynomial ? place + at.s + j * at.k_row : place + at.xt[turn] + j * at.k_row, row,
-                                old);
+          read_values<SPLIT, 4>(place + at.s + j * at.k_row, row, old);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[e] = STAGE == kPolynomial ? fmaf(s.c, v[e], s.b * old[e]) : fmaf(s.a, old[e], v[e]);
+            v[4 * q + e] = fmaf(s.c, v[4 * q + e], s.b * old[e]) + (row + e == j ? s.a * kScale : 0.f);
         }
-        if constexpr (STAGE == kLast) {
-          const bool tall = t.rows[i] > t.columns[i];
-          T* p = (T*)t.p[i];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (row + e < at.k && j < at.l) {
-              const int64_t to = tall ? j * at.k + row + e : (row + e) * at.l + j;
-              const float update = v[e] * kDown;
-              p[to] = (T)(t.m[i] ? (float)p[to] * s.keep - t.rate[i] * update : update);
-            }
-        } else {
-          char* rows_to = place + (STAGE == kGram ? at.s : STAGE == kPolynomial ? at.p : at.x);
-          char* columns_to = STAGE == kNext ? place + at.xt[turn ^ 1] : rows_to;
-          const int64_t rows_bytes = STAGE == kNext ? at.l_row : at.k_row;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float one[1] = {v[e]};
-            write_values<SPLIT, 1>(rows_to + (row + e) * rows_bytes, j, one);
-          }
-          if (!mirrored) write_values<SPLIT, 4>(columns_to + j * at.k_row, row, v);
-        }
+      }
+      if constexpr (STAGE == kLast) {
+        const bool tall = t.rows[i] > t.columns[i];
+        write_result<T>(v, scratch, lane, (T*)t.p[i], tall ? at.k : at.l, tall, tall ? j0 : i0, tall ? i0 : j0,
+                        tall ? at.l : at.k, tall ? at.k : at.l, t.m[i] != nullptr, s.keep, t.rate[i]);
+      } else {
+        char* rows_to = place + (STAGE == kGram ? at.s : STAGE == kPolynomial ? at.p : at.x);
+        char* columns_to = STAGE == kNext ? place + at.xt[turn ^ 1] : rows_to;
+        const int64_t rows_bytes = STAGE == kNext ? at.l_row : at.k_row;
+        write_block<SPLIT>(v, scratch, lane, place_of<SPLIT>(rows_to + i0 * rows_bytes, j0), rows_bytes,
+                           mirrored ? nullptr : place_of<SPLIT>(columns_to + j0 * at.k_row, i0), at.k_row);
       }
     }
 }
@@ -355,20 +433,21 @@ int64_t deal(Table& t, int used, Of of) {
 
 int64_t triangle(int64_t n) { return n * (n + 1) / 2; }
 
-template <typename T, bool SPLIT, int TILE>
-void iterate(Table& t, int used, const Settings& s, int steps, char* workspace, hipStream_t stream) {
-  Table square = t;
-  const int64_t squares_of = deal(square, used, [](const Layout& at) { return triangle(ceil_div(at.kp, TILE)); });
-  const int64_t all = deal(t, used, [](const Layout& at) { return ceil_div(at.kp, TILE) * ceil_div(at.lp, TILE); });
-  for (int step = 0; step < steps; ++step) {
-    const int turn = step & 1;
-    launch(product<SPLIT, TILE, kGram, f16>, dim3((unsigned)squares_of), dim3(256), stream, square, s, workspace, turn);
-    launch(product<SPLIT, TILE, kPolynomial, f16>, dim3((unsigned)squares_of), dim3(256), stream, square, s, workspace, turn);
-    if (step + 1 < steps)
-      launch(product<SPLIT, TILE, kNext, f16>, dim3((unsigned)all), dim3(256), stream, t, s, workspace, turn);
-    else
-      launch(product<SPLIT, TILE, kLast, T>, dim3((unsigned)all), dim3(256), stream, t, s, workspace, turn);
-  }
+template <bool SPLIT, int TILE, int STAGE, typename T>
+void multiply(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream) {
+  const int64_t groups = deal(t, used, [](const Layout& at) {
+    const int64_t down = ceil_div(at.kp, TILE);
+    return STAGE <= kPolynomial ? triangle(down) : down * ceil_div(at.lp, TILE);
+  });
+  launch(product<SPLIT, TILE, STAGE, T>, dim3((unsigned)groups), dim3(Shape<TILE>::THREADS), stream, t, s, workspace, turn);
+}
+
+template <bool SPLIT, int STAGE, typename T>
+void stage(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream, int tile) {
+  if (tile == 128)
+    multiply<SPLIT, 128, STAGE, T>(t, used, s, workspace, turn, stream);
+  else
+    multiply<SPLIT, 64, STAGE, T>(t, used, s, workspace, turn, stream);
 }
 
 template <typename T>
@@ -379,10 +458,16 @@ void run_group(Table& t, int used, const Settings& s, int steps, char* workspace
   groups = deal(t, used, [](const Layout& at) { return at.kp / 64 * (at.lp / 64); });
   launch(lay_out<T, SPLIT>, dim3((unsigned)groups), dim3(256), stream, t, s, workspace);
   // tiles of 128 where they fill the GPU
-  if (groups >= 1024)
-    iterate<T, SPLIT, 128>(t, used, s, steps, workspace, stream);
-  else
-    iterate<T, SPLIT, 64>(t, used, s, steps, workspace, stream);
+  const int tile = groups >= 1024 ? 128 : 64;
+  for (int step = 0; step < steps; ++step) {
+    const int turn = step & 1;
+    stage<SPLIT, kGram, f16>(t, used, s, workspace, turn, stream, tile);
+    stage<SPLIT, kPolynomial, f16>(t, used, s, workspace, turn, stream, tile);
+    if (step + 1 < steps)
+      stage<SPLIT, kNext, f16>(t, used, s, workspace, turn, stream, tile);
+    else
+      stage<SPLIT, kLast, T>(t, used, s, workspace, turn, stream, tile);
+  }
 }
 
 // Deals the matrices to groups that share the workspace one after another: 64 at most, and as many workgroups as a

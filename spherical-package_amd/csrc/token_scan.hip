@@ -6,15 +6,19 @@
 //
 // Each channel by itself.  A span of tokens acts on the state before it as h -> A h + H, and spans join: (A, H) then
 // (A', H') is (A A', A' H + H').  So a workgroup takes 64 channels in 16 bits (32 in float32: 128 bytes of a token either
-// way) and a tile of 128 tokens, of which each thread walks four in order; the threads' (A, H) are joined over the tile,
-// and each walks its four again from the state in front of them.  The tile's values stay in registers meanwhile.
-// Sequences with too few channels for the GPU are cut into segments: a first launch forms the (A, H) of each, the
-// second begins each segment with the state that the ones before it leave.
+// way; a quarter of that where the width is no larger) and a tile of tokens, of which each thread walks two or four in
+// order; the threads' spans are joined over the tile, and each walks its tokens again from the state in front of them.  The
+// tile's values stay in registers meanwhile.  Where batch and channels fill the GPU a workgroup goes through a whole
+// sequence; otherwise it takes one tile, and tiles hand each other their spans while the kernel runs (scan_tiles).
 //
 // Bound by memory: three values read or written a token and channel forward, six backward (the gradients read h as
-// it was rounded to the tensors' type); segments read two of them twice.  The state, its gradient, (A, H) and the gates
-// are float32.  u is formed as sigmoid(-gate) and weighs the distance x - h: 1 - f of a rounded f near one would be
-// off by a part of all that a long memory sums up.
+// it was rounded to the tensors' type).  2 x 8192 tokens of 1024 channels in bfloat16: forward 30 us (3.4 TB/s), backward 54
+// (3.7 TB/s); all tiles of the forward are on the GPU at once, so that reading, waiting and writing follow each other.  A
+// first launch for the spans of longer segments, which then were read again, took 49 and 74 us.  131072 tokens of 256
+// channels in float16 forward: 60 us (3.4 TB/s; 95 with two launches).
+//
+// The state, its gradient, the spans and the gates are float32.  u weighs the distance x - h: 1 - f of a rounded f near one
+// would be off by a part of all that a long memory sums up.
 #include <algorithm>
 
 #include "token_types.hpp"
@@ -23,8 +27,8 @@ namespace sdk {
 namespace token {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRows = 4;                       // tokens of a tile that a thread walks
+constexpr int kThreads = 256;                  // of a workgroup that walks a whole sequence
+constexpr int kWaiting = 512;                  // of one that takes a single tile of it
 
 struct Scan {
   const void *x, *gate;
@@ -36,7 +40,7 @@ struct Scan {
   const float* grad_last;      // may be NULL
   void *grad_x, *grad_gate;    // [batch][tokens][width] dense, may be NULL
   float* grad_state;           // may be NULL
-  float* sums;                 // [2][batch of the launch][segments][width]: A, H of the segments
+  unsigned long long* words;   // tickets and the tiles' spans
   int64_t x_strides[2], gate_strides[2], grad_strides[2];   // batch, token
   int64_t tokens, segment;     // segment: tokens of one, a multiple of the tile unless there is one alone
   int width, segments, blocks; // blocks: of channels
@@ -45,20 +49,25 @@ struct Scan {
   int reverse;
 };
 
-// f = sigmoid(g), u = 1 - f, both to a few units of their last place: e = exp(-|g|) by the power of two, whose argument
-// is carried in two parts.
+// u = 1 - sigmoid(g) = 1 / (1 + e^g) and f = sigmoid(g) = e^g u.  Both keep their relative precision wherever they are
+// small; e^g stops at 2^126, NaN passes.  FINE: to a few units of the last place (the power's argument in two parts, a
+// correction of the reciprocal); 16-bit gates, whose results round to 16 bits, do without (5e-7 of u at gates of 8).
+template <bool FINE>
 __device__ __forceinline__ void gates(float g, float& f, float& u) {
   constexpr float kLog2e = 1.44269502e+00f, kLog2eRest = 1.92596303e-08f, kLn2 = 6.93147182e-01f;
-  const float m = fminf(fabsf(g), 128.f), t = m * kLog2e;
-  const float rest = fmaf(m, kLog2eRest, fmaf(m, kLog2e, -t));
-  float e = __builtin_amdgcn_exp2f(-t);
-  e = fmaf(e * rest, -kLn2, e);
+  float t = g * kLog2e;
+  const bool large = t > 126.f;
+  t = large ? 126.f : t;
+  float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (FINE) {
+    // t below -150 gives zero, whatever its rest (an infinity's is no number)
+    const float rest = fmaf(g, kLog2eRest, fmaf(g, kLog2e, -t));
+    if (fabsf(t) < 126.f) e = fmaf(e * rest, kLn2, e);
+  }
   const float d = 1.f + e;
-  float r = __builtin_amdgcn_rcpf(d);
-  r = fmaf(fmaf(-d, r, 1.f), r, r);
-  f = g >= 0.f ? r : e * r;
-  u = g >= 0.f ? e * r : r;
-  if (g != g) f = u = g;
+  u = __builtin_amdgcn_rcpf(d);
+  if constexpr (FINE) u = large ? u : fmaf(fmaf(-d, u, 1.f), u, u);
+  f = e * u;
 }
 
 // h -> a h + b, for each of V channels
@@ -73,11 +82,11 @@ __device__ __forceinline__ void unit(Span<V>& s) {
   for (int e = 0; e < V; ++e) s.a[e] = 1.f, s.b[e] = 0.f;
 }
 
-// Joins the spans of the workgroup's threads in the order of their time lanes (thread = time lane * LANES + channel lane):
-// on return `in` is the state in front of this thread's span, and `carry`, the state in front of all of them, the one
-// behind.  slots: [2][4 waves][LANES * V] floats, free to be written (the caller takes two in turn).
-template <int V, int LANES>
-__device__ __forceinline__ void over_tile(Span<V> s, float (&carry)[V], float (&in)[V], float* slots) {
+// Joins the spans of the workgroup's threads in the order of their time lanes (thread = time lane * LANES + channel lane)
+// up to the wave: on return `s` is the span of the threads before this one in its wave, and the waves' whole spans are in
+// slots, [2][waves][LANES * V] floats that are free to be written.
+template <int V, int LANES, int WAVES>
+__device__ __forceinline__ void over_waves(Span<V>& s, float* slots) {
   constexpr int C = LANES * V;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (threadIdx.x % LANES) * V;
 #pragma unroll
@@ -91,23 +100,29 @@ __device__ __forceinline__ void over_tile(Span<V> s, float (&carry)[V], float (&
   }
   if (lane >= 64 - LANES) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) slots[wave * C + c + e] = s.a[e], slots[(4 + wave) * C + c + e] = s.b[e];
+    for (int e = 0; e < V; ++e) slots[wave * C + c + e] = s.a[e], slots[(WAVES + wave) * C + c + e] = s.b[e];
   }
-  // the span of the threads before this one in the wave
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const float a = __shfl_up(s.a[e], LANES), b = __shfl_up(s.b[e], LANES);
     s.a[e] = lane >= LANES ? a : 1.f;
     s.b[e] = lane >= LANES ? b : 0.f;
   }
-  __syncthreads();
+}
+
+// After a barrier: `in` is the state in front of this thread's span, and `carry`, the state in front of all of them, the
+// one behind.
+template <int V, int LANES, int WAVES>
+__device__ __forceinline__ void from_waves(const Span<V>& s, float (&carry)[V], float (&in)[V], const float* slots) {
+  constexpr int C = LANES * V;
+  const int wave = threadIdx.x >> 6, c = (threadIdx.x % LANES) * V;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     float h = carry[e];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       if (w == wave) in[e] = fmaf(s.a[e], h, s.b[e]);
-      h = fmaf(slots[w * C + c + e], h, slots[(4 + w) * C + c + e]);
+      h = fmaf(slots[w * C + c + e], h, slots[(WAVES + w) * C + c + e]);
     }
     carry[e] = h;
   }
@@ -117,51 +132,26 @@ __device__ __forceinline__ void over_tile(Span<V> s, float (&carry)[V], float (&
 template <typename T, int LANES>
 struct Place {
   int64_t b, from, to, first_token, after_last;   // batch element, tokens of the segment, those that count (by `at`)
+  int64_t lane_state;                             // of the thread's first channel in [batch][width]
   int segment, channel, left, time;
-  __device__ __forceinline__ Place(const Scan& p) {
-    unsigned id = blockIdx.x;
+  __device__ __forceinline__ Place(const Scan& p, unsigned id, int segment_) {
     const int block = (int)(id % (unsigned)p.blocks);
-    id /= (unsigned)p.blocks;
-    segment = (int)(id % (unsigned)p.segments);
-    b = id / (unsigned)p.segments;
+    segment = segment_;
+    b = p.first + id / (unsigned)p.blocks;
     from = segment * p.segment;
     to = from + p.segment < p.tokens ? from + p.segment : p.tokens;
     channel = (block * LANES + (int)(threadIdx.x % LANES)) * kWide<T>;
     left = p.width - channel;
+    lane_state = b * p.width + channel;
     time = threadIdx.x / LANES;
     int64_t n = p.tokens;
-    if (p.lengths) n = p.lengths[p.first + b], n = n < 0 ? 0 : n > p.tokens ? p.tokens : n;
+    if (p.lengths) n = p.lengths[b], n = n < 0 ? 0 : n > p.tokens ? p.tokens : n;
     first_token = p.reverse ? p.tokens - n : 0;
     after_last = p.reverse ? p.tokens : n;
   }
   __device__ __forceinline__ int64_t row(const Scan& p, int64_t at) const { return p.reverse ? p.tokens - 1 - at : at; }
   __device__ __forceinline__ bool counts(int64_t at) const { return left > 0 && at >= first_token && at < after_last; }
 };
-
-// The state in front of segment `at.segment` in the order that its sums go (backward: from the last segment down): the
-// segments' spans are dealt to the time lanes.
-template <typename T, int LANES, bool BACKWARD>
-__device__ __forceinline__ void state_before(const Scan& p, const Place<T, LANES>& at, float (&carry)[kWide<T>], float* slots) {
-  constexpr int V = kWide<T>, TIMES = kThreads / LANES;
-  const int before = BACKWARD ? p.segments - 1 - at.segment : at.segment;
-  if (before == 0) return;
-  const int each = (before + TIMES - 1) / TIMES;
-  Span<V> s;
-  unit(s);
-  const float* a = p.sums + ((int64_t)at.b * p.segments) * p.width + at.channel;
-  const float* b = a + (int64_t)p.batches * p.segments * p.width;
-  for (int i = at.time * each; i < (at.time + 1) * each && i < before; ++i) {
-    const int64_t to = (int64_t)(BACKWARD ? p.segments - 1 - i : i) * p.width;
-    float fa[V], fb[V];
-    load_part<float, V>(a + to, fa, at.left);
-    load_part<float, V>(b + to, fb, at.left);
-#pragma unroll
-    for (int e = 0; e < V; ++e) s.b[e] = fmaf(fa[e], s.b[e], fb[e]), s.a[e] *= fa[e];
-  }
-  float in[V];
-  over_tile<V, LANES>(s, carry, in, slots);
-  __syncthreads();
-}
 
 template <int V>
 __device__ __forceinline__ void load_state(const float* p, int64_t at, float (&f)[V], int left) {
@@ -170,202 +160,259 @@ __device__ __forceinline__ void load_state(const float* p, int64_t at, float (&f
   if (p && left > 0) load_part<float, V>(p + at, f, left);
 }
 
-// The span of each segment: a time lane walks its part of the segment, without waiting for others until the end.
-template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
-__global__ __launch_bounds__(kThreads) void scan_spans(const Scan p) {
-  constexpr int V = kWide<T>, TIMES = kThreads / LANES;
-  __shared__ float slots[8 * LANES * V];
-  const Place<T, LANES> place(p);
-  const void* source = BACKWARD ? p.grad : p.x;
-  const int64_t(&strides)[2] = BACKWARD ? p.grad_strides : p.x_strides;
-  const T* x = source ? (const T*)source + (p.first + place.b) * strides[0] + place.channel : nullptr;
-  const T* gate = (const T*)p.gate + (p.first + place.b) * p.gate_strides[0] + place.channel;
-  const int64_t each = p.segment / TIMES;   // a multiple of kRows
-  Span<V> s;
-  unit(s);
-  for (int64_t i = 0; i < each; i += kRows) {
-    const int64_t begin = place.time * each + i;
-    float fx[kRows][V], fg[kRows][V];
-    bool counts[kRows];
+// ROWS tokens of a thread in the order of the walk, as they lie in memory, and what the walk does with them.  Forward they
+// are at, at + 1, ..; backward at, at - 1, ..
+template <typename T, int LANES, bool ALIGNED, bool BACKWARD, int ROWS>
+struct Walk {
+  static constexpr int V = kWide<T>;
+  static constexpr bool FINE = sizeof(T) == 4;
+  static constexpr int STEP = BACKWARD ? -1 : 1;
+  float u[ROWS][V];                       // the gate until span()
+  Pack<T, V> x[ROWS], g[BACKWARD ? ROWS : 1], h[BACKWARD ? ROWS : 1];
+  bool inside[ROWS], counts[ROWS];
+
+  __device__ __forceinline__ void load(const Scan& p, const Place<T, LANES>& place, int64_t at) {
+    const T* px = (const T*)p.x + place.b * p.x_strides[0] + place.channel;
+    const T* pgate = (const T*)p.gate + place.b * p.gate_strides[0] + place.channel;
+    const T* pgrad = (const T*)p.grad + place.b * p.grad_strides[0] + place.channel;
+    const T* ph = (const T*)p.out + place.b * p.tokens * p.width + place.channel;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int64_t at = BACKWARD ? place.from + p.segment - 1 - begin - r : place.from + begin + r;
-      counts[r] = at < place.to && place.counts(at);
+    for (int r = 0; r < ROWS; ++r) {
+      const int64_t t = at + STEP * r;
+      inside[r] = t >= place.from && t < place.to && place.left > 0;
+      counts[r] = inside[r] && place.counts(t);
+      if constexpr (BACKWARD) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) fx[r][e] = 0.f;
+        for (int e = 0; e < V; ++e) g[r].v[e] = (T)0.f;
+      }
       if (counts[r]) {
-        const int64_t row = place.row(p, at);
-        if (x) get<T, V, ALIGNED>(x + row * strides[1], fx[r], place.left);
-        get<T, V, ALIGNED>(gate + row * p.gate_strides[1], fg[r], place.left);
+        const int64_t row = place.row(p, t);
+        get<T, V, ALIGNED>(pgate + row * p.gate_strides[1], u[r], place.left);
+        get_raw<T, V, ALIGNED>(px + row * p.x_strides[1], x[r], place.left);
+        if constexpr (BACKWARD) {
+          if (p.grad) get_raw<T, V, ALIGNED>(pgrad + row * p.grad_strides[1], g[r], place.left);
+          if (t > place.first_token) get_raw<T, V, ALIGNED>(ph + place.row(p, t - 1) * p.width, h[r], place.left);
+        }
       }
     }
+  }
+
+  // What the tokens do to the state in front of them.
+  __device__ __forceinline__ Span<V> span() {
+    Span<V> s;
+    unit(s);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int r = 0; r < ROWS; ++r)
       if (counts[r]) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          float f, u;
-          gates(fg[r][e], f, u);
+          float f;
+          gates<FINE>(u[r][e], f, u[r][e]);
           if constexpr (BACKWARD) {
-            const float c = fx[r][e] + s.b[e];
-            s.b[e] = fmaf(-u, c, c);
+            const float c = (float)g[r].v[e] + s.b[e];
+            s.b[e] = fmaf(-u[r][e], c, c);
           } else {
-            s.b[e] = fmaf(u, fx[r][e] - s.b[e], s.b[e]);
+            s.b[e] = fmaf(u[r][e], (float)x[r].v[e] - s.b[e], s.b[e]);
           }
-          s.a[e] = fmaf(-u, s.a[e], s.a[e]);
+          s.a[e] = fmaf(-u[r][e], s.a[e], s.a[e]);
         }
       }
+    return s;
   }
-  float product[V], carry[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) carry[e] = 0.f;
-  over_tile<V, LANES>(s, carry, product, slots);
-#pragma unroll
-  for (int e = 0; e < V; ++e) {   // the slots hold the waves' spans
-    product[e] = 1.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) product[e] *= slots[w * LANES * V + (threadIdx.x % LANES) * V + e];
-  }
-  if (place.left <= 0 || place.time != 0) return;
-  float* a = p.sums + ((int64_t)place.b * p.segments + place.segment) * p.width + place.channel;
-  store_part<float, V>(a, product, place.left);
-  store_part<float, V>(a + (int64_t)p.batches * p.segments * p.width, carry, place.left);
-}
 
-template <typename T, int LANES, bool ALIGNED>
-__global__ __launch_bounds__(kThreads) void scan_forward(const Scan p) {
-  constexpr int V = kWide<T>, TILE = kThreads / LANES * kRows;
-  __shared__ float slots[2][8 * LANES * V];
-  const Place<T, LANES> place(p);
-  const int64_t b = p.first + place.b, lane_state = b * p.width + place.channel;
-  const T* x = (const T*)p.x + b * p.x_strides[0] + place.channel;
-  const T* gate = (const T*)p.gate + b * p.gate_strides[0] + place.channel;
-  T* out = (T*)p.out + b * p.tokens * p.width + place.channel;
-  float carry[V];
-  load_state<V>(p.state, lane_state, carry, place.left);
-  state_before<T, LANES, false>(p, place, carry, slots[1]);
-  int turn = 0;
-  for (int64_t tile = place.from; tile < place.to; tile += TILE, turn ^= 1) {
-    const int64_t at = tile + place.time * kRows;
-    float fx[kRows][V], fg[kRows][V], in[V];
-    bool counts[kRows];
-    Span<V> s;
-    unit(s);
+  // The results of the tokens, given the state in front of them.
+  __device__ __forceinline__ void finish(const Scan& p, const Place<T, LANES>& place, int64_t at, float (&in)[V]) {
+    const int64_t begin = place.b * p.tokens * p.width + place.channel;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      counts[r] = at + r < place.to && place.counts(at + r);
-      if (counts[r]) {
-        const int64_t row = place.row(p, at + r);
-        get<T, V, ALIGNED>(x + row * p.x_strides[1], fx[r], place.left);
-        get<T, V, ALIGNED>(gate + row * p.gate_strides[1], fg[r], place.left);
-      }
-    }
+    for (int r = 0; r < ROWS; ++r) {
+      if (!inside[r]) continue;
+      const int64_t row = begin + place.row(p, at + STEP * r) * p.width;
+      float y[V], z[V], before[V];
+      if constexpr (BACKWARD) {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (counts[r]) {
+        for (int e = 0; e < V; ++e) before[e] = (float)h[r].v[e];
+        if (at + STEP * r == place.first_token) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float f, u;
-          gates(fg[r][e], f, u);
-          fg[r][e] = u;
-          s.b[e] = fmaf(u, fx[r][e] - s.b[e], s.b[e]);
-          s.a[e] = fmaf(-u, s.a[e], s.a[e]);
+          for (int e = 0; e < V; ++e) before[e] = p.state && e < place.left ? p.state[place.lane_state + e] : 0.f;
         }
       }
-    over_tile<V, LANES>(s, carry, in, slots[turn]);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      if (at + r >= place.to || place.left <= 0) continue;
-      float h[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        h[e] = 0.f;
-        if (counts[r]) h[e] = in[e] = fmaf(fg[r][e], fx[r][e] - in[e], in[e]);
-      }
-      put<T, V, ALIGNED>(out + place.row(p, at + r) * p.width, h, place.left);
-    }
-  }
-  if (place.left > 0 && place.time == 0 && place.segment == p.segments - 1)
-    store_part<float, V>(p.last + lane_state, carry, place.left);
-}
-
-// The same from the last token down.  Time lane 0 has the tile's last tokens.
-template <typename T, int LANES, bool ALIGNED>
-__global__ __launch_bounds__(kThreads) void scan_backward(const Scan p) {
-  constexpr int V = kWide<T>, TILE = kThreads / LANES * kRows;
-  __shared__ float slots[2][8 * LANES * V];
-  const Place<T, LANES> place(p);
-  const int64_t b = p.first + place.b, lane_state = b * p.width + place.channel;
-  const T* x = (const T*)p.x + b * p.x_strides[0] + place.channel;
-  const T* gate = (const T*)p.gate + b * p.gate_strides[0] + place.channel;
-  const T* grad = p.grad ? (const T*)p.grad + b * p.grad_strides[0] + place.channel : nullptr;
-  const T* h = (const T*)p.out + b * p.tokens * p.width + place.channel;
-  T* grad_x = p.grad_x ? (T*)p.grad_x + b * p.tokens * p.width + place.channel : nullptr;
-  T* grad_gate = p.grad_gate ? (T*)p.grad_gate + b * p.tokens * p.width + place.channel : nullptr;
-  float carry[V];
-  load_state<V>(p.grad_last, lane_state, carry, place.left);
-  state_before<T, LANES, true>(p, place, carry, slots[1]);
-  const int64_t tiles = (place.to - place.from + TILE - 1) / TILE;
-  int turn = 0;
-  for (int64_t tile = tiles - 1; tile >= 0; --tile, turn ^= 1) {
-    // row r of the thread is token at - r
-    const int64_t at = place.from + (tile + 1) * TILE - 1 - place.time * kRows;
-    float fg[kRows][V], gg[kRows][V], fx[kRows][V], fh[kRows][V], in[V];
-    bool counts[kRows];
-    Span<V> s;
-    unit(s);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      counts[r] = at - r < place.to && place.counts(at - r);
-#pragma unroll
-      for (int e = 0; e < V; ++e) gg[r][e] = 0.f;
-      if (counts[r]) {
-        const int64_t row = place.row(p, at - r);
-        get<T, V, ALIGNED>(gate + row * p.gate_strides[1], fg[r], place.left);
-        if (grad) get<T, V, ALIGNED>(grad + row * p.grad_strides[1], gg[r], place.left);
-        get<T, V, ALIGNED>(x + row * p.x_strides[1], fx[r], place.left);
-        if (at - r > place.first_token)
-          get<T, V, ALIGNED>(h + place.row(p, at - r - 1) * p.width, fh[r], place.left);
-        else
-          load_state<V>(p.state, lane_state, fh[r], place.left);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (counts[r]) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float f, u;
-          gates(fg[r][e], f, u);
-          const float c = gg[r][e] + s.b[e];
-          s.b[e] = fmaf(-u, c, c);
-          s.a[e] = fmaf(-u, s.a[e], s.a[e]);
-        }
-      }
-    over_tile<V, LANES>(s, carry, in, slots[turn]);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      if (at - r >= place.to || place.left <= 0) continue;
-      float dx[V], dg[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        dx[e] = dg[e] = 0.f;
+        y[e] = z[e] = 0.f;
         if (counts[r]) {
-          float f, u;
-          gates(fg[r][e], f, u);
-          const float c = gg[r][e] + in[e];
-          dx[e] = c * u;
-          dg[e] = c * (fh[r][e] - fx[r][e]) * (f * u);
-          in[e] = fmaf(-u, c, c);
+          if constexpr (BACKWARD) {
+            const float c = (float)g[r].v[e] + in[e];
+            in[e] = fmaf(-u[r][e], c, c);
+            y[e] = c * u[r][e];
+            z[e] = (c - y[e]) * u[r][e] * (before[e] - (float)x[r].v[e]);
+          } else {
+            y[e] = in[e] = fmaf(u[r][e], (float)x[r].v[e] - in[e], in[e]);
+          }
         }
       }
-      const int64_t row = place.row(p, at - r) * p.width;
-      if (grad_x) put<T, V, ALIGNED>(grad_x + row, dx, place.left);
-      if (grad_gate) put<T, V, ALIGNED>(grad_gate + row, dg, place.left);
+      if constexpr (BACKWARD) {
+        if (p.grad_x) put<T, V, ALIGNED>((T*)p.grad_x + row, y, place.left);
+        if (p.grad_gate) put<T, V, ALIGNED>((T*)p.grad_gate + row, z, place.left);
+      } else {
+        put<T, V, ALIGNED>((T*)p.out + row, y, place.left);
+      }
     }
   }
-  if (place.left > 0 && place.time == 0 && place.segment == 0 && p.grad_state)
-    store_part<float, V>(p.grad_state + lane_state, carry, place.left);
+};
+
+template <bool BACKWARD>
+__device__ __forceinline__ const float* first_state(const Scan& p) { return BACKWARD ? p.grad_last : p.state; }
+
+template <typename T, int LANES, bool BACKWARD>
+__device__ __forceinline__ void store_last(const Scan& p, const Place<T, LANES>& place, const float (&carry)[kWide<T>]) {
+  float* to = BACKWARD ? p.grad_state : p.last;
+  if (to && place.left > 0 && place.time == 0) store_part<float, kWide<T>>(to + place.lane_state, carry, place.left);
+}
+
+// Tokens of a tile that a thread walks: a backward holds four tensors' values of each, a forward two.
+template <bool BACKWARD>
+constexpr int kRows = BACKWARD ? 2 : 4;
+
+// Whole sequences, tile by tile: a workgroup a batch element and block of channels.
+template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void scan_whole(const Scan p) {
+  constexpr int V = kWide<T>, WAVES = kThreads / 64, ROWS = kRows<BACKWARD>, TILE = kThreads / LANES * ROWS;
+  __shared__ float slots[2][2 * WAVES * LANES * V];
+  const Place<T, LANES> place(p, blockIdx.x, 0);
+  float carry[V];
+  load_state<V>(first_state<BACKWARD>(p), place.lane_state, carry, place.left);
+  const int64_t tiles = (p.tokens + TILE - 1) / TILE;
+  for (int64_t i = 0; i < tiles; ++i) {
+    const int64_t at = BACKWARD ? (tiles - i) * TILE - 1 - place.time * ROWS : i * TILE + place.time * ROWS;
+    Walk<T, LANES, ALIGNED, BACKWARD, ROWS> walk;
+    walk.load(p, place, at);
+    Span<V> s = walk.span();
+    float in[V];
+    over_waves<V, LANES, WAVES>(s, slots[i & 1]);
+    __syncthreads();
+    from_waves<V, LANES, WAVES>(s, carry, in, slots[i & 1]);
+    walk.finish(p, place, at, in);
+  }
+  store_last<T, LANES, BACKWARD>(p, place, carry);
+}
+
+// What other workgroups read of a tile: for each channel words {A, 1} and {H, 1} of its span, and of the last tile of a
+// run the state behind it instead; zeros until they are written.  Value and tag arrive together, so nothing else has to be
+// ordered.
+typedef unsigned long long Word;
+__device__ __forceinline__ Word word_of(float v, unsigned tag) { return (Word)tag << 32 | __float_as_uint(v); }
+__device__ __forceinline__ void publish(Word* to, Word w) {
+  __hip_atomic_store(to, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ Word seen(const Word* from) {
+  return __hip_atomic_load(const_cast<Word*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+constexpr int kTicket = 16;       // words of a group's ticket: a line of its own
+constexpr int kPolls = 1 << 20;   // a second: a wait ends whatever happens, with NaN
+
+__global__ __launch_bounds__(256) void clear(Word* words, int64_t count) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) words[i] = 0;
+}
+
+// One tile of a sequence a workgroup, read once and held in registers while its span goes out and the state in front of it
+// comes in.  Tiles form runs, of 32 where a workgroup has 64 channels: the state in front of a tile is the one behind the
+// run before, carried over the spans of the tiles before it in its run, always in this order, so that results do not depend
+// on who comes first.  Workgroups take the tiles of a group by its ticket, so those before a tile in its sequence have begun when it
+// begins; each publishes its tile's span before it waits for others, and the last of a run waits for nothing that comes
+// after it: every wait ends.
+constexpr int kLook = 4;
+
+template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
+__global__ __launch_bounds__(kWaiting, 4) void scan_tiles(const Scan p) {
+  constexpr int ROWS = kRows<BACKWARD>, V = kWide<T>, WAVES = kWaiting / 64, C = LANES * V, SLOTS = kWaiting / C;
+  __shared__ float slots[2 * WAVES * C], looked[2][SLOTS][C], entry[WAVES][C];
+  __shared__ unsigned ticket;
+  const unsigned groups = (unsigned)p.batches * p.blocks, id = blockIdx.x % groups;
+  if (threadIdx.x == 0)
+    ticket = __hip_atomic_fetch_add((unsigned*)(p.words + (int64_t)id * kTicket), 1u, __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int turn = (int)ticket;   // of the tile in the order of the walk
+  const Place<T, LANES> place(p, id, BACKWARD ? p.segments - 1 - turn : turn);
+  const int64_t at = BACKWARD ? place.from + p.segment - 1 - place.time * ROWS : place.from + place.time * ROWS;
+  Walk<T, LANES, ALIGNED, BACKWARD, ROWS> walk;
+  walk.load(p, place, at);
+  Span<V> s = walk.span();
+  over_waves<V, LANES, WAVES>(s, slots);
+  __syncthreads();
+
+  // a channel a thread: words of tile `turn` are at [2][tiles][groups][C] behind the tickets
+  const int c = threadIdx.x % C, slot = threadIdx.x / C;
+  const int64_t step = (int64_t)groups * C;
+  Word* products = p.words + groups * kTicket + (int64_t)id * C + c;
+  Word* states = products + p.segments * step;
+  constexpr int RUN = SLOTS * kLook;
+  const bool closes = turn % RUN == RUN - 1;
+  if (slot == 0 && !closes) {
+    float a = 1.f, b = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      b = fmaf(slots[w * C + c], b, slots[(WAVES + w) * C + c]);
+      a *= slots[w * C + c];
+    }
+    publish(products + turn * step, word_of(a, 1));
+    publish(states + turn * step, word_of(b, 1));
+  }
+  // a channel a thread: four tiles of the run before this one, by slot
+  const int start = turn / RUN * RUN, begin = start + slot * kLook;
+  Word product[kLook], state[kLook];
+#pragma unroll
+  for (int i = 0; i < kLook; ++i) {
+    const int other = begin + i < turn ? begin + i : 0;
+    product[i] = seen(products + other * step);
+    state[i] = seen(states + other * step);
+  }
+  float la = 1.f, lb = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLook; ++i) {
+    if (begin + i >= turn) continue;
+    for (int polls = 0; !(state[i] >> 32 && product[i] >> 32) && polls < kPolls; ++polls) {
+      __builtin_amdgcn_s_sleep(1);
+      product[i] = seen(products + (begin + i) * step);
+      state[i] = seen(states + (begin + i) * step);
+    }
+    const bool there = state[i] >> 32 && product[i] >> 32;
+    const float oa = __uint_as_float((unsigned)product[i]);
+    lb = fmaf(oa, lb, there ? __uint_as_float((unsigned)state[i]) : __builtin_nanf(""));
+    la *= oa;
+  }
+  looked[0][slot][c] = la;
+  looked[1][slot][c] = lb;
+  __syncthreads();
+  if (slot == 0) {
+    const int channel = (int)(id % (unsigned)p.blocks) * C + c;
+    const int64_t lane_state = place.b * p.width + channel;
+    const float* first = first_state<BACKWARD>(p);
+    float h = first && channel < p.width ? first[lane_state] : 0.f;
+    if (start > 0) {
+      Word w = seen(states + (start - 1) * step);
+      for (int polls = 0; !(w >> 32) && polls < kPolls; ++polls) {
+        __builtin_amdgcn_s_sleep(1);
+        w = seen(states + (start - 1) * step);
+      }
+      h = w >> 32 ? __uint_as_float((unsigned)w) : __builtin_nanf("");
+    }
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) h = fmaf(looked[0][i][c], h, looked[1][i][c]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      entry[w][c] = h;
+      h = fmaf(slots[w * C + c], h, slots[(WAVES + w) * C + c]);
+    }
+    float* last = BACKWARD ? p.grad_state : p.last;
+    if (closes) publish(states + turn * step, word_of(h, 1));
+    if (turn + 1 == p.segments && last && channel < p.width) last[lane_state] = h;
+  }
+  __syncthreads();
+  float in[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) in[e] = fmaf(s.a[e], entry[threadIdx.x >> 6][threadIdx.x % LANES * V + e], s.b[e]);
+  walk.finish(p, place, at, in);
 }
 
 // No tokens: the state, or its gradient, passes through.
@@ -390,26 +437,32 @@ __global__ __launch_bounds__(256) void scan_step(const T* x, int64_t x_stride, c
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     float f, u;
-    gates(fg[e], f, u);
+    gates<sizeof(T) == 4>(fg[e], f, u);
     h[e] = fmaf(u, fx[e] - h[e], h[e]);
   }
   store_part<float, V>(state + b * state_stride + c, h, left);
   put<T, V, ALIGNED>(out + b * width + c, h, left);
 }
 
-// Workgroups that fill the GPU: four a CU.
-constexpr int64_t kFill = 1024;
-
 // Channel lanes of a workgroup: the fewest of 2 and 8 that take the width.
 int lanes_of(int64_t width, int wide) { return width <= 2 * wide ? 2 : 8; }
 
-// Tokens of a segment: all, or as many tiles as leave four workgroups a CU.
-int64_t segment_of(int64_t batch, int64_t tokens, int64_t width, int dtype) {
-  const int wide = dtype == SDK_F32 ? 4 : 8, lanes = lanes_of(width, wide), tile = kThreads / lanes * kRows;
-  const int64_t groups = batch * ceil_div(width, lanes * wide);
-  if (groups >= kFill || tokens <= tile) return tokens;
-  const int64_t segments = std::min(ceil_div(kFill, groups), ceil_div(tokens, tile));
-  return std::min(tokens, ceil_div(ceil_div(tokens, segments), tile) * tile);
+// Tokens of a workgroup: all where batch and channels alone make four workgroups a CU, or a sequence is hardly longer than
+// a tile; a tile otherwise.
+constexpr int64_t kFill = 1024;
+int64_t segment_of(int64_t batch, int64_t tokens, int64_t width, int dtype, bool backward) {
+  const int wide = dtype == SDK_F32 ? 4 : 8, lanes = lanes_of(width, wide);
+  const int64_t groups = batch * ceil_div(width, lanes * wide), tile = kWaiting / lanes * (backward ? kRows<true> : kRows<false>);
+  return groups >= kFill || tokens <= tile || groups * ceil_div(tokens, tile) > most_groups(kWaiting) ? tokens : tile;
+}
+
+// Bytes for the tiles' words: a ticket's line a group, and two words a tile and channel (of whole blocks).
+size_t words_of(const sdk_gated_scan* a, bool backward) {
+  const int64_t segment = segment_of(a->batch, a->tokens, a->width, a->dtype, backward);
+  if (segment == a->tokens) return 0;
+  const int wide = a->dtype == SDK_F32 ? 4 : 8, c = lanes_of(a->width, wide) * wide;
+  const int64_t groups = a->batch * ceil_div(a->width, c);
+  return (size_t)(8 * groups * (kTicket + 2 * ceil_div(a->tokens, segment) * c));
 }
 
 int check(const sdk_gated_scan* a) {
@@ -422,29 +475,37 @@ int check(const sdk_gated_scan* a) {
   return SDK_OK;
 }
 
-// The launch's arguments; batch elements go in launches of as many workgroups as one holds.
-template <typename Run>
-void in_launches(const sdk_gated_scan* a, Scan p, int lanes, int wide, Run run) {
-  p.blocks = (int)ceil_div(p.width, lanes * wide);
-  p.segments = (int)ceil_div(p.tokens, p.segment);
-  const int64_t each = most_groups(kThreads) / ((int64_t)p.blocks * p.segments);
-  for (p.first = 0; p.first < a->batch; p.first += each) {
-    p.batches = (int)std::min(each, a->batch - p.first);
-    run(p, dim3((unsigned)((int64_t)p.batches * p.blocks * p.segments)));
-  }
-}
-
-Scan on_device(const sdk_gated_scan* a, void* workspace) {
+Scan on_device(const sdk_gated_scan* a, void* workspace, int lanes, int wide, bool backward) {
   Scan p = {};
   p.x = a->x, p.gate = a->gate, p.state = a->state, p.lengths = a->lengths, p.out = a->output, p.last = a->last;
   p.grad = a->grad_output, p.grad_last = a->grad_last, p.grad_x = a->grad_x, p.grad_gate = a->grad_gate;
-  p.grad_state = a->grad_state, p.sums = (float*)workspace;
+  p.grad_state = a->grad_state, p.words = (unsigned long long*)workspace;
   for (int i = 0; i < 2; ++i)
     p.x_strides[i] = a->x_strides[i], p.gate_strides[i] = a->gate_strides[i],
     p.grad_strides[i] = a->grad_output_strides[i];
   p.tokens = a->tokens, p.width = (int)a->width, p.reverse = a->reverse != 0;
-  p.segment = segment_of(a->batch, a->tokens, a->width, a->dtype);
+  p.segment = segment_of(a->batch, a->tokens, a->width, a->dtype, backward);
+  p.blocks = (int)ceil_div(p.width, lanes * wide);
+  p.segments = (int)ceil_div(p.tokens, p.segment);
   return p;
+}
+
+template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
+void run(const sdk_gated_scan* a, void* workspace, hipStream_t s) {
+  Scan p = on_device(a, workspace, LANES, kWide<T>, BACKWARD);
+  if (p.segments > 1) {   // fewer than kFill workgroups for a segment
+    const int64_t words = (int64_t)(words_of(a, BACKWARD) / 8);
+    launch(clear, dim3((unsigned)std::min<int64_t>(ceil_div(words, 256), 1024)), dim3(256), s, p.words, words);
+    p.batches = (int)a->batch;
+    launch(scan_tiles<T, LANES, ALIGNED, BACKWARD>,
+           dim3((unsigned)((int64_t)p.batches * p.blocks * p.segments)), dim3(kWaiting), s, p);
+    return;
+  }
+  const int64_t each = most_groups(kThreads) / p.blocks;   // batch elements of a launch
+  for (p.first = 0; p.first < a->batch; p.first += each) {
+    p.batches = (int)std::min(each, a->batch - p.first);
+    launch(scan_whole<T, LANES, ALIGNED, BACKWARD>, dim3((unsigned)((int64_t)p.batches * p.blocks)), dim3(kThreads), s, p);
+  }
 }
 
 template <typename T>
@@ -466,10 +527,10 @@ bool fits(const void* p, const int64_t (&strides)[2]) {
     }                                                                         \
   } while (0)
 
-int check_workspace(const sdk_gated_scan* a, const void* workspace, size_t bytes) {
-  const size_t need = sdk_gated_scan_workspace_bytes(a);
-  if (need && (!workspace || bytes < need))
-    return fail(SDK_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", bytes, need);
+int check_workspace(const sdk_gated_scan* a, const void* workspace, size_t bytes, bool backward) {
+  const size_t need = words_of(a, backward);
+  if (need && (!workspace || bytes < need || (uintptr_t)workspace % 8))
+    return fail(SDK_ERR_WORKSPACE, "workspace of %zu bytes at a multiple of 8, %zu needed", bytes, need);
   return SDK_OK;
 }
 
@@ -482,11 +543,9 @@ using namespace sdk::token;
 
 extern "C" {
 
-size_t sdk_gated_scan_workspace_bytes(const sdk_gated_scan* a) {
+size_t sdk_gated_scan_workspace_bytes(const sdk_gated_scan* a, int32_t backward) {
   if (check(a) != SDK_OK || !a->batch || !a->tokens || !a->width) return 0;
-  const int64_t segment = segment_of(a->batch, a->tokens, a->width, a->dtype);
-  const int64_t segments = ceil_div(a->tokens, segment);
-  return segments == 1 ? 0 : (size_t)(2 * a->batch * segments * a->width * (int64_t)sizeof(float));
+  return words_of(a, backward != 0);
 }
 
 int sdk_gated_scan_forward(const sdk_gated_scan* a, void* workspace, size_t workspace_bytes, sdk_stream_t stream) {
@@ -499,16 +558,13 @@ int sdk_gated_scan_forward(const sdk_gated_scan* a, void* workspace, size_t work
     return SDK_OK;
   }
   SDK_REQUIRE(a->x && a->gate && a->output && a->last, "x, gate, output and last must not be NULL");
-  if (int rc = check_workspace(a, workspace, workspace_bytes)) return rc;
+  if (int rc = check_workspace(a, workspace, workspace_bytes, false)) return rc;
   hipStream_t s = (hipStream_t)stream;
   SDK_DISPATCH_TOKEN_DTYPE(a->dtype, {
     const int lanes = lanes_of(a->width, kWide<T>);
     const bool wide = a->width % kWide<T> == 0 && fits<T>(a->x, a->x_strides) && fits<T>(a->gate, a->gate_strides) &&
                       aligned16(a->output);
-    SCAN_SHAPE(in_launches(a, on_device(a, workspace), LANES, kWide<T>, [&](const Scan& p, dim3 grid) {
-      if (p.segments > 1) launch(scan_spans<T, LANES, ALIGNED, false>, grid, dim3(kThreads), s, p);
-      launch(scan_forward<T, LANES, ALIGNED>, grid, dim3(kThreads), s, p);
-    }));
+    SCAN_SHAPE(run<T, LANES, ALIGNED, false>(a, workspace, s));
   });
   SDK_LAUNCH_CHECK("gated_scan_forward");
   return SDK_OK;
@@ -525,17 +581,14 @@ int sdk_gated_scan_backward(const sdk_gated_scan* a, void* workspace, size_t wor
   }
   SDK_REQUIRE(a->x && a->gate && a->output, "x, gate and output must not be NULL");
   SDK_REQUIRE(a->grad_x || a->grad_gate || a->grad_state, "one gradient at least must not be NULL");
-  if (int rc = check_workspace(a, workspace, workspace_bytes)) return rc;
+  if (int rc = check_workspace(a, workspace, workspace_bytes, true)) return rc;
   hipStream_t s = (hipStream_t)stream;
   SDK_DISPATCH_TOKEN_DTYPE(a->dtype, {
     const int lanes = lanes_of(a->width, kWide<T>);
     const bool wide = a->width % kWide<T> == 0 && fits<T>(a->x, a->x_strides) && fits<T>(a->gate, a->gate_strides) &&
                       fits<T>(a->grad_output, a->grad_output_strides) && aligned16(a->output) && aligned16(a->grad_x) &&
                       aligned16(a->grad_gate);
-    SCAN_SHAPE(in_launches(a, on_device(a, workspace), LANES, kWide<T>, [&](const Scan& p, dim3 grid) {
-      if (p.segments > 1) launch(scan_spans<T, LANES, ALIGNED, true>, grid, dim3(kThreads), s, p);
-      launch(scan_backward<T, LANES, ALIGNED>, grid, dim3(kThreads), s, p);
-    }));
+    SCAN_SHAPE(run<T, LANES, ALIGNED, true>(a, workspace, s));
   });
   SDK_LAUNCH_CHECK("gated_scan_backward");
   return SDK_OK;

@@ -80,6 +80,19 @@ __device__ __forceinline__ void put(T* p, const float (&f)[V], int left) {
     store_part<T, V>(p, f, left);
 }
 
+// The same without conversion.
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void get_raw(const T* p, Pack<T, V>& x, int left) {
+  if constexpr (ALIGNED) {
+    x = *reinterpret_cast<const Pack<T, V>*>(p);
+  } else if (left >= V) {
+    __builtin_memcpy(&x, p, sizeof(x));
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) x.v[e] = e < left ? p[e] : (T)0.f;
+  }
+}
+
 // V values of a weight that is held in the rows' type or in float32.
 template <typename T, int V, bool ALIGNED>
 __device__ __forceinline__ void load_weight(const void* w, int is_float, int64_t at, float (&f)[V], int left) {
@@ -128,6 +141,13 @@ __device__ __forceinline__ float over_group(float x, float* slots) {
     for (int i = 1; i < THREADS / 64; ++i) x = Op::of(x, slots[first + i]);
   }
   return x;
+}
+
+// Between a wave's writes to LDS and its other lanes' reads: LDS keeps a wave's order, so it is the compiler alone
+// that must not exchange them.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // Workgroups follow each other round the eight dies; consecutive tiles of one head or matrix share its operands, so

@@ -398,7 +398,7 @@ std::tuple<Tensor, Tensor> gated_scan_forward(Tensor x, Tensor gate, OptTensor s
   Tensor out = at::empty(x.sizes(), x.options());
   Tensor last = at::empty({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
   a.output = ptr(out), a.last = (float*)ptr(last);
-  const size_t need = sdk_gated_scan_workspace_bytes(&a);
+  const size_t need = sdk_gated_scan_workspace_bytes(&a, 0);
   Tensor ws = workspace(x, need);
   TOKEN_CALL(sdk_gated_scan_forward, &a, need ? ptr(ws) : nullptr, need, stream_of(x));
   return {out, last};
@@ -436,7 +436,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_backward(OptTensor grad, OptTensor
   if (need_x) a.grad_x = ptr(dx);
   if (need_gate) a.grad_gate = ptr(dgate);
   if (need_state) a.grad_state = (float*)ptr(dstate);
-  const size_t need = sdk_gated_scan_workspace_bytes(&a);
+  const size_t need = sdk_gated_scan_workspace_bytes(&a, 1);
   Tensor ws = workspace(x, need);
   TOKEN_CALL(sdk_gated_scan_backward, &a, need ? ptr(ws) : nullptr, need, stream_of(x));
   return {dx, dgate, dstate};
