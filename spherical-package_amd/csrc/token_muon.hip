@@ -60,13 +60,13 @@ constexpr int kLine = SPLIT ? 32 : 64;
 
 // Where the buffers of a matrix lie; sides padded with zeros to multiples of kPad.
 struct Layout {
-  int64_t k, l, kp, lp, x, xt[2], s, p, sums, end;   // byte offsets from the matrix's place
+  int64_t k, l, kp, lp, x0, x1, s, p, sums, end;    // byte offsets from the matrix's place; X of even and odd steps
   int64_t k_row, l_row;                             // bytes of a row of k and of l values
   __host__ __device__ Layout(int64_t rows, int64_t columns, bool split) {
     k = rows < columns ? rows : columns, l = rows < columns ? columns : rows;
     kp = (k + kPad - 1) / kPad * kPad, lp = (l + kPad - 1) / kPad * kPad;
     k_row = kp * (split ? 4 : 2), l_row = lp * (split ? 4 : 2);
-    x = 0, xt[0] = x + kp * l_row, xt[1] = xt[0] + lp * k_row, s = xt[1] + lp * k_row, p = s + kp * k_row;
+    x0 = 0, x1 = x0 + kp * l_row, s = x1 + kp * l_row, p = s + kp * k_row;
     sums = p + kp * k_row;
     end = sums + ((rows * columns + kPerGroup - 1) / kPerGroup * 8 + 127) / 128 * 128;
   }
@@ -77,16 +77,22 @@ __device__ __forceinline__ char* place_of(char* row, int64_t at) {
   return row + at / kLine<SPLIT> * 128 + at % kLine<SPLIT> * 2;
 }
 
+// v = hi + lo.  The value is kept from the compiler's view: it would form hi of a product twice, for the store from the
+// rounded product and for lo by one fused rounding, and where the two differ lo misses a half of hi's last place (1e-5 of a
+// matrix instead of 2e-7).
+__device__ __forceinline__ void split_f16(float v, f16& hi, f16& lo) {
+  asm("" : "+v"(v));
+  hi = (f16)v;
+  lo = (f16)(v - (float)hi);
+}
+
 // N consecutive values (a power of two up to 8, at a multiple of N) into or out of a row.
 template <bool SPLIT, int N>
 __device__ __forceinline__ void write_values(char* row, int64_t at, const float (&v)[N]) {
   char* to = place_of<SPLIT>(row, at);
   Pack<f16, N> hi, lo;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    hi.v[e] = (f16)v[e];
-    lo.v[e] = (f16)(v[e] - (float)hi.v[e]);
-  }
+  for (int e = 0; e < N; ++e) split_f16(v[e], hi.v[e], lo.v[e]);
   *reinterpret_cast<Pack<f16, N>*>(to) = hi;
   if constexpr (SPLIT) *reinterpret_cast<Pack<f16, N>*>(to + 64) = lo;
 }
@@ -137,12 +143,13 @@ __global__ __launch_bounds__(256) void squares(const Table t, const Settings s, 
   }
 }
 
-// The normalised update as operands, 64 x 64 values of X and of its transpose a workgroup.
+// The normalised update as X, 64 x 64 values a workgroup.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void lay_out(const Table t, const Settings s, char* workspace) {
   __shared__ float tile[64][65];
   __shared__ double sums[4];
-  const int i = matrix_of(t.start, blockIdx.x), rows = t.rows[i], columns = t.columns[i];
+  const unsigned group = gridDim.x - 1 - blockIdx.x;   // last first: what squares() touched last is still in the caches
+  const int i = matrix_of(t.start, group), rows = t.rows[i], columns = t.columns[i];
   const Layout at(rows, columns, SPLIT);
   char* place = workspace + t.at[i];
   const T* g = (const T*)t.g[i];
@@ -154,80 +161,75 @@ __global__ __launch_bounds__(256) void lay_out(const Table t, const Settings s, 
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  const float up = kScale / ((float)sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + s.eps);
   // the tile as it lies in the matrix
   const bool tall = rows > columns;
-  const int64_t cp = tall ? at.kp : at.lp, id = blockIdx.x - t.start[i];
+  const int64_t cp = tall ? at.kp : at.lp, id = group - t.start[i];
   const int64_t r0 = id / (cp / 64) * 64, c0 = id % (cp / 64) * 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int r = wave; r < 64; r += 4) {
-    const bool there = r0 + r < rows && c0 + lane < columns;
-    tile[r][lane] = there ? update_of(g, m, (r0 + r) * columns + c0 + lane, s) * up : 0.f;
+#pragma unroll
+  for (int r = 0; r < 64; r += 4) {
+    const bool there = r0 + r + wave < rows && c0 + lane < columns;
+    tile[r + wave][lane] = there ? update_of(g, m, (r0 + r + wave) * columns + c0 + lane, s) : 0.f;
   }
   __syncthreads();
-  char* by_row = place + (tall ? at.xt[0] : at.x);
-  char* by_column = place + (tall ? at.x : at.xt[0]);
-  const int64_t row_bytes = tall ? at.k_row : at.l_row, column_bytes = tall ? at.l_row : at.k_row;
+  const float up = kScale / ((float)sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + s.eps);
+  const int64_t k0 = tall ? c0 : r0, l0 = tall ? r0 : c0;
   for (int c = threadIdx.x; c < 64 * 8; c += 256) {
     const int r = c / 8, from = c % 8 * 8;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[r][from + e];
-    write_values<SPLIT, 8>(by_row + (r0 + r) * row_bytes, c0 + from, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[from + e][r];
-    write_values<SPLIT, 8>(by_column + (c0 + r) * column_bytes, r0 + from, v);
+    for (int e = 0; e < 8; ++e) v[e] = (tall ? tile[from + e][r] : tile[r][from + e]) * up;
+    write_values<SPLIT, 8>(place + at.x0 + (k0 + r) * at.l_row, l0 + from, v);
   }
 }
 
 typedef const __attribute__((address_space(1))) void* Global;
 typedef __attribute__((address_space(3))) void* Lds;
 
-// Between the steps of a product: every wave's requests have landed and its reads are done.
+// Between the steps of a product: all but the wave's last LEFT requests have landed, its reads are done, and so have every
+// other wave's.
+template <int LEFT>
 __device__ __forceinline__ void step_barrier() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | 7 << 4 | (LEFT >> 4) << 14);   // vmcnt(LEFT) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
 constexpr int kGram = 0, kPolynomial = 1, kNext = 2, kLast = 3;
 
-// Waves of a workgroup, down and across, and 32 x 32 blocks of a wave.
-template <int TILE>
+// A workgroup's block of F rows of the first operand and G of the second, dealt to waves of at most 64 x 64.
+template <int F_, int G_, int ACROSS_ = 2>
 struct Shape {
-  static constexpr int DOWN = 2, ACROSS = TILE == 256 ? 4 : 2, THREADS = 64 * DOWN * ACROSS;
-  static constexpr int Y = TILE / 32 / DOWN, X = TILE / 32 / ACROSS;
-  static constexpr int LOADS = 2 * TILE * 128 / 16 / THREADS;   // 16-byte requests of a thread and step
+  static constexpr int F = F_, G = G_, DOWN = F == 64 ? 2 : F / 64, ACROSS = ACROSS_, WAVES = DOWN * ACROSS, THREADS = 64 * WAVES;
+  static constexpr int Y = F / 32 / DOWN, X = G / 32 / ACROSS;   // 32 x 32 blocks of a wave
+  static constexpr int STAGES = F == 64 ? 4 : 2;  // steps in LDS
+  static constexpr int F_LOADS = F * 8 / THREADS, LOADS = (F + G) * 8 / THREADS;   // 16-byte requests of a thread and step
+  static constexpr int STEP = (F + G) * 128;                     // bytes of a step
 };
 
 // A wave's 32 x 32 block on its way to memory: in LDS as rows of 128 bytes whose 16-byte chunks are exchanged by the row's
 // number, so that neither the lanes' columns nor the rows meet in one bank.
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) * 16); }
 
-// From the lanes (column lane % 32, rows 8 q + 4 (lane / 32) + e of value 4 q + e) to the lines of `rows` and `columns`
-// (NULL: not written), rows of the matrix in rows of operands and in columns of them.
-template <bool SPLIT>
+// From the lanes (column lane % 32, rows 8 q + 4 (lane / 32) + e of value 4 q + e) to lines of memory: its rows to `rows`, its
+// columns to `columns` (NULL: not written); without ROWS_TOO to `columns` alone.
+template <bool SPLIT, bool ROWS_TOO>
 __device__ __forceinline__ void write_block(const floatx16& v, char* scratch, int lane, char* rows, int64_t rows_bytes,
                                             char* columns, int64_t columns_bytes) {
   constexpr int PIECES = SPLIT ? 2 : 1;
   const int half = lane / 32, c = lane % 32;
   f16 piece[2][16];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    piece[0][e] = (f16)v[e];
-    piece[1][e] = (f16)(v[e] - (float)piece[0][e]);
-  }
+  for (int e = 0; e < 16; ++e) split_f16(v[e], piece[0][e], piece[1][e]);
 #pragma unroll
   for (int p = 0; p < PIECES; ++p)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *(f16*)(scratch + chunk_at(8 * q + 4 * half + e, p * 4 + c / 8) + c % 8 * 2) = piece[p][4 * q + e];
-      if (columns) {
+        if (ROWS_TOO) *(f16*)(scratch + chunk_at(8 * q + 4 * half + e, p * 4 + c / 8) + c % 8 * 2) = piece[p][4 * q + e];
+      if (!ROWS_TOO || columns) {
         Pack<f16, 4> four;
 #pragma unroll
         for (int e = 0; e < 4; ++e) four.v[e] = piece[p][4 * q + e];
@@ -240,9 +242,11 @@ __device__ __forceinline__ void write_block(const floatx16& v, char* scratch, in
 #pragma unroll
   for (int r = 0; r < 32; r += ROWS) {
     const int row = r + lane / CHUNKS, chunk = lane % CHUNKS;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(scratch + chunk_at(row, chunk));
-    *reinterpret_cast<u32x4*>(rows + row * rows_bytes + chunk * 16) = x;
-    if (columns) {
+    if (ROWS_TOO) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(scratch + chunk_at(row, chunk));
+      *reinterpret_cast<u32x4*>(rows + row * rows_bytes + chunk * 16) = x;
+    }
+    if (!ROWS_TOO || columns) {
       const u32x4 y = *reinterpret_cast<const u32x4*>(scratch + 4096 + chunk_at(row, chunk));
       *reinterpret_cast<u32x4*>(columns + row * columns_bytes + chunk * 16) = y;
     }
@@ -250,86 +254,142 @@ __device__ __forceinline__ void write_block(const floatx16& v, char* scratch, in
   wave_order();
 }
 
-// A block of the last product into the matrix: element (row, column) at p[row * stride + column]; `turned`: the block's
-// columns are the matrix's rows.
+// Where the last product goes: element (row, column) at p[row * columns + column], alone or as a parameter's step.
 template <typename T>
-__device__ __forceinline__ void write_result(const floatx16& v, char* scratch, int lane, T* p, int64_t stride, bool turned,
-                                             int64_t row0, int64_t column0, int64_t rows, int64_t columns, bool step,
-                                             float keep, float rate) {
-  const int half = lane / 32, c = lane % 32;
-  float x[16];
+struct Result {
+  T* p;
+  int64_t rows, columns;
+  bool turned;               // the block's columns are the matrix's rows
+  bool step, wide;           // wide: rows of whole 16-byte vectors
+  float keep, rate;
+
+  static constexpr int V = kWide<T>, PARTS = 32 / V, ROWS = 64 / PARTS, N = 32 / ROWS;   // vectors of a block's row, rows of
+                                                                                         // a wave's request, requests
+  typedef Pack<T, V> Old[N];
+
+  __device__ __forceinline__ bool there(int64_t row0, int64_t column0, int lane, int n, int64_t& at) const {
+    const int64_t row = row0 + n * ROWS + lane / PARTS, column = column0 + lane % PARTS * V;
+    at = row * columns + column;
+    return row < rows && column < columns;
+  }
+  // The parameters of a block, requested before the block is worked on.
+  __device__ __forceinline__ void load(Old& old, int lane, int64_t row0, int64_t column0) const {
+    if (!wide || !step) return;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] = v[e];
-  if (turned) {
+    for (int n = 0; n < N; ++n) {
+      int64_t at;
+      if (there(row0, column0, lane, n, at)) old[n] = *reinterpret_cast<const Pack<T, V>*>(p + at);
+    }
+  }
+  __device__ __forceinline__ T value(T old, float x) const { return (T)(step ? (float)old * keep - rate * x : x); }
+
+  // The block through LDS: memory's rows in rows there.
+  __device__ __forceinline__ void store(const floatx16& v, const Old& old, char* scratch, int lane, int64_t row0,
+                                        int64_t column0) const {
+    const int half = lane / 32, c = lane % 32;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float4 four = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-      *reinterpret_cast<float4*>(scratch + chunk_at(c, 2 * q + half)) = four;
+      if (turned) {
+        const float4 four = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        *reinterpret_cast<float4*>(scratch + chunk_at(c, 2 * q + half)) = four;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *(float*)(scratch + chunk_at(8 * q + 4 * half + e, c / 4) + c % 4 * 4) = v[4 * q + e];
+      }
     }
     wave_order();
+    if (wide) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = *(const float*)(scratch + chunk_at(2 * e + half, c / 4) + c % 4 * 4);
+      for (int n = 0; n < N; ++n) {
+        int64_t at;
+        const bool inside = there(row0, column0, lane, n, at);
+        const int row = n * ROWS + lane / PARTS, chunk = lane % PARTS * V / 4;
+        Pack<T, V> out;
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(scratch + chunk_at(row, chunk + e / 4));
+          out.v[e] = value(old[n].v[e], x.x), out.v[e + 1] = value(old[n].v[e + 1], x.y);
+          out.v[e + 2] = value(old[n].v[e + 2], x.z), out.v[e + 3] = value(old[n].v[e + 3], x.w);
+        }
+        if (inside) *reinterpret_cast<Pack<T, V>*>(p + at) = out;
+      }
+    } else {
+      T one[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t row = row0 + 2 * e + half;
+        if (step && row < rows && column0 + c < columns) one[e] = p[row * columns + column0 + c];
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t row = row0 + 2 * e + half;
+        const float x = *(const float*)(scratch + chunk_at(2 * e + half, c / 4) + c % 4 * 4);
+        if (row < rows && column0 + c < columns) p[row * columns + column0 + c] = value(one[e], x);
+      }
+    }
     wave_order();
   }
-  T old[16];
-  bool there[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int row = turned ? 2 * e + half : 8 * (e / 4) + 4 * half + e % 4;
-    there[e] = row0 + row < rows && column0 + c < columns;
-    if (step && there[e]) old[e] = p[(row0 + row) * stride + column0 + c];
-  }
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int row = turned ? 2 * e + half : 8 * (e / 4) + 4 * half + e % 4;
-    if (there[e]) p[(row0 + row) * stride + column0 + c] = (T)(step ? (float)old[e] * keep - rate * x[e] : x[e]);
-  }
-}
+};
 
-// One product of TILE x TILE values a workgroup, rows i of A with rows j of B, of which step k has 128 bytes each in LDS,
-// brought there without registers on the way while the step before is multiplied.  A row's eight 16-byte chunks are
-// exchanged by its number, so that the lanes of a read meet no bank twice.
-template <bool SPLIT, int TILE, int STAGE, typename T>
-__global__ __launch_bounds__(Shape<TILE>::THREADS, TILE == 64 ? 4 : 2) void product(const Table t, const Settings s, char* workspace, int turn) {
-  using S = Shape<TILE>;
-  __shared__ __attribute__((aligned(128))) char lds[2][2 * TILE * 128];
+// One product of F x G values a workgroup, of which a step has 128 bytes of each of the F + G rows in LDS, brought there
+// without registers on the way while the steps before are multiplied.
+//   S, P: rows i of X (of S) with rows j of it, tiles i <= j, written both ways.
+//   X':   columns j of X with rows i of P: the block's rows are X's columns, so that a lane has four of a row of X' beside
+//         each other.  X lies with its columns beside each other: those operands are transposed on the way out of LDS.
+// The 16-byte chunks of a row are exchanged by its number, so that the lanes of a read meet no bank twice: of rows of 128
+// bytes by row % 8, of the steps of X by 4 (row % 4) (rows of 128 bytes: by half of that).
+template <bool SPLIT, typename S, int STAGE, typename T>
+__global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Settings s, char* workspace, int turn) {
+  constexpr bool SQUARE = STAGE <= kPolynomial;
+  static_assert(!SQUARE || S::F == S::G, "tiles on the diagonal");
+  constexpr int CHUNKS = S::F * (SPLIT ? 4 : 2) / 16;       // of a row of X's step
+  constexpr int LINE = kLine<SPLIT>, KK = LINE / 16, PIECES = SPLIT ? 2 : 1;
+  __shared__ __attribute__((aligned(128))) char lds[S::STAGES * S::STEP];
   const unsigned group = by_die(blockIdx.x, gridDim.x);
   const int i = matrix_of(t.start, group);
   const Layout at(t.rows[i], t.columns[i], SPLIT);
   char* place = workspace + t.at[i];
   const int64_t id = group - t.start[i];
-  int64_t ti, tj;
-  if constexpr (STAGE <= kPolynomial) {      // tiles ti <= tj, counted column by column
+  int64_t ti, tj;                             // tile of the block's rows, of its columns
+  if constexpr (SQUARE) {                     // ti <= tj, counted column by column
     tj = (int64_t)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
     while (tj * (tj + 1) / 2 > id) --tj;
     while ((tj + 1) * (tj + 2) / 2 <= id) ++tj;
     ti = id - tj * (tj + 1) / 2;
   } else {
-    const int64_t down = (at.kp + TILE - 1) / TILE;
-    ti = id % down, tj = id / down;
+    const int64_t across = (at.kp + S::G - 1) / S::G;
+    tj = id % across, ti = id / across;
   }
-  const char* A = place + (STAGE == kGram ? at.x : STAGE == kPolynomial ? at.s : at.p);
-  const char* B = place + (STAGE == kGram ? at.x : STAGE == kPolynomial ? at.s : at.xt[turn]);
+  const char* X = place + (turn ? at.x1 : at.x0);
+  const char* rows_of = STAGE == kGram ? X : place + (STAGE == kPolynomial ? at.s : at.p);   // of 128 bytes a step
   const int64_t row_bytes = STAGE == kGram ? at.l_row : at.k_row;
-  const int64_t b_rows = STAGE <= kPolynomial ? at.kp : at.lp;
   const int steps = (int)(row_bytes / 128);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const char* from[S::LOADS];
 #pragma unroll
   for (int r = 0; r < S::LOADS; ++r) {
-    const int row = r * (S::THREADS / 8) + wave * 8 + lane / 8;   // of A's rows, then B's
-    const bool second = r >= S::LOADS / 2;
-    int64_t global = second ? tj * TILE + row - TILE : ti * TILE + row;
-    const int64_t most = (second ? b_rows : at.kp) - 1;
-    global = global < most ? global : most;         // tiles that pass the end: their last rows again, not written
-    from[r] = (second ? B : A) + global * row_bytes + ((lane % 8) ^ (lane / 8)) * 16;
+    const bool first = r < S::F_LOADS;
+    const int chunk = (first ? r : r - S::F_LOADS) * S::THREADS + (int)threadIdx.x;   // of its operand's part of the step
+    if (SQUARE || !first) {
+      const int row = chunk / 8;
+      int64_t global = first ? ti * S::F + row : tj * S::G + row;
+      global = global < at.kp ? global : at.kp - 1;   // tiles that pass the end: the last row again, not written
+      from[r] = rows_of + global * row_bytes + ((chunk % 8) ^ (row & 7)) * 16;
+    } else {
+      const int row = chunk / CHUNKS, turned = CHUNKS >= 16 ? row % 4 * 4 : row / 2 % 2 * 4;
+      int64_t byte = ti * (CHUNKS * 16) + ((chunk % CHUNKS) ^ turned) * 16;
+      byte = byte < at.l_row ? byte : at.l_row - 16;
+      from[r] = X + row * at.l_row + byte;
+    }
   }
+  const int64_t first_step = SQUARE ? 128 : LINE * at.l_row;
   auto request = [&](int step) {
-    char* to = lds[step & 1] + wave * 8 * 128;
+    char* to = lds + step % S::STAGES * S::STEP + wave * 1024;
 #pragma unroll
     for (int r = 0; r < S::LOADS; ++r)
-      __builtin_amdgcn_global_load_lds((Global)(from[r] + (int64_t)step * 128), (Lds)(to + r * S::THREADS * 16), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((Global)(from[r] + step * (r < S::F_LOADS ? first_step : 128)),
+                                       (Lds)(to + r * S::THREADS * 16), 16, 0, 0);
   };
 
   floatx16 acc[S::Y][S::X];
@@ -341,47 +401,105 @@ __global__ __launch_bounds__(Shape<TILE>::THREADS, TILE == 64 ? 4 : 2) void prod
       for (int v = 0; v < 16; ++v) acc[y][x][v] = 0.f;
 
   const int half = lane / 32, wy = wave / S::ACROSS * S::Y * 32, wx = wave % S::ACROSS * S::X * 32;
-  request(0);
+#pragma unroll
+  for (int step = 0; step < S::STAGES - 1; ++step)
+    if (step < steps) request(step);
   for (int step = 0; step < steps; ++step) {
-    step_barrier();
-    if (step + 1 < steps) request(step + 1);
-    const char* buffer = lds[step & 1];
+    if (step + S::STAGES - 1 <= steps)   // as many steps requested as there is room for
+      step_barrier<(S::STAGES - 2) * S::LOADS>();
+    else
+      step_barrier<0>();
+    const bool more = step + S::STAGES - 1 < steps;
+    const char* buffer = lds + step % S::STAGES * S::STEP;
     auto operand = [&](int row, int chunk) { return *reinterpret_cast<const f16x8*>(buffer + chunk_at(row, chunk)); };
+    // columns first .. first + 31 of 16 rows of X from row `row` on
+    auto turned_operand = [&](int first, int row, int piece) {
+      const int r = row + 8 * half + lane % 16 / 4;   // and r + 4, whose chunks lie alike
+      const int column = first + lane / 16 % 2 * 16;
+      const int chunk = column / LINE * 8 + piece * 4 + column % LINE / 8 + lane % 4 / 2;
+      const char* lo = buffer + r * (CHUNKS * 16) + ((chunk ^ (CHUNKS >= 16 ? r % 4 * 4 : r / 2 % 2 * 4)) * 16) + lane % 2 * 8;
+      return __builtin_bit_cast(f16x8, tr_frag(lo, lo + 4 * CHUNKS * 16).v);
+    };
+    f16x8 a[KK][S::Y][PIECES];
+    if constexpr (SQUARE) {
+      if (more) request(step + S::STAGES - 1);
+    } else {
+      // the compiler waits for every request in flight before a transposing read: these come first
 #pragma unroll
-    for (int kk = 0; kk < (SPLIT ? 2 : 4); ++kk) {
-      f16x8 a[S::Y][2], b[S::X][2];
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int piece = 0; piece < (SPLIT ? 2 : 1); ++piece) {
+        for (int y = 0; y < S::Y; ++y)
 #pragma unroll
-        for (int x = 0; x < S::X; ++x) b[x][piece] = operand(TILE + wx + x * 32 + lane % 32, piece * 4 + kk * 2 + half);
+          for (int piece = 0; piece < PIECES; ++piece) a[kk][y][piece] = turned_operand(wy + y * 32, kk * 16, piece);
+      asm volatile("" ::: "memory");
+      if (more) request(step + S::STAGES - 1);
+      asm volatile("" ::: "memory");
+    }
 #pragma unroll
-        for (int y = 0; y < S::Y; ++y) a[y][piece] = operand(wy + y * 32 + lane % 32, piece * 4 + kk * 2 + half);
+    for (int kk = 0; kk < KK; ++kk) {
+      f16x8 b[S::X][PIECES];
+#pragma unroll
+      for (int piece = 0; piece < PIECES; ++piece) {
+#pragma unroll
+        for (int x = 0; x < S::X; ++x) b[x][piece] = operand(S::F + wx + x * 32 + lane % 32, piece * 4 + kk * 2 + half);
+        if constexpr (SQUARE) {
+#pragma unroll
+          for (int y = 0; y < S::Y; ++y) a[kk][y][piece] = operand(wy + y * 32 + lane % 32, piece * 4 + kk * 2 + half);
+        }
       }
 #pragma unroll
       for (int y = 0; y < S::Y; ++y)
 #pragma unroll
         for (int x = 0; x < S::X; ++x) {
           if constexpr (SPLIT) {
-            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[y][1], b[x][0], acc[y][x], 0, 0, 0);
-            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[y][0], b[x][1], acc[y][x], 0, 0, 0);
+            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][1], b[x][0], acc[y][x], 0, 0, 0);
+            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][0], b[x][1], acc[y][x], 0, 0, 0);
           }
-          acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[y][0], b[x][0], acc[y][x], 0, 0, 0);
+          acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][0], b[x][0], acc[y][x], 0, 0, 0);
         }
     }
   }
-  step_barrier();   // the buffers are free
+  step_barrier<0>();   // the buffers are free
 
-  char* scratch = &lds[0][0] + wave * 8192;
-  const bool mirrored = STAGE <= kPolynomial && ti == tj;
+  char* scratch = lds + wave * 8192;
+  const int64_t i_end = SQUARE ? at.kp : at.lp;
+  auto scaled = [&](int y, int x) {
+    floatx16 v;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = acc[y][x][e] * (STAGE == kLast ? kDown * kDown : kDown);
+    return v;
+  };
+  if constexpr (STAGE == kLast) {
+    const bool tall = t.rows[i] > t.columns[i];
+    T* p = (T*)t.p[i];
+    const int64_t columns = tall ? at.k : at.l;
+    const Result<T> result = {p, tall ? at.l : at.k, columns, !tall, t.m[i] != nullptr,
+                              columns % kWide<T> == 0 && (uintptr_t)p % 16 == 0, s.keep, t.rate[i]};
+#pragma unroll
+    for (int y = 0; y < S::Y; ++y) {
+      typename Result<T>::Old old[S::X];
+      const int64_t i0 = ti * S::F + wy + y * 32;
+#pragma unroll
+      for (int x = 0; x < S::X; ++x) {
+        const int64_t j0 = tj * S::G + wx + x * 32;
+        result.load(old[x], lane, tall ? i0 : j0, tall ? j0 : i0);
+      }
+#pragma unroll
+      for (int x = 0; x < S::X; ++x) {
+        const int64_t j0 = tj * S::G + wx + x * 32;
+        if (i0 < i_end && j0 < at.kp)
+          result.store(scaled(y, x), old[x], scratch, lane, tall ? i0 : j0, tall ? j0 : i0);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int y = 0; y < S::Y; ++y)
 #pragma unroll
     for (int x = 0; x < S::X; ++x) {
-      const int64_t i0 = ti * TILE + wy + y * 32, j0 = tj * TILE + wx + x * 32;
-      if (i0 >= at.kp || j0 >= b_rows) continue;
-      floatx16 v;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = acc[y][x][e] * (STAGE == kLast ? kDown * kDown : kDown);
+      const int64_t i0 = ti * S::F + wy + y * 32, j0 = tj * S::G + wx + x * 32;
+      if (i0 >= i_end || j0 >= at.kp) continue;
+      floatx16 v = scaled(y, x);
       if constexpr (STAGE == kPolynomial) {   // a I + b S + c S S; S is its own transpose
         const int64_t j = j0 + lane % 32;
 #pragma unroll
@@ -394,16 +512,13 @@ __global__ __launch_bounds__(Shape<TILE>::THREADS, TILE == 64 ? 4 : 2) void prod
             v[4 * q + e] = fmaf(s.c, v[4 * q + e], s.b * old[e]) + (row + e == j ? s.a * kScale : 0.f);
         }
       }
-      if constexpr (STAGE == kLast) {
-        const bool tall = t.rows[i] > t.columns[i];
-        write_result<T>(v, scratch, lane, (T*)t.p[i], tall ? at.k : at.l, tall, tall ? j0 : i0, tall ? i0 : j0,
-                        tall ? at.l : at.k, tall ? at.k : at.l, t.m[i] != nullptr, s.keep, t.rate[i]);
+      if constexpr (SQUARE) {
+        char* to = place + (STAGE == kGram ? at.s : at.p);
+        write_block<SPLIT, true>(v, scratch, lane, place_of<SPLIT>(to + i0 * at.k_row, j0), at.k_row,
+                           ti == tj ? nullptr : place_of<SPLIT>(to + j0 * at.k_row, i0), at.k_row);
       } else {
-        char* rows_to = place + (STAGE == kGram ? at.s : STAGE == kPolynomial ? at.p : at.x);
-        char* columns_to = STAGE == kNext ? place + at.xt[turn ^ 1] : rows_to;
-        const int64_t rows_bytes = STAGE == kNext ? at.l_row : at.k_row;
-        write_block<SPLIT>(v, scratch, lane, place_of<SPLIT>(rows_to + i0 * rows_bytes, j0), rows_bytes,
-                           mirrored ? nullptr : place_of<SPLIT>(columns_to + j0 * at.k_row, i0), at.k_row);
+        write_block<SPLIT, false>(v, scratch, lane, nullptr, 0, place_of<SPLIT>(place + (turn ? at.x0 : at.x1) + j0 * at.l_row, i0),
+                           at.l_row);
       }
     }
 }
@@ -433,21 +548,30 @@ int64_t deal(Table& t, int used, Of of) {
 
 int64_t triangle(int64_t n) { return n * (n + 1) / 2; }
 
-template <bool SPLIT, int TILE, int STAGE, typename T>
-void multiply(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream) {
-  const int64_t groups = deal(t, used, [](const Layout& at) {
-    const int64_t down = ceil_div(at.kp, TILE);
-    return STAGE <= kPolynomial ? triangle(down) : down * ceil_div(at.lp, TILE);
+template <int STAGE, typename S>
+int64_t groups_of(Table& t, int used) {
+  return deal(t, used, [](const Layout& at) {
+    const int64_t across = ceil_div(at.kp, S::G);
+    return STAGE <= kPolynomial ? triangle(across) : across * ceil_div(at.lp, S::F);
   });
-  launch(product<SPLIT, TILE, STAGE, T>, dim3((unsigned)groups), dim3(Shape<TILE>::THREADS), stream, t, s, workspace, turn);
 }
 
+template <bool SPLIT, typename S, int STAGE, typename T>
+void multiply(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream) {
+  const int64_t groups = groups_of<STAGE, S>(t, used);
+  launch(product<SPLIT, S, STAGE, T>, dim3((unsigned)groups), dim3(S::THREADS), stream, t, s, workspace, turn);
+}
+
+// Tiles of 128 x 128 where they make a workgroup a CU, of 64 x 64 otherwise.  Eight waves a tile keep the matrix unit busier
+// than four (S of 32 matrices of up to 640 x 2560 in bfloat16 45 us for 48, X' 67 for 71), but leave too few registers for
+// the last stage's parameters (247 us for 190 in float32).
 template <bool SPLIT, int STAGE, typename T>
-void stage(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream, int tile) {
-  if (tile == 128)
-    multiply<SPLIT, 128, STAGE, T>(t, used, s, workspace, turn, stream);
+void stage(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream) {
+  using Large = Shape<128, 128, STAGE == kLast ? 2 : 4>;
+  if (groups_of<STAGE, Large>(t, used) >= 256)
+    multiply<SPLIT, Large, STAGE, T>(t, used, s, workspace, turn, stream);
   else
-    multiply<SPLIT, 64, STAGE, T>(t, used, s, workspace, turn, stream);
+    multiply<SPLIT, Shape<64, 64>, STAGE, T>(t, used, s, workspace, turn, stream);
 }
 
 template <typename T>
@@ -457,16 +581,14 @@ void run_group(Table& t, int used, const Settings& s, int steps, char* workspace
   launch(squares<T>, dim3((unsigned)groups), dim3(256), stream, t, s, workspace, (int)SPLIT);
   groups = deal(t, used, [](const Layout& at) { return at.kp / 64 * (at.lp / 64); });
   launch(lay_out<T, SPLIT>, dim3((unsigned)groups), dim3(256), stream, t, s, workspace);
-  // tiles of 128 where they fill the GPU
-  const int tile = groups >= 1024 ? 128 : 64;
   for (int step = 0; step < steps; ++step) {
     const int turn = step & 1;
-    stage<SPLIT, kGram, f16>(t, used, s, workspace, turn, stream, tile);
-    stage<SPLIT, kPolynomial, f16>(t, used, s, workspace, turn, stream, tile);
+    stage<SPLIT, kGram, f16>(t, used, s, workspace, turn, stream);
+    stage<SPLIT, kPolynomial, f16>(t, used, s, workspace, turn, stream);
     if (step + 1 < steps)
-      stage<SPLIT, kNext, f16>(t, used, s, workspace, turn, stream, tile);
+      stage<SPLIT, kNext, f16>(t, used, s, workspace, turn, stream);
     else
-      stage<SPLIT, kLast, T>(t, used, s, workspace, turn, stream, tile);
+      stage<SPLIT, kLast, T>(t, used, s, workspace, turn, stream);
   }
 }
 

@@ -134,16 +134,26 @@ struct Place {
   int64_t b, from, to, first_token, after_last;   // batch element, tokens of the segment, those that count (by `at`)
   int64_t lane_state;                             // of the thread's first channel in [batch][width]
   int segment, channel, left, time;
+  // the thread of a workgroup that takes segment `segment_` of a block of channels
   __device__ __forceinline__ Place(const Scan& p, unsigned id, int segment_) {
-    const int block = (int)(id % (unsigned)p.blocks);
     segment = segment_;
-    b = p.first + id / (unsigned)p.blocks;
+    channel = ((int)(id % (unsigned)p.blocks) * LANES + (int)(threadIdx.x % LANES)) * kWide<T>;
+    time = threadIdx.x / LANES;
+    begin(p, p.first + id / (unsigned)p.blocks);
+  }
+  // thread `id` of those that take a sequence's channels alone
+  __device__ __forceinline__ Place(const Scan& p, int64_t id) {
+    const int vectors = (p.width + kWide<T> - 1) / kWide<T>;
+    segment = time = 0;
+    channel = (int)(id % vectors) * kWide<T>;
+    begin(p, p.first + id / vectors);
+  }
+  __device__ __forceinline__ void begin(const Scan& p, int64_t element) {
+    b = element;
     from = segment * p.segment;
     to = from + p.segment < p.tokens ? from + p.segment : p.tokens;
-    channel = (block * LANES + (int)(threadIdx.x % LANES)) * kWide<T>;
     left = p.width - channel;
     lane_state = b * p.width + channel;
-    time = threadIdx.x / LANES;
     int64_t n = p.tokens;
     if (p.lengths) n = p.lengths[b], n = n < 0 ? 0 : n > p.tokens ? p.tokens : n;
     first_token = p.reverse ? p.tokens - n : 0;
@@ -167,7 +177,7 @@ struct Walk {
   static constexpr int V = kWide<T>;
   static constexpr bool FINE = sizeof(T) == 4;
   static constexpr int STEP = BACKWARD ? -1 : 1;
-  float u[ROWS][V];                       // the gate until span()
+  float u[ROWS][V];                       // the gate until open() or span()
   Pack<T, V> x[ROWS], g[BACKWARD ? ROWS : 1], h[BACKWARD ? ROWS : 1];
   bool inside[ROWS], counts[ROWS];
 
@@ -197,7 +207,18 @@ struct Walk {
     }
   }
 
-  // What the tokens do to the state in front of them.
+  // The gates of the tokens.
+  __device__ __forceinline__ void open() {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float f;
+        if (counts[r]) gates<FINE>(u[r][e], f, u[r][e]);
+      }
+  }
+
+  // The same, and what the tokens do to the state in front of them.
   __device__ __forceinline__ Span<V> span() {
     Span<V> s;
     unit(s);
@@ -294,6 +315,25 @@ __global__ __launch_bounds__(kThreads) void scan_whole(const Scan p) {
     walk.finish(p, place, at, in);
   }
   store_last<T, LANES, BACKWARD>(p, place, carry);
+}
+
+// Short sequences: a thread takes 16 bytes of channels through all tokens.
+template <typename T, bool ALIGNED, bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void scan_short(const Scan p) {
+  constexpr int V = kWide<T>, ROWS = kRows<BACKWARD>;
+  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (id >= (int64_t)p.batches * ((p.width + V - 1) / V)) return;
+  const Place<T, 1> place(p, id);
+  float carry[V];
+  load_state<V>(first_state<BACKWARD>(p), place.lane_state, carry, place.left);
+  for (int64_t i = 0; i < p.tokens; i += ROWS) {
+    const int64_t at = BACKWARD ? p.tokens - 1 - i : i;
+    Walk<T, 1, ALIGNED, BACKWARD, ROWS> walk;
+    walk.load(p, place, at);
+    walk.open();
+    walk.finish(p, place, at, carry);
+  }
+  store_last<T, 1, BACKWARD>(p, place, carry);
 }
 
 // What other workgroups read of a tile: for each channel words {A, 1} and {H, 1} of its span, and of the last tile of a
@@ -450,6 +490,12 @@ int lanes_of(int64_t width, int wide) { return width <= 2 * wide ? 2 : 8; }
 // Tokens of a workgroup: all where batch and channels alone make four workgroups a CU, or a sequence is hardly longer than
 // a tile; a tile otherwise.
 constexpr int64_t kFill = 1024;
+// Short sequences go to threads that walk them alone: up to 8 tokens, or 32 where such threads fill the GPU.  Forward in
+// bfloat16, 1024 channels: 1024 sequences of 16 tokens 21 us (146 by tiles of 128 tokens), 512 of 32 28 (75), 256 of 64 48
+// (42), 64 of 32 20 (10).
+bool is_short(int64_t batch, int64_t tokens, int64_t vectors) {
+  return tokens <= 8 || (tokens <= 32 && batch * vectors >= 32768);
+}
 int64_t segment_of(int64_t batch, int64_t tokens, int64_t width, int dtype, bool backward) {
   const int wide = dtype == SDK_F32 ? 4 : 8, lanes = lanes_of(width, wide);
   const int64_t groups = batch * ceil_div(width, lanes * wide), tile = kWaiting / lanes * (backward ? kRows<true> : kRows<false>);
@@ -493,6 +539,14 @@ Scan on_device(const sdk_gated_scan* a, void* workspace, int lanes, int wide, bo
 template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
 void run(const sdk_gated_scan* a, void* workspace, hipStream_t s) {
   Scan p = on_device(a, workspace, LANES, kWide<T>, BACKWARD);
+  const int64_t vectors = ceil_div(p.width, kWide<T>), most = most_groups(kThreads) * kThreads / vectors;
+  if (is_short(a->batch, p.tokens, vectors)) {
+    for (p.first = 0; p.first < a->batch; p.first += most) {
+      p.batches = (int)std::min(most, a->batch - p.first);
+      launch(scan_short<T, ALIGNED, BACKWARD>, dim3((unsigned)ceil_div(p.batches * vectors, kThreads)), dim3(kThreads), s, p);
+    }
+    return;
+  }
   if (p.segments > 1) {   // fewer than kFill workgroups for a segment
     const int64_t words = (int64_t)(words_of(a, BACKWARD) / 8);
     launch(clear, dim3((unsigned)std::min<int64_t>(ceil_div(words, 256), 1024)), dim3(256), s, p.words, words);
