@@ -196,16 +196,58 @@ __device__ __forceinline__ void step_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// The lanes' columns of 16 KK rows of ROW bytes: KK operands, from the lane's place in the first four rows.  Waits for them
+// itself.
+template <int KK, int ROW>
+__device__ __forceinline__ void turned_reads(const char* first, f16x8 (&operands)[KK]) {
+  typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+  const unsigned at = (unsigned)(uintptr_t)(Lds)(first);
+  u32x2_t lo[KK], hi[KK];
+  if constexpr (KK == 2) {
+    asm volatile("ds_read_b64_tr_b16 %0, %4\n\t"
+                 "ds_read_b64_tr_b16 %1, %4 offset:%5\n\t"
+                 "ds_read_b64_tr_b16 %2, %4 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %3, %4 offset:%7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+                 : "v"(at), "i"(4 * ROW), "i"(16 * ROW), "i"(20 * ROW)
+                 : "memory");
+  } else {
+    static_assert(KK == 4, "lines of 32 or 64 values");
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\t"
+                 "ds_read_b64_tr_b16 %1, %8 offset:%9\n\t"
+                 "ds_read_b64_tr_b16 %2, %8 offset:%10\n\t"
+                 "ds_read_b64_tr_b16 %3, %8 offset:%11\n\t"
+                 "ds_read_b64_tr_b16 %4, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %5, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %8 offset:%14\n\t"
+                 "ds_read_b64_tr_b16 %7, %8 offset:%15\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]),
+                   "=&v"(hi[3])
+                 : "v"(at), "i"(4 * ROW), "i"(16 * ROW), "i"(20 * ROW), "i"(32 * ROW), "i"(36 * ROW), "i"(48 * ROW),
+                   "i"(52 * ROW)
+                 : "memory");
+  }
+#pragma unroll
+  for (int k = 0; k < KK; ++k) {
+    typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+    operands[k] = __builtin_bit_cast(f16x8, u32x4_t{lo[k].x, lo[k].y, hi[k].x, hi[k].y});
+  }
+}
+
 constexpr int kGram = 0, kPolynomial = 1, kNext = 2, kLast = 3;
 
 // A workgroup's block of F rows of the first operand and G of the second, dealt to waves of at most 64 x 64.
-template <int F_, int G_, int ACROSS_ = 2>
+// LINES: of 128 bytes of each row that a step takes, by as many groups of waves, each with a sum of its own.
+template <int F_, int G_, int ACROSS_, int LINES_, int STAGES_>
 struct Shape {
-  static constexpr int F = F_, G = G_, DOWN = F == 64 ? 2 : F / 64, ACROSS = ACROSS_, WAVES = DOWN * ACROSS, THREADS = 64 * WAVES;
+  static constexpr int F = F_, G = G_, DOWN = 2, ACROSS = ACROSS_, LINES = LINES_, WAVES = DOWN * ACROSS, THREADS = 64 * WAVES * LINES;
   static constexpr int Y = F / 32 / DOWN, X = G / 32 / ACROSS;   // 32 x 32 blocks of a wave
-  static constexpr int STAGES = F == 64 ? 4 : 2;  // steps in LDS
-  static constexpr int F_LOADS = F * 8 / THREADS, LOADS = (F + G) * 8 / THREADS;   // 16-byte requests of a thread and step
-  static constexpr int STEP = (F + G) * 128;                     // bytes of a step
+  static constexpr int STAGES = STAGES_;                         // steps in LDS
+  static constexpr int F_LOADS = F * 8 / (64 * WAVES), LOADS = (F + G) * 8 / (64 * WAVES);   // 16-byte requests of a thread
+                                                                                              // and step
+  static constexpr int LINE_BYTES = (F + G) * 128, STEP = LINES * LINE_BYTES;                // in LDS
 };
 
 // A wave's 32 x 32 block on its way to memory: in LDS as rows of 128 bytes whose 16-byte chunks are exchanged by the row's
@@ -363,14 +405,17 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
   const char* X = place + (turn ? at.x1 : at.x0);
   const char* rows_of = STAGE == kGram ? X : place + (STAGE == kPolynomial ? at.s : at.p);   // of 128 bytes a step
   const int64_t row_bytes = STAGE == kGram ? at.l_row : at.k_row;
-  const int steps = (int)(row_bytes / 128);
+  const int lines = (int)(row_bytes / 128), steps = (lines + S::LINES - 1) / S::LINES;
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // a group of waves takes every LINES-th line of the rows
+  const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = any_wave % S::WAVES, line = any_wave / S::WAVES;
+  const int thread = threadIdx.x % (64 * S::WAVES);
   const char* from[S::LOADS];
 #pragma unroll
   for (int r = 0; r < S::LOADS; ++r) {
     const bool first = r < S::F_LOADS;
-    const int chunk = (first ? r : r - S::F_LOADS) * S::THREADS + (int)threadIdx.x;   // of its operand's part of the step
+    const int chunk = (first ? r : r - S::F_LOADS) * 64 * S::WAVES + thread;   // of its operand's part of the line
     if (SQUARE || !first) {
       const int row = chunk / 8;
       int64_t global = first ? ti * S::F + row : tj * S::G + row;
@@ -383,13 +428,15 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
       from[r] = X + row * at.l_row + byte;
     }
   }
-  const int64_t first_step = SQUARE ? 128 : LINE * at.l_row;
-  auto request = [&](int step) {
-    char* to = lds + step % S::STAGES * S::STEP + wave * 1024;
+  const int64_t first_line = SQUARE ? 128 : LINE * at.l_row;
+  auto request = [&](int step) {   // of lines behind the rows' end: the last one, not used
+    char* to = lds + step % S::STAGES * S::STEP + line * S::LINE_BYTES + wave * 1024;
+    int64_t here = step * S::LINES + line;
+    if constexpr (S::LINES > 1) here = here < lines ? here : lines - 1;
 #pragma unroll
     for (int r = 0; r < S::LOADS; ++r)
-      __builtin_amdgcn_global_load_lds((Global)(from[r] + step * (r < S::F_LOADS ? first_step : 128)),
-                                       (Lds)(to + r * S::THREADS * 16), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((Global)(from[r] + here * (r < S::F_LOADS ? first_line : 128)),
+                                       (Lds)(to + r * S::WAVES * 1024), 16, 0, 0);
   };
 
   floatx16 acc[S::Y][S::X];
@@ -410,58 +457,99 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
     else
       step_barrier<0>();
     const bool more = step + S::STAGES - 1 < steps;
-    const char* buffer = lds + step % S::STAGES * S::STEP;
+    const char* buffer = lds + step % S::STAGES * S::STEP + line * S::LINE_BYTES;
     auto operand = [&](int row, int chunk) { return *reinterpret_cast<const f16x8*>(buffer + chunk_at(row, chunk)); };
     // columns first .. first + 31 of 16 rows of X from row `row` on
-    auto turned_operand = [&](int first, int row, int piece) {
+    auto turned_at = [&](int first, int row, int piece) {
       const int r = row + 8 * half + lane % 16 / 4;   // and r + 4, whose chunks lie alike
       const int column = first + lane / 16 % 2 * 16;
       const int chunk = column / LINE * 8 + piece * 4 + column % LINE / 8 + lane % 4 / 2;
-      const char* lo = buffer + r * (CHUNKS * 16) + ((chunk ^ (CHUNKS >= 16 ? r % 4 * 4 : r / 2 % 2 * 4)) * 16) + lane % 2 * 8;
-      return __builtin_bit_cast(f16x8, tr_frag(lo, lo + 4 * CHUNKS * 16).v);
+      return buffer + r * (CHUNKS * 16) + ((chunk ^ (CHUNKS >= 16 ? r % 4 * 4 : r / 2 % 2 * 4)) * 16) + lane % 2 * 8;
     };
     f16x8 a[KK][S::Y][PIECES];
     if constexpr (SQUARE) {
       if (more) request(step + S::STAGES - 1);
-    } else {
+    } else if constexpr (S::STAGES == 2) {
       // the compiler waits for every request in flight before a transposing read: these come first
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int y = 0; y < S::Y; ++y)
 #pragma unroll
-          for (int piece = 0; piece < PIECES; ++piece) a[kk][y][piece] = turned_operand(wy + y * 32, kk * 16, piece);
+          for (int piece = 0; piece < PIECES; ++piece) {
+            const char* lo = turned_at(wy + y * 32, kk * 16, piece);
+            a[kk][y][piece] = __builtin_bit_cast(f16x8, tr_frag(lo, lo + 4 * CHUNKS * 16).v);
+          }
       asm volatile("" ::: "memory");
       if (more) request(step + S::STAGES - 1);
       asm volatile("" ::: "memory");
-    }
+    } else {
+      if (more) request(step + S::STAGES - 1);
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      f16x8 b[S::X][PIECES];
+      for (int y = 0; y < S::Y; ++y)
+#pragma unroll
+        for (int piece = 0; piece < PIECES; ++piece) {
+          f16x8 all[KK];
+          turned_reads<KK, CHUNKS * 16>(turned_at(wy + y * 32, 0, piece), all);
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) a[kk][y][piece] = all[kk];
+        }
+    }
+    if (S::LINES > 1 && step * S::LINES + line >= lines) continue;
+    f16x8 b[KK][S::X][PIECES];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int piece = 0; piece < PIECES; ++piece) {
 #pragma unroll
-        for (int x = 0; x < S::X; ++x) b[x][piece] = operand(S::F + wx + x * 32 + lane % 32, piece * 4 + kk * 2 + half);
+        for (int x = 0; x < S::X; ++x) b[kk][x][piece] = operand(S::F + wx + x * 32 + lane % 32, piece * 4 + kk * 2 + half);
         if constexpr (SQUARE) {
 #pragma unroll
           for (int y = 0; y < S::Y; ++y) a[kk][y][piece] = operand(wy + y * 32 + lane % 32, piece * 4 + kk * 2 + half);
         }
       }
+    if constexpr (S::LINES > 1) __builtin_amdgcn_sched_barrier(0);   // few products: all reads before the first
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int y = 0; y < S::Y; ++y)
 #pragma unroll
         for (int x = 0; x < S::X; ++x) {
           if constexpr (SPLIT) {
-            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][1], b[x][0], acc[y][x], 0, 0, 0);
-            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][0], b[x][1], acc[y][x], 0, 0, 0);
+            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][1], b[kk][x][0], acc[y][x], 0, 0, 0);
+            acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][0], b[kk][x][1], acc[y][x], 0, 0, 0);
           }
-          acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][0], b[x][0], acc[y][x], 0, 0, 0);
+          acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][0], b[kk][x][0], acc[y][x], 0, 0, 0);
         }
-    }
   }
   step_barrier<0>();   // the buffers are free
 
-  char* scratch = lds + wave * 8192;
+  if constexpr (S::LINES > 1) {   // the groups' sums, in their order
+    float* sums = (float*)lds;
+    if (line > 0) {
+#pragma unroll
+      for (int y = 0; y < S::Y; ++y)
+#pragma unroll
+        for (int x = 0; x < S::X; ++x)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            sums[((((line - 1) * S::Y + y) * S::X + x) * 16 + v) * (64 * S::WAVES) + thread] = acc[y][x][v];
+    }
+    __syncthreads();
+    if (line > 0) return;
+#pragma unroll
+    for (int more = 0; more < S::LINES - 1; ++more)
+#pragma unroll
+      for (int y = 0; y < S::Y; ++y)
+#pragma unroll
+        for (int x = 0; x < S::X; ++x)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            acc[y][x][v] += sums[(((more * S::Y + y) * S::X + x) * 16 + v) * (64 * S::WAVES) + thread];
+  }
+  // behind the sums that were just read
+  char* scratch = lds + (S::LINES - 1) * S::F * S::G * 4 + wave * 8192;
+  static_assert((S::LINES - 1) * S::F * S::G * 4 + S::WAVES * 8192 <= S::STAGES * S::STEP, "scratch lies in the buffers");
   const int64_t i_end = SQUARE ? at.kp : at.lp;
   auto scaled = [&](int y, int x) {
     floatx16 v;
@@ -567,11 +655,11 @@ void multiply(Table& t, int used, const Settings& s, char* workspace, int turn, 
 // the last stage's parameters (247 us for 190 in float32).
 template <bool SPLIT, int STAGE, typename T>
 void stage(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream) {
-  using Large = Shape<128, 128, STAGE == kLast ? 2 : 4>;
+  using Large = Shape<128, 128, STAGE == kLast ? 2 : 4, 1, 2>;
   if (groups_of<STAGE, Large>(t, used) >= 256)
     multiply<SPLIT, Large, STAGE, T>(t, used, s, workspace, turn, stream);
   else
-    multiply<SPLIT, Shape<64, 64>, STAGE, T>(t, used, s, workspace, turn, stream);
+    multiply<SPLIT, Shape<64, 64, 2, 2, 4>, STAGE, T>(t, used, s, workspace, turn, stream);
 }
 
 template <typename T>
