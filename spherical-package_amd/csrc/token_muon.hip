@@ -14,7 +14,8 @@
 // the 1.7e-3 of its own rounding.  Every singular value stays below about 1.2 on its way with the usual coefficients, so
 // entries of X and S are at most 1.5; up to 15 fit.  Sums are float32, of the norm double.
 //
-// All matrices of a call go through a stage in one launch; their table is a kernel argument.
+// All matrices of a call go through a stage in one launch; their table is a kernel argument.  Small ones go through all
+// stages in a workgroup of their own.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -611,6 +612,269 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
     }
 }
 
+// Small matrices, k up to 64: one workgroup takes a matrix through all steps, in LDS throughout.  X, S and P lie there as
+// lines of 128 bytes, a row after the other, their chunks exchanged by the row's number.
+template <bool SPLIT>
+struct Small {
+  static constexpr int THREADS = 512, LP = SPLIT ? 384 : 640;   // and l up to LP
+  static constexpr int SQUARE = 64 * (64 / kLine<SPLIT>) * 128, X = SQUARE / 64 * LP;
+  static constexpr int BYTES = X + SQUARE + 16384;              // X, S, P; from P's place on sums of S in float32
+};
+
+// 16 bytes of a row's line.
+__device__ __forceinline__ char* line_at(char* base, int row, int pitch, int line, int chunk) {
+  return base + row * pitch + line * 128 + ((chunk ^ (row & 7)) * 16);
+}
+
+// A block's columns into lines: value 4 q + e of a lane is row 8 q + 4 (lane / 32) + e, column lane % 32; its column goes to
+// row `row0` + column of `base`, from value `at` of the row on (a multiple of 32).
+template <bool SPLIT>
+__device__ __forceinline__ void keep_block(const floatx16& v, int lane, char* base, int pitch, int row0, int at) {
+  const int half = lane / 32, row = row0 + lane % 32, line = at / kLine<SPLIT>, first = at % kLine<SPLIT> / 8;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    Pack<f16, 4> hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split_f16(v[4 * q + e], hi.v[e], lo.v[e]);
+    *reinterpret_cast<Pack<f16, 4>*>(line_at(base, row, pitch, line, first + q) + half * 8) = hi;
+    if constexpr (SPLIT) *reinterpret_cast<Pack<f16, 4>*>(line_at(base, row, pitch, line, 4 + q) + half * 8) = lo;
+  }
+}
+
+// acc += the products of two operands' pieces
+template <bool SPLIT>
+__device__ __forceinline__ void add_product(floatx16& acc, const f16x8 (&a)[2], const f16x8 (&b)[2]) {
+  if constexpr (SPLIT) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], acc, 0, 0, 0);
+  }
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc, 0, 0, 0);
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void small_matrix(const Table t, const Settings s, int steps) {
+  constexpr bool SPLIT = !std::is_same<T, bf16>::value;
+  constexpr int LINE = kLine<SPLIT>, KK = LINE / 16, PIECES = SPLIT ? 2 : 1, SQUARE_PITCH = 64 / LINE * 128;
+  using Z = Small<SPLIT>;
+  __shared__ __attribute__((aligned(128))) char lds[Z::BYTES];
+  __shared__ double sums[8];
+  const int i = blockIdx.x, rows = t.rows[i], columns = t.columns[i];
+  const bool tall = rows > columns;
+  const int k = tall ? columns : rows, l = tall ? rows : columns, lp = (l + 63) / 64 * 64, pitch = lp / LINE * 128;
+  const T* g = (const T*)t.g[i];
+  float* m = t.m[i];
+  char *X = lds, *S = lds + Z::X, *P = S + Z::SQUARE;
+  float* blocks = (float*)P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane / 32;
+
+  // momentum and norm; the update stays in registers, X begins as zeros
+  // four columns of a row at once, a thread's vectors THREADS apart
+  constexpr int EACH = Z::LP * 64 / 4 / Z::THREADS;
+  const int vectors = (columns + 3) / 4, rows_on = Z::THREADS / vectors, vectors_on = Z::THREADS % vectors;
+  const int row0 = (int)threadIdx.x / vectors, vector0 = (int)threadIdx.x % vectors;
+  auto next_vector = [&](int& row, int& vector) {
+    row += rows_on, vector += vectors_on;
+    if (vector >= vectors) vector -= vectors, ++row;
+  };
+  float u[EACH][4], old[EACH][4];
+  int row = row0, vector = vector0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) u[e][c] = old[e][c] = 0.f;
+    if (row < rows) {
+      load_part<T, 4>(g + row * columns + vector * 4, u[e], columns - vector * 4);
+      if (m) load_part<float, 4>(m + row * columns + vector * 4, old[e], columns - vector * 4);
+    }
+    next_vector(row, vector);
+  }
+  double sum = 0;
+  row = row0, vector = vector0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (m && row < rows) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float grad = u[e][c];
+        old[e][c] = s.mu * old[e][c] + s.rest * grad;
+        u[e][c] = s.nesterov ? s.mu * old[e][c] + s.rest * grad : old[e][c];
+      }
+      store_part<float, 4>(m + row * columns + vector * 4, old[e], columns - vector * 4);
+    }
+    // four squares in double: float32's range would not do
+    sum += ((double)u[e][0] * u[e][0] + (double)u[e][1] * u[e][1]) + ((double)u[e][2] * u[e][2] + (double)u[e][3] * u[e][3]);
+    next_vector(row, vector);
+  }
+  for (int at = threadIdx.x * 16; at < 64 * pitch; at += Z::THREADS * 16) *(float4*)(X + at) = float4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += sums[w];
+  const float up = kScale / ((float)sqrt(sum) + s.eps);
+  row = row0, vector = vector0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (row < rows) {
+      Pack<f16, 4> hi, lo;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) split_f16(u[e][c] * up, hi.v[c], lo.v[c]);
+      if (tall) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {   // up to three rows behind the matrix's: zeros
+          const int y = vector * 4 + c;
+          *(f16*)(line_at(X, y, pitch, row / LINE, row % LINE / 8) + row % 8 * 2) = hi.v[c];
+          if constexpr (SPLIT) *(f16*)(line_at(X, y, pitch, row / LINE, 4 + row % LINE / 8) + row % 8 * 2) = lo.v[c];
+        }
+      } else {
+        const int x = vector * 4;
+        *reinterpret_cast<Pack<f16, 4>*>(line_at(X, row, pitch, x / LINE, x % LINE / 8) + x % 8 * 2) = hi;
+        if constexpr (SPLIT)
+          *reinterpret_cast<Pack<f16, 4>*>(line_at(X, row, pitch, x / LINE, 4 + x % LINE / 8) + x % 8 * 2) = lo;
+      }
+    }
+    next_vector(row, vector);
+  }
+  __syncthreads();
+
+  auto operand = [&](char* base, int row_pitch, int row, int line, int kk, f16x8 (&x)[2]) {
+#pragma unroll
+    for (int piece = 0; piece < PIECES; ++piece)
+      x[piece] = *reinterpret_cast<const f16x8*>(line_at(base, row + lane % 32, row_pitch, line, piece * 4 + kk * 2 + half));
+  };
+  // columns j .. j + 31 of P X times `down`, as rows: the rows of P in two halves
+  auto multiply = [&](int j, floatx16 (&next)[2], float down) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) next[0][v] = next[1][v] = 0.f;
+    f16x8 x[4][2];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int piece = 0; piece < PIECES; ++piece) {
+        const int row = kk * 16 + 8 * half + lane % 16 / 4, column = j + lane / 16 % 2 * 16;
+        const int chunk = piece * 4 + column % LINE / 8 + lane % 4 / 2;
+        const char* lo = line_at(X, row, pitch, column / LINE, chunk) + lane % 2 * 8;
+        const char* hi = line_at(X, row + 4, pitch, column / LINE, chunk) + lane % 2 * 8;
+        x[kk][piece] = __builtin_bit_cast(f16x8, tr_frag(lo, hi).v);
+      }
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        f16x8 p[2];
+        operand(P, SQUARE_PITCH, y * 32, kk / KK, kk % KK, p);
+        add_product<SPLIT>(next[y], x[kk], p);
+      }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) next[0][v] *= down, next[1][v] *= down;
+  };
+  const int by = wave / 2 % 2 * 32, bx = wave % 2 * 32;   // of S and P, by waves 0 to 3
+  for (int step = 0; step < steps; ++step) {
+    floatx16 acc;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+    // S: four waves take even lines, four odd ones
+    for (int line = wave / 4; line < lp / LINE; line += 2) {
+      f16x8 a[KK][2], b[KK][2];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) operand(X, pitch, by, line, kk, a[kk]), operand(X, pitch, bx, line, kk, b[kk]);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) add_product<SPLIT>(acc, a[kk], b[kk]);
+    }
+    float* part = blocks + wave % 4 * 1024 + lane;
+    if (wave >= 4) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) part[v * 64] = acc[v];
+    }
+    __syncthreads();
+    if (wave < 4) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[v] = (acc[v] + part[v * 64]) * kDown;
+      keep_block<SPLIT>(acc, lane, S, SQUARE_PITCH, bx, by);   // S is its own transpose
+    }
+    __syncthreads();
+    if (wave < 4) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+#pragma unroll
+      for (int line = 0; line < 64 / LINE; ++line)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          f16x8 a[2], b[2];
+          operand(S, SQUARE_PITCH, by, line, kk, a), operand(S, SQUARE_PITCH, bx, line, kk, b);
+          add_product<SPLIT>(acc, a, b);
+        }
+      const int row = bx + lane % 32;   // where this lane's column of S lies
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int line = by / LINE, chunk = by % LINE / 8 + q;
+        const Pack<f16, 4> hi = *reinterpret_cast<const Pack<f16, 4>*>(line_at(S, row, SQUARE_PITCH, line, chunk) + half * 8);
+        Pack<f16, 4> lo;
+        if constexpr (SPLIT)
+          lo = *reinterpret_cast<const Pack<f16, 4>*>(line_at(S, row, SQUARE_PITCH, line, 4 + q) + half * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float old = (float)hi.v[e] + (SPLIT ? (float)lo.v[e] : 0.f);
+          acc[4 * q + e] = fmaf(s.c, acc[4 * q + e] * kDown, s.b * old) +
+                           (by + 8 * q + 4 * half + e == row ? s.a * kScale : 0.f);
+        }
+      }
+      keep_block<SPLIT>(acc, lane, P, SQUARE_PITCH, bx, by);
+    }
+    __syncthreads();
+    if (step + 1 == steps) break;
+    // X' = P X in place: a wave has 32 columns of X to itself
+    for (int j = wave * 32; j < lp; j += Z::THREADS / 2) {
+      floatx16 next[2];
+      multiply(j, next, kDown);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) keep_block<SPLIT>(next[y], lane, X, pitch, y * 32, j);
+    }
+    __syncthreads();
+  }
+  T* p = (T*)t.p[i];
+  const float keep = m ? s.keep : 0.f, rate = m ? -t.rate[i] : 1.f;
+  for (int j = wave * 32; j < lp; j += Z::THREADS / 2) {
+    floatx16 next[2];
+    multiply(j, next, kDown * kDown);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int row = y * 32 + lane % 32, left = row < k ? l - j - 4 * half : 0;   // columns of this lane's from its first on
+      float old[4][4];
+      if (left <= 0) continue;
+      if (tall) {
+        T* to = p + row + (j + 4 * half) * k;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int column = 8 * (v / 4) + v % 4;
+          old[v / 4][v % 4] = m && column < left ? (float)to[column * k] : 0.f;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int column = 8 * (v / 4) + v % 4;
+          if (column < left) to[column * k] = (T)(old[v / 4][v % 4] * keep + rate * next[y][v]);
+        }
+      } else {
+        T* to = p + row * l + j + 4 * half;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) old[q][c] = 0.f;
+          if (m && 8 * q < left) load_part<T, 4>(to + 8 * q, old[q], left - 8 * q);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) old[q][c] = old[q][c] * keep + rate * next[y][4 * q + c];
+          if (8 * q < left) store_part<T, 4>(to + 8 * q, old[q], left - 8 * q);
+        }
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------ host
 struct Matrix {
   void* p;
@@ -680,10 +944,16 @@ void run_group(Table& t, int used, const Settings& s, int steps, char* workspace
   }
 }
 
+// Whether one workgroup takes the matrix: three matrices of 16 x 27 to 64 x 288 in float32, a step of each, 20 us for 85.
+bool is_small(int64_t rows, int64_t columns, int dtype) {
+  return std::min(rows, columns) <= 64 && std::max(rows, columns) <= (split(dtype) ? Small<true>::LP : Small<false>::LP);
+}
+
 // Deals the matrices to groups that share the workspace one after another: 64 at most, and as many workgroups as a
 // launch holds.  `run` gets a table and how many it holds; returns the bytes of the largest group.
+// small: those that a workgroup takes alone, or the others.
 template <typename Get, typename Run>
-size_t in_groups(int64_t count, int dtype, Get get, Run run) {
+size_t in_groups(int64_t count, int dtype, bool small, Get get, Run run) {
   Table t = {};
   int used = 0;
   int64_t bytes = 0, most = 0, tiles = 0;
@@ -694,7 +964,7 @@ size_t in_groups(int64_t count, int dtype, Get get, Run run) {
   };
   for (int64_t i = 0; i < count; ++i) {
     const Matrix x = get(i);
-    if (x.rows < 1 || x.columns < 1) continue;
+    if (x.rows < 1 || x.columns < 1 || is_small(x.rows, x.columns, dtype) != small) continue;
     const Layout at(x.rows, x.columns, split(dtype));
     const int64_t mine = std::max(at.kp / 64 * (at.lp / 64), ceil_div(x.rows * x.columns, kPerGroup));
     if (used == kMatrices || tiles + mine > most_groups(256)) done();
@@ -736,10 +1006,13 @@ Settings settings_of(const double* c, double eps) {
 int run_all(int64_t count, int steps, const Settings& s, void* workspace, size_t workspace_bytes, int dtype,
             sdk_stream_t stream, Matrix (*get)(const void*, int64_t), const void* context) {
   auto of = [&](int64_t i) { return get(context, i); };
-  const size_t need = in_groups(count, dtype, of, [](Table&, int) {});
+  const size_t need = in_groups(count, dtype, false, of, [](Table&, int) {});
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 128))
     return fail(SDK_ERR_WORKSPACE, "workspace of %zu bytes at a multiple of 128, %zu needed", workspace_bytes, need);
-  in_groups(count, dtype, of, [&](Table& t, int used) {
+  in_groups(count, dtype, true, of, [&](Table& t, int used) {
+    SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(small_matrix<T>, dim3(used), dim3(512), (hipStream_t)stream, t, s, steps));
+  });
+  in_groups(count, dtype, false, of, [&](Table& t, int used) {
     SDK_DISPATCH_TOKEN_DTYPE(dtype, run_group<T>(t, used, s, steps, (char*)workspace, (hipStream_t)stream));
   });
   return SDK_OK;
@@ -770,7 +1043,7 @@ extern "C" {
 size_t sdk_orthogonalize_workspace_bytes(int64_t rows, int64_t columns, int64_t count, int32_t dtype) {
   if (check_matrix(rows, columns) != SDK_OK || !known(dtype) || count < 0) return 0;
   count = std::min<int64_t>(count, kMatrices);
-  return in_groups(count, dtype, [&](int64_t) { return Matrix{nullptr, nullptr, nullptr, rows, columns, 0.f}; },
+  return in_groups(count, dtype, false, [&](int64_t) { return Matrix{nullptr, nullptr, nullptr, rows, columns, 0.f}; },
                    [](Table&, int) {});
 }
 
@@ -797,7 +1070,7 @@ size_t sdk_muon_step_workspace_bytes(const int64_t* rows, const int64_t* columns
   if (!known(dtype) || count < 1 || !rows || !columns) return 0;
   for (int64_t i = 0; i < count; ++i)
     if (check_matrix(rows[i], columns[i]) != SDK_OK) return 0;
-  return in_groups(count, dtype, [&](int64_t i) { return Matrix{nullptr, nullptr, nullptr, rows[i], columns[i], 0.f}; },
+  return in_groups(count, dtype, false, [&](int64_t i) { return Matrix{nullptr, nullptr, nullptr, rows[i], columns[i], 0.f}; },
                    [](Table&, int) {});
 }
 
