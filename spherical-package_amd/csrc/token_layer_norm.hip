@@ -25,79 +25,154 @@ template <typename T>
 constexpr int kChunks = 16 / kWide<T>;
 constexpr int64_t kMostWidth = 16384;
 
-template <int THREADS>
-__device__ __forceinline__ float row_sum(float x, float* slots) {
-  if constexpr (THREADS < 64)
-    return over_lanes<Add, THREADS>(x);
-  else
-    return over_group<Add, THREADS>(x, slots);
+// The sums of COUNT values over the row's threads.  slots: COUNT floats a wave, used again only after a barrier of another
+// call.
+template <int THREADS, int COUNT>
+__device__ __forceinline__ void row_sums(float (&x)[COUNT], float (*slots)[COUNT]) {
+#pragma unroll
+  for (int c = 0; c < COUNT; ++c) x[c] = lane_sum<(THREADS < 64 ? THREADS : 64)>(x[c]);
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int c = 0; c < COUNT; ++c) slots[threadIdx.x >> 6][c] = x[c];
+    }
+    __syncthreads();
+    const int first = threadIdx.x / THREADS * (THREADS / 64);
+#pragma unroll
+    for (int c = 0; c < COUNT; ++c) {
+      x[c] = slots[first][c];
+#pragma unroll
+      for (int w = 1; w < THREADS / 64; ++w) x[c] += slots[first + w][c];
+    }
+  }
 }
 
+// 16 bytes of a row as they lie in memory, `left` of their V values in the row.  A row that fits no vector ends inside one:
+// what follows is the next row (`more`: there is one) and is read with it; the user leaves it out (in_row).  Words, not
+// values: of values the compiler makes a request each.
+typedef unsigned Words __attribute__((ext_vector_type(4)));
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ Words row_get(const T* p, int left, bool more) {
+  typedef Words AnyWords __attribute__((aligned(2)));
+  if (ALIGNED) return *reinterpret_cast<const Words*>(p);
+  if (left >= V || more) return *reinterpret_cast<const AnyWords*>(p);
+  Pack<T, V> x;
+#pragma unroll
+  for (int e = 0; e < V; ++e) x.v[e] = e < left ? p[e] : (T)0.f;
+  return __builtin_bit_cast(Words, x);
+}
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void in_row(Words w, float (&f)[V], int left) {
+  const Pack<T, V> x = __builtin_bit_cast(Pack<T, V>, w);
+#pragma unroll
+  for (int e = 0; e < V; ++e) f[e] = ALIGNED || e < left ? (float)x.v[e] : 0.f;
+}
+
+// The same into memory: what a vector does not hold goes in halves, quarters, ...
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void row_put(T* p, const float (&f)[V], int left) {
+  if (ALIGNED || left >= V) {
+    put<T, V, ALIGNED>(p, f, left);
+    return;
+  }
+  Pack<T, V> x;
+#pragma unroll
+  for (int e = 0; e < V; ++e) x.v[e] = (T)f[e];
+  if constexpr (V == 8) {
+    if (left & 4) {
+      __builtin_memcpy(p, &x, 4 * sizeof(T));
+      p += 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.v[e] = x.v[e + 4];
+    }
+  }
+  if (left & 2) {
+    __builtin_memcpy(p, &x, 2 * sizeof(T));
+    p += 2;
+    x.v[0] = x.v[2];
+  }
+  if (left & 1) *p = x.v[0];
+}
+
+// Rows of whole vectors: a workgroup a row (or the rows that share one).  Others: workgroup b takes rows b, b + gridDim.x, ..,
+// so that the weight's end, which has to be read in single values, is read once.
 template <typename T, int THREADS, bool ALIGNED>
 __global__ __launch_bounds__(kGroup<THREADS>) void layer_forward(const T* x, const T* residual, const void* weight,
                                                                  const void* bias, int weight_float, T* out, T* summed,
                                                                  float* mean, float* inverse, int64_t rows, int width,
                                                                  float eps) {
-  constexpr int V = kWide<T>, N = kChunks<T>;
-  __shared__ float slots[kGroup<THREADS> / 64];
+  constexpr int V = kWide<T>, N = kChunks<T>, SHARE = kGroup<THREADS> / THREADS;
+  __shared__ float slots[2][kGroup<THREADS> / 64][1];
   const int t = threadIdx.x % THREADS;
-  const int64_t row = (int64_t)blockIdx.x * (kGroup<THREADS> / THREADS) + threadIdx.x / THREADS;
-  const bool live = row < rows;
-  const int64_t base = row * width;
-  float h[N][V];
-  float sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
+  float w[N][V], b[N][V];
+  auto weights = [&](int k) {
     const int j = (k * THREADS + t) * V;
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[k][e] = 0.f;
-    if (live && j < width) {
-      get<T, V, ALIGNED>(x + base + j, h[k], width - j);
-      if (residual) {
-        float r[V];
-        get<T, V, ALIGNED>(residual + base + j, r, width - j);
-#pragma unroll
-        for (int e = 0; e < V; ++e) h[k][e] += r[e];
-      }
+    for (int e = 0; e < V; ++e) w[k][e] = b[k][e] = 0.f;
+    if (j < width) {
+      load_weight<T, V, ALIGNED>(weight, weight_float, j, w[k], width - j);
+      if (bias) load_weight<T, V, ALIGNED>(bias, weight_float, j, b[k], width - j);
     }
+  };
+  if (!ALIGNED) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum += h[k][e];
+    for (int k = 0; k < N; ++k) weights(k);
   }
-  if (summed) {
+  for (int64_t first = (int64_t)blockIdx.x * SHARE; first < rows; first += (int64_t)gridDim.x * SHARE) {
+    const int64_t row = first + threadIdx.x / THREADS, base = row * width;
+    const bool live = row < rows, more = row + 1 < rows && width >= V;
+    float h[N][V];
+    float sum[1] = {0.f}, sq[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int j = (k * THREADS + t) * V;
-      if (live && j < width) put<T, V, ALIGNED>(summed + base + j, h[k], width - j);
+      Words a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+      if (live && j < width) {
+        a = row_get<T, V, ALIGNED>(x + base + j, width - j, more);
+        if (residual) b = row_get<T, V, ALIGNED>(residual + base + j, width - j, more);
+      }
+      float r[V];
+      in_row<T, V, ALIGNED>(a, h[k], width - j);
+      in_row<T, V, ALIGNED>(b, r, width - j);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        h[k][e] += r[e];
+        sum[0] += h[k][e];
+      }
     }
-  }
-  const float mu = row_sum<THREADS>(sum, slots) / (float)width;
-  float sq = 0.f;
+    if (summed) {
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int left = width - (k * THREADS + t) * V;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      h[k][e] -= mu;
-      if (e < left) sq += h[k][e] * h[k][e];
+      for (int k = 0; k < N; ++k) {
+        const int j = (k * THREADS + t) * V;
+        if (live && j < width) row_put<T, V, ALIGNED>(summed + base + j, h[k], width - j);
+      }
     }
-  }
-  const float inv = 1.f / sqrtf(row_sum<THREADS>(sq, slots) / (float)width + eps);
-  if (live && t == 0) {
-    if (mean) mean[row] = mu;
-    if (inverse) inverse[row] = inv;
-  }
+    row_sums<THREADS>(sum, slots[0]);
+    const float mu = sum[0] / (float)width;
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int j = (k * THREADS + t) * V;
-    if (live && j < width) {
-      float w[V], b[V];
-      load_weight<T, V, ALIGNED>(weight, weight_float, j, w, width - j);
+    for (int k = 0; k < N; ++k) {
+      const int left = width - (k * THREADS + t) * V;
 #pragma unroll
-      for (int e = 0; e < V; ++e) b[e] = 0.f;
-      if (bias) load_weight<T, V, ALIGNED>(bias, weight_float, j, b, width - j);
+      for (int e = 0; e < V; ++e) {
+        h[k][e] -= mu;
+        if (e < left) sq[0] += h[k][e] * h[k][e];
+      }
+    }
+    row_sums<THREADS>(sq, slots[1]);
+    const float inv = 1.f / sqrtf(sq[0] / (float)width + eps);
+    if (live && t == 0) {
+      if (mean) mean[row] = mu;
+      if (inverse) inverse[row] = inv;
+    }
 #pragma unroll
-      for (int e = 0; e < V; ++e) h[k][e] = h[k][e] * inv * w[e] + b[e];
-      put<T, V, ALIGNED>(out + base + j, h[k], width - j);
+    for (int k = 0; k < N; ++k) {
+      const int j = (k * THREADS + t) * V;
+      if (live && j < width) {
+        if (ALIGNED) weights(k);
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[k][e] = h[k][e] * inv * w[k][e] + b[k][e];
+        row_put<T, V, ALIGNED>(out + base + j, h[k], width - j);
+      }
     }
   }
 }
@@ -110,7 +185,7 @@ __global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad,
                                                                   const float* mean, const float* inverse, T* grad_x,
                                                                   float* parts, int64_t rows, int width) {
   constexpr int V = kWide<T>, N = kChunks<T>, SHARE = kGroup<THREADS> / THREADS;
-  __shared__ float slots[2][kGroup<THREADS> / 64];
+  __shared__ float slots[2][kGroup<THREADS> / 64][2];
   const int t = threadIdx.x % THREADS, sub = threadIdx.x / THREADS;
   float w[N][V], dw[N][V], db[N][V];
 #pragma unroll
@@ -120,50 +195,74 @@ __global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad,
     for (int e = 0; e < V; ++e) w[k][e] = dw[k][e] = db[k][e] = 0.f;
     if (j < width) load_weight<T, V, ALIGNED>(weight, weight_float, j, w[k], width - j);
   }
-  for (int64_t first = (int64_t)blockIdx.x * SHARE; first < rows; first += (int64_t)gridDim.x * SHARE) {
+  // a row as it lies in memory; the next one is requested while this one is worked on (75 us without that for 43, 32768
+  // rows of 768 bfloat16 values), but for 1024 threads, whose registers do not hold two
+  constexpr bool AHEAD = THREADS < 1024;
+  struct Row {
+    Words h[N], g[N], s[N];
+    float mu, inv;
+    bool live;
+  };
+  auto request = [&](Row& r, int64_t first) {
     const int64_t row = first + sub, base = row * width;
-    const bool live = row < rows;
-    const float inv = live ? inverse[row] : 0.f, mu = live ? mean[row] : 0.f;
-    float z[N][V], q[N][V], flat = 0.f, along = 0.f;
+    const bool more = row + 1 < rows && width >= V;
+    r.live = row < rows;
+    r.inv = r.live ? inverse[row] : 0.f;
+    r.mu = r.live ? mean[row] : 0.f;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int j = (k * THREADS + t) * V;
-#pragma unroll
-      for (int e = 0; e < V; ++e) z[k][e] = q[k][e] = 0.f;
-      if (live && j < width) {
-        get<T, V, ALIGNED>(h_in + base + j, z[k], width - j);
-        get<T, V, ALIGNED>(grad + base + j, q[k], width - j);
+      r.h[k] = r.g[k] = r.s[k] = Words{0, 0, 0, 0};
+      if (r.live && j < width) {
+        r.h[k] = row_get<T, V, ALIGNED>(h_in + base + j, width - j, more);
+        r.g[k] = row_get<T, V, ALIGNED>(grad + base + j, width - j, more);
+        if (grad_sum) r.s[k] = row_get<T, V, ALIGNED>(grad_sum + base + j, width - j, more);
       }
     }
+  };
+  const int64_t begin = (int64_t)blockIdx.x * SHARE, step = (int64_t)gridDim.x * SHARE;
+  Row now;
+  if (AHEAD) request(now, begin);
+  int turn = 0;
+  for (int64_t first = begin; first < rows; first += step, turn ^= 1) {
+    Row next;
+    if (!AHEAD)
+      request(now, first);
+    else if (first + step < rows)
+      request(next, first + step);
+    float z[N][V], q[N][V], both[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < N; ++k)
+    for (int k = 0; k < N; ++k) {
+      // beyond the row's end q and w are zeros: z counts nowhere
+      const int left = width - (k * THREADS + t) * V;
+      in_row<T, V, ALIGNED>(now.h[k], z[k], left);
+      in_row<T, V, ALIGNED>(now.g[k], q[k], left);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        // beyond the row's end q and w are zeros: z counts nowhere
-        z[k][e] = (z[k][e] - mu) * inv;
+        z[k][e] = (z[k][e] - now.mu) * now.inv;
         dw[k][e] += q[k][e] * z[k][e];
         db[k][e] += q[k][e];
         q[k][e] *= w[k][e];
-        flat += q[k][e];
-        along += q[k][e] * z[k][e];
+        both[0] += q[k][e];
+        both[1] += q[k][e] * z[k][e];
       }
-    flat = row_sum<THREADS>(flat, slots[0]) / (float)width;
-    along = row_sum<THREADS>(along, slots[1]) / (float)width;
+    }
+    row_sums<THREADS>(both, slots[turn]);
+    const float flat = both[0] / (float)width, along = both[1] / (float)width;
     if (grad_x) {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         const int j = (k * THREADS + t) * V;
-        if (live && j < width) {
+        if (now.live && j < width) {
           float s[V];
+          in_row<T, V, true>(now.s[k], s, width - j);
 #pragma unroll
-          for (int e = 0; e < V; ++e) s[e] = 0.f;
-          if (grad_sum) get<T, V, ALIGNED>(grad_sum + base + j, s, width - j);
-#pragma unroll
-          for (int e = 0; e < V; ++e) s[e] += inv * (q[k][e] - flat - z[k][e] * along);
-          put<T, V, ALIGNED>(grad_x + base + j, s, width - j);
+          for (int e = 0; e < V; ++e) s[e] += now.inv * (q[k][e] - flat - z[k][e] * along);
+          row_put<T, V, ALIGNED>(grad_x + (first + sub) * width + j, s, width - j);
         }
       }
     }
+    if (AHEAD) now = next;
   }
   if (!parts) return;
   float* to = parts + (int64_t)blockIdx.x * 2 * width;
@@ -268,7 +367,9 @@ void run_forward(const T* x, const T* residual, const void* weight, const void* 
   constexpr int64_t EACH = most_groups(kGroup<THREADS>) * SHARE;
   for (int64_t row = 0; row < rows; row += EACH) {
     const int64_t count = std::min(EACH, rows - row), at = row * width;
-    launch(layer_forward<T, THREADS, ALIGNED>, dim3((unsigned)ceil_div(count, SHARE)), dim3(kGroup<THREADS>), s, x + at,
+    const int64_t groups = ceil_div(count, SHARE);
+    launch(layer_forward<T, THREADS, ALIGNED>, dim3((unsigned)(ALIGNED ? groups : std::min<int64_t>(groups, 2048))),
+           dim3(kGroup<THREADS>), s, x + at,
            residual ? residual + at : nullptr, weight, bias, weight_float, out + at, summed ? summed + at : nullptr,
            mean ? mean + row : nullptr, inverse ? inverse + row : nullptr, count, width, eps);
   }

@@ -3,6 +3,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "sdk_host.hpp"
 
 namespace sdk {
@@ -117,11 +119,25 @@ __device__ __forceinline__ float over_wave(float x) {
   return x;
 }
 
-// Over the LANES (a power of two up to 64) consecutive lanes of a group that starts at a multiple of LANES.
-template <typename Op, int LANES>
-__device__ __forceinline__ float over_lanes(float x) {
-#pragma unroll
-  for (int d = LANES / 2; d > 0; d >>= 1) x = Op::of(x, __shfl_xor(x, d));
+// The sum over the LANES (4 to 64) consecutive lanes of a group that starts at a multiple of LANES, in every one of them:
+// exchanges within the vector unit, without LDS.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float x) {
+  const auto moved = [](float v, auto control) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(control)::value, 0xf, 0xf, false));
+  };
+  x += moved(x, std::integral_constant<int, 0xb1>());                        // lanes 1 0 3 2
+  x += moved(x, std::integral_constant<int, 0x4e>());                        // 2 3 0 1
+  if constexpr (LANES >= 8) x += moved(x, std::integral_constant<int, 0x141>());    // eight lanes turned
+  if constexpr (LANES >= 16) x += moved(x, std::integral_constant<int, 0x140>());   // sixteen lanes turned
+  if constexpr (LANES >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+    x = __int_as_float(r[0]) + __int_as_float(r[1]);
+  }
+  if constexpr (LANES >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    x = __int_as_float(r[0]) + __int_as_float(r[1]);
+  }
   return x;
 }
 
