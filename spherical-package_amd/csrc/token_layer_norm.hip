@@ -377,7 +377,7 @@ void run_forward(const T* x, const T* residual, const void* weight, const void* 
 
 int64_t backward_groups(int64_t rows, int64_t width) {
   const int threads = threads_of(width), share = threads < 256 ? 256 / threads : 1;
-  const int64_t groups = threads > 256 ? 512 : 1024;
+  const int64_t groups = threads > 512 ? 256 : threads > 256 ? 512 : 1024;
   return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, share), groups));
 }
 

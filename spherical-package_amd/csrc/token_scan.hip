@@ -20,6 +20,7 @@
 // The state, its gradient, the spans and the gates are float32.  u weighs the distance x - h: 1 - f of a rounded f near one
 // would be off by a part of all that a long memory sums up.
 #include <algorithm>
+#include <type_traits>
 
 #include "token_types.hpp"
 
@@ -49,25 +50,20 @@ struct Scan {
   int reverse;
 };
 
-// u = 1 - sigmoid(g) = 1 / (1 + e^g) and f = sigmoid(g) = e^g u.  Both keep their relative precision wherever they are
-// small; e^g stops at 2^126, NaN passes.  FINE: to a few units of the last place (the power's argument in two parts, a
-// correction of the reciprocal); 16-bit gates, whose results round to 16 bits, do without (5e-7 of u at gates of 8).
+// u = 1 - sigmoid(g) = 1 / (1 + e^g), to its relative precision also where it is small; f is only ever formed as c - c u.
+// FINE: to a few units of the last place (the power's argument in two parts, a correction of the reciprocal); 16-bit gates,
+// whose results round to 16 bits, do without (5e-7 of u at gates of 8).
 template <bool FINE>
-__device__ __forceinline__ void gates(float g, float& f, float& u) {
+__device__ __forceinline__ float unkept(float g) {
   constexpr float kLog2e = 1.44269502e+00f, kLog2eRest = 1.92596303e-08f, kLn2 = 6.93147182e-01f;
-  float t = g * kLog2e;
-  const bool large = t > 126.f;
-  t = large ? 126.f : t;
+  const float t = g * kLog2e;
   float e = __builtin_amdgcn_exp2f(t);
-  if constexpr (FINE) {
-    // t below -150 gives zero, whatever its rest (an infinity's is no number)
-    const float rest = fmaf(g, kLog2eRest, fmaf(g, kLog2e, -t));
-    if (fabsf(t) < 126.f) e = fmaf(e * rest, kLn2, e);
-  }
-  const float d = 1.f + e;
-  u = __builtin_amdgcn_rcpf(d);
-  if constexpr (FINE) u = large ? u : fmaf(fmaf(-d, u, 1.f), u, u);
-  f = e * u;
+  if constexpr (!FINE) return __builtin_amdgcn_rcpf(1.f + e);
+  const bool middle = fabsf(t) < 126.f;   // beyond it u is e^-g or 1 (or NaN), and corrections would be no numbers
+  const float rest = fmaf(g, kLog2eRest, fmaf(g, kLog2e, -t));
+  if (middle) e = fmaf(e * rest, kLn2, e);
+  const float d = 1.f + e, u = __builtin_amdgcn_rcpf(d);
+  return middle ? fmaf(fmaf(-d, u, 1.f), u, u) : u;
 }
 
 // h -> a h + b, for each of V channels
@@ -171,7 +167,7 @@ __device__ __forceinline__ void load_state(const float* p, int64_t at, float (&f
 }
 
 // ROWS tokens of a thread in the order of the walk, as they lie in memory, and what the walk does with them.  Forward they
-// are at, at + 1, ..; backward at, at - 1, ..
+// are at, at + 1, ..; backward at, at - 1, ..  FULL: all of the workgroup's tokens and channels count.
 template <typename T, int LANES, bool ALIGNED, bool BACKWARD, int ROWS>
 struct Walk {
   static constexpr int V = kWide<T>;
@@ -181,27 +177,32 @@ struct Walk {
   Pack<T, V> x[ROWS], g[BACKWARD ? ROWS : 1], h[BACKWARD ? ROWS : 1];
   bool inside[ROWS], counts[ROWS];
 
+  template <bool FULL>
   __device__ __forceinline__ void load(const Scan& p, const Place<T, LANES>& place, int64_t at) {
-    const T* px = (const T*)p.x + place.b * p.x_strides[0] + place.channel;
-    const T* pgate = (const T*)p.gate + place.b * p.gate_strides[0] + place.channel;
-    const T* pgrad = (const T*)p.grad + place.b * p.grad_strides[0] + place.channel;
-    const T* ph = (const T*)p.out + place.b * p.tokens * p.width + place.channel;
+    // the thread's first token in memory, and the way from there to its others
+    const int64_t row = place.row(p, at), way = (p.reverse != 0) != BACKWARD ? -1 : 1;
+    const int64_t x_way = way * p.x_strides[1], gate_way = way * p.gate_strides[1], grad_way = way * p.grad_strides[1],
+                  h_way = way * p.width;
+    const T* px = (const T*)p.x + place.b * p.x_strides[0] + place.channel + row * p.x_strides[1];
+    const T* pgate = (const T*)p.gate + place.b * p.gate_strides[0] + place.channel + row * p.gate_strides[1];
+    const T* pgrad = (const T*)p.grad + place.b * p.grad_strides[0] + place.channel + row * p.grad_strides[1];
+    const T* ph = (const T*)p.out + (place.b * p.tokens + row) * p.width + place.channel;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int64_t t = at + STEP * r;
-      inside[r] = t >= place.from && t < place.to && place.left > 0;
-      counts[r] = inside[r] && place.counts(t);
+      inside[r] = FULL || (t >= place.from && t < place.to && place.left > 0);
+      counts[r] = FULL || (inside[r] && place.counts(t));
       if constexpr (BACKWARD) {
 #pragma unroll
         for (int e = 0; e < V; ++e) g[r].v[e] = (T)0.f;
       }
       if (counts[r]) {
-        const int64_t row = place.row(p, t);
-        get<T, V, ALIGNED>(pgate + row * p.gate_strides[1], u[r], place.left);
-        get_raw<T, V, ALIGNED>(px + row * p.x_strides[1], x[r], place.left);
+        get<T, V, ALIGNED>(pgate + r * gate_way, u[r], place.left);
+        get_raw<T, V, ALIGNED>(px + r * x_way, x[r], place.left);
         if constexpr (BACKWARD) {
-          if (p.grad) get_raw<T, V, ALIGNED>(pgrad + row * p.grad_strides[1], g[r], place.left);
-          if (t > place.first_token) get_raw<T, V, ALIGNED>(ph + place.row(p, t - 1) * p.width, h[r], place.left);
+          if (p.grad) get_raw<T, V, ALIGNED>(pgrad + r * grad_way, g[r], place.left);
+          // the token before: backward that is the thread's next
+          if (t > place.first_token) get_raw<T, V, ALIGNED>(ph + (r + 1) * h_way, h[r], place.left);
         }
       }
     }
@@ -212,23 +213,21 @@ struct Walk {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float f;
-        if (counts[r]) gates<FINE>(u[r][e], f, u[r][e]);
-      }
+      for (int e = 0; e < V; ++e)
+        if (counts[r]) u[r][e] = unkept<FINE>(u[r][e]);
   }
 
   // The same, and what the tokens do to the state in front of them.
+  template <bool FULL>
   __device__ __forceinline__ Span<V> span() {
     Span<V> s;
     unit(s);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (counts[r]) {
+      if (FULL || counts[r]) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          float f;
-          gates<FINE>(u[r][e], f, u[r][e]);
+          u[r][e] = unkept<FINE>(u[r][e]);
           if constexpr (BACKWARD) {
             const float c = (float)g[r].v[e] + s.b[e];
             s.b[e] = fmaf(-u[r][e], c, c);
@@ -242,12 +241,14 @@ struct Walk {
   }
 
   // The results of the tokens, given the state in front of them.
+  template <bool FULL>
   __device__ __forceinline__ void finish(const Scan& p, const Place<T, LANES>& place, int64_t at, float (&in)[V]) {
-    const int64_t begin = place.b * p.tokens * p.width + place.channel;
+    const int64_t way = ((p.reverse != 0) != BACKWARD ? -1 : 1) * p.width;
+    const int64_t begin = (place.b * p.tokens + place.row(p, at)) * p.width + place.channel;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      if (!inside[r]) continue;
-      const int64_t row = begin + place.row(p, at + STEP * r) * p.width;
+      if (!FULL && !inside[r]) continue;
+      const int64_t row = begin + r * way;
       float y[V], z[V], before[V];
       if constexpr (BACKWARD) {
 #pragma unroll
@@ -259,13 +260,13 @@ struct Walk {
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        y[e] = z[e] = 0.f;
-        if (counts[r]) {
+        if (!FULL) y[e] = z[e] = 0.f;
+        if (FULL || counts[r]) {
           if constexpr (BACKWARD) {
             const float c = (float)g[r].v[e] + in[e];
             in[e] = fmaf(-u[r][e], c, c);
             y[e] = c * u[r][e];
-            z[e] = (c - y[e]) * u[r][e] * (before[e] - (float)x[r].v[e]);
+            z[e] = in[e] * u[r][e] * (before[e] - (float)x[r].v[e]);
           } else {
             y[e] = in[e] = fmaf(u[r][e], (float)x[r].v[e] - in[e], in[e]);
           }
@@ -280,6 +281,15 @@ struct Walk {
     }
   }
 };
+
+// Whether all of `count` tokens from `first` on and all channels of the workgroup's block count.
+template <typename T, int LANES, bool ALIGNED>
+__device__ __forceinline__ bool is_full(const Scan& p, const Place<T, LANES>& place, int64_t first, int64_t count) {
+  const int block_end = (place.channel / (LANES * kWide<T>) + 1) * LANES * kWide<T>;
+  return ALIGNED && __builtin_amdgcn_readfirstlane(first >= place.from && first >= place.first_token &&
+                                                   first + count <= place.to && first + count <= place.after_last &&
+                                                   block_end <= p.width);
+}
 
 template <bool BACKWARD>
 __device__ __forceinline__ const float* first_state(const Scan& p) { return BACKWARD ? p.grad_last : p.state; }
@@ -306,13 +316,20 @@ __global__ __launch_bounds__(kThreads) void scan_whole(const Scan p) {
   for (int64_t i = 0; i < tiles; ++i) {
     const int64_t at = BACKWARD ? (tiles - i) * TILE - 1 - place.time * ROWS : i * TILE + place.time * ROWS;
     Walk<T, LANES, ALIGNED, BACKWARD, ROWS> walk;
-    walk.load(p, place, at);
-    Span<V> s = walk.span();
-    float in[V];
-    over_waves<V, LANES, WAVES>(s, slots[i & 1]);
-    __syncthreads();
-    from_waves<V, LANES, WAVES>(s, carry, in, slots[i & 1]);
-    walk.finish(p, place, at, in);
+    auto tile = [&](auto full) {
+      constexpr bool FULL = decltype(full)::value;
+      walk.template load<FULL>(p, place, at);
+      Span<V> s = walk.template span<FULL>();
+      float in[V];
+      over_waves<V, LANES, WAVES>(s, slots[i & 1]);
+      __syncthreads();
+      from_waves<V, LANES, WAVES>(s, carry, in, slots[i & 1]);
+      walk.template finish<FULL>(p, place, at, in);
+    };
+    if (is_full<T, LANES, ALIGNED>(p, place, (BACKWARD ? tiles - 1 - i : i) * TILE, TILE))
+      tile(std::true_type());
+    else
+      tile(std::false_type());
   }
   store_last<T, LANES, BACKWARD>(p, place, carry);
 }
@@ -329,9 +346,9 @@ __global__ __launch_bounds__(kThreads) void scan_short(const Scan p) {
   for (int64_t i = 0; i < p.tokens; i += ROWS) {
     const int64_t at = BACKWARD ? p.tokens - 1 - i : i;
     Walk<T, 1, ALIGNED, BACKWARD, ROWS> walk;
-    walk.load(p, place, at);
+    walk.template load<false>(p, place, at);
     walk.open();
-    walk.finish(p, place, at, carry);
+    walk.template finish<false>(p, place, at, carry);
   }
   store_last<T, 1, BACKWARD>(p, place, carry);
 }
@@ -376,8 +393,15 @@ __global__ __launch_bounds__(kWaiting, 4) void scan_tiles(const Scan p) {
   const Place<T, LANES> place(p, id, BACKWARD ? p.segments - 1 - turn : turn);
   const int64_t at = BACKWARD ? place.from + p.segment - 1 - place.time * ROWS : place.from + place.time * ROWS;
   Walk<T, LANES, ALIGNED, BACKWARD, ROWS> walk;
-  walk.load(p, place, at);
-  Span<V> s = walk.span();
+  const bool full = is_full<T, LANES, ALIGNED>(p, place, place.from, p.segment);
+  Span<V> s;
+  if (full) {
+    walk.template load<true>(p, place, at);
+    s = walk.template span<true>();
+  } else {
+    walk.template load<false>(p, place, at);
+    s = walk.template span<false>();
+  }
   over_waves<V, LANES, WAVES>(s, slots);
   __syncthreads();
 
@@ -452,7 +476,10 @@ __global__ __launch_bounds__(kWaiting, 4) void scan_tiles(const Scan p) {
   float in[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) in[e] = fmaf(s.a[e], entry[threadIdx.x >> 6][threadIdx.x % LANES * V + e], s.b[e]);
-  walk.finish(p, place, at, in);
+  if (full)
+    walk.template finish<true>(p, place, at, in);
+  else
+    walk.template finish<false>(p, place, at, in);
 }
 
 // No tokens: the state, or its gradient, passes through.
@@ -476,9 +503,7 @@ __global__ __launch_bounds__(256) void scan_step(const T* x, int64_t x_stride, c
   load_part<float, V>(state + b * state_stride + c, h, left);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    float f, u;
-    gates<sizeof(T) == 4>(fg[e], f, u);
-    h[e] = fmaf(u, fx[e] - h[e], h[e]);
+    h[e] = fmaf(unkept<sizeof(T) == 4>(fg[e]), fx[e] - h[e], h[e]);
   }
   store_part<float, V>(state + b * state_stride + c, h, left);
   put<T, V, ALIGNED>(out + b * width + c, h, left);
