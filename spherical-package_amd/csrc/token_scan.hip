@@ -301,13 +301,13 @@ __device__ __forceinline__ void store_last(const Scan& p, const Place<T, LANES>&
 }
 
 // Tokens of a tile that a thread walks: a backward holds four tensors' values of each, a forward two.
-template <bool BACKWARD>
-constexpr int kRows = BACKWARD ? 2 : 4;
+template <bool BACKWARD, int V>
+constexpr int kRows = (BACKWARD ? 16 : 32) / V;
 
 // Whole sequences, tile by tile: a workgroup a batch element and block of channels.
 template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
 __global__ __launch_bounds__(kThreads) void scan_whole(const Scan p) {
-  constexpr int V = kWide<T>, WAVES = kThreads / 64, ROWS = kRows<BACKWARD>, TILE = kThreads / LANES * ROWS;
+  constexpr int V = kWide<T>, WAVES = kThreads / 64, ROWS = kRows<BACKWARD, V>, TILE = kThreads / LANES * ROWS;
   __shared__ float slots[2][2 * WAVES * LANES * V];
   const Place<T, LANES> place(p, blockIdx.x, 0);
   float carry[V];
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kThreads) void scan_whole(const Scan p) {
 // Short sequences: a thread takes 16 bytes of channels through all tokens.
 template <typename T, bool ALIGNED, bool BACKWARD>
 __global__ __launch_bounds__(kThreads) void scan_short(const Scan p) {
-  constexpr int V = kWide<T>, ROWS = kRows<BACKWARD>;
+  constexpr int V = kWide<T>, ROWS = kRows<BACKWARD, V>;
   const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (id >= (int64_t)p.batches * ((p.width + V - 1) / V)) return;
   const Place<T, 1> place(p, id);
@@ -381,7 +381,7 @@ constexpr int kLook = 4;
 
 template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
 __global__ __launch_bounds__(kWaiting, 4) void scan_tiles(const Scan p) {
-  constexpr int ROWS = kRows<BACKWARD>, V = kWide<T>, WAVES = kWaiting / 64, C = LANES * V, SLOTS = kWaiting / C;
+  constexpr int V = kWide<T>, ROWS = kRows<BACKWARD, V>, WAVES = kWaiting / 64, C = LANES * V, SLOTS = kWaiting / C;
   __shared__ float slots[2 * WAVES * C], looked[2][SLOTS][C], entry[WAVES][C];
   __shared__ unsigned ticket;
   const unsigned groups = (unsigned)p.batches * p.blocks, id = blockIdx.x % groups;
@@ -523,7 +523,8 @@ bool is_short(int64_t batch, int64_t tokens, int64_t vectors) {
 }
 int64_t segment_of(int64_t batch, int64_t tokens, int64_t width, int dtype, bool backward) {
   const int wide = dtype == SDK_F32 ? 4 : 8, lanes = lanes_of(width, wide);
-  const int64_t groups = batch * ceil_div(width, lanes * wide), tile = kWaiting / lanes * (backward ? kRows<true> : kRows<false>);
+  const int64_t groups = batch * ceil_div(width, lanes * wide), rows = (backward ? kRows<true, 1> : kRows<false, 1>) / wide;
+  const int64_t tile = kWaiting / lanes * rows;
   return groups >= kFill || tokens <= tile || groups * ceil_div(tokens, tile) > most_groups(kWaiting) ? tokens : tile;
 }
 
