@@ -897,11 +897,13 @@ int sdk_add_layer_norm(const void* x, const void* residual, const void* weight, 
                        void* summed, float* mean, float* inverse, int64_t rows, int64_t width, double eps,
                        int32_t dtype, int32_t weight_dtype, sdk_stream_t stream);
 /* grad_x (the gradient of x and of residual): that of `grad` through the norm plus grad_sum (may be NULL).
- * Gradients that are NULL are not formed; the workspace is needed for those of weight and bias. */
+ * x and residual (NULL: none) as the forward got them, or its summed and NULL: one read less, and with 16-bit types
+ * gradients off by the rounding of the sum.  Gradients that are NULL are not formed; the workspace is needed for those
+ * of weight and bias. */
 size_t sdk_add_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width);
-int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const void* summed, const void* weight,
-                                const float* mean, const float* inverse, void* grad_x, void* grad_weight,
-                                void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t width,
+int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const void* x, const void* residual,
+                                const void* weight, const float* mean, const float* inverse, void* grad_x,
+                                void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t width,
                                 int32_t dtype, int32_t weight_dtype, sdk_stream_t stream);
 
 /* Gated linear recurrence along the tokens, each channel by itself:

@@ -113,7 +113,7 @@ SIGNATURES = {
     "sdk_adamw_step_8bit": [_vp] * 7 + _step_settings,
     "sdk_adamw_moment_values": [_vp] * 3 + [_i64] + [_i32] * 2 + [_vp],
     "sdk_add_layer_norm": [_vp] * 8 + [_i64] * 2 + [ctypes.c_double] + [_i32] * 2 + [_vp],
-    "sdk_add_layer_norm_backward": [_vp] * 10 + [_sz] + [_i64] * 2 + [_i32] * 2 + [_vp],
+    "sdk_add_layer_norm_backward": [_vp] * 11 + [_sz] + [_i64] * 2 + [_i32] * 2 + [_vp],
     "sdk_gated_scan_forward": [_scan, _vp, _sz, _vp],
     "sdk_gated_scan_backward": [_scan, _vp, _sz, _vp],
     "sdk_gated_scan_step": [_vp, _i64, _vp, _i64, _vp, _i64, _vp] + [_i64] * 2 + [_i32, _vp],

@@ -362,33 +362,34 @@ def add_layer_norm(x, residual, weight, bias, eps):
     return out, summed, mean, inverse
 
 
-def add_layer_norm_backward(grad, grad_sum, summed, weight, mean, inverse, need_x, need_weight, need_bias):
-    """-> (gradient of x and of residual, of weight, of bias); those not asked for are empty tensors."""
-    _check_norm(summed, None, weight)
-    _on_gpu(summed, grad=grad, grad_sum=grad_sum, mean=mean, inverse=inverse)
+def add_layer_norm_backward(grad, grad_sum, x, residual, weight, mean, inverse, need_x, need_weight, need_bias):
+    """-> (gradient of x and of residual, of weight, of bias); those not asked for are empty tensors.  x and residual as
+    the forward got them, or its sum alone (one read less; 16-bit gradients are then off by the sum's rounding)."""
+    _check_norm(x, residual, weight)
+    _on_gpu(x, grad=grad, grad_sum=grad_sum, mean=mean, inverse=inverse)
     for name, t in (("grad", grad), ("grad_sum", grad_sum)):
-        if t is not None and (t.shape != summed.shape or t.dtype != summed.dtype):
-            raise RuntimeError("%s must be like the sums: %s %s, got %s %s"
-                               % (name, tuple(summed.shape), summed.dtype, tuple(t.shape), t.dtype))
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise RuntimeError("%s must be like x: %s %s, got %s %s"
+                               % (name, tuple(x.shape), x.dtype, tuple(t.shape), t.dtype))
     _dense(grad=grad, grad_sum=grad_sum, mean=mean, inverse=inverse)
-    width = summed.shape[-1]
-    rows = summed.numel() // width
+    width = x.shape[-1]
+    rows = x.numel() // width
     for t in (mean, inverse):
         if t.dtype != torch.float32 or t.numel() != rows:
             raise RuntimeError("mean and inverse must be float32 with one value for each row")
-    dx = torch.empty_like(summed) if need_x else summed.new_empty(0)
+    dx = torch.empty_like(x) if need_x else x.new_empty(0)
     dw, db = (torch.empty_like(weight) if need else weight.new_empty(0) for need in (need_weight, need_bias))
     if not need_x and not need_weight and not need_bias:
         return dx, dw, db
-    with torch.cuda.device(summed.device):
+    with torch.cuda.device(x.device):
         need = 0
         if need_weight or need_bias:
             need = _capi.load().sdk_add_layer_norm_backward_workspace_bytes(rows, width)
-        ws = torch.empty(need, dtype=torch.uint8, device=summed.device) if need else None
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         _capi.call("sdk_add_layer_norm_backward",
-                   *(_ops._ptr(t) for t in (grad, grad_sum, summed, weight, mean, inverse, dx if need_x else None,
+                   *(_ops._ptr(t) for t in (grad, grad_sum, x, residual, weight, mean, inverse, dx if need_x else None,
                                             dw if need_weight else None, db if need_bias else None, ws)), need,
-                   rows, width, _DTYPES[summed.dtype], _DTYPES[weight.dtype], _ops._stream(summed))
+                   rows, width, _DTYPES[x.dtype], _DTYPES[weight.dtype], _ops._stream(x))
     return dx, dw, db
 
 
@@ -613,8 +614,8 @@ _SCHEMAS = (
      "(Tensor x, Tensor? residual, Tensor weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor, Tensor)",
      add_layer_norm),
     ("add_layer_norm_backward",
-     "(Tensor grad, Tensor? grad_sum, Tensor summed, Tensor weight, Tensor mean, Tensor inverse, bool need_x,"
-     " bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)", add_layer_norm_backward),
+     "(Tensor grad, Tensor? grad_sum, Tensor x, Tensor? residual, Tensor weight, Tensor mean, Tensor inverse,"
+     " bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)", add_layer_norm_backward),
     ("gated_scan", "(Tensor x, Tensor gate, Tensor? state, Tensor? lengths, bool reverse) -> Tensor[]", gated_scan),
     ("gated_scan_forward", "(Tensor x, Tensor gate, Tensor? state, Tensor? lengths, bool reverse) -> (Tensor, Tensor)",
      gated_scan_forward),

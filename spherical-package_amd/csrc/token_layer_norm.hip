@@ -6,9 +6,10 @@
 //   dw_j = sum over rows of g_j z_j,  db_j = sum over rows of g_j
 //
 // Bound by memory: a row is read once and held in registers, where the mean is formed first and the squares of the
-// distances from it after (their difference from sums of squares would lose a mean's square).  Sums are float32.  The
-// forward normalises the sum before it is rounded to the tensors' type; the backward reads the rounded h, which the
-// forward wrote.
+// distances from it after (their difference from sums of squares would lose a mean's square).  Sums are float32, and h is
+// normalised before it is rounded to the tensors' type, in the backward too: there it is formed again from x and r.  h as
+// the forward wrote it would be one read less (42 us for 46.7, 32768 rows of 768 bfloat16 values), but dw then carries h's
+// rounding beside its own (2.5e-3 of its size for 1.8e-3).  In float32 that does not show, and h is read.
 #include <algorithm>
 
 #include "token_types.hpp"
@@ -180,8 +181,8 @@ __global__ __launch_bounds__(kGroup<THREADS>) void layer_forward(const T* x, con
 // Workgroup b takes rows b, b + gridDim.x, ... (times the rows that share a workgroup) and keeps its parts of dw and db
 // in registers; the parts [group][dw, db][width] are joined in their order by join_parts.
 template <typename T, int THREADS, bool ALIGNED>
-__global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad, const T* grad_sum, const T* h_in,
-                                                                  const void* weight, int weight_float,
+__global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad, const T* grad_sum, const T* x,
+                                                                  const T* residual, const void* weight, int weight_float,
                                                                   const float* mean, const float* inverse, T* grad_x,
                                                                   float* parts, int64_t rows, int width) {
   constexpr int V = kWide<T>, N = kChunks<T>, SHARE = kGroup<THREADS> / THREADS;
@@ -195,11 +196,11 @@ __global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad,
     for (int e = 0; e < V; ++e) w[k][e] = dw[k][e] = db[k][e] = 0.f;
     if (j < width) load_weight<T, V, ALIGNED>(weight, weight_float, j, w[k], width - j);
   }
-  // a row as it lies in memory; the next one is requested while this one is worked on (75 us without that for 43, 32768
+  // a row as it lies in memory; the next one is requested while this one is worked on (75 us without that for 42 when h was read, 32768
   // rows of 768 bfloat16 values), but for 1024 threads, whose registers do not hold two
   constexpr bool AHEAD = THREADS < 1024;
   struct Row {
-    Words h[N], g[N], s[N];
+    Words h[N], r[N], g[N], s[N];
     float mu, inv;
     bool live;
   };
@@ -212,9 +213,10 @@ __global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad,
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int j = (k * THREADS + t) * V;
-      r.h[k] = r.g[k] = r.s[k] = Words{0, 0, 0, 0};
+      r.h[k] = r.r[k] = r.g[k] = r.s[k] = Words{0, 0, 0, 0};
       if (r.live && j < width) {
-        r.h[k] = row_get<T, V, ALIGNED>(h_in + base + j, width - j, more);
+        r.h[k] = row_get<T, V, ALIGNED>(x + base + j, width - j, more);
+        if (residual) r.r[k] = row_get<T, V, ALIGNED>(residual + base + j, width - j, more);
         r.g[k] = row_get<T, V, ALIGNED>(grad + base + j, width - j, more);
         if (grad_sum) r.s[k] = row_get<T, V, ALIGNED>(grad_sum + base + j, width - j, more);
       }
@@ -235,11 +237,13 @@ __global__ __launch_bounds__(kGroup<THREADS>) void layer_backward(const T* grad,
     for (int k = 0; k < N; ++k) {
       // beyond the row's end q and w are zeros: z counts nowhere
       const int left = width - (k * THREADS + t) * V;
+      float r[V];
       in_row<T, V, ALIGNED>(now.h[k], z[k], left);
+      in_row<T, V, ALIGNED>(now.r[k], r, left);
       in_row<T, V, ALIGNED>(now.g[k], q[k], left);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        z[k][e] = (z[k][e] - now.mu) * now.inv;
+        z[k][e] = ((z[k][e] + r[e]) - now.mu) * now.inv;
         dw[k][e] += q[k][e] * z[k][e];
         db[k][e] += q[k][e];
         q[k][e] *= w[k][e];
@@ -423,13 +427,13 @@ size_t sdk_add_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width) 
   return (size_t)backward_groups(rows, width) * 2 * width * sizeof(float);
 }
 
-int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const void* summed, const void* weight,
-                                const float* mean, const float* inverse, void* grad_x, void* grad_weight,
+int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const void* x, const void* residual,
+                                const void* weight, const float* mean, const float* inverse, void* grad_x, void* grad_weight,
                                 void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t width,
                                 int32_t dtype, int32_t weight_dtype, sdk_stream_t stream) {
   if (int rc = check(rows, width, dtype, weight_dtype)) return rc;
   SDK_REQUIRE(weight && (grad_x || grad_weight || grad_bias), "weight and one gradient at least must not be NULL");
-  SDK_REQUIRE(rows == 0 || (grad && summed && mean && inverse), "grad, summed, mean and inverse must not be NULL");
+  SDK_REQUIRE(rows == 0 || (grad && x && mean && inverse), "grad, x, mean and inverse must not be NULL");
   const bool sums = grad_weight || grad_bias;
   const size_t need = sums ? sdk_add_layer_norm_backward_workspace_bytes(rows, width) : 0;
   if (need && (!workspace || workspace_bytes < need))
@@ -438,11 +442,11 @@ int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const vo
   const int64_t groups = rows ? backward_groups(rows, width) : 0;
   float* parts = sums ? (float*)workspace : nullptr;
   SDK_DISPATCH_TOKEN_DTYPE(dtype, {
-    const bool wide = width % kWide<T> == 0 && aligned16(grad) && aligned16(grad_sum) && aligned16(summed) &&
-                      aligned16(weight) && aligned16(grad_x);
+    const bool wide = width % kWide<T> == 0 && aligned16(grad) && aligned16(grad_sum) && aligned16(x) &&
+                      aligned16(residual) && aligned16(weight) && aligned16(grad_x);
     if (rows)
       LAYER_SHAPE(launch(layer_backward<T, THREADS, ALIGNED>, dim3((unsigned)groups), dim3(kGroup<THREADS>), s,
-                         (const T*)grad, (const T*)grad_sum, (const T*)summed, weight,
+                         (const T*)grad, (const T*)grad_sum, (const T*)x, (const T*)residual, weight,
                          (int)(weight_dtype == SDK_F32), mean, inverse, (T*)grad_x, parts, rows, (int)width));
     if (sums)
       launch(join_parts<T>, dim3((unsigned)ceil_div(2 * width, 64)), dim3(1024), s, (const float*)parts, groups,

@@ -322,33 +322,33 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> add_layer_norm(const Tensor& x, const
 }
 
 std::tuple<Tensor, Tensor, Tensor> add_layer_norm_backward(const Tensor& grad, const OptTensor& grad_sum,
-                                                           const Tensor& summed, const Tensor& weight,
+                                                           const Tensor& x, const OptTensor& residual, const Tensor& weight,
                                                            const Tensor& mean, const Tensor& inverse, bool need_x,
                                                            bool need_weight, bool need_bias) {
-  check_norm(summed, OptTensor(), weight);
-  beside(summed, "grad", grad), beside(summed, "grad_sum", grad_sum);
-  beside(summed, "mean", mean), beside(summed, "inverse", inverse);
+  check_norm(x, residual, weight);
+  beside(x, "grad", grad), beside(x, "grad_sum", grad_sum);
+  beside(x, "mean", mean), beside(x, "inverse", inverse);
   for (const auto& t : {std::pair<const char*, OptTensor>{"grad", grad}, {"grad_sum", grad_sum}})
     if (has(t.second))
-      TORCH_CHECK(t.second->sizes() == summed.sizes() && t.second->scalar_type() == summed.scalar_type(), t.first,
-                  " must be like the sums: ", summed.sizes(), " ", summed.scalar_type(), ", got ", t.second->sizes(),
+      TORCH_CHECK(t.second->sizes() == x.sizes() && t.second->scalar_type() == x.scalar_type(), t.first,
+                  " must be like x: ", x.sizes(), " ", x.scalar_type(), ", got ", t.second->sizes(),
                   " ", t.second->scalar_type());
   dense("grad", grad), dense("grad_sum", grad_sum), dense("mean", mean), dense("inverse", inverse);
-  const int64_t width = summed.size(-1), rows = summed.numel() / width;
+  const int64_t width = x.size(-1), rows = x.numel() / width;
   for (const Tensor& t : {mean, inverse})
     TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == rows,
                 "mean and inverse must be float32 with one value for each row");
-  c10::DeviceGuard guard(summed.device());
-  Tensor dx = need_x ? at::empty_like(summed) : nothing(summed);
+  c10::DeviceGuard guard(x.device());
+  Tensor dx = need_x ? at::empty_like(x) : nothing(x);
   Tensor dw = need_weight ? at::empty_like(weight) : nothing(weight);
   Tensor db = need_bias ? at::empty_like(weight) : nothing(weight);
   if (!need_x && !need_weight && !need_bias) return {dx, dw, db};
   const size_t need = need_weight || need_bias ? sdk_add_layer_norm_backward_workspace_bytes(rows, width) : 0;
-  Tensor ws = workspace(summed, need);
-  TOKEN_CALL(sdk_add_layer_norm_backward, ptr(grad), ptr(grad_sum), ptr(summed), ptr(weight), (const float*)ptr(mean),
+  Tensor ws = workspace(x, need);
+  TOKEN_CALL(sdk_add_layer_norm_backward, ptr(grad), ptr(grad_sum), ptr(x), ptr(residual), ptr(weight), (const float*)ptr(mean),
              (const float*)ptr(inverse), need_x ? ptr(dx) : nullptr, need_weight ? ptr(dw) : nullptr,
              need_bias ? ptr(db) : nullptr, need ? ptr(ws) : nullptr, need, rows, width,
-             dtype_of(summed.scalar_type(), "summed"), dtype_of(weight.scalar_type(), "weight"), stream_of(summed));
+             dtype_of(x.scalar_type(), "x"), dtype_of(weight.scalar_type(), "weight"), stream_of(x));
   return {dx, dw, db};
 }
 
@@ -717,7 +717,9 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
     auto [out, summed, mean, inverse] = add_layer_norm(x, residual, weight, bias, eps);
     ctx->saved_data["alone"] = alone;
     ctx->saved_data["bias"] = has(bias);
-    ctx->save_for_backward({alone ? x : summed, weight, mean, inverse});
+    // 16-bit sums would bring their rounding into the gradients
+    const bool sum = !alone && x.scalar_type() == at::kFloat;
+    ctx->save_for_backward({sum ? summed : x, alone || sum ? Tensor() : *residual, weight, mean, inverse});
     ctx->set_materialize_grads(false);
     return alone ? variable_list{out} : variable_list{out, summed};
   }
@@ -730,11 +732,12 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
     const Tensor sum = grads.size() > 1 ? grads[1] : Tensor();
     at::AutoDispatchBelowADInplaceOrView guard;
     if (!grads[0].defined())   // only the sum was used, or nothing
-      return {need_x ? sum : Tensor(), need_w ? at::zeros_like(saved[1]) : Tensor(), need_r ? sum : Tensor(),
-              need_b ? at::zeros_like(saved[1]) : Tensor(), Tensor()};
+      return {need_x ? sum : Tensor(), need_w ? at::zeros_like(saved[2]) : Tensor(), need_r ? sum : Tensor(),
+              need_b ? at::zeros_like(saved[2]) : Tensor(), Tensor()};
     auto [dx, dw, db] = add_layer_norm_backward(
-        grads[0].contiguous(), sum.defined() ? OptTensor(sum.contiguous()) : OptTensor(), saved[0], saved[1], saved[2],
-        saved[3], need_x || need_r, need_w, need_b);
+        grads[0].contiguous(), sum.defined() ? OptTensor(sum.contiguous()) : OptTensor(), saved[0],
+        saved[1].defined() ? OptTensor(saved[1]) : OptTensor(), saved[2], saved[3], saved[4], need_x || need_r, need_w,
+        need_b);
     return {need_x ? dx : Tensor(), need_w ? dw : Tensor(), need_r ? dx : Tensor(), need_b ? db : Tensor(), Tensor()};
   }
 };

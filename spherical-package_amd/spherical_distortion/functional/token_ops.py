@@ -150,7 +150,9 @@ class AddLayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps):
         out, summed, mean, inverse = _sdk_ops.add_layer_norm(x, residual, weight, bias, eps)
-        ctx.save_for_backward(x if residual is None else summed, weight, mean, inverse)
+        # 16-bit sums would bring their rounding into the gradients
+        rows = (summed, None) if residual is not None and x.dtype == torch.float32 else (x, residual)
+        ctx.save_for_backward(*rows, weight, mean, inverse)
         ctx.alone = residual is None
         ctx.set_materialize_grads(False)
         return (out, x.view_as(x)) if ctx.alone else (out, summed)
@@ -158,13 +160,13 @@ class AddLayerNormFunction(torch.autograd.Function):
     @staticmethod
     @_only_first
     def backward(ctx, grad, grad_sum):
-        summed, weight, mean, inverse = ctx.saved_tensors
+        x, residual, weight, mean, inverse = ctx.saved_tensors
         need_x, need_r, need_w, need_b, _ = ctx.needs_input_grad
         if grad is None:   # only the sum was used
             return (grad_sum if need_x else None, grad_sum if need_r else None,
                     torch.zeros_like(weight) if need_w else None, torch.zeros_like(weight) if need_b else None, None)
         dx, dw, db = _sdk_ops.add_layer_norm_backward(
-            grad.contiguous(), None if grad_sum is None else grad_sum.contiguous(), summed, weight, mean, inverse,
+            grad.contiguous(), None if grad_sum is None else grad_sum.contiguous(), x, residual, weight, mean, inverse,
             need_x or need_r, need_w, need_b)
         return (dx if need_x else None, dx if need_r else None, dw if need_w else None, db if need_b else None, None)
 
