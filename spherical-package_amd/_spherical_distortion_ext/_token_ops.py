@@ -515,6 +515,12 @@ def _coefficients(values):
     return (ctypes.c_double * 3)(*values)
 
 
+def check_newton_schulz(steps, coefficients, eps):
+    """Raises where orthogonalize and muon_step would refuse these settings; touches no device."""
+    _capi.call("sdk_orthogonalize", None, None, 0, 0, 0, steps, _coefficients(coefficients), eps, None, 0,
+               _DTYPES[torch.float32], None)
+
+
 def orthogonalize(x, steps, coefficients, eps):
     """-> a dense tensor like x [.., rows, columns]."""
     _on_gpu(x)
@@ -538,6 +544,8 @@ def muon_step(params, grads, momenta, lr, momentum, nesterov, weight_decay, step
     _check_lists(params, {"params": (params, None, None), "grads": (grads, None, None),
                           "momenta": (momenta, torch.float32, None)})
     if not params:
+        if len(grads) or len(momenta):
+            raise RuntimeError("gradients or momenta without params")
         return
     for i, p in enumerate(params):
         if p.dim() < 2:

@@ -11,13 +11,16 @@
 // Operands are float16 times 2^12.  float32 and float16 matrices take two pieces a value, v = hi + lo, and three products
 // hi hi + hi lo + lo hi: 22 bits, 2.5e-7 of the result, below what float32 products leave (2e-6), at a third of the
 // float16 rate where the float32 unit runs at an eighth.  bfloat16 matrices take one piece: 1.3e-3 of the result, beside
-// the 1.7e-3 of its own rounding.  Every singular value stays below about 1.2 on its way with the usual coefficients, so
-// entries of X and S are at most 1.5; up to 15 fit.  Sums are float32, of the norm double.
+// the 1.7e-3 of its own rounding.  Entries of X, S and P have to stay below 16: no entry is larger than the largest singular
+// value, which the coefficients alone bound (check_coefficients).  Sums are float32, of the norm double.
 //
 // All matrices of a call go through a stage in one launch; their table is a kernel argument.  Small ones go through all
 // stages in a workgroup of their own.
 #include <algorithm>
 #include <cmath>
+#include <functional>
+#include <memory>
+#include <new>
 #include <type_traits>
 
 #include "sdk_mfma.hpp"
@@ -944,7 +947,8 @@ void run_group(Table& t, int used, const Settings& s, int steps, char* workspace
   }
 }
 
-// Whether one workgroup takes the matrix: three matrices of 16 x 27 to 64 x 288 in float32, a step of each, 20 us for 85.
+// Whether one workgroup takes the matrix: three matrices of 16 x 27 to 64 x 288 in float32, a step of each, 43 us
+// for 110 through the launches.
 bool is_small(int64_t rows, int64_t columns, int dtype) {
   return std::min(rows, columns) <= 64 && std::max(rows, columns) <= (split(dtype) ? Small<true>::LP : Small<false>::LP);
 }
@@ -986,6 +990,34 @@ int check_matrix(int64_t rows, int64_t columns) {
   return SDK_OK;
 }
 
+// X begins with a norm of 1 at most, and a step makes of a singular value x the value x q(x^2), q(s) = a + b s + c s^2.
+// Followed from 1 on, no value may pass 3.8, so that S stays below 15, and no q of one 15.
+int check_coefficients(int64_t steps, const double* k) {
+  const double a = k[0], b = k[1], c = k[2];
+  auto q = [&](double s) { return std::fabs(a + (b + c * s) * s); };
+  double most = 1;
+  for (int64_t step = 0; step < steps; ++step) {
+    const double end = most * most;
+    double of_q = std::max(q(0), q(end)), next = most * q(end);
+    auto inside = [&](double s, bool of_product) {   // where q's or x q(x^2)'s slope is zero
+      if (!(s > 0 && s < end)) return;
+      if (of_product)
+        next = std::max(next, std::sqrt(s) * q(s));
+      else
+        of_q = std::max(of_q, q(s));
+    };
+    inside(-b / (2 * c), false);   // c = 0: no number, or none inside
+    const double root = 9 * b * b - 20 * a * c;
+    if (root >= 0) inside((-3 * b + std::sqrt(root)) / (10 * c), true), inside((-3 * b - std::sqrt(root)) / (10 * c), true);
+    if (c == 0) inside(-a / (3 * b), true);
+    SDK_REQUIRE(of_q <= 15 && next <= 3.8,
+                "coefficients %g, %g, %g let singular values or the polynomial grow too far (3.8 and 15) in step %lld", a, b, c,
+                (long long)step + 1);
+    most = std::max(1e-30, next);
+  }
+  return SDK_OK;
+}
+
 int check_settings(int64_t count, int64_t steps, const double* coefficients, double eps, int dtype) {
   SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
   SDK_REQUIRE(count >= 0, "count must not be negative");
@@ -994,7 +1026,7 @@ int check_settings(int64_t count, int64_t steps, const double* coefficients, dou
   for (int i = 0; i < 3; ++i)
     SDK_REQUIRE(std::fabs(coefficients[i]) <= 100, "coefficients must be numbers up to 100 in magnitude");
   SDK_REQUIRE(eps >= 0x1p-100 && eps <= 1, "eps = %g must be between 2^-100 and 1", eps);
-  return SDK_OK;
+  return check_coefficients(steps, coefficients);
 }
 
 Settings settings_of(const double* c, double eps) {
@@ -1030,6 +1062,21 @@ struct Lists {
   const int64_t *rows, *columns;
   double lr;
 };
+
+// A parameter or momentum that is in the lists twice would be changed by two workgroups at once.
+int check_once(const Lists& l, int64_t count) {
+  std::unique_ptr<const void*[]> written(new (std::nothrow) const void*[2 * count]);
+  SDK_REQUIRE(written, "no memory for the addresses of %lld matrices", (long long)count);
+  const void** end = written.get();
+  for (int64_t i = 0; i < count; ++i)
+    if (l.rows[i] && l.columns[i]) *end++ = l.p[i], *end++ = l.m[i];
+  std::sort(written.get(), end, std::less<const void*>());
+  SDK_REQUIRE(std::adjacent_find(written.get(), end) == end, "a parameter or momentum is in the lists twice");
+  for (int64_t i = 0; i < count; ++i)
+    SDK_REQUIRE(!l.rows[i] || !l.columns[i] || !std::binary_search(written.get(), end, l.g[i], std::less<const void*>()),
+                "gradient %lld is a parameter or a momentum too", (long long)i);
+  return SDK_OK;
+}
 
 }  // namespace
 }  // namespace token
@@ -1083,15 +1130,19 @@ int sdk_muon_step(void* const* params, const void* const* grads, float* const* m
               "lr and weight_decay must not be negative, momentum in [0, 1)");
   if (!count) return SDK_OK;
   SDK_REQUIRE(params && grads && momenta && rows && columns, "the lists must not be NULL");
+  bool any = false;
   for (int64_t i = 0; i < count; ++i) {
     if (int rc = check_matrix(rows[i], columns[i])) return rc;
-    SDK_REQUIRE(!rows[i] || !columns[i] || (params[i] && grads[i] && momenta[i]), "matrix %lld: a tensor is NULL",
-                (long long)i);
+    if (!rows[i] || !columns[i]) continue;
+    SDK_REQUIRE(params[i] && grads[i] && momenta[i], "matrix %lld: a tensor is NULL", (long long)i);
+    any = true;
   }
+  if (!any) return SDK_OK;
   Settings s = settings_of(coefficients, eps);
   s.mu = (float)momentum, s.rest = (float)(1 - momentum), s.keep = (float)(1 - lr * weight_decay);
   s.nesterov = nesterov != 0;
   const Lists lists = {params, grads, momenta, rows, columns, lr};
+  if (int rc = check_once(lists, count)) return rc;
   const int rc = run_all(count, steps, s, workspace, workspace_bytes, dtype, stream,
                          [](const void* context, int64_t i) {
                            const Lists& l = *(const Lists*)context;

@@ -654,8 +654,8 @@ int sdk_gated_scan_backward(const sdk_gated_scan* a, void* workspace, size_t wor
   if (int rc = check(a)) return rc;
   if (!a->batch || !a->width) return SDK_OK;
   if (!a->tokens) {
-    if (a->grad_state)
-      launch(pass_state, dim3(64), dim3(256), (hipStream_t)stream, a->grad_last, a->grad_state, a->batch * a->width);
+    if (!a->grad_state) return SDK_OK;
+    launch(pass_state, dim3(64), dim3(256), (hipStream_t)stream, a->grad_last, a->grad_state, a->batch * a->width);
     SDK_LAUNCH_CHECK("gated_scan_backward");
     return SDK_OK;
   }

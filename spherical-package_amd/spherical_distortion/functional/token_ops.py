@@ -277,9 +277,9 @@ def orthogonalize(input, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Matrices [.., rows, columns] with their singular values brought towards one by products alone: X = input / (its
     Frobenius norm + eps), then `steps` times X = a X + (b S + c S S) X with S = X X^T of the smaller side.
 
-    float32 and float16 matrices are multiplied with 22 bits a value, bfloat16 with 11; sums are float32.  Singular
-    values have to stay below 3.8 on the way (entries beyond 15 overflow and give NaN), as with the coefficients given
-    here.  eps: 2 ** -100 to 1.  No gradients."""
+    float32 and float16 matrices are multiplied with 22 bits a value, bfloat16 with 11; sums are float32.
+    Coefficients with which a singular value could pass 3.8, or a + b s + c s ** 2 pass 15 (s: its square), within the
+    steps raise.  eps: 2 ** -100 to 1.  No gradients."""
     with torch.no_grad():
         return _sdk_ops.orthogonalize(input, steps, coefficients, eps)
 
@@ -289,7 +289,8 @@ def muon_step(params, grads, momenta, *, lr=2e-2, momentum=0.95, nesterov=True, 
     """One Muon step over lists of parameters, in place and in few launches (64 parameters at a time).
 
     params and grads: float32, bfloat16 or float16, all of one type, two axes at least: [out, ..] counts as a matrix of
-    `out` rows (weights [out, in, taps] of mapped convolutions among them); momenta float32.  No two tensors may overlap.
+    `out` rows (weights [out, in, taps] of mapped convolutions among them); momenta float32.  No two tensors may overlap;
+    one that is in the lists twice raises.
     m = momentum m + (1 - momentum) g;  u = momentum m + (1 - momentum) g with nesterov, else m;
     p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / columns)) orthogonalize(u)."""
     if _no_tensors(params, grads, momenta):

@@ -1,6 +1,8 @@
 """Muon over the framework's kernels: the update of each matrix made orthogonal, all matrices of a step in few launches."""
 import torch
 
+from _spherical_distortion_ext import _token_ops
+
 from .. import functional as F
 from . import adamw
 
@@ -14,21 +16,30 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr=2e-2, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
                  coefficients=F.NEWTON_SCHULZ, eps=1e-7):
-        if not lr >= 0 or not weight_decay >= 0:
-            raise ValueError("lr and weight_decay must not be negative")
-        if not 0 <= momentum < 1:
-            raise ValueError("momentum must be in [0, 1), got %s" % momentum)
-        if not 1 <= steps <= 100 or len(coefficients) != 3 or not 2.0 ** -100 <= eps <= 1:
-            raise ValueError("steps must be between 1 and 100, coefficients three, eps between 2^-100 and 1")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=tuple(coefficients), eps=eps))
 
+    @staticmethod
+    def _check(group):
+        if not group["lr"] >= 0 or not group["weight_decay"] >= 0:
+            raise ValueError("lr and weight_decay must not be negative")
+        if not 0 <= group["momentum"] < 1:
+            raise ValueError("momentum must be in [0, 1), got %s" % group["momentum"])
+        try:
+            _token_ops.check_newton_schulz(group["steps"], group["coefficients"], group["eps"])
+        except RuntimeError as e:
+            raise ValueError(str(e)) from None
+        for p in group["params"]:
+            if p.dim() < 2:
+                raise ValueError("Muon takes parameters of two axes at least, got one of shape %s" % (tuple(p.shape),))
+
     def add_param_group(self, group):
         super().add_param_group(group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                self.param_groups.pop()
-                raise ValueError("Muon takes parameters of two axes at least, got one of shape %s" % (tuple(p.shape),))
+        try:
+            self._check(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     @torch.no_grad()
     def step(self, closure=None):
