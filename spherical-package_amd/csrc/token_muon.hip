@@ -53,9 +53,33 @@ struct Settings {
 };
 static_assert(sizeof(Table) + sizeof(Settings) + 64 <= 4096, "kernel arguments are limited to 4 KB");
 
-__device__ __forceinline__ int matrix_of(const unsigned* start, unsigned group) {
-  const unsigned long long before = __ballot(start[threadIdx.x & 63] <= group);
-  return __builtin_amdgcn_readfirstlane(__popcll(before) - 1);
+// The matrix of a workgroup.  Every lane reads one matrix's entries before the workgroup knows which is its own: one trip to
+// the arguments where one for the index and one for the entries would follow each other (65 x 65: 85 us for 90 in 17 launches).
+struct Mine {
+  int rows, columns;
+  int64_t at, id;     // place in the workspace; which workgroup of the matrix
+  char* p;
+  const char* g;
+  float* m;
+  float rate;
+};
+__device__ __forceinline__ int64_t lane_of(int64_t x, int lane) {
+  const unsigned low = __builtin_amdgcn_readlane((int)x, lane);
+  return (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 | low;
+}
+__device__ __forceinline__ Mine matrix_of(const Table& t, unsigned group) {
+  const int lane = threadIdx.x & 63;
+  const unsigned start = t.start[lane];
+  const int rows = t.rows[lane], columns = t.columns[lane];
+  const int64_t at = t.at[lane], p = (int64_t)t.p[lane], g = (int64_t)t.g[lane], m = (int64_t)t.m[lane];
+  const float rate = t.rate[lane];
+  const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(start <= group)) - 1);
+  Mine mine;
+  mine.rows = __builtin_amdgcn_readlane(rows, i), mine.columns = __builtin_amdgcn_readlane(columns, i);
+  mine.at = lane_of(at, i), mine.id = group - (unsigned)__builtin_amdgcn_readlane((int)start, i);
+  mine.p = (char*)lane_of(p, i), mine.g = (const char*)lane_of(g, i), mine.m = (float*)lane_of(m, i);
+  mine.rate = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rate), i));
+  return mine;
 }
 
 // A row of an operand is a sequence of lines of 128 bytes: 64 values, or 32 values' hi and then their lo pieces.
@@ -113,37 +137,62 @@ __device__ __forceinline__ void read_values(const char* row, int64_t at, float (
   }
 }
 
-template <typename T>
-__device__ __forceinline__ float update_of(const T* g, const float* m, int64_t i, const Settings& s) {
-  if (!m) return (float)g[i];
-  return s.nesterov ? s.mu * m[i] + s.rest * (float)g[i] : m[i];
+__device__ __forceinline__ float update_of(bool momentum, float g, float m, const Settings& s) {
+  if (!momentum) return g;
+  return s.nesterov ? s.mu * m + s.rest * g : m;
 }
 
-// The momentum, and the sum of squares of the update, 4096 values a workgroup.
-template <typename T>
-__global__ __launch_bounds__(256) void squares(const Table t, const Settings s, char* workspace, int split) {
-  __shared__ double sums[4];
-  const int i = matrix_of(t.start, blockIdx.x);
-  const int64_t n = (int64_t)t.rows[i] * t.columns[i], group = blockIdx.x - t.start[i];
-  const T* g = (const T*)t.g[i];
-  float* m = t.m[i];
+// The momentum and the sum of squares of kPerGroup values, four beside each other a thread; all are requested before the
+// first is used.  WHOLE: all are in the matrix, and 16-byte vectors fit the addresses.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ double squares_of(const T* g, float* m, int64_t left, const Settings& s) {
+  constexpr int N = kPerGroup / 1024;
+  float from[N][4], held[N][4];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const int at = r * 1024 + threadIdx.x * 4;
+    const int here = (int)(left - at < 4 ? left - at : 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) from[r][e] = held[r][e] = 0.f;
+    if (WHOLE || here > 0) {
+      get<T, 4, WHOLE>(g + at, from[r], here);
+      if (m) get<float, 4, WHOLE>(m + at, held[r], here);
+    }
+  }
   double sum = 0;
-#pragma unroll 4
-  for (int r = 0; r < kPerGroup / 256; ++r) {
-    const int64_t at = group * kPerGroup + r * 256 + threadIdx.x;
-    if (at < n) {
-      if (m) m[at] = s.mu * m[at] + s.rest * (float)g[at];
-      const double u = update_of(g, m, at, s);
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const int at = r * 1024 + threadIdx.x * 4;
+    const int here = (int)(left - at < 4 ? left - at : 4);
+    if (m) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) held[r][e] = s.mu * held[r][e] + s.rest * from[r][e];
+      if (WHOLE || here > 0) put<float, 4, WHOLE>(m + at, held[r], here);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const double u = update_of(m != nullptr, from[r][e], held[r][e], s);
       sum += u * u;
     }
   }
+  return sum;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void squares(const Table t, const Settings s, char* workspace, int split) {
+  __shared__ double sums[4];
+  const Mine mine = matrix_of(t, blockIdx.x);
+  const int64_t n = (int64_t)mine.rows * mine.columns, first = mine.id * kPerGroup;
+  const T* g = (const T*)mine.g + first;
+  float* m = mine.m ? mine.m + first : nullptr;
+  const bool whole = first + kPerGroup <= n && (uintptr_t)g % 16 == 0 && (uintptr_t)m % 16 == 0;
+  double sum = whole ? squares_of<T, true>(g, m, n - first, s) : squares_of<T, false>(g, m, n - first, s);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
-    const Layout at(t.rows[i], t.columns[i], split);
-    ((double*)(workspace + t.at[i] + at.sums))[group] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const Layout at(mine.rows, mine.columns, split);
+    ((double*)(workspace + mine.at + at.sums))[mine.id] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   }
 }
 
@@ -153,28 +202,34 @@ __global__ __launch_bounds__(256) void lay_out(const Table t, const Settings s, 
   __shared__ float tile[64][65];
   __shared__ double sums[4];
   const unsigned group = gridDim.x - 1 - blockIdx.x;   // last first: what squares() touched last is still in the caches
-  const int i = matrix_of(t.start, group), rows = t.rows[i], columns = t.columns[i];
+  const Mine mine = matrix_of(t, group);
+  const int rows = mine.rows, columns = mine.columns;
   const Layout at(rows, columns, SPLIT);
-  char* place = workspace + t.at[i];
-  const T* g = (const T*)t.g[i];
-  const float* m = t.m[i];
+  char* place = workspace + mine.at;
+  const T* g = (const T*)mine.g;
+  const float* m = mine.m;
+  // the tile as it lies in the matrix
+  const bool tall = rows > columns;
+  const int64_t cp = tall ? at.kp : at.lp, id = mine.id;
+  const int64_t r0 = id / (cp / 64) * 64, c0 = id % (cp / 64) * 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float from[16], held[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const bool there = r0 + 4 * r + wave < rows && c0 + lane < columns;
+    const int64_t i = (r0 + 4 * r + wave) * columns + c0 + lane;
+    from[r] = there ? (float)g[i] : 0.f;
+    held[r] = there && m ? m[i] : 0.f;
+  }
   const double* parts = (const double*)(place + at.sums);
   const int64_t count = ((int64_t)rows * columns + kPerGroup - 1) / kPerGroup;
   double sum = 0;
   for (int64_t j = threadIdx.x; j < count; j += 256) sum += parts[j];
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
-  // the tile as it lies in the matrix
-  const bool tall = rows > columns;
-  const int64_t cp = tall ? at.kp : at.lp, id = group - t.start[i];
-  const int64_t r0 = id / (cp / 64) * 64, c0 = id % (cp / 64) * 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) sums[wave] = sum;
 #pragma unroll
-  for (int r = 0; r < 64; r += 4) {
-    const bool there = r0 + r + wave < rows && c0 + lane < columns;
-    tile[r + wave][lane] = there ? update_of(g, m, (r0 + r + wave) * columns + c0 + lane, s) : 0.f;
-  }
+  for (int r = 0; r < 16; ++r) tile[4 * r + wave][lane] = update_of(m != nullptr, from[r], held[r], s);
   __syncthreads();
   const float up = kScale / ((float)sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + s.eps);
   const int64_t k0 = tall ? c0 : r0, l0 = tall ? r0 : c0;
@@ -246,7 +301,7 @@ constexpr int kGram = 0, kPolynomial = 1, kNext = 2, kLast = 3;
 // LINES: of 128 bytes of each row that a step takes, by as many groups of waves, each with a sum of its own.
 template <int F_, int G_, int ACROSS_, int LINES_, int STAGES_>
 struct Shape {
-  static constexpr int F = F_, G = G_, DOWN = 2, ACROSS = ACROSS_, LINES = LINES_, WAVES = DOWN * ACROSS, THREADS = 64 * WAVES * LINES;
+  static constexpr int F = F_, G = G_, DOWN = F_ < 64 ? 1 : 2, ACROSS = ACROSS_, LINES = LINES_, WAVES = DOWN * ACROSS, THREADS = 64 * WAVES * LINES;
   static constexpr int Y = F / 32 / DOWN, X = G / 32 / ACROSS;   // 32 x 32 blocks of a wave
   static constexpr int STAGES = STAGES_;                         // steps in LDS
   static constexpr int F_LOADS = F * 8 / (64 * WAVES), LOADS = (F + G) * 8 / (64 * WAVES);   // 16-byte requests of a thread
@@ -392,10 +447,10 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
   constexpr int LINE = kLine<SPLIT>, KK = LINE / 16, PIECES = SPLIT ? 2 : 1;
   __shared__ __attribute__((aligned(128))) char lds[S::STAGES * S::STEP];
   const unsigned group = by_die(blockIdx.x, gridDim.x);
-  const int i = matrix_of(t.start, group);
-  const Layout at(t.rows[i], t.columns[i], SPLIT);
-  char* place = workspace + t.at[i];
-  const int64_t id = group - t.start[i];
+  const Mine mine = matrix_of(t, group);
+  const Layout at(mine.rows, mine.columns, SPLIT);
+  char* place = workspace + mine.at;
+  const int64_t id = mine.id;
   int64_t ti, tj;                             // tile of the block's rows, of its columns
   if constexpr (SQUARE) {                     // ti <= tj, counted column by column
     tj = (int64_t)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
@@ -562,11 +617,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
     return v;
   };
   if constexpr (STAGE == kLast) {
-    const bool tall = t.rows[i] > t.columns[i];
-    T* p = (T*)t.p[i];
+    const bool tall = mine.rows > mine.columns;
+    T* p = (T*)mine.p;
     const int64_t columns = tall ? at.k : at.l;
-    const Result<T> result = {p, tall ? at.l : at.k, columns, !tall, t.m[i] != nullptr,
-                              columns % kWide<T> == 0 && (uintptr_t)p % 16 == 0, s.keep, t.rate[i]};
+    const Result<T> result = {p, tall ? at.l : at.k, columns, !tall, mine.m != nullptr,
+                              columns % kWide<T> == 0 && (uintptr_t)p % 16 == 0, s.keep, mine.rate};
 #pragma unroll
     for (int y = 0; y < S::Y; ++y) {
       typename Result<T>::Old old[S::X];
@@ -919,14 +974,20 @@ void multiply(Table& t, int used, const Settings& s, char* workspace, int turn, 
 
 // Tiles of 128 x 128 where they make a workgroup a CU, of 64 x 64 otherwise.  Eight waves a tile keep the matrix unit busier
 // than four (S of 32 matrices of up to 640 x 2560 in bfloat16 45 us for 48, X' 67 for 71), but leave too few registers for
-// the last stage's parameters (247 us for 190 in float32).
+// the last stage's parameters (247 us for 190 in float32).  S and P of so few tiles that those of 32 x 32 still make one
+// workgroup a CU, take them, eight waves along the sums (five steps of 701 x 1100 in float32 153 us for 184, 400 x 4000 214
+// for 289; with two workgroups for some CUs 900 x 1000 226 for 199).
 template <bool SPLIT, int STAGE, typename T>
 void stage(Table& t, int used, const Settings& s, char* workspace, int turn, hipStream_t stream) {
   using Large = Shape<128, 128, STAGE == kLast ? 2 : 4, 1, 2>;
+  using Middle = Shape<64, 64, 2, 2, 4>;
+  using Little = std::conditional_t<(STAGE <= kPolynomial), Shape<32, 32, 1, 8, 2>, Middle>;
   if (groups_of<STAGE, Large>(t, used) >= 256)
     multiply<SPLIT, Large, STAGE, T>(t, used, s, workspace, turn, stream);
+  else if (STAGE <= kPolynomial && groups_of<STAGE, Little>(t, used) <= 256)
+    multiply<SPLIT, Little, STAGE, T>(t, used, s, workspace, turn, stream);
   else
-    multiply<SPLIT, Shape<64, 64, 2, 2, 4>, STAGE, T>(t, used, s, workspace, turn, stream);
+    multiply<SPLIT, Middle, STAGE, T>(t, used, s, workspace, turn, stream);
 }
 
 template <typename T>
