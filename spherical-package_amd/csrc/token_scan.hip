@@ -6,16 +6,16 @@
 //
 // Each channel by itself.  A span of tokens acts on the state before it as h -> A h + H, and spans join: (A, H) then
 // (A', H') is (A A', A' H + H').  So a workgroup takes 64 channels in 16 bits (32 in float32: 128 bytes of a token either
-// way; a quarter of that where the width is no larger) and a tile of tokens, of which each thread walks two or four in
-// order; the threads' spans are joined over the tile, and each walks its tokens again from the state in front of them.  The
+// way; a quarter of that where the width is no larger) and a tile of tokens, of which each thread walks 32 values
+// (backward 16: two to eight tokens) in order; the threads' spans are joined over the tile, and each walks its tokens again from the state in front of them.  The
 // tile's values stay in registers meanwhile.  Where batch and channels fill the GPU a workgroup goes through a whole
 // sequence; otherwise it takes one tile, and tiles hand each other their spans while the kernel runs (scan_tiles).
 //
 // Bound by memory: three values read or written a token and channel forward, six backward (the gradients read h as
-// it was rounded to the tensors' type).  2 x 8192 tokens of 1024 channels in bfloat16: forward 30 us (3.4 TB/s), backward 54
-// (3.7 TB/s); all tiles of the forward are on the GPU at once, so that reading, waiting and writing follow each other.  A
+// it was rounded to the tensors' type).  2 x 8192 tokens of 1024 channels in bfloat16: forward 28 us (3.6 TB/s), backward 48
+// (4.2 TB/s); all tiles of the forward are on the GPU at once, so that reading, waiting and writing follow each other.  A
 // first launch for the spans of longer segments, which then were read again, took 49 and 74 us.  131072 tokens of 256
-// channels in float16 forward: 60 us (3.4 TB/s; 95 with two launches).
+// channels in float16 forward: 53 us (3.8 TB/s; 95 with two launches).
 //
 // The state, its gradient, the spans and the gates are float32.  u weighs the distance x - h: 1 - f of a rounded f near one
 // would be off by a part of all that a long memory sums up.
@@ -300,7 +300,8 @@ __device__ __forceinline__ void store_last(const Scan& p, const Place<T, LANES>&
   if (to && place.left > 0 && place.time == 0) store_part<float, kWide<T>>(to + place.lane_state, carry, place.left);
 }
 
-// Tokens of a tile that a thread walks: a backward holds four tensors' values of each, a forward two.
+// Tokens of a tile that a thread walks: a backward holds four tensors' values of each, a forward two.  (Half as many in
+// float32: long scans 4 to 15 % slower.)
 template <bool BACKWARD, int V>
 constexpr int kRows = (BACKWARD ? 16 : 32) / V;
 
