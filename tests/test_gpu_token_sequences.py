@@ -172,6 +172,50 @@ def test_one_tensor_in_several_places():
     assert torch.equal(torch.autograd.grad(F.gated_scan(leaf, leaf)[0], leaf, dt)[0], want[0] + want[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_parameters_in_one_buffer(dtype):
+    """Muon on views at any address of flat buffers: what copies give, and nothing beside them changes.  Tiles, lines and sums
+    are the same, so the bits are too."""
+    from spherical_distortion import functional as F
+    shapes = [(7, 9), (64, 31), (100, 201), (130, 129), (5, 3, 9)]
+    sizes = [torch.Size(s).numel() for s in shapes]
+    flat = [torch.full((sum(sizes) + 2 * len(sizes) + 1,), 7.0, dtype=d, device=DEV) for d in (dtype, dtype, torch.float32)]
+    lists, at = [[], [], []], 1
+    for i, (shape, n) in enumerate(zip(shapes, sizes)):
+        for to, buffer in zip(lists, flat):
+            to.append(buffer[at:at + n].view(shape))
+            to[-1].copy_(_randn(*shape, seed=len(to)))
+        at += n + 2
+    twins = [[t.clone() for t in ts] for ts in lists]
+    F.muon_step(*lists, lr=0.1, weight_decay=0.1)
+    F.muon_step(*twins, lr=0.1, weight_decay=0.1)
+    for ts, us in zip(lists, twins):
+        assert all(torch.equal(t, u) for t, u in zip(ts, us))
+    for buffer in flat:
+        at = 0
+        for n in sizes:
+            assert float(buffer[at]) == 7
+            at += n + 1
+            assert float(buffer[at]) == 7
+            at += 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_a_backward_reads_must_not_change_before_it(dtype):
+    from spherical_distortion import functional as F
+    x, r = (_randn(4, 16, seed=i, dtype=dtype) for i in range(2))
+    w = _randn(16).requires_grad_()
+    y, h = F.add_layer_norm(x, r, w)
+    (h if dtype == torch.float32 else r).add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    x, state = _randn(2, 5, 16, dtype=dtype).requires_grad_(), _randn(2, 16)
+    out, _ = F.gated_scan(x, x.detach(), state)
+    F.gated_scan_step(x[:, 0].detach(), x[:, 0].detach(), state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
 def test_inference_tensors():
     from spherical_distortion import functional as F
     from spherical_distortion.optim import Muon
