@@ -298,6 +298,49 @@ def test_another_stream(name, dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_two_streams_at_once():
+    """Scans whose tiles wait for each other, norms and steps on two streams at the same time: the bits of one after another."""
+    works = [_work(torch.bfloat16), _work(torch.bfloat16)]
+    want = {name: [t.clone() for t in works[0][name][1]()] for name in ("norm", "scan", "orthogonal")}
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in works], [[], []]
+    for _ in range(5):
+        for work, stream, result in zip(works, streams, results):
+            with torch.cuda.stream(stream):
+                result.append({name: work[name][1]() for name in want})
+    torch.cuda.synchronize()
+    for result in results:
+        for got in result:
+            for name in want:
+                assert all(torch.equal(a, b) for a, b in zip(got[name], want[name])), name
+
+
+def test_a_backward_may_run_twice():
+    from spherical_distortion import functional as F
+    x, gate, w = _randn(2, 700, 16).requires_grad_(), _randn(2, 700, 16, seed=1).requires_grad_(), _randn(16).requires_grad_()
+    y, h = F.add_layer_norm(x, gate, w)
+    out, last = F.gated_scan(y, h)
+    first, second = (torch.autograd.grad([out.sum(), last.sum()], [x, gate, w], retain_graph=keep) for keep in (True, False))
+    assert all(torch.equal(a, c) for a, c in zip(first, second))
+
+
+def test_one_row():
+    """A vector is a row; float32 weights get float32 gradients beside 16-bit rows."""
+    from spherical_distortion import functional as F
+    for dtype in (torch.float32, torch.float16):
+        x, w, b, dy = _randn(40, dtype=dtype), _randn(40, seed=1), _randn(40, seed=2), _randn(40, seed=3, dtype=dtype)
+        results = []
+        for shape in ((40,), (1, 40), (1, 1, 1, 40)):
+            leaves = [x.view(shape).clone().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()]
+            y, h = F.add_layer_norm(leaves[0], None, *leaves[1:])
+            assert y.shape == shape and h is leaves[0]
+            grads = torch.autograd.grad(y, leaves, dy.view(shape))
+            assert grads[1].dtype == grads[2].dtype == torch.float32
+            results.append([t.flatten() for t in (y, *grads)])
+        for other in results[1:]:
+            assert all(torch.equal(a, c) for a, c in zip(results[0], other))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("name", WORK)
 def test_two_graphs(name, dtype):
