@@ -10,14 +10,18 @@
 //
 // Operands are float16 times 2^12.  float32 and float16 matrices take two pieces a value, v = hi + lo, and three products
 // hi hi + hi lo + lo hi: 22 bits, 2.5e-7 of the result, below what float32 products leave (2e-6), at a third of the
-// float16 rate where the float32 unit runs at an eighth.  bfloat16 matrices take one piece: 1.3e-3 of the result, beside
-// the 1.7e-3 of its own rounding.  Entries of X, S and P have to stay below 16: no entry is larger than the largest singular
-// value, which the coefficients alone bound (check_coefficients).  Sums are float32, of the norm double.
+// float16 rate where the float32 unit runs at an eighth.  bfloat16 matrices take one piece, but for the diagonals of S and P,
+// whose rests are kept: they weigh whole rows, so their roundings add up where others average out (3 x 240 would be 4.5e-3
+// off for 1.7e-3, 400 x 4000 2.6e-3 for 1.8e-3; of these the result's own rounding is 1.66e-3).  With D the rests of S, S S
+// is formed as S S + D S + S D; with D those of P, X' = P X + D X.
+//
+// Entries of X, S and P have to stay below 16: no entry is larger than the largest singular value, which the coefficients
+// alone bound (check_coefficients).  Sums are float32, of the norm double.
 //
 // 32 matrices of 640 x 640 to 640 x 2560, 39 million values, a step in float32: 1.81 ms.  S takes 110 us (820 TFLOP/s of
 // products of pieces; its workgroups' sums are 640 to 2560 long), P 43 (710), X' 165 (910), momentum and norm 77, X_0 85, the
-// last X' into the parameters 190.  A large library product of float16 reaches 1165.  bfloat16: 0.86 ms (S 43, P 20, X' 65,
-// 61, 75 and 95).
+// last X' into the parameters 190.  A large library product of float16 reaches 1165.  bfloat16: 0.84 to 0.89 ms (S 43 to 46,
+// P 20 to 23, X' 68 to 74, 61, 78 and 100; without the diagonals' rests X' 65 to 70).
 //
 // All matrices of a call go through a stage in one launch; their table is a kernel argument.  Small ones go through all
 // stages in a workgroup of their own.
@@ -93,14 +97,15 @@ constexpr int kLine = SPLIT ? 32 : 64;
 
 // Where the buffers of a matrix lie; sides padded with zeros to multiples of kPad.
 struct Layout {
-  int64_t k, l, kp, lp, x0, x1, s, p, sums, end;    // byte offsets from the matrix's place; X of even and odd steps
+  int64_t k, l, kp, lp, x0, x1, s, p, s_rest, p_rest, sums, end;   // byte offsets from the matrix's place; X of even and
+                                                                   // odd steps
   int64_t k_row, l_row;                             // bytes of a row of k and of l values
   __host__ __device__ Layout(int64_t rows, int64_t columns, bool split) {
     k = rows < columns ? rows : columns, l = rows < columns ? columns : rows;
     kp = (k + kPad - 1) / kPad * kPad, lp = (l + kPad - 1) / kPad * kPad;
     k_row = kp * (split ? 4 : 2), l_row = lp * (split ? 4 : 2);
     x0 = 0, x1 = x0 + kp * l_row, s = x1 + kp * l_row, p = s + kp * k_row;
-    sums = p + kp * k_row;
+    s_rest = p + kp * k_row, p_rest = s_rest + (split ? 0 : kp * 4), sums = p_rest + (split ? 0 : kp * 4);
     end = sums + ((rows * columns + kPerGroup - 1) / kPerGroup * 8 + 127) / 128 * 128;
   }
 };
@@ -361,6 +366,27 @@ __device__ __forceinline__ void write_block(const floatx16& v, char* scratch, in
   wave_order();
 }
 
+// What a block on a diagonal keeps beside its float16 values: of each column the rest of its diagonal's value.
+__device__ __forceinline__ void keep_rest(const floatx16& v, int lane, float* to) {
+  const int c = lane % 32;
+  float own = v[0];
+#pragma unroll
+  for (int e = 1; e < 16; ++e) own = e == c / 8 * 4 + c % 4 ? v[e] : own;
+  if (c / 4 % 2 == lane / 32) to[c] = own - (float)(f16)own;
+}
+
+// The diagonal of 32 rests, one of each lane's column, as two operands of 16.
+struct Rests {
+  f16x8 v[2];
+  __device__ __forceinline__ Rests() = default;
+  __device__ __forceinline__ Rests(float rest, int lane) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[kk][e] = kk * 16 + lane / 32 * 8 + e == lane % 32 ? (f16)rest : (f16)0.f;
+  }
+};
+
 // Where the last product goes: element (row, column) at p[row * columns + column], alone or as a parameter's step.
 template <typename T>
 struct Result {
@@ -513,6 +539,17 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
       for (int v = 0; v < 16; ++v) acc[y][x][v] = 0.f;
 
   const int half = lane / 32, wy = wave / S::ACROSS * S::Y * 32, wx = wave % S::ACROSS * S::X * 32;
+  // the rests of the diagonals of S and, as operands that are zero beside it, of the blocks' rows of P
+  constexpr bool DIAGONAL = !SPLIT && !SQUARE;
+  float *s_rest = (float*)(place + at.s_rest), *p_rest = (float*)(place + at.p_rest);
+  Rests rest[DIAGONAL ? S::X : 1];
+  if constexpr (DIAGONAL) {
+#pragma unroll
+    for (int x = 0; x < S::X; ++x) {
+      const int64_t j = tj * S::G + wx + x * 32 + lane % 32;
+      rest[x] = Rests(j < at.kp ? p_rest[j] : 0.f, lane);
+    }
+  }
 #pragma unroll
   for (int step = 0; step < S::STAGES - 1; ++step)
     if (step < steps) request(step);
@@ -586,6 +623,25 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
           }
           acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kk][y][0], b[kk][x][0], acc[y][x], 0, 0, 0);
         }
+    if constexpr (DIAGONAL) {
+#pragma unroll
+      for (int x = 0; x < S::X; ++x) {
+        const int64_t j0 = tj * S::G + wx + x * 32;
+        if (j0 / LINE != step * S::LINES + line) continue;
+        auto add = [&](auto first) {   // its 32 of the line's rows of X
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int y = 0; y < S::Y; ++y)
+              acc[y][x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[decltype(first)::value + kk][y][0], rest[x].v[kk], acc[y][x],
+                                                                 0, 0, 0);
+        };
+        if (j0 % LINE == 0)
+          add(std::integral_constant<int, 0>());
+        else
+          add(std::integral_constant<int, 2>());
+      }
+    }
   }
   step_barrier<0>();   // the buffers are free
 
@@ -653,17 +709,29 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
       const int64_t i0 = ti * S::F + wy + y * 32, j0 = tj * S::G + wx + x * 32;
       if (i0 >= i_end || j0 >= at.kp) continue;
       floatx16 v = scaled(y, x);
+      if (!SPLIT && STAGE == kGram && i0 == j0) keep_rest(v, lane, s_rest + i0);
       if constexpr (STAGE == kPolynomial) {   // a I + b S + c S S; S is its own transpose
         const int64_t j = j0 + lane % 32;
+        const float own_rest = SPLIT ? 0.f : s_rest[j];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int64_t row = i0 + 8 * q + 4 * half;
           float old[4];
           read_values<SPLIT, 4>(place + at.s + j * at.k_row, row, old);
+          if constexpr (!SPLIT) {
+            const float4 rests = *reinterpret_cast<const float4*>(s_rest + row);
+            const float d[4] = {rests.x, rests.y, rests.z, rests.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[4 * q + e] = fmaf((d[e] + own_rest) * kDown, old[e], v[4 * q + e]);
+              old[e] += row + e == j ? own_rest : 0.f;
+            }
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             v[4 * q + e] = fmaf(s.c, v[4 * q + e], s.b * old[e]) + (row + e == j ? s.a * kScale : 0.f);
         }
+        if (!SPLIT && i0 == j0) keep_rest(v, lane, p_rest + i0);
       }
       if constexpr (SQUARE) {
         char* to = place + (STAGE == kGram ? at.s : at.p);
@@ -722,6 +790,7 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
   using Z = Small<SPLIT>;
   __shared__ __attribute__((aligned(128))) char lds[Z::BYTES];
   __shared__ double sums[8];
+  __shared__ __attribute__((aligned(16))) float s_rest[SPLIT ? 4 : 64], p_rest[SPLIT ? 4 : 64];   // of the diagonals
   const int i = blockIdx.x, rows = t.rows[i], columns = t.columns[i];
   const bool tall = rows > columns;
   const int k = tall ? columns : rows, l = tall ? rows : columns, lp = (l + 63) / 64 * 64, pitch = lp / LINE * 128;
@@ -808,6 +877,7 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
     for (int piece = 0; piece < PIECES; ++piece)
       x[piece] = *reinterpret_cast<const f16x8*>(line_at(base, row + lane % 32, row_pitch, line, piece * 4 + kk * 2 + half));
   };
+  Rests rest[2];   // of P's diagonal
   // columns j .. j + 31 of P X times `down`, as rows: the rows of P in two halves
   auto multiply = [&](int j, floatx16 (&next)[2], float down) {
 #pragma unroll
@@ -831,6 +901,13 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
         operand(P, SQUARE_PITCH, y * 32, kk / KK, kk % KK, p);
         add_product<SPLIT>(next[y], x[kk], p);
       }
+    if constexpr (!SPLIT) {   // the rests of P's diagonal
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+          next[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[2 * y + kk][0], rest[y].v[kk], next[y], 0, 0, 0);
+    }
 #pragma unroll
     for (int v = 0; v < 16; ++v) next[0][v] *= down, next[1][v] *= down;
   };
@@ -857,6 +934,7 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[v] = (acc[v] + part[v * 64]) * kDown;
       keep_block<SPLIT>(acc, lane, S, SQUARE_PITCH, bx, by);   // S is its own transpose
+      if (!SPLIT && by == bx) keep_rest(acc, lane, s_rest + bx);
     }
     __syncthreads();
     if (wave < 4) {
@@ -871,6 +949,7 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
           add_product<SPLIT>(acc, a, b);
         }
       const int row = bx + lane % 32;   // where this lane's column of S lies
+      const float own_rest = SPLIT ? 0.f : s_rest[row];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int line = by / LINE, chunk = by % LINE / 8 + q;
@@ -878,16 +957,28 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
         Pack<f16, 4> lo;
         if constexpr (SPLIT)
           lo = *reinterpret_cast<const Pack<f16, 4>*>(line_at(S, row, SQUARE_PITCH, line, 4 + q) + half * 8);
+        float4 rests = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (!SPLIT) rests = *reinterpret_cast<const float4*>(s_rest + by + 8 * q + 4 * half);
+        const float d[4] = {rests.x, rests.y, rests.z, rests.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float old = (float)hi.v[e] + (SPLIT ? (float)lo.v[e] : 0.f);
+          float old = (float)hi.v[e] + (SPLIT ? (float)lo.v[e] : 0.f);
+          if constexpr (!SPLIT) {
+            acc[4 * q + e] = fmaf(d[e] + own_rest, old, acc[4 * q + e]);
+            old += by + 8 * q + 4 * half + e == row ? own_rest : 0.f;
+          }
           acc[4 * q + e] = fmaf(s.c, acc[4 * q + e] * kDown, s.b * old) +
                            (by + 8 * q + 4 * half + e == row ? s.a * kScale : 0.f);
         }
       }
       keep_block<SPLIT>(acc, lane, P, SQUARE_PITCH, bx, by);
+      if (!SPLIT && by == bx) keep_rest(acc, lane, p_rest + bx);
     }
     __syncthreads();
+    if constexpr (!SPLIT) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) rest[y] = Rests(p_rest[y * 32 + lane % 32], lane);
+    }
     if (step + 1 == steps) break;
     // X' = P X in place: a wave has 32 columns of X to itself
     for (int j = wave * 32; j < lp; j += Z::THREADS / 2) {

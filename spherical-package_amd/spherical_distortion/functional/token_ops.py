@@ -277,7 +277,8 @@ def orthogonalize(input, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Matrices [.., rows, columns] with their singular values brought towards one by products alone: X = input / (its
     Frobenius norm + eps), then `steps` times X = a X + (b S + c S S) X with S = X X^T of the smaller side.
 
-    float32 and float16 matrices are multiplied with 22 bits a value, bfloat16 with 11; sums are float32.
+    float32 and float16 matrices are multiplied with 22 bits a value, bfloat16 with 11 (but for S's diagonal and the
+    polynomial's); sums are float32.
     Coefficients with which a singular value could pass 3.8, or a + b s + c s ** 2 pass 15 (s: its square), within the
     steps raise.  eps: 2 ** -100 to 1.  No gradients."""
     with torch.no_grad():

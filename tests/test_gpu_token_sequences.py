@@ -474,6 +474,25 @@ def test_a_matrix_of_gigabytes():
         assert float((got[rows].double() - want).norm()) <= 5e-6 * float(want.norm())
 
 
+@pytest.mark.parametrize("shape", [(3, 240), (3, 428), (412, 4), (34, 1855), (40, 1834), (64, 300), (400, 4000)])
+def test_bfloat16_matrices_of_few_long_rows(shape):
+    """Rows that are nearly orthogonal to each other: S and P are nearly diagonal, and their roundings weigh whole rows.
+
+    The result's own rounding is 2^-8 / sqrt(3) = 2.3e-3 at most in the root of the mean square.  X is rounded to 11 bits in
+    each step, 2^-11 / sqrt(3), which a step multiplies by 1.3 at most where singular values have arrived (0.68 to 1.14):
+    sqrt(1 + 1.3^2 + .. + 1.3^8) = 4.3 of them, 1.2e-3.  Together 2.6e-3; 2^-8 leaves half as much again."""
+    from spherical_distortion import functional as F
+    x = _randn(*shape, dtype=torch.bfloat16)
+    y = x.double()
+    y = y.t() if shape[0] > shape[1] else y
+    y = y / (y.norm() + 1e-7)
+    for _ in range(5):
+        s = y @ y.t()
+        y = NS[0] * y + (NS[1] * s + NS[2] * (s @ s)) @ y
+    y = y.t() if shape[0] > shape[1] else y
+    assert float((F.orthogonalize(x).double() - y).norm()) <= 2.0 ** -8 * float(y.norm())
+
+
 # --------------------------------------------------------------------------- together
 class _Block(torch.nn.Module):
     """Norm with residual, gated scan, norm with residual, two linear layers."""
