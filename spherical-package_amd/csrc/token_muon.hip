@@ -9,9 +9,9 @@
 // above the diagonal are formed and written twice.
 //
 // Operands are float16 times 2^12.  float32 and float16 matrices take two pieces a value, v = hi + lo, and three products
-// hi hi + hi lo + lo hi: 22 bits, 2.5e-7 of the result, below what float32 products leave (2e-6), at a third of the
-// float16 rate where the float32 unit runs at an eighth.  bfloat16 matrices take one piece, but for the diagonals of S and P,
-// whose rests are kept: they weigh whole rows, so their roundings add up where others average out (3 x 240 would be 4.5e-3
+// hi hi + hi lo + lo hi: 22 bits, 1.2e-6 of the result (701 x 1100) where float32 products leave 3.2e-6, at a third
+// of the float16 rate where the float32 unit runs at an eighth.  bfloat16 matrices take one piece, but for the diagonals of S
+// and P, whose rests are kept: they weigh whole rows, so their roundings add up where others average out (3 x 240 would be 4.5e-3
 // off for 1.7e-3, 400 x 4000 2.6e-3 for 1.8e-3; of these the result's own rounding is 1.66e-3).  With D the rests of S, S S
 // is formed as S S + D S + S D; with D those of P, X' = P X + D X.
 //
@@ -24,7 +24,7 @@
 // P 20 to 23, X' 68 to 74, 61, 78 and 100; without the diagonals' rests X' 65 to 70).
 //
 // All matrices of a call go through a stage in one launch; their table is a kernel argument.  Small ones go through all
-// stages in a workgroup of their own.
+// stages in a workgroup of their own, those of up to 16 rows on S alone, in 64 bits.
 #include <algorithm>
 #include <cmath>
 #include <functional>
@@ -59,6 +59,7 @@ struct Table {
 struct Settings {
   float a, b, c, eps, mu, rest, keep;   // rest: 1 - mu; keep: 1 - lr decay
   int nesterov;
+  double a64, b64, c64;                 // a, b, c as they were given
 };
 static_assert(sizeof(Table) + sizeof(Settings) + 64 <= 4096, "kernel arguments are limited to 4 KB");
 
@@ -744,8 +745,122 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
     }
 }
 
+// Matrices of up to 16 rows (or columns): the steps on S alone, in 64 bits, where squares of small singular values keep 1e-16
+// of the largest.  All matrices of a step are polynomials of S, so they commute and are symmetric, and with Q the product
+// of all P so far
+//   Q = P Q    S = P S P = P P S        X_steps = Q X_0
+// reads the matrix twice however many steps there are: one workgroup, in float64 products of 16 x 16 x 4.  A lane's four
+// values of a product are rows 4 i + lane / 16 of column lane % 16, which is how it takes the second operand, and of a
+// symmetric matrix the first: products follow each other in registers, in every wave by itself.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f64x4 product_of(const f64x4& a, const f64x4& b) {
+  f64x4 sum = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f64_16x16x4f64(a[i], b[i], sum, 0, 0, 0);
+  return sum;
+}
+
+// Five steps against those of X in LDS or through the launches: 16 x 27 10 us for 18, 16 x 384 13 for 33, 16 x 1000 21 for 88
+// (float32), 4e-8 off for 1e-6.  One workgroup reads a long matrix slowly: 16 x 4096 in bfloat16 75 us for 102, but 16 x 8192
+// 140 for 131; in two pieces the launches are behind up to the longest (16 x 131072 1.87 ms for 2.28).
+constexpr int kThin = 16, kThinWaves = 8;
+__host__ __device__ inline bool is_thin(int64_t rows, int64_t columns, bool split) {
+  const int64_t k = rows < columns ? rows : columns, l = rows < columns ? columns : rows;
+  return k <= kThin && (split || l <= 4096);
+}
+
+template <typename T>
+__device__ void thin_matrix(const T* g, float* m, T* p, int rows, int columns, float rate, const Settings& s, int steps,
+                            double (*parts)[4][64]) {
+  constexpr int TILES = 4, STRIDE = 16 * kThinWaves;   // tiles of 16 columns of a wave that are requested at once; to its next
+  const bool tall = rows > columns;
+  const int k = tall ? columns : rows, l = tall ? rows : columns;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, across = lane % 16, down = lane / 16;
+  auto place = [&](int row, int column) { return tall ? column * k + row : row * l + column; };
+
+  // the momentum, and S: a lane has row `across` of four columns
+  f64x4 S = {0, 0, 0, 0};
+  for (int base = wave * 16; base < l; base += TILES * STRIDE) {
+    float u[TILES][4], held[TILES][4];
+#pragma unroll
+    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int column = base + n * STRIDE + 4 * e + down;
+        const bool there = across < k && column < l;
+        u[n][e] = there ? (float)g[place(across, column)] : 0.f;
+        held[n][e] = there && m ? m[place(across, column)] : 0.f;
+      }
+#pragma unroll
+    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int column = base + n * STRIDE + 4 * e + down;
+        if (m) {
+          held[n][e] = s.mu * held[n][e] + s.rest * u[n][e];
+          if (across < k && column < l) m[place(across, column)] = held[n][e];
+        }
+        const double x = update_of(m != nullptr, u[n][e], held[n][e], s);
+        S = __builtin_amdgcn_mfma_f64_16x16x4f64(x, x, S, 0, 0, 0);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) parts[wave][i][lane] = S[i];
+  __syncthreads();
+  double norm = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    S[i] = parts[0][i][lane];
+#pragma unroll
+    for (int w = 1; w < kThinWaves; ++w) S[i] += parts[w][i][lane];
+    if (4 * i + down == across) norm += S[i];
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) norm += __shfl_xor(norm, d);
+  const double scale = 1. / (sqrt(norm) + (double)s.eps);
+  f64x4 Q, P;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) S[i] *= scale * scale, Q[i] = 4 * i + down == across ? scale : 0.;
+  for (int step = 0; step < steps; ++step) {
+    const f64x4 square = product_of(S, S);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      P[i] = (4 * i + down == across ? s.a64 : 0.) + s.b64 * S[i] + s.c64 * square[i];
+    Q = product_of(P, Q);
+    if (step + 1 < steps) S = product_of(P, product_of(P, S));
+  }
+
+  // Q X_0: a lane has four rows of column `across`
+  for (int base = wave * 16; base < l; base += TILES * STRIDE) {
+    float u[TILES][4], held[TILES][4], old[TILES][4];
+#pragma unroll
+    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 4 * i + down, column = base + n * STRIDE + across;
+        const bool there = row < k && column < l;
+        u[n][i] = there ? (float)g[place(row, column)] : 0.f;
+        held[n][i] = there && m ? m[place(row, column)] : 0.f;
+        old[n][i] = there && m ? (float)p[place(row, column)] : 0.f;
+      }
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) {
+      f64x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = update_of(m != nullptr, u[n][i], held[n][i], s);
+      x = product_of(Q, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 4 * i + down, column = base + n * STRIDE + across;
+        const float out = (float)x[i];
+        if (row < k && column < l) p[place(row, column)] = (T)(m ? old[n][i] * s.keep - rate * out : out);
+      }
+    }
+  }
+}
+
 // Small matrices, k up to 64: one workgroup takes a matrix through all steps, in LDS throughout.  X, S and P lie there as
-// lines of 128 bytes, a row after the other, their chunks exchanged by the row's number.
+// lines of 128 bytes, a row after the other, their chunks exchanged by the row's number.  Thin ones are steps of S alone.
 template <bool SPLIT>
 struct Small {
   static constexpr int THREADS = 512, LP = SPLIT ? 384 : 640;   // and l up to LP
@@ -792,6 +907,11 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
   __shared__ double sums[8];
   __shared__ __attribute__((aligned(16))) float s_rest[SPLIT ? 4 : 64], p_rest[SPLIT ? 4 : 64];   // of the diagonals
   const int i = blockIdx.x, rows = t.rows[i], columns = t.columns[i];
+  if (is_thin(rows, columns, SPLIT)) {
+    static_assert(Z::THREADS == 64 * kThinWaves && Z::BYTES >= kThinWaves * 4 * 64 * 8, "threads and LDS of both");
+    thin_matrix((const T*)t.g[i], t.m[i], (T*)t.p[i], rows, columns, t.rate[i], s, steps, (double (*)[4][64])lds);
+    return;
+  }
   const bool tall = rows > columns;
   const int k = tall ? columns : rows, l = tall ? rows : columns, lp = (l + 63) / 64 * 64, pitch = lp / LINE * 128;
   const T* g = (const T*)t.g[i];
@@ -1105,10 +1225,12 @@ void run_group(Table& t, int used, const Settings& s, int steps, char* workspace
   }
 }
 
-// Whether one workgroup takes the matrix: three matrices of 16 x 27 to 64 x 288 in float32, a step of each, 43 us
-// for 110 through the launches.
+// Whether one workgroup takes the matrix.  Three matrices of 16 x 27 to 64 x 288 in float32, a step of each, 43 us for 110
+// through the launches.
 bool is_small(int64_t rows, int64_t columns, int dtype) {
-  return std::min(rows, columns) <= 64 && std::max(rows, columns) <= (split(dtype) ? Small<true>::LP : Small<false>::LP);
+  const int64_t k = std::min(rows, columns), l = std::max(rows, columns);
+  return is_thin(rows, columns, split(dtype)) ||
+         (k <= 64 && l <= (split(dtype) ? Small<true>::LP : Small<false>::LP));
 }
 
 // Deals the matrices to groups that share the workspace one after another: 64 at most, and as many workgroups as a
@@ -1190,6 +1312,7 @@ int check_settings(int64_t count, int64_t steps, const double* coefficients, dou
 Settings settings_of(const double* c, double eps) {
   Settings s = {};
   s.a = (float)c[0], s.b = (float)c[1], s.c = (float)c[2], s.eps = (float)eps;
+  s.a64 = c[0], s.b64 = c[1], s.c64 = c[2];
   return s;
 }
 

@@ -493,6 +493,47 @@ def test_bfloat16_matrices_of_few_long_rows(shape):
     assert float((F.orthogonalize(x).double() - y).norm()) <= 2.0 ** -8 * float(y.norm())
 
 
+@pytest.mark.parametrize("shape", [(1, 1), (1, 700), (16, 16), (17, 5), (3, 1000), (2050, 16), (16, 4096), (11, 4097), (9, 20000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_matrices_of_few_rows(shape, dtype):
+    """Up to 16 rows or columns.  The steps are 64 bits where they go by S alone: the result's rounding, half a step of each value.
+    Longer ones in bfloat16 (4097 and 20000) go through products of 11 bits: 2^-8 again."""
+    from spherical_distortion import functional as F
+    x = _randn(2, *shape, dtype=dtype)
+    x[1] *= 1e-2
+    got = F.orthogonalize(x)
+    for i in range(2):
+        y = x[i].double()
+        y = y.t() if shape[0] > shape[1] else y
+        y = y / (y.norm() + 1e-7)
+        for _ in range(5):
+            s = y @ y.t()
+            y = NS[0] * y + (NS[1] * s + NS[2] * (s @ s)) @ y
+        y = y.t() if shape[0] > shape[1] else y
+        off = (got[i].double() - y).abs()
+        if dtype == torch.bfloat16 and max(shape) > 4096:
+            assert float(off.norm()) <= 2.0 ** -8 * float(y.norm())
+        else:
+            # eps is rounded to 32 bits, beside norms of 1e-2 and more: 1e-12; float16 values below 2^-14 by halves of 2^-24
+            u = torch.finfo(dtype).eps / 2
+            assert bool((off <= u * (1 + 1e-3) * y.abs() + 1e-9 + (2.0 ** -25 if dtype == torch.float16 else 0)).all())
+
+
+def test_singular_values_far_apart():
+    """Of 1 to 1e-4 of the largest, in few rows: squares of 1e-8 keep eight digits of 64 bits.  The matrix's own rounding to 32
+    bits (2^-24 of the largest beside 1e-4 of it) is in the oracle's input too; 2^-24 of the result is its rounding."""
+    from spherical_distortion import functional as F
+    g = torch.Generator().manual_seed(5)
+    u, v = (torch.linalg.qr(torch.randn(n, 8, generator=g, dtype=torch.float64))[0] for n in (8, 500))
+    x = ((u * torch.logspace(0, -4, 8, dtype=torch.float64)) @ v.t()).float().to(DEV)
+    y = x.double()
+    y = y / (y.norm() + 1e-7)
+    for _ in range(5):
+        s = y @ y.t()
+        y = NS[0] * y + (NS[1] * s + NS[2] * (s @ s)) @ y
+    assert float((F.orthogonalize(x).double() - y).norm()) <= 2.0 ** -24 * float(y.norm()) * 1.001
+
+
 # --------------------------------------------------------------------------- together
 class _Block(torch.nn.Module):
     """Norm with residual, gated scan, norm with residual, two linear layers."""
