@@ -11,9 +11,9 @@
 // Operands are float16 times 2^12.  float32 and float16 matrices take two pieces a value, v = hi + lo, and three products
 // hi hi + hi lo + lo hi: 22 bits, 1.2e-6 of the result (701 x 1100) where float32 products leave 3.2e-6, at a third
 // of the float16 rate where the float32 unit runs at an eighth.  bfloat16 matrices take one piece, but for the diagonals of S
-// and P, whose rests are kept: they weigh whole rows, so their roundings add up where others average out (3 x 240 would be 4.5e-3
-// off for 1.7e-3, 400 x 4000 2.6e-3 for 1.8e-3; of these the result's own rounding is 1.66e-3).  With D the rests of S, S S
-// is formed as S S + D S + S D; with D those of P, X' = P X + D X.
+// and P, whose rests are kept: they weigh whole rows, so their roundings add up where others average out (34 x 1855 would be
+// 3.1e-3 off for 1.7e-3, 400 x 4000 2.6e-3 for 1.8e-3; of these the result's own rounding is 1.66e-3).  With D the rests of S,
+// S S is formed as S S + D S + S D; with D those of P, X' = P X + D X.
 //
 // Entries of X, S and P have to stay below 16: no entry is larger than the largest singular value, which the coefficients
 // alone bound (check_coefficients).  Sums are float32, of the norm double.
@@ -761,7 +761,7 @@ __device__ __forceinline__ f64x4 product_of(const f64x4& a, const f64x4& b) {
 }
 
 // Five steps against those of X in LDS or through the launches: 16 x 27 10 us for 18, 16 x 384 13 for 33, 16 x 1000 21 for 88
-// (float32), 4e-8 off for 1e-6.  One workgroup reads a long matrix slowly: 16 x 4096 in bfloat16 75 us for 102, but 16 x 8192
+// (float32), 2.5e-8 off for 1e-6.  One workgroup reads a long matrix slowly: 16 x 4096 in bfloat16 75 us for 102, but 16 x 8192
 // 140 for 131; in two pieces the launches are behind up to the longest (16 x 131072 1.87 ms for 2.28).
 constexpr int kThin = 16, kThinWaves = 8;
 __host__ __device__ inline bool is_thin(int64_t rows, int64_t columns, bool split) {
