@@ -948,7 +948,8 @@ int sdk_gated_scan_step(const void* x, int64_t x_stride, const void* gate, int64
  * bits); bfloat16: from one (11 bits), but for the diagonals of S and b S + c S S (22).  Sums are float32.  Entries are
  * held below 16: coefficients with which a singular value could pass 3.8, or a + b s + c s s pass 15 (s: its square),
  * within the steps are refused.  Sides up to 131072, matrices of up to 2^31 values; out may be x.  eps: 2^-100 to 1.
- * The workspace begins at a multiple of 128. */
+ * Up to 16 rows or columns: 64 bits while the steps are few (six of the default coefficients), the others' bits beyond.
+ * The workspace begins at a multiple of 128; the bytes are enough for any steps and coefficients. */
 size_t sdk_orthogonalize_workspace_bytes(int64_t rows, int64_t columns, int64_t count, int32_t dtype);
 int sdk_orthogonalize(const void* x, void* out, int64_t rows, int64_t columns, int64_t count, int32_t steps,
                       const double* coefficients, double eps, void* workspace, size_t workspace_bytes, int32_t dtype,

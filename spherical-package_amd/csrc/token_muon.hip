@@ -24,7 +24,7 @@
 // P 20 to 23, X' 68 to 74, 61, 78 and 100; without the diagonals' rests X' 65 to 70).
 //
 // All matrices of a call go through a stage in one launch; their table is a kernel argument.  Small ones go through all
-// stages in a workgroup of their own, those of up to 16 rows on S alone, in 64 bits.
+// stages in a workgroup of their own, those of up to 16 rows on S alone, in 64 bits, where the steps are few.
 #include <algorithm>
 #include <cmath>
 #include <functional>
@@ -59,6 +59,7 @@ struct Table {
 struct Settings {
   float a, b, c, eps, mu, rest, keep;   // rest: 1 - mu; keep: 1 - lr decay
   int nesterov;
+  int thin;                             // whether matrices of up to 16 rows go by S alone
   double a64, b64, c64;                 // a, b, c as they were given
 };
 static_assert(sizeof(Table) + sizeof(Settings) + 64 <= 4096, "kernel arguments are limited to 4 KB");
@@ -752,6 +753,15 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
 // reads the matrix twice however many steps there are: one workgroup, in float64 products of 16 x 16 x 4.  A lane's four
 // values of a product are rows 4 i + lane / 16 of column lane % 16, which is how it takes the second operand, and of a
 // symmetric matrix the first: products follow each other in registers, in every wave by itself.
+//
+// X is not read again, so nothing takes back what rounding does to S.  A step makes of an eigenvalue s the value f(s) = s q(s)^2,
+// and of an error E of S, in S's eigenvectors, the differences of f: E_ij (f(s_i) - f(s_j)) / (s_i - s_j), at most max |f'|
+// times E.  (For that S has to be symmetric, and is made so in each step: a product taken by its transpose moves the rest of an
+// S that is not by more, 16 x 27 2e-6 off after 12 steps of the default coefficients for 3e-15.)  Where f' is not small the
+// error grows, and once an eigenvalue of zero is rounded to less, it leaves for minus infinity: equal rows are 3e-13 off after
+// 5 steps, 4e-11 after 8, and infinite after 20.  So this is the way of as many steps as keep the product of
+// max |f'| below 2^24 (check_coefficients), which leaves 16 roundings of 2^-53 below 2^-25 of S: six steps of the default
+// coefficients, twelve of 1.875, -1.25, 0.375.  More go by X, whose S is a sum of squares anew in each step.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f64x4 product_of(const f64x4& a, const f64x4& b) {
   f64x4 sum = {0, 0, 0, 0};
@@ -764,6 +774,7 @@ __device__ __forceinline__ f64x4 product_of(const f64x4& a, const f64x4& b) {
 // (float32), 2.5e-8 off for 1e-6.  One workgroup reads a long matrix slowly: 16 x 4096 in bfloat16 75 us for 102, but 16 x 8192
 // 140 for 131; in two pieces the launches are behind up to the longest (16 x 131072 1.87 ms for 2.28).
 constexpr int kThin = 16, kThinWaves = 8;
+constexpr double kMostGrowth = 1 << 24;
 __host__ __device__ inline bool is_thin(int64_t rows, int64_t columns, bool split) {
   const int64_t k = rows < columns ? rows : columns, l = rows < columns ? columns : rows;
   return k <= kThin && (split || l <= 4096);
@@ -818,14 +829,20 @@ __device__ void thin_matrix(const T* g, float* m, T* p, int rows, int columns, f
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) norm += __shfl_xor(norm, d);
   const double scale = 1. / (sqrt(norm) + (double)s.eps);
-  f64x4 Q, P;
+  f64x4 Q, P, unit;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) S[i] *= scale * scale, Q[i] = 4 * i + down == across ? scale : 0.;
+  for (int i = 0; i < 4; ++i) {
+    unit[i] = 4 * i + down == across ? 1. : 0.;
+    S[i] *= scale * scale, Q[i] = unit[i] * scale;
+  }
   for (int step = 0; step < steps; ++step) {
+    const f64x4 turned = product_of(S, unit);   // S's transpose, exactly
+#pragma unroll
+    for (int i = 0; i < 4; ++i) S[i] = 0.5 * (S[i] + turned[i]);
     const f64x4 square = product_of(S, S);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      P[i] = (4 * i + down == across ? s.a64 : 0.) + s.b64 * S[i] + s.c64 * square[i];
+      P[i] = unit[i] * s.a64 + s.b64 * S[i] + s.c64 * square[i];
     Q = product_of(P, Q);
     if (step + 1 < steps) S = product_of(P, product_of(P, S));
   }
@@ -860,7 +877,8 @@ __device__ void thin_matrix(const T* g, float* m, T* p, int rows, int columns, f
 }
 
 // Small matrices, k up to 64: one workgroup takes a matrix through all steps, in LDS throughout.  X, S and P lie there as
-// lines of 128 bytes, a row after the other, their chunks exchanged by the row's number.  Thin ones are steps of S alone.
+// lines of 128 bytes, a row after the other, their chunks exchanged by the row's number.  Thin ones of few steps are steps
+// of S alone.
 template <bool SPLIT>
 struct Small {
   static constexpr int THREADS = 512, LP = SPLIT ? 384 : 640;   // and l up to LP
@@ -907,7 +925,7 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
   __shared__ double sums[8];
   __shared__ __attribute__((aligned(16))) float s_rest[SPLIT ? 4 : 64], p_rest[SPLIT ? 4 : 64];   // of the diagonals
   const int i = blockIdx.x, rows = t.rows[i], columns = t.columns[i];
-  if (is_thin(rows, columns, SPLIT)) {
+  if (s.thin && is_thin(rows, columns, SPLIT)) {
     static_assert(Z::THREADS == 64 * kThinWaves && Z::BYTES >= kThinWaves * 4 * 64 * 8, "threads and LDS of both");
     thin_matrix((const T*)t.g[i], t.m[i], (T*)t.p[i], rows, columns, t.rate[i], s, steps, (double (*)[4][64])lds);
     return;
@@ -1226,10 +1244,10 @@ void run_group(Table& t, int used, const Settings& s, int steps, char* workspace
 }
 
 // Whether one workgroup takes the matrix.  Three matrices of 16 x 27 to 64 x 288 in float32, a step of each, 43 us for 110
-// through the launches.
-bool is_small(int64_t rows, int64_t columns, int dtype) {
+// through the launches.  thin: whether the steps may go by S alone.
+bool is_small(int64_t rows, int64_t columns, int dtype, bool thin) {
   const int64_t k = std::min(rows, columns), l = std::max(rows, columns);
-  return is_thin(rows, columns, split(dtype)) ||
+  return (thin && is_thin(rows, columns, split(dtype))) ||
          (k <= 64 && l <= (split(dtype) ? Small<true>::LP : Small<false>::LP));
 }
 
@@ -1237,7 +1255,7 @@ bool is_small(int64_t rows, int64_t columns, int dtype) {
 // launch holds.  `run` gets a table and how many it holds; returns the bytes of the largest group.
 // small: those that a workgroup takes alone, or the others.
 template <typename Get, typename Run>
-size_t in_groups(int64_t count, int dtype, bool small, Get get, Run run) {
+size_t in_groups(int64_t count, int dtype, bool thin, bool small, Get get, Run run) {
   Table t = {};
   int used = 0;
   int64_t bytes = 0, most = 0, tiles = 0;
@@ -1248,7 +1266,7 @@ size_t in_groups(int64_t count, int dtype, bool small, Get get, Run run) {
   };
   for (int64_t i = 0; i < count; ++i) {
     const Matrix x = get(i);
-    if (x.rows < 1 || x.columns < 1 || is_small(x.rows, x.columns, dtype) != small) continue;
+    if (x.rows < 1 || x.columns < 1 || is_small(x.rows, x.columns, dtype, thin) != small) continue;
     const Layout at(x.rows, x.columns, split(dtype));
     const int64_t mine = std::max(at.kp / 64 * (at.lp / 64), ceil_div(x.rows * x.columns, kPerGroup));
     if (used == kMatrices || tiles + mine > most_groups(256)) done();
@@ -1259,6 +1277,13 @@ size_t in_groups(int64_t count, int dtype, bool small, Get get, Run run) {
   }
   done();
   return (size_t)most;
+}
+
+// The workspace that is enough for any steps and coefficients.
+template <typename Get>
+size_t most_bytes(int64_t count, int dtype, Get get) {
+  const auto none = [](Table&, int) {};
+  return std::max(in_groups(count, dtype, true, false, get, none), in_groups(count, dtype, false, false, get, none));
 }
 
 constexpr int64_t kMostSide = 1 << 17;
@@ -1272,10 +1297,13 @@ int check_matrix(int64_t rows, int64_t columns) {
 
 // X begins with a norm of 1 at most, and a step makes of a singular value x the value x q(x^2), q(s) = a + b s + c s^2.
 // Followed from 1 on, no value may pass 3.8, so that S stays below 15, and no q of one 15.
-int check_coefficients(int64_t steps, const double* k) {
+// thin: whether errors of S grow little enough for the steps to go by S alone: f(s) = s q(s)^2 has the slope q(s) r(s),
+// r(s) = a + 3 b s + 5 c s^2.
+int check_coefficients(int64_t steps, const double* k, bool& thin) {
   const double a = k[0], b = k[1], c = k[2];
   auto q = [&](double s) { return std::fabs(a + (b + c * s) * s); };
-  double most = 1;
+  auto r = [&](double s) { return std::fabs(a + (3 * b + 5 * c * s) * s); };
+  double most = 1, growth = 1;
   for (int64_t step = 0; step < steps; ++step) {
     const double end = most * most;
     double of_q = std::max(q(0), q(end)), next = most * q(end);
@@ -1293,12 +1321,16 @@ int check_coefficients(int64_t steps, const double* k) {
     SDK_REQUIRE(of_q <= 15 && next <= 3.8,
                 "coefficients %g, %g, %g let singular values or the polynomial grow too far (3.8 and 15) in step %lld", a, b, c,
                 (long long)step + 1);
+    const double turn = -3 * b / (10 * c);   // c = 0: no number, or none inside
+    const double of_r = std::max({r(0), r(end), turn > 0 && turn < end ? r(turn) : 0.});
+    growth = std::min(growth * std::max(1., of_q * of_r), 2 * kMostGrowth);
     most = std::max(1e-30, next);
   }
+  thin = growth <= kMostGrowth;
   return SDK_OK;
 }
 
-int check_settings(int64_t count, int64_t steps, const double* coefficients, double eps, int dtype) {
+int check_settings(int64_t count, int64_t steps, const double* coefficients, double eps, int dtype, bool& thin) {
   SDK_REQUIRE(known(dtype), "unknown dtype %d (float32, bfloat16 and float16 only)", dtype);
   SDK_REQUIRE(count >= 0, "count must not be negative");
   SDK_REQUIRE(steps >= 1 && steps <= 100, "steps = %lld must be between 1 and 100", (long long)steps);
@@ -1306,26 +1338,27 @@ int check_settings(int64_t count, int64_t steps, const double* coefficients, dou
   for (int i = 0; i < 3; ++i)
     SDK_REQUIRE(std::fabs(coefficients[i]) <= 100, "coefficients must be numbers up to 100 in magnitude");
   SDK_REQUIRE(eps >= 0x1p-100 && eps <= 1, "eps = %g must be between 2^-100 and 1", eps);
-  return check_coefficients(steps, coefficients);
+  return check_coefficients(steps, coefficients, thin);
 }
 
-Settings settings_of(const double* c, double eps) {
+Settings settings_of(const double* c, double eps, bool thin) {
   Settings s = {};
   s.a = (float)c[0], s.b = (float)c[1], s.c = (float)c[2], s.eps = (float)eps;
-  s.a64 = c[0], s.b64 = c[1], s.c64 = c[2];
+  s.a64 = c[0], s.b64 = c[1], s.c64 = c[2], s.thin = thin;
   return s;
 }
 
 int run_all(int64_t count, int steps, const Settings& s, void* workspace, size_t workspace_bytes, int dtype,
             sdk_stream_t stream, Matrix (*get)(const void*, int64_t), const void* context) {
   auto of = [&](int64_t i) { return get(context, i); };
-  const size_t need = in_groups(count, dtype, false, of, [](Table&, int) {});
+  const bool thin = s.thin;
+  const size_t need = in_groups(count, dtype, thin, false, of, [](Table&, int) {});
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 128))
     return fail(SDK_ERR_WORKSPACE, "workspace of %zu bytes at a multiple of 128, %zu needed", workspace_bytes, need);
-  in_groups(count, dtype, true, of, [&](Table& t, int used) {
+  in_groups(count, dtype, thin, true, of, [&](Table& t, int used) {
     SDK_DISPATCH_TOKEN_DTYPE(dtype, launch(small_matrix<T>, dim3(used), dim3(512), (hipStream_t)stream, t, s, steps));
   });
-  in_groups(count, dtype, false, of, [&](Table& t, int used) {
+  in_groups(count, dtype, thin, false, of, [&](Table& t, int used) {
     SDK_DISPATCH_TOKEN_DTYPE(dtype, run_group<T>(t, used, s, steps, (char*)workspace, (hipStream_t)stream));
   });
   return SDK_OK;
@@ -1371,19 +1404,19 @@ extern "C" {
 size_t sdk_orthogonalize_workspace_bytes(int64_t rows, int64_t columns, int64_t count, int32_t dtype) {
   if (check_matrix(rows, columns) != SDK_OK || !known(dtype) || count < 0) return 0;
   count = std::min<int64_t>(count, kMatrices);
-  return in_groups(count, dtype, false, [&](int64_t) { return Matrix{nullptr, nullptr, nullptr, rows, columns, 0.f}; },
-                   [](Table&, int) {});
+  return most_bytes(count, dtype, [&](int64_t) { return Matrix{nullptr, nullptr, nullptr, rows, columns, 0.f}; });
 }
 
 int sdk_orthogonalize(const void* x, void* out, int64_t rows, int64_t columns, int64_t count, int32_t steps,
                       const double* coefficients, double eps, void* workspace, size_t workspace_bytes, int32_t dtype,
                       sdk_stream_t stream) {
-  if (int rc = check_settings(count, steps, coefficients, eps, dtype)) return rc;
+  bool thin = false;
+  if (int rc = check_settings(count, steps, coefficients, eps, dtype, thin)) return rc;
   if (int rc = check_matrix(rows, columns)) return rc;
   if (!count || !rows || !columns) return SDK_OK;
   SDK_REQUIRE(x && out, "x and out must not be NULL");
   const Stack stack = {(const char*)x, (char*)out, rows, columns, rows * columns * (int64_t)bytes_of(dtype)};
-  const int rc = run_all(count, steps, settings_of(coefficients, eps), workspace, workspace_bytes, dtype, stream,
+  const int rc = run_all(count, steps, settings_of(coefficients, eps, thin), workspace, workspace_bytes, dtype, stream,
                          [](const void* context, int64_t i) {
                            const Stack& s = *(const Stack*)context;
                            return Matrix{s.out + i * s.bytes, s.x + i * s.bytes, nullptr, s.rows, s.columns, 0.f};
@@ -1398,15 +1431,15 @@ size_t sdk_muon_step_workspace_bytes(const int64_t* rows, const int64_t* columns
   if (!known(dtype) || count < 1 || !rows || !columns) return 0;
   for (int64_t i = 0; i < count; ++i)
     if (check_matrix(rows[i], columns[i]) != SDK_OK) return 0;
-  return in_groups(count, dtype, false, [&](int64_t i) { return Matrix{nullptr, nullptr, nullptr, rows[i], columns[i], 0.f}; },
-                   [](Table&, int) {});
+  return most_bytes(count, dtype, [&](int64_t i) { return Matrix{nullptr, nullptr, nullptr, rows[i], columns[i], 0.f}; });
 }
 
 int sdk_muon_step(void* const* params, const void* const* grads, float* const* momenta, const int64_t* rows,
                   const int64_t* columns, int64_t count, double lr, double momentum, int32_t nesterov,
                   double weight_decay, int32_t steps, const double* coefficients, double eps, void* workspace,
                   size_t workspace_bytes, int32_t dtype, sdk_stream_t stream) {
-  if (int rc = check_settings(count, steps, coefficients, eps, dtype)) return rc;
+  bool thin = false;
+  if (int rc = check_settings(count, steps, coefficients, eps, dtype, thin)) return rc;
   SDK_REQUIRE(lr >= 0 && weight_decay >= 0 && momentum >= 0 && momentum < 1 && lr <= 1e30 && weight_decay <= 1e30,
               "lr and weight_decay must not be negative, momentum in [0, 1)");
   if (!count) return SDK_OK;
@@ -1419,7 +1452,7 @@ int sdk_muon_step(void* const* params, const void* const* grads, float* const* m
     any = true;
   }
   if (!any) return SDK_OK;
-  Settings s = settings_of(coefficients, eps);
+  Settings s = settings_of(coefficients, eps, thin);
   s.mu = (float)momentum, s.rest = (float)(1 - momentum), s.keep = (float)(1 - lr * weight_decay);
   s.nesterov = nesterov != 0;
   const Lists lists = {params, grads, momenta, rows, columns, lr};
