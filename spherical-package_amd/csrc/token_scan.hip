@@ -1,14 +1,14 @@
 // Gated linear recurrence along the tokens of sequences, with gradients, and its step for single tokens.
 //
-//   f_t = sigmoid(gate_t),  u_t = 1 - f_t        h_t = f_t h_{t-1} + u_t x_t = h_{t-1} + u_t (x_t - h_{t-1})
+//   f_t = sigmoid(gate_t),  u_t = 1 - f_t        h_t = f_t h_{t-1} + u_t x_t
 //   e_t = g_t + c_t,  c_{t-1} = f_t e_t          (g: the gradient of h_t; c behind the last token: that of the last state)
 //   dx_t = u_t e_t    dgate_t = e_t (h_{t-1} - x_t) f_t u_t    gradient of the first state = c in front of the first token
 //
 // Each channel by itself.  A span of tokens acts on the state before it as h -> A h + H, and spans join: (A, H) then
 // (A', H') is (A A', A' H + H').  So a workgroup takes 64 channels in 16 bits (32 in float32: 128 bytes of a token either
 // way; a quarter of that where the width is no larger) and a tile of tokens, of which each thread walks 32 values
-// (backward 16: two to eight tokens) in order; the threads' spans are joined over the tile, and each walks its tokens again from the state in front of them.  The
-// tile's values stay in registers meanwhile.  Where batch and channels fill the GPU a workgroup goes through a whole
+// (backward 16: two to eight tokens) in order; the threads' spans are joined over the tile, and each walks its tokens again
+// from the state in front of them.  The tile's values stay in registers meanwhile.  Where batch and channels fill the GPU a workgroup goes through a whole
 // sequence; otherwise it takes one tile, and tiles hand each other their spans while the kernel runs (scan_tiles).
 //
 // Bound by memory: three values read or written a token and channel forward, six backward (the gradients read h as
@@ -17,8 +17,12 @@
 // first launch for the spans of longer segments, which then were read again, took 49 and 74 us.  131072 tokens of 256
 // channels in float16 forward: 53 us (3.8 TB/s; 95 with two launches).
 //
-// The state, its gradient, the spans and the gates are float32.  u weighs the distance x - h: 1 - f of a rounded f near one
-// would be off by a part of all that a long memory sums up.
+// The state, its gradient, the spans and the gates are float32.  Of f and u the lesser is formed, to its own relative
+// precision, and weighs the distance of h and x:
+//   open, f >= u:  h_t = h + u (x - h)        closed:  h_t = x + f (h - x)
+// 1 - f of a rounded f near one would be off by a part of all that a long memory sums up, 1 - u of a rounded u near one by
+// all that a closed gate leaves: at a gate of -14 by 3e-3 of f, from -18 on by f itself, in the gates' gradient and that of
+// the states before, and a state of 1e4 would leave 2^-24 of itself where 1e-4 replaces it.
 #include <algorithm>
 #include <type_traits>
 
@@ -50,21 +54,29 @@ struct Scan {
   int reverse;
 };
 
-// u = 1 - sigmoid(g) = 1 / (1 + e^g), to its relative precision also where it is small; f is only ever formed as c - c u.
+// The lesser of f = sigmoid(g) and u = 1 - f, e / (1 + e) with e = e^-|g|, to its relative precision; its sign says which it
+// is: f where it is +, a closed gate, u where it is -.
 // FINE: to a few units of the last place (the power's argument in two parts, a correction of the reciprocal); 16-bit gates,
-// whose results round to 16 bits, do without (5e-7 of u at gates of 8).
+// whose results round to 16 bits, do without (5e-7 of it at gates of 8, 2e-6 at 30).
 template <bool FINE>
-__device__ __forceinline__ float unkept(float g) {
+__device__ __forceinline__ float gate_of(float g) {
   constexpr float kLog2e = 1.44269502e+00f, kLog2eRest = 1.92596303e-08f, kLn2 = 6.93147182e-01f;
-  const float t = g * kLog2e;
+  const float m = -fabsf(g), t = m * kLog2e;
   float e = __builtin_amdgcn_exp2f(t);
-  if constexpr (!FINE) return __builtin_amdgcn_rcpf(1.f + e);
-  const bool middle = fabsf(t) < 126.f;   // beyond it u is e^-g or 1 (or NaN), and corrections would be no numbers
-  const float rest = fmaf(g, kLog2eRest, fmaf(g, kLog2e, -t));
-  if (middle) e = fmaf(e * rest, kLn2, e);
-  const float d = 1.f + e, u = __builtin_amdgcn_rcpf(d);
-  return middle ? fmaf(fmaf(-d, u, 1.f), u, u) : u;
+  if constexpr (FINE) {
+    const float rest = fmaf(m, kLog2eRest, fmaf(m, kLog2e, -t));
+    if (t > -126.f) e = fmaf(e * rest, kLn2, e);   // beyond it e is zero or nearly, and the rest may be no number
+  }
+  const float d = 1.f + e;
+  float inverse = __builtin_amdgcn_rcpf(d);
+  if constexpr (FINE) inverse = fmaf(fmaf(-d, inverse, 1.f), inverse, inverse);
+  return copysignf(e * inverse, -g);
 }
+__device__ __forceinline__ bool closed(float s) { return __float_as_int(s) >= 0; }
+// f h + u x
+__device__ __forceinline__ float mixed(float s, float h, float x) { return fmaf(s, h - x, closed(s) ? x : h); }
+// f c
+__device__ __forceinline__ float kept(float s, float c) { return fmaf(s, c, closed(s) ? 0.f : c); }
 
 // h -> a h + b, for each of V channels
 template <int V>
@@ -166,6 +178,15 @@ __device__ __forceinline__ void load_state(const float* p, int64_t at, float (&f
   if (p && left > 0) load_part<float, V>(p + at, f, left);
 }
 
+// 16 bytes of which the compiler no longer knows what has been made of them.
+template <typename Raw>
+__device__ __forceinline__ void anew(Raw& raw) {
+  typedef unsigned Words __attribute__((ext_vector_type(4)));
+  Words w = __builtin_bit_cast(Words, raw);
+  asm("" : "+v"(w));
+  raw = __builtin_bit_cast(Raw, w);
+}
+
 // ROWS tokens of a thread in the order of the walk, as they lie in memory, and what the walk does with them.  Forward they
 // are at, at + 1, ..; backward at, at - 1, ..  FULL: all of the workgroup's tokens and channels count.
 template <typename T, int LANES, bool ALIGNED, bool BACKWARD, int ROWS>
@@ -173,7 +194,7 @@ struct Walk {
   static constexpr int V = kWide<T>;
   static constexpr bool FINE = sizeof(T) == 4;
   static constexpr int STEP = BACKWARD ? -1 : 1;
-  float u[ROWS][V];                       // the gate until open() or span()
+  float s[ROWS][V];                       // the gate until open() or span(), which make it gate_of()
   Pack<T, V> x[ROWS], g[BACKWARD ? ROWS : 1], h[BACKWARD ? ROWS : 1];
   bool inside[ROWS], counts[ROWS];
 
@@ -197,7 +218,7 @@ struct Walk {
         for (int e = 0; e < V; ++e) g[r].v[e] = (T)0.f;
       }
       if (counts[r]) {
-        get<T, V, ALIGNED>(pgate + r * gate_way, u[r], place.left);
+        get<T, V, ALIGNED>(pgate + r * gate_way, s[r], place.left);
         get_raw<T, V, ALIGNED>(px + r * x_way, x[r], place.left);
         if constexpr (BACKWARD) {
           if (p.grad) get_raw<T, V, ALIGNED>(pgrad + r * grad_way, g[r], place.left);
@@ -214,30 +235,28 @@ struct Walk {
     for (int r = 0; r < ROWS; ++r)
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (counts[r]) u[r][e] = unkept<FINE>(u[r][e]);
+        if (counts[r]) s[r][e] = gate_of<FINE>(s[r][e]);
   }
 
   // The same, and what the tokens do to the state in front of them.
   template <bool FULL>
   __device__ __forceinline__ Span<V> span() {
-    Span<V> s;
-    unit(s);
+    Span<V> all;
+    unit(all);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
       if (FULL || counts[r]) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          u[r][e] = unkept<FINE>(u[r][e]);
-          if constexpr (BACKWARD) {
-            const float c = (float)g[r].v[e] + s.b[e];
-            s.b[e] = fmaf(-u[r][e], c, c);
-          } else {
-            s.b[e] = fmaf(u[r][e], (float)x[r].v[e] - s.b[e], s.b[e]);
-          }
-          s.a[e] = fmaf(-u[r][e], s.a[e], s.a[e]);
+          s[r][e] = gate_of<FINE>(s[r][e]);
+          if constexpr (BACKWARD)
+            all.b[e] = kept(s[r][e], (float)g[r].v[e] + all.b[e]);
+          else
+            all.b[e] = mixed(s[r][e], all.b[e], (float)x[r].v[e]);
+          all.a[e] = kept(s[r][e], all.a[e]);
         }
       }
-    return s;
+    return all;
   }
 
   // The results of the tokens, given the state in front of them.
@@ -245,6 +264,12 @@ struct Walk {
   __device__ __forceinline__ void finish(const Scan& p, const Place<T, LANES>& place, int64_t at, float (&in)[V]) {
     const int64_t way = ((p.reverse != 0) != BACKWARD ? -1 : 1) * p.width;
     const int64_t begin = (place.b * p.tokens + place.row(p, at)) * p.width + place.channel;
+    if constexpr (BACKWARD) {
+      // x and g are converted again here: kept from span() in 32 bits they leave no registers (scan_whole in 16 bits: 135 us
+      // for 101; of the forward's one tensor they do not count)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) anew(x[r]), anew(g[r]);
+    }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       if (!FULL && !inside[r]) continue;
@@ -263,12 +288,13 @@ struct Walk {
         if (!FULL) y[e] = z[e] = 0.f;
         if (FULL || counts[r]) {
           if constexpr (BACKWARD) {
-            const float c = (float)g[r].v[e] + in[e];
-            in[e] = fmaf(-u[r][e], c, c);
-            y[e] = c * u[r][e];
-            z[e] = in[e] * u[r][e] * (before[e] - (float)x[r].v[e]);
+            const float c = (float)g[r].v[e] + in[e], lesser = fabsf(s[r][e]);
+            const float less = lesser * c, more = fmaf(-lesser, c, c);
+            in[e] = closed(s[r][e]) ? less : more;
+            y[e] = closed(s[r][e]) ? more : less;
+            z[e] = more * lesser * (before[e] - (float)x[r].v[e]);
           } else {
-            y[e] = in[e] = fmaf(u[r][e], (float)x[r].v[e] - in[e], in[e]);
+            y[e] = in[e] = mixed(s[r][e], in[e], (float)x[r].v[e]);
           }
         }
       }
@@ -306,8 +332,10 @@ template <bool BACKWARD, int V>
 constexpr int kRows = (BACKWARD ? 16 : 32) / V;
 
 // Whole sequences, tile by tile: a workgroup a batch element and block of channels.
+// (Backward two waves a SIMD, without which the compiler takes registers for one: 64 x 512 tokens of 1024 channels in
+// bfloat16 188 us for 101.  Forward it arrives at two by itself, and is slower if told: 48 us for 45.)
 template <typename T, int LANES, bool ALIGNED, bool BACKWARD>
-__global__ __launch_bounds__(kThreads) void scan_whole(const Scan p) {
+__global__ __launch_bounds__(kThreads, BACKWARD ? 2 : 1) void scan_whole(const Scan p) {
   constexpr int V = kWide<T>, WAVES = kThreads / 64, ROWS = kRows<BACKWARD, V>, TILE = kThreads / LANES * ROWS;
   __shared__ float slots[2][2 * WAVES * LANES * V];
   const Place<T, LANES> place(p, blockIdx.x, 0);
@@ -504,7 +532,7 @@ __global__ __launch_bounds__(256) void scan_step(const T* x, int64_t x_stride, c
   load_part<float, V>(state + b * state_stride + c, h, left);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    h[e] = fmaf(unkept<sizeof(T) == 4>(fg[e]), fx[e] - h[e], h[e]);
+    h[e] = mixed(gate_of<sizeof(T) == 4>(fg[e]), h[e], fx[e]);
   }
   store_part<float, V>(state + b * state_stride + c, h, left);
   put<T, V, ALIGNED>(out + b * width + c, h, left);

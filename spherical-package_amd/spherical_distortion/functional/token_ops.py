@@ -211,8 +211,9 @@ def gated_scan(input, gate, state=None, lengths=None, reverse=False):
     (others are copied); h like them, dense.  state: h in front of the first token, float32 [B, width] (None: zeros);
     the last state, float32 too, is h behind the last token.  lengths (int32 [B]): tokens from lengths[b] on do not
     count; input and gate are not read there, h and the gradients are zeros.  reverse: from the last token that counts
-    to the first.  The state is float32 throughout and h is rounded once; inputs or states that are not finite give NaN
-    from there on.  With gradients for input, gate and state; second derivatives and forward mode raise.
+    to the first.  The state is float32 throughout and h is rounded once; of f and 1 - f the lesser is formed to its own
+    precision, so closed gates (of -8 and below) have all their digits too.  Inputs or states that are not finite give NaN
+    or infinities from there on.  With gradients for input, gate and state; second derivatives and forward mode raise.
 
     Long sequences of few channels are cut into segments that are worked on side by side."""
     if "gated_scan" in _token_ops.NATIVE_OPS:
