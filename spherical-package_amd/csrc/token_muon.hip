@@ -1316,8 +1316,10 @@ int check_coefficients(int64_t steps, const double* k, bool& thin) {
     };
     inside(-b / (2 * c), false);   // c = 0: no number, or none inside
     const double root = 9 * b * b - 20 * a * c;
-    if (root >= 0) inside((-3 * b + std::sqrt(root)) / (10 * c), true), inside((-3 * b - std::sqrt(root)) / (10 * c), true);
-    if (c == 0) inside(-a / (3 * b), true);
+    if (root >= 0) {   // of r; the second from their product, where -3 b less a root of nearly 3 b would leave nothing
+      const double sum = -3 * b - std::copysign(std::sqrt(root), b);
+      inside(sum / (10 * c), true), inside(2 * a / sum, true);
+    }
     SDK_REQUIRE(of_q <= 15 && next <= 3.8,
                 "coefficients %g, %g, %g let singular values or the polynomial grow too far (3.8 and 15) in step %lld", a, b, c,
                 (long long)step + 1);

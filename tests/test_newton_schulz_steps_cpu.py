@@ -3,6 +3,7 @@ touches the device."""
 import ctypes
 
 import pytest
+import torch
 
 ONE = ctypes.c_void_p(256)   # aligned, never dereferenced
 NS = (3.4445, -4.7750, 2.0315)
@@ -42,3 +43,42 @@ def test_workspaces_hold_either_way(lib):
     rows, columns = (ctypes.c_int64 * n)(*[16] * 65, 100), (ctypes.c_int64 * n)(*[1000] * 65, 100)
     assert lib.sdk_muon_step_workspace_bytes(rows, columns, n, 0) == max(64 * thin, thin + large, large)
     assert size(16, 300, 9, 0) == 0   # short ones need none either way
+
+
+def _allowed(steps, c):
+    from _spherical_distortion_ext import _token_ops
+    try:
+        _token_ops.check_newton_schulz(steps, c, 1e-7)
+    except RuntimeError as e:
+        assert "grow too far" in str(e)
+        return False
+    return True
+
+
+@pytest.mark.parametrize("c", [1e-20, -1e-20, 1e-300, 5e-324, 1e-12, -1e-9, 0.0])
+def test_extremes_beside_a_last_coefficient_of_nearly_nothing(c):
+    """15 x - 15 x^3 is 5.77 at sqrt(1/3), 9 x - 9 x^3 3.46; 3 x - x^3 reaches 2 at 1, from where it goes to -2 at 2; 6 x + 3.2 x^3
+    only grows; 1.5 x - 0.5 x^3 stays at one."""
+    assert not _allowed(1, (15.0, -15.0, c)) and not _allowed(2, (15.0, -15.0, c)) and not _allowed(1, (-15.0, 15.0, c))
+    assert _allowed(1, (9.0, -9.0, c)) and _allowed(1, (-9.0, 9.0, c)) and not _allowed(2, (9.0, -9.0, c))
+    assert _allowed(3, (3.0, -1.0, c))
+    assert not _allowed(1, (6.0, 3.2, c)) and _allowed(100, (1.5, -0.5, c))
+
+
+def test_extremes_of_small_last_coefficients():
+    """Against the polynomial at many points, which miss an extreme by 1e-8 of it."""
+    g = torch.Generator().manual_seed(1)
+    seen = set()
+    for _ in range(300):
+        a, b, c = ((torch.rand(3, generator=g, dtype=torch.float64) * 2 - 1) * torch.tensor([15.0, 20.0, 1.0])).tolist()
+        c *= 10.0 ** -float(torch.randint(1, 22, (1,), generator=g))
+        most, good, near = 1.0, True, False
+        for _ in range(2):
+            x = torch.linspace(0, most, 20001, dtype=torch.float64)
+            q = (a + b * x ** 2 + c * x ** 4).abs()
+            good = good and float(q.max()) <= 15 and float((x * q).max()) <= 3.8
+            near = near or abs(float(q.max()) - 15) < 1e-5 or abs(float((x * q).max()) - 3.8) < 1e-5
+            most = float((x * q).max())
+        assert near or _allowed(2, (a, b, c)) == good, (a, b, c)
+        seen.add(good)
+    assert seen == {True, False}
