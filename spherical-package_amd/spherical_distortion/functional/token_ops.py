@@ -270,7 +270,7 @@ def adamw_moment_values(codes, scales, dtype=torch.float32):
 
 
 #: a, b, c of orthogonalize: steep at zero (3.4 times a step), so that five steps bring singular values from 0.002 of the
-#: norm on to between 0.68 and 1.14.
+#: norm on to between 0.68 and 1.21.
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 

@@ -102,3 +102,28 @@ def test_matrices_of_few_rows_beside_others(steps, dtype):
         F.muon_step(*(ts[i:i + 1] for ts in alone), lr=0.1, steps=steps)
     for ts, us in zip(lists, alone):
         assert all(torch.equal(t, u) and bool(t.isfinite().all()) for t, u in zip(ts, us))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(12, 40), (60, 60), (200, 90)])
+def test_singular_values_go_where_the_polynomial_takes_them(shape, dtype):
+    """Spread over 0.001 to 0.7 of the norm, so that some end near its maximum of 1.2024.  Of the slack each value takes what the
+    slope of five steps makes of it (the product of their slopes, at most 3.4445^5 for the smallest): bounded over the matrix
+    as the largest slope times the rounding of the matrix and a step, 2^-22 or 2^-12, and the slack itself."""
+    from spherical_distortion import functional as F
+    g = torch.Generator().manual_seed(sum(shape))
+    k = min(shape)
+    u, v = (torch.linalg.qr(torch.randn(n, k, generator=g, dtype=torch.float64))[0] for n in shape)
+    x = ((u * torch.logspace(0, -2.5, k, dtype=torch.float64)) @ v.t()).to(dtype).to(DEV)
+    s = _values(x)
+    s = s / s.norm()
+    slope = torch.ones_like(s)
+    for _ in range(5):
+        slope = slope * (NS[0] + 3 * NS[1] * s ** 2 + 5 * NS[2] * s ** 4).abs()
+        s = NS[0] * s + NS[1] * s ** 3 + NS[2] * s ** 5
+    got = _values(F.orthogonalize(x))
+    assert float(s.max()) > 1.19
+    unit = 2.0 ** (-12 if dtype == torch.bfloat16 else -22)
+    off = (got - s.sort(descending=True).values).abs().max()
+    assert float(off) <= _slack(dtype) + float(slope.max()) * unit
+    assert float(got.max()) <= 1.2024 + _slack(dtype)

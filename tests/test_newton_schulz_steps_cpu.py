@@ -82,3 +82,17 @@ def test_extremes_of_small_last_coefficients():
         assert near or _allowed(2, (a, b, c)) == good, (a, b, c)
         seen.add(good)
     assert seen == {True, False}
+
+
+def test_five_default_steps_as_documented():
+    """Singular values of 0.002 of the norm and more end between 0.68 and 1.21, as the documentation of NEWTON_SCHULZ says: the
+    polynomial at 2 * 10^6 points, between which five steps of a slope of 3.4445 at most move it by 5e-7 * 3.4445^5 = 2.4e-4."""
+    import inspect
+
+    from spherical_distortion.functional import token_ops
+    a, b, c = token_ops.NEWTON_SCHULZ
+    x = torch.linspace(0.002, 1, 2000001, dtype=torch.float64)
+    for _ in range(5):
+        x = a * x + b * x ** 3 + c * x ** 5
+    assert 0.68 + 2.4e-4 <= float(x.min()) and float(x.max()) <= 1.21 - 2.4e-4
+    assert "between 0.68 and 1.21" in inspect.getsource(token_ops) and float(x.max()) > 1.2
