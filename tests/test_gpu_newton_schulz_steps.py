@@ -127,3 +127,15 @@ def test_singular_values_go_where_the_polynomial_takes_them(shape, dtype):
     off = (got - s.sort(descending=True).values).abs().max()
     assert float(off) <= _slack(dtype) + float(slope.max()) * unit
     assert float(got.max()) <= 1.2024 + _slack(dtype)
+
+
+def test_gradients_are_refused_or_not_wanted():
+    from spherical_distortion import functional as F
+    x = torch.randn(20, 30, device=DEV)
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        F.orthogonalize(leaf)
+    want = F.orthogonalize(x)
+    assert not want.requires_grad and torch.equal(F.orthogonalize(leaf.detach()), want)
+    with torch.no_grad():
+        assert torch.equal(F.orthogonalize(leaf), want)
