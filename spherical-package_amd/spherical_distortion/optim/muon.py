@@ -12,7 +12,7 @@ class Muon(torch.optim.Optimizer):
 
     params: float32, bfloat16 or float16, contiguous, two axes at least; [out, ..] counts as a matrix of `out` rows.  Others
     (biases, norms' weights, tables looked up by row) belong to another optimizer.  Momenta are float32.  One without a
-    gradient is left as it is.  A step checks every parameter before it changes one."""
+    gradient is left as it is.  A step checks every group and parameter before it changes one."""
 
     def __init__(self, params, lr=2e-2, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
                  coefficients=F.NEWTON_SCHULZ, eps=1e-7):
@@ -20,23 +20,50 @@ class Muon(torch.optim.Optimizer):
                                       coefficients=tuple(coefficients), eps=eps))
 
     @staticmethod
-    def _check(group):
-        if not group["lr"] >= 0 or not group["weight_decay"] >= 0:
-            raise ValueError("lr and weight_decay must not be negative")
+    def _check_settings(group):
+        if not 0 <= group["lr"] <= 1e30 or not 0 <= group["weight_decay"] <= 1e30:
+            raise ValueError("lr and weight_decay must not be negative (or beyond 1e30)")
         if not 0 <= group["momentum"] < 1:
             raise ValueError("momentum must be in [0, 1), got %s" % group["momentum"])
         try:
             _token_ops.check_newton_schulz(group["steps"], group["coefficients"], group["eps"])
         except RuntimeError as e:
             raise ValueError(str(e)) from None
-        for p in group["params"]:
-            if p.dim() < 2:
-                raise ValueError("Muon takes parameters of two axes at least, got one of shape %s" % (tuple(p.shape),))
+
+    @staticmethod
+    def _check_shape(p):
+        if p.dim() < 2:
+            raise ValueError("Muon takes parameters of two axes at least, got one of shape %s" % (tuple(p.shape),))
+        rows = p.shape[0]
+        if max(rows, p.numel() // rows if rows else 0) > 1 << 17 or p.numel() > 1 << 31:
+            raise ValueError("Muon takes matrices with sides up to 131072 and 2^31 values, got a parameter of shape %s"
+                             % (tuple(p.shape),))
+
+    def _check_step(self):
+        """All that a call would refuse, of every group before one is stepped."""
+        stepped = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
+        for group in self.param_groups:
+            self._check_settings(group)
+        for p in stepped:
+            adamw.check_parameter("Muon", p)
+            m = self.state[p].get("momentum") if p in self.state else None
+            if m is not None and not (m.shape == p.shape and m.dtype == torch.float32 and m.device == p.device
+                                      and m.is_contiguous()):
+                raise RuntimeError("a momentum must be float32, contiguous and beside its parameter of shape %s, got %s %s on %s"
+                                   % (tuple(p.shape), m.dtype, tuple(m.shape), m.device))
+        written = [p.data_ptr() for p in stepped if p.numel()]
+        addresses = set(written)
+        if len(addresses) < len(written):
+            raise RuntimeError("a parameter is listed twice")
+        if any(p.grad.data_ptr() in addresses for p in stepped if p.numel()):
+            raise RuntimeError("a gradient is a parameter too")
 
     def add_param_group(self, group):
         super().add_param_group(group)
         try:
-            self._check(self.param_groups[-1])
+            self._check_settings(self.param_groups[-1])
+            for p in self.param_groups[-1]["params"]:
+                self._check_shape(p)
         except ValueError:
             self.param_groups.pop()
             raise
@@ -47,10 +74,7 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.grad is not None:
-                    adamw.check_parameter("Muon", p)
+        self._check_step()
         for group in self.param_groups:
             settings = {k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps")}
             calls = {}   # (type, device) -> lists of tensors
