@@ -81,7 +81,8 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                m = self.state[p]["momentum"] if p in self.state else torch.zeros(p.shape, device=p.device)
+                m = (self.state[p]["momentum"] if p in self.state
+                     else torch.zeros(p.shape, dtype=torch.float32, device=p.device))
                 for to, t in zip(calls.setdefault((p.dtype, p.device), ([], [], [])), (p, p.grad.contiguous(), m)):
                     to.append(t)
             for lists in calls.values():

@@ -86,3 +86,17 @@ def test_sides_that_no_call_takes():
             optimizer.add_param_group(dict(params=[big]))
         assert len(optimizer.param_groups) == 1
     Muon([torch.nn.Parameter(torch.empty(1).expand(1 << 17, 1 << 14)), torch.nn.Parameter(torch.empty(0, 1 << 20))])
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_momenta_are_float32_whatever_the_default_type(steps, default):
+    from spherical_distortion.optim import Muon
+    p = _param(4, 5)
+    optimizer = Muon([p])
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        optimizer.step()
+    finally:
+        torch.set_default_dtype(before)
+    assert optimizer.state[p]["momentum"].dtype == torch.float32
