@@ -39,6 +39,9 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("Muon takes matrices with sides up to 131072 and 2^31 values, got a parameter of shape %s"
                              % (tuple(p.shape),))
 
+    def _momentum(self, p):
+        return self.state.get(p, {}).get("momentum")   # looking it up by [] would make an entry
+
     def _check_step(self):
         """All that a call would refuse, of every group before one is stepped."""
         stepped = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
@@ -46,7 +49,7 @@ class Muon(torch.optim.Optimizer):
             self._check_settings(group)
         for p in stepped:
             adamw.check_parameter("Muon", p)
-            m = self.state[p].get("momentum") if p in self.state else None
+            m = self._momentum(p)
             if m is not None and not (m.shape == p.shape and m.dtype == torch.float32 and m.device == p.device
                                       and m.is_contiguous()):
                 raise RuntimeError("a momentum must be float32, contiguous and beside its parameter of shape %s, got %s %s on %s"
@@ -81,8 +84,9 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                m = (self.state[p]["momentum"] if p in self.state
-                     else torch.zeros(p.shape, dtype=torch.float32, device=p.device))
+                m = self._momentum(p)
+                if m is None:
+                    m = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 for to, t in zip(calls.setdefault((p.dtype, p.device), ([], [], [])), (p, p.grad.contiguous(), m)):
                     to.append(t)
             for lists in calls.values():

@@ -100,3 +100,13 @@ def test_momenta_are_float32_whatever_the_default_type(steps, default):
     finally:
         torch.set_default_dtype(before)
     assert optimizer.state[p]["momentum"].dtype == torch.float32
+
+
+def test_a_state_that_was_only_looked_at(steps):
+    """optimizer.state makes an entry for whoever is looked up."""
+    from spherical_distortion.optim import Muon
+    p = _param(4, 5)
+    optimizer = Muon([p])
+    assert not optimizer.state[p]
+    optimizer.step()
+    assert torch.equal(optimizer.state[p]["momentum"], p.grad)
