@@ -12,7 +12,8 @@ class Muon(torch.optim.Optimizer):
 
     params: float32, bfloat16 or float16, contiguous, two axes at least; [out, ..] counts as a matrix of `out` rows.  Others
     (biases, norms' weights, tables looked up by row) belong to another optimizer.  Momenta are float32.  One without a
-    gradient is left as it is.  A step checks every group and parameter before it changes one."""
+    gradient is left as it is.  A step checks every group and parameter before it changes one.  In a graph a
+    step keeps the settings of its capture; a parameter's first step, which makes its momentum, is refused there."""
 
     def __init__(self, params, lr=2e-2, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
                  coefficients=F.NEWTON_SCHULZ, eps=1e-7):
@@ -54,6 +55,8 @@ class Muon(torch.optim.Optimizer):
                                       and m.is_contiguous()):
                 raise RuntimeError("a momentum must be float32, contiguous and beside its parameter of shape %s, got %s %s on %s"
                                    % (tuple(p.shape), m.dtype, tuple(m.shape), m.device))
+        if any(p.is_cuda and self._momentum(p) is None for p in stepped) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a parameter's first step cannot be captured: its momentum would begin as zeros in every replay")
         written = [p.data_ptr() for p in stepped if p.numel()]
         addresses = set(written)
         if len(addresses) < len(written):
