@@ -914,7 +914,8 @@ int sdk_add_layer_norm_backward(const void* grad, const void* grad_sum, const vo
  * output and gradients are zeros.  reverse: from the last token that counts down to the first.
  * Backward: grad_output (its strides) and grad_last may be NULL (zeros); gradients that are NULL are not formed;
  * grad_x, grad_gate [batch, tokens, width] dense.  output is the forward's.
- * width: up to 2^20.  Every sum is formed in an order that depends on the sizes alone. */
+ * width: up to 2^20.  Every sum is formed in an order that depends on the sizes alone.  Workgroups of long sequences wait
+ * for each other, a second at most each: a device that keeps one from running for longer gets NaN from there on. */
 typedef struct sdk_gated_scan {
   const void* x;
   const void* gate;

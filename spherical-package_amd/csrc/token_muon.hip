@@ -761,7 +761,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void product(const Table t, const Se
 // error grows, and once an eigenvalue of zero is rounded to less, it leaves for minus infinity: equal rows are 3e-13 off after
 // 5 steps, 4e-11 after 8, and infinite after 20.  So this is the way of as many steps as keep the product of
 // max |f'| below 2^24 (check_coefficients), which leaves 16 roundings of 2^-53 below 2^-25 of S: six steps of the default
-// coefficients, twelve of 1.875, -1.25, 0.375.  More go by X, whose S is a sum of squares anew in each step.
+// coefficients, thirteen of 1.875, -1.25, 0.375.  More go by X, whose S is a sum of squares anew in each step.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f64x4 product_of(const f64x4& a, const f64x4& b) {
   f64x4 sum = {0, 0, 0, 0};
@@ -770,9 +770,10 @@ __device__ __forceinline__ f64x4 product_of(const f64x4& a, const f64x4& b) {
   return sum;
 }
 
-// Five steps against those of X in LDS or through the launches: 16 x 27 10 us for 18, 16 x 384 13 for 33, 16 x 1000 21 for 88
-// (float32), 2.5e-8 off for 1e-6.  One workgroup reads a long matrix slowly: 16 x 4096 in bfloat16 75 us for 102, but 16 x 8192
-// 140 for 131; in two pieces the launches are behind up to the longest (16 x 131072 1.87 ms for 2.28).
+// Five steps against those of X in LDS or through the launches, float32, 16 rows of 17 values 11 us for 18, of 400 16 for 78,
+// of 1000 24 for 86, of 4096 70 for 134, of 16384 257 for 340, of 131072 1.76 ms for 2.27; 64 of 16 x 16384 at once 268 us for
+// 1160; 3 rows of 1000 18 for 86, of 131072 1.21 ms for 2.28; 2.5e-8 off for 1e-6.  In one piece the launches read half as
+// much: bfloat16, 16 rows of 1000 25 us for 76, of 4096 79 for 101, but of 8192 140 for 131.
 constexpr int kThin = 16, kThinWaves = 8;
 constexpr double kMostGrowth = 1 << 24;
 __host__ __device__ inline bool is_thin(int64_t rows, int64_t columns, bool split) {

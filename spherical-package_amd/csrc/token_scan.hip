@@ -8,14 +8,16 @@
 // (A', H') is (A A', A' H + H').  So a workgroup takes 64 channels in 16 bits (32 in float32: 128 bytes of a token either
 // way; a quarter of that where the width is no larger) and a tile of tokens, of which each thread walks 32 values
 // (backward 16: two to eight tokens) in order; the threads' spans are joined over the tile, and each walks its tokens again
-// from the state in front of them.  The tile's values stay in registers meanwhile.  Where batch and channels fill the GPU a workgroup goes through a whole
-// sequence; otherwise it takes one tile, and tiles hand each other their spans while the kernel runs (scan_tiles).
+// from the state in front of them.  The tile's values stay in registers meanwhile.  Where batch and channels fill the GPU a
+// workgroup goes through a whole sequence; otherwise it takes one tile, and tiles hand each other their spans while the
+// kernel runs (scan_tiles).
 //
 // Bound by memory: three values read or written a token and channel forward, six backward (the gradients read h as
-// it was rounded to the tensors' type).  2 x 8192 tokens of 1024 channels in bfloat16: forward 28 us (3.6 TB/s), backward 48
-// (4.2 TB/s); all tiles of the forward are on the GPU at once, so that reading, waiting and writing follow each other.  A
+// it was rounded to the tensors' type).  2 x 8192 tokens of 1024 channels in bfloat16: forward 28 us (3.6 TB/s), backward 49
+// (4.1 TB/s); all tiles of the forward are on the GPU at once, so that reading, waiting and writing follow each other.  A
 // first launch for the spans of longer segments, which then were read again, took 49 and 74 us.  131072 tokens of 256
-// channels in float16 forward: 53 us (3.8 TB/s; 95 with two launches).
+// channels in float16 forward: 53 us (3.8 TB/s; 95 with two launches).  Whole sequences, 64 of 512 tokens of 1024 channels in
+// bfloat16: forward 45 us (4.5 TB/s), backward 101 (4.0 TB/s).
 //
 // The state, its gradient, the spans and the gates are float32.  Of f and u the lesser is formed, to its own relative
 // precision, and weighs the distance of h and x:
@@ -394,7 +396,9 @@ __device__ __forceinline__ Word seen(const Word* from) {
   return __hip_atomic_load(const_cast<Word*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 constexpr int kTicket = 16;       // words of a group's ticket: a line of its own
-constexpr int kPolls = 1 << 20;   // a second: a wait ends whatever happens, with NaN
+// About a second: a wait ends whatever happens, with NaN.  No wait gets there: it is for a workgroup that has begun (see
+// scan_tiles) and waits for none behind it.
+constexpr int kPolls = 1 << 20;
 
 __global__ __launch_bounds__(256) void clear(Word* words, int64_t count) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) words[i] = 0;
@@ -403,8 +407,8 @@ __global__ __launch_bounds__(256) void clear(Word* words, int64_t count) {
 // One tile of a sequence a workgroup, read once and held in registers while its span goes out and the state in front of it
 // comes in.  Tiles form runs, of 32 where a workgroup has 64 channels: the state in front of a tile is the one behind the
 // run before, carried over the spans of the tiles before it in its run, always in this order, so that results do not depend
-// on who comes first.  Workgroups take the tiles of a group by its ticket, so those before a tile in its sequence have begun when it
-// begins; each publishes its tile's span before it waits for others, and the last of a run waits for nothing that comes
+// on who comes first.  Workgroups take the tiles of a group by its ticket, so those before a tile in its sequence have begun
+// when it begins; each publishes its tile's span before it waits for others, and the last of a run waits for nothing that comes
 // after it: every wait ends.
 constexpr int kLook = 4;
 
