@@ -947,8 +947,8 @@ int sdk_gated_scan_step(const void* x, int64_t x_stride, const void* gate, int64
  *   S = X X^T (of the smaller side)      X = a X + (b S + c S S) X        coefficients: a, b, c (host array)
  * which brings the singular values towards one.  float32 and float16: products from two float16 pieces a value (22
  * bits); bfloat16: from one (11 bits), but for the diagonals of S and b S + c S S (22).  Sums are float32.  Entries are
- * held below 16: coefficients with which a singular value could pass 3.8, or a + b s + c s s pass 15 (s: its square),
- * within the steps are refused.  Sides up to 131072, matrices of up to 2^31 values; out may be x.  eps: 2^-100 to 1.
+ * held below 16: coefficients with which a singular value that may gain 2^-10 of itself a step could pass 3.8, or
+ * a + b s + c s s pass 15 (s: its square), within the steps are refused.  Sides up to 131072, matrices of up to 2^31 values; out may be x.  eps: 2^-100 to 1.
  * Up to 16 rows or columns: 64 bits while the steps are few (six of the default coefficients), the others' bits beyond.
  * The workspace begins at a multiple of 128; the bytes are enough for any steps and coefficients. */
 size_t sdk_orthogonalize_workspace_bytes(int64_t rows, int64_t columns, int64_t count, int32_t dtype);

@@ -1297,14 +1297,17 @@ int check_matrix(int64_t rows, int64_t columns) {
 }
 
 // X begins with a norm of 1 at most, and a step makes of a singular value x the value x q(x^2), q(s) = a + b s + c s^2.
-// Followed from 1 on, no value may pass 3.8, so that S stays below 15, and no q of one 15.
+// Followed from 1 on, no value may pass 3.8, so that S stays below 15, and no q of one 15.  Roundings take values further, in
+// pieces of 11 bits by up to about three times 2^-12 of them a step, and where the polynomial is steep behind its largest
+// value they do not come back: 3 x - x^3 stays within 2 and left float16 after 6 steps.  So 2^-10 goes on top in each step.
 // thin: whether errors of S grow little enough for the steps to go by S alone: f(s) = s q(s)^2 has the slope q(s) r(s),
 // r(s) = a + 3 b s + 5 c s^2.
 int check_coefficients(int64_t steps, const double* k, bool& thin) {
   const double a = k[0], b = k[1], c = k[2];
   auto q = [&](double s) { return std::fabs(a + (b + c * s) * s); };
   auto r = [&](double s) { return std::fabs(a + (3 * b + 5 * c * s) * s); };
-  double most = 1, growth = 1;
+  constexpr double kMore = 1 + 0x1p-10;
+  double most = kMore, growth = 1;
   for (int64_t step = 0; step < steps; ++step) {
     const double end = most * most;
     double of_q = std::max(q(0), q(end)), next = most * q(end);
@@ -1327,7 +1330,7 @@ int check_coefficients(int64_t steps, const double* k, bool& thin) {
     const double turn = -3 * b / (10 * c);   // c = 0: no number, or none inside
     const double of_r = std::max({r(0), r(end), turn > 0 && turn < end ? r(turn) : 0.});
     growth = std::min(growth * std::max(1., of_q * of_r), 2 * kMostGrowth);
-    most = std::max(1e-30, next);
+    most = std::max(1e-30, next * kMore);
   }
   thin = growth <= kMostGrowth;
   return SDK_OK;

@@ -281,7 +281,7 @@ def orthogonalize(input, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     float32 and float16 matrices are multiplied with 22 bits a value, bfloat16 with 11 (but for S's diagonal and the
     polynomial's); sums are float32.
     Coefficients with which a singular value could pass 3.8, or a + b s + c s ** 2 pass 15 (s: its square), within the
-    steps raise.  eps: 2 ** -100 to 1.  No gradients: raises where one would be wanted."""
+    steps raise, also where only roundings (2 ** -10 a step) would take it there.  eps: 2 ** -100 to 1.  No gradients: raises where one would be wanted."""
     if _wants_gradient(input):
         raise RuntimeError("orthogonalize has no gradients: call it under torch.no_grad(), or of a detached input")
     return _sdk_ops.orthogonalize(input, steps, coefficients, eps)

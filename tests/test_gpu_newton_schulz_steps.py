@@ -139,3 +139,26 @@ def test_gradients_are_refused_or_not_wanted():
     assert not want.requires_grad and torch.equal(F.orthogonalize(leaf.detach()), want)
     with torch.no_grad():
         assert torch.equal(F.orthogonalize(leaf), want)
+
+
+def test_coefficients_that_are_taken_stay_in_range():
+    """Whatever the coefficients, what is not refused ends finite, with singular values that pass 3.8 by roundings alone (2^-10 a
+    step, and the slack): of one singular value, which takes the extremes, and of many."""
+    from spherical_distortion import functional as F
+    g = torch.Generator().manual_seed(9)
+    taken = 0
+    for i in range(120):
+        c = ((torch.rand(3, generator=g) * 2 - 1) * torch.tensor([4.0, 6.0, 4.0 * (i % 3 > 0)])).tolist()
+        c = [(3.0, -1.0, 0.0), NS, NEWTON, (2.6, -1.0, 0.0)][i] if i < 4 else c
+        steps = 1 + i % 12
+        for dtype in TYPES:
+            for kind, shape in (("rank one", (8, 50)), ("equal", (40, 30)), ("rank one", (100, 130)), ("full", (70, 70))):
+                try:
+                    got = F.orthogonalize(_matrix(kind, shape, dtype), steps, c)
+                except RuntimeError as e:
+                    assert "grow too far" in str(e)
+                    continue
+                taken += 1
+                assert bool(got.isfinite().all()), (c, steps, kind, shape, dtype)
+                assert float(_values(got)[0]) <= 3.8 * (1 + 2.0 ** -10) + _slack(dtype), (c, steps, kind, shape, dtype)
+    assert taken >= 100   # of 1440 the most are refused

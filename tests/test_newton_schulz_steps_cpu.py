@@ -96,3 +96,13 @@ def test_five_default_steps_as_documented():
         x = a * x + b * x ** 3 + c * x ** 5
     assert 0.68 + 2.4e-4 <= float(x.min()) and float(x.max()) <= 1.21 - 2.4e-4
     assert "between 0.68 and 1.21" in inspect.getsource(token_ops) and float(x.max()) > 1.2
+
+
+def test_coefficients_whose_roundings_grow():
+    """3 x - x^3 takes 1 to 2 and 2 to -2, and 2 (1 + e) to -2 (1 + 9 e): what is rounded past 2 leaves.  2.6 x - x^3 stays within
+    1.62, its largest value, whatever is rounded (2.6 * 1.62 - 1.62^3 = -0.04)."""
+    assert _allowed(3, (3.0, -1.0, 0.0))
+    for steps in (6, 8, 30, 100):
+        assert not _allowed(steps, (3.0, -1.0, 0.0)) and not _allowed(steps, (-3.0, 1.0, 0.0))
+        assert _allowed(steps, (2.6, -1.0, 0.0)) and _allowed(steps, NS) and _allowed(steps, (1.875, -1.25, 0.375))
+        assert _allowed(steps, (1.5, -0.5, 0.0)) and _allowed(steps, (2.0, -1.5, 0.5))
