@@ -149,6 +149,13 @@ __device__ __forceinline__ void read_values(const char* row, int64_t at, float (
   }
 }
 
+// kScale / (norm + eps) for the sum of squares `sum`.  The norm may be beyond float32's largest value, so it and eps are
+// taken down by a power of two, which changes no bit of the others.
+__device__ __forceinline__ float scale_of(double sum, float eps) {
+  constexpr float kNear = 0x1p-24f;
+  return kScale * kNear / ((float)(sqrt(sum) * kNear) + eps * kNear);
+}
+
 __device__ __forceinline__ float update_of(bool momentum, float g, float m, const Settings& s) {
   if (!momentum) return g;
   return s.nesterov ? s.mu * m + s.rest * g : m;
@@ -243,7 +250,7 @@ __global__ __launch_bounds__(256) void lay_out(const Table t, const Settings s, 
 #pragma unroll
   for (int r = 0; r < 16; ++r) tile[4 * r + wave][lane] = update_of(m != nullptr, from[r], held[r], s);
   __syncthreads();
-  const float up = kScale / ((float)sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + s.eps);
+  const float up = scale_of((sums[0] + sums[1]) + (sums[2] + sums[3]), s.eps);
   const int64_t k0 = tall ? c0 : r0, l0 = tall ? r0 : c0;
   for (int c = threadIdx.x; c < 64 * 8; c += 256) {
     const int r = c / 8, from = c % 8 * 8;
@@ -985,7 +992,7 @@ __global__ __launch_bounds__(512) void small_matrix(const Table t, const Setting
   sum = 0;
 #pragma unroll
   for (int w = 0; w < 8; ++w) sum += sums[w];
-  const float up = kScale / ((float)sqrt(sum) + s.eps);
+  const float up = scale_of(sum, s.eps);
   row = row0, vector = vector0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {

@@ -162,3 +162,19 @@ def test_coefficients_that_are_taken_stay_in_range():
                 assert bool(got.isfinite().all()), (c, steps, kind, shape, dtype)
                 assert float(_values(got)[0]) <= 3.8 * (1 + 2.0 ** -10) + _slack(dtype), (c, steps, kind, shape, dtype)
     assert taken >= 100   # of 1440 the most are refused
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(16, 1000), (50, 60), (300, 200)])
+def test_norms_beyond_float32(shape, dtype):
+    """Values of up to 2^127, whose norm float32 does not hold: the bits of the same matrix times 2^-100, as powers of two
+    change nothing but eps' share (2^-122 beside 1)."""
+    from spherical_distortion import functional as F
+    x = _matrix("full", shape, dtype).float()
+    x = (x / x.abs().max()).to(dtype)
+    big = (x.double() * 2.0 ** 127).to(dtype)
+    assert bool(big.isfinite().all()) and float(big.double().norm()) > torch.finfo(torch.float32).max
+    assert torch.equal(F.orthogonalize(big), F.orthogonalize((big.double() * 2.0 ** -100).to(dtype)))
+    p, m = torch.zeros_like(x), big.float().clone()
+    F.muon_step([p], [big], [m], lr=1.0, momentum=0.5)
+    assert torch.equal(m, big.float()) and bool(p.isfinite().all()) and float(p.double().norm()) > 0.5
