@@ -32,24 +32,24 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(str(e)) from None
 
     @staticmethod
-    def _check_shape(p):
-        if p.dim() < 2:
-            raise ValueError("Muon takes parameters of two axes at least, got one of shape %s" % (tuple(p.shape),))
+    def _check_sides(p):
         rows = p.shape[0]
         if max(rows, p.numel() // rows if rows else 0) > 1 << 17 or p.numel() > 1 << 31:
-            raise ValueError("Muon takes matrices with sides up to 131072 and 2^31 values, got a parameter of shape %s"
+            raise RuntimeError("Muon takes matrices with sides up to 131072 and 2^31 values, got a parameter of shape %s"
                              % (tuple(p.shape),))
 
     def _momentum(self, p):
         return self.state.get(p, {}).get("momentum")   # looking it up by [] would make an entry
 
     def _check_step(self):
-        """All that a call would refuse, of every group before one is stepped."""
+        """All that a call would refuse, of every group that is stepped before one is."""
         stepped = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
         for group in self.param_groups:
-            self._check_settings(group)
+            if any(p.grad is not None for p in group["params"]):
+                self._check_settings(group)
         for p in stepped:
             adamw.check_parameter("Muon", p)
+            self._check_sides(p)
             m = self._momentum(p)
             if m is not None and not (m.shape == p.shape and m.dtype == torch.float32 and m.device == p.device
                                       and m.is_contiguous()):
@@ -69,7 +69,8 @@ class Muon(torch.optim.Optimizer):
         try:
             self._check_settings(self.param_groups[-1])
             for p in self.param_groups[-1]["params"]:
-                self._check_shape(p)
+                if p.dim() < 2:
+                    raise ValueError("Muon takes parameters of two axes at least, got one of shape %s" % (tuple(p.shape),))
         except ValueError:
             self.param_groups.pop()
             raise

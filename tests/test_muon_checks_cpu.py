@@ -41,6 +41,9 @@ def test_settings_that_were_changed_since(steps, change):
     optimizer = Muon([dict(params=[_param(4, 5)]), dict(params=[_param(6, 5)])])
     optimizer.param_groups[1].update(change)
     _refused(optimizer, steps)
+    optimizer.param_groups[1]["params"][0].grad = None   # a group that is not stepped
+    optimizer.step()
+    assert steps == [1]
 
 
 @pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate parameters")
@@ -74,18 +77,22 @@ def test_momenta_of_another_model(steps):
     assert not steps and all(torch.equal(p, v) for p, v in zip([p for g in new.param_groups for p in g["params"]], values))
 
 
-def test_sides_that_no_call_takes():
-    """At once: no step would take them."""
+def test_sides_that_no_call_takes(steps):
+    """Refused with a gradient; one without is left as it is."""
     from spherical_distortion.optim import Muon
-    for shape in (((1 << 17) + 1, 2), (1 << 20, 0), (2, (1 << 17) + 1), (1 << 17, 1 << 15), (3, 1 << 9, 1 << 9)):
-        big = torch.nn.Parameter(torch.empty(1).expand(*shape))
-        with pytest.raises(ValueError, match="131072"):
-            Muon([big])
-        optimizer = Muon([_param(4, 5)])
-        with pytest.raises(ValueError, match="131072"):
-            optimizer.add_param_group(dict(params=[big]))
-        assert len(optimizer.param_groups) == 1
-    Muon([torch.nn.Parameter(torch.empty(1).expand(1 << 17, 1 << 14)), torch.nn.Parameter(torch.empty(0, 1 << 20))])
+    for shape in (((1 << 17) + 1, 2), (1 << 20, 0), (2, (1 << 17) + 1), (3, 1 << 9, 1 << 9)):
+        big = _param(*shape)
+        optimizer = Muon([dict(params=[_param(4, 5)]), dict(params=[big])])
+        _refused(optimizer, steps)
+        big.grad = None
+        optimizer.step()
+        assert steps == [1]
+        steps.clear()
+    for shape in ((1 << 17, (1 << 14) + 1), (1 << 16, 1 << 16)):
+        with pytest.raises(RuntimeError, match="131072"):
+            Muon._check_sides(torch.empty(shape, device="meta"))
+    for shape in ((1 << 17, 1 << 14), (0, 1 << 20), (1 << 17, 0)):
+        Muon._check_sides(torch.empty(shape, device="meta"))
 
 
 @pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
