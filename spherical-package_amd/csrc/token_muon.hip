@@ -18,10 +18,10 @@
 // Entries of X, S and P have to stay below 16: no entry is larger than the largest singular value, which the coefficients
 // alone bound (check_coefficients).  Sums are float32, of the norm double.
 //
-// 32 matrices of 640 x 640 to 640 x 2560, 39 million values, a step in float32: 1.81 to 1.88 ms on four cards.  S takes 110 us (820 TFLOP/s of
-// products of pieces; its workgroups' sums are 640 to 2560 long), P 43 (710), X' 165 (910), momentum and norm 77, X_0 85, the
-// last X' into the parameters 190.  A large library product of float16 reaches 1165.  bfloat16: 0.84 to 0.90 ms (S 43 to 46,
-// P 20 to 23, X' 68 to 74, 61, 78 and 100; without the diagonals' rests X' 65 to 70).
+// 32 matrices of 640 x 640 to 640 x 2560, 39 million values, a step in float32: 1.81 to 1.88 ms, as cards differ.  S takes
+// 110 us (820 TFLOP/s of products of pieces; its workgroups' sums are 640 to 2560 long), P 43 (710), X' 165 (910), momentum
+// and norm 77, X_0 85, the last X' into the parameters 190.  A large library product of float16 reaches 1165.  bfloat16: 0.84
+// to 0.90 ms (S 43 to 46, P 20 to 23, X' 68 to 74, 61, 78 and 100; without the diagonals' rests X' 65 to 70).
 //
 // All matrices of a call go through a stage in one launch; their table is a kernel argument.  Small ones go through all
 // stages in a workgroup of their own, those of up to 16 rows on S alone, in 64 bits, where the steps are few.
